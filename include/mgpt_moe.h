@@ -366,6 +366,88 @@ int mgpt_gpt_bin_read_block(const char* path, int num_experts, int hidden_dim, i
 int mgpt_moe_load_gpt_bin(mgpt_moe* h, const char* path, int layer, float* ln2_gamma,
                           void* stream);
 
+/* ---- The training step around the block --------------------------------
+ * Operators without a handle: a config, device pointers and a workspace of
+ * the caller's.  They run on the current HIP device, which the pointers and
+ * the stream belong to; nothing is allocated, copied or waited for, so each
+ * call may be captured into a HIP graph.  The same call on the same inputs
+ * gives the same bits.  Outputs must not overlap inputs except where said. */
+
+/* One AdamW step over any number of tensors, replacing AdamWOptimizer::step
+ * (nn/optimisers/AdamWOptimiser.h:13-97, Tensor::adamw_step,
+ * utils/Tensor.cpp:683-701).  With g = gradient * (*grad_scale), t the number
+ * of the step, c = 1 / (1 - beta^t), every operation rounded to fp32:
+ *   m = b1 m + (1 - b1) g,  v = b2 v + ((1 - b2) g) g,
+ *   p = p - (lr wd) p,  p = p - (lr (m c1)) / (sqrt(v c2) + eps). */
+typedef struct mgpt_adamw_config {
+  float lr, beta1, beta2, eps, weight_decay;   /* betas in [0, 1) */
+  int state_bits;   /* 32: moments in fp32; 8: in 8 bits (layout below) */
+  int grad_dtype;   /* MGPT_DTYPE_F32 or MGPT_DTYPE_BF16 */
+} mgpt_adamw_config;
+
+/* Bytes of the moments of num_tensors tensors with sizes[i] elements (0 ..
+ * 2^34 each).  The state is the caller's, 16-byte aligned, and all zero
+ * bytes before the first step.  Its layout: every tensor takes whole blocks
+ * of 256 elements, in order (element j of tensor i is state element 256 *
+ * (blocks of the tensors before) + j); with B blocks in all, first moments
+ * [256 B], second moments [256 B] in state_bits each, and for 8 bits one
+ * exponent byte per block for the first [B] and for the second moments [B]:
+ *   m = e4m3(code) * 2^(e - 134) (e counts as 16 at least), nearest even;
+ *   v = the fp32 with bits ((e - 31) << 23) + (code << 20) (e counts as 32 at
+ *       least), code 0 is 0, 255 a value that is not finite; rounded up with
+ *       the probability of the part cut off (16 bits of a hash of element and
+ *       step), and never to 0 from above. */
+int mgpt_adamw_state_bytes(int num_tensors, const int64_t* sizes, int state_bits, size_t* bytes);
+
+/* params[i]: fp32, updated in place; grads[i]: grad_dtype, read; copies (may
+ * be null, or hold nulls): bf16 copies of the updated params.  All device
+ * memory, aligned to their elements (16-byte aligned ones are faster), while
+ * the arrays of pointers and sizes are host memory, read during the call.  A
+ * tensor whose grads[i] is null is left as it is, its moments too.  step: 1
+ * for the first; if step_device is not null the device reads the number
+ * there instead (a captured step that is replayed; below 1 counts as 1).
+ * grad_scale: device float, or null for 1 (a clip coefficient). */
+int mgpt_adamw_step(const mgpt_adamw_config* cfg, int num_tensors, const int64_t* sizes,
+                    float* const* params, const void* const* grads, void* const* copies,
+                    void* state, size_t state_bytes, int step, const int32_t* step_device,
+                    const float* grad_scale, void* stream);
+
+/* The norms around a block, with its gate and the scaled residual stream:
+ *   n = h / sqrt(mean(h^2) + eps),  out = residual_scale x + gate (n gamma_post),
+ *   y = out / sqrt(mean(out^2) + eps) * gamma_pre
+ * x (residual stream), h (the block's output), out, y: [N,C] in dtype; the
+ * gains fp32, gamma_post and gamma_pre [C], gate [gate_rows,C], row g for
+ * tokens g N / gate_rows .. (g + 1) N / gate_rows - 1.  y is formed from out
+ * before it is rounded.  A null gain is left out: gamma_post with its norm (n =
+ * h), gate (1, whatever gate_rows says), gamma_pre with y.  The reference has
+ * the pre-norm (RMSNormLayer, utils/Tensor.cpp:785-800). */
+typedef struct mgpt_norm_config {
+  int embed_dim;          /* C: 1 .. 16384 */
+  int dtype;              /* MGPT_DTYPE_F32 or MGPT_DTYPE_BF16 */
+  int gate_rows;          /* >= 1; divides num_tokens */
+  float eps;
+  float residual_scale;
+} mgpt_norm_config;
+
+/* rstd_post, rstd_pre [N] fp32: the two 1/rms, for the backward (null where
+ * their gain is). */
+int mgpt_norm_forward(const mgpt_norm_config* cfg, const void* x, const void* h,
+                      const float* gamma_post, const float* gate, const float* gamma_pre, void* out,
+                      void* y, float* rstd_post, float* rstd_pre, int num_tokens, void* stream);
+
+int mgpt_norm_backward_workspace_bytes(const mgpt_norm_config* cfg, int num_tokens, size_t* bytes);
+
+/* Gradients of mgpt_norm_forward for the upstream gradients dout of out (null:
+ * none, allowed with gamma_pre) and dy of y, from the same x, h and gains and
+ * the rstd that it wrote: dx, dh [N,C] in dtype, and where not null
+ * dgamma_post [C], dgate [gate_rows,C], dgamma_pre [C] fp32, all written,
+ * not added to.  workspace: 256-byte aligned. */
+int mgpt_norm_backward(const mgpt_norm_config* cfg, const void* x, const void* h,
+                       const float* gamma_post, const float* gate, const float* gamma_pre,
+                       const float* rstd_post, const float* rstd_pre, const void* dout, const void* dy,
+                       void* dx, void* dh, float* dgamma_post, float* dgate, float* dgamma_pre,
+                       int num_tokens, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Description of the last error on this host thread ("" if none). */
 const char* mgpt_moe_last_error(void);
 

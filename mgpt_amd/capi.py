@@ -52,6 +52,17 @@ class GptBinInfo(ctypes.Structure):
                 ("block_floats", ctypes.c_int64), ("moe_floats", ctypes.c_int64)]
 
 
+class AdamWConfig(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_float), ("beta1", ctypes.c_float), ("beta2", ctypes.c_float),
+                ("eps", ctypes.c_float), ("weight_decay", ctypes.c_float),
+                ("state_bits", ctypes.c_int), ("grad_dtype", ctypes.c_int)]
+
+
+class NormConfig(ctypes.Structure):
+    _fields_ = [("embed_dim", ctypes.c_int), ("dtype", ctypes.c_int), ("gate_rows", ctypes.c_int),
+                ("eps", ctypes.c_float), ("residual_scale", ctypes.c_float)]
+
+
 class MoEError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"mgpt_moe status {status}: {message}")
@@ -103,6 +114,11 @@ def lib() -> ctypes.CDLL:
         "mgpt_gpt_bin_inspect": [ctypes.c_char_p, i, i, ctypes.POINTER(GptBinInfo)],
         "mgpt_gpt_bin_read_block": [ctypes.c_char_p, i, i, i, vp, vp, sz],
         "mgpt_moe_load_gpt_bin": [vp, ctypes.c_char_p, i, vp, vp],
+        "mgpt_adamw_state_bytes": [i, vp, i, ctypes.POINTER(sz)],
+        "mgpt_adamw_step": [ctypes.POINTER(AdamWConfig), i, vp, vp, vp, vp, vp, sz, i, vp, vp, vp],
+        "mgpt_norm_forward": [ctypes.POINTER(NormConfig)] + [vp] * 9 + [i, vp],
+        "mgpt_norm_backward_workspace_bytes": [ctypes.POINTER(NormConfig), i, ctypes.POINTER(sz)],
+        "mgpt_norm_backward": [ctypes.POINTER(NormConfig)] + [vp] * 14 + [i, vp, sz, vp],
     }
     for name, args in sig.items():
         f = getattr(L, name)

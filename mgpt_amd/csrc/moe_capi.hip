@@ -135,14 +135,6 @@ using namespace mgpt;
 
 namespace {
 
-#define HIP_TRY(expr)                                                                  \
-  do {                                                                                 \
-    hipError_t _e = (expr);                                                            \
-    if (_e != hipSuccess)                                                              \
-      return fail(MGPT_ERR_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(_e), \
-                  __FILE__, __LINE__);                                                 \
-  } while (0)
-
 constexpr size_t kAlign = 256;
 constexpr size_t kGemmPartialBytes = 512 * 128 * 4;   // one 256x256 fp32 tile
 constexpr int kRowPad = 256;   // rows of slack after activation buffers (GEMM tile overrun)

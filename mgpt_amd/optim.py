@@ -1,0 +1,102 @@
+"""AdamW: one step over all tensors of a model in one launch per 96 of them.
+
+Mirrors the engine's AdamWOptimizer
+(/root/reference/src/main/neuralnetwork/optimisers/AdamWOptimiser.h:13-97)
+over the C ABI (mgpt_adamw_step).  The moments are fp32 or 8 bits per value;
+the parameters are fp32 CUDA tensors, updated in place, e.g. the 2 + 6E
+tensors a MoELayer loads, with the gradients of MoELayer.get_gradients().
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import capi
+
+_GRAD = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16}
+
+
+class AdamW:
+    """params: contiguous float32 CUDA tensors of one device.  copies: None, or
+    per parameter a bfloat16 tensor of its size (or None) that every step
+    refreshes.  state_bits: 32 or 8.  device_step: keep the step's number on
+    the device, so that a step captured into a HIP graph counts on when it is
+    replayed (step_count then stays where it was)."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.01, state_bits: int = 32, copies=None, device_step: bool = False):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("no parameters")
+        self.lr, self.betas, self.eps, self.weight_decay = lr, tuple(betas), eps, weight_decay
+        self.state_bits = state_bits
+        self.device = self.params[0].device
+        self.copies = list(copies) if copies is not None else None
+        if self.copies is not None and len(self.copies) != len(self.params):
+            raise ValueError("copies must have an entry per parameter")
+        for i, p in enumerate(self.params):
+            self._check(p, torch.float32, p.numel(), f"params[{i}]")
+            if self.copies is not None and self.copies[i] is not None:
+                self._check(self.copies[i], torch.bfloat16, p.numel(), f"copies[{i}]")
+        self.step_count = 0
+        n = len(self.params)
+        self._sizes = (ctypes.c_int64 * n)(*[p.numel() for p in self.params])
+        need = ctypes.c_size_t()
+        capi.check(capi.lib().mgpt_adamw_state_bytes(n, self._sizes, state_bits, ctypes.byref(need)))
+        self.state = torch.zeros(need.value, dtype=torch.uint8, device=self.device)
+        self._step_device = (torch.zeros(1, dtype=torch.int32, device=self.device) if device_step else None)
+        blocks = sum((p.numel() + 255) // 256 for p in self.params)
+        held = blocks * 256 * state_bits // 8
+        kinds = (torch.float32, torch.float32) if state_bits == 32 else (torch.float8_e4m3fn, torch.uint8)
+        # views of the state, in its own order (a tensor takes whole blocks of 256)
+        self.m = self.state[:held].view(kinds[0])
+        self.v = self.state[held:2 * held].view(kinds[1])
+        self.m_exp = self.state[2 * held:2 * held + blocks] if state_bits == 8 else None
+        self.v_exp = self.state[2 * held + blocks:] if state_bits == 8 else None
+
+    def _check(self, t, dtype, numel, what):
+        if t.device != self.device or not t.is_cuda:
+            raise ValueError(f"{what} must be a CUDA tensor on {self.device}")
+        if t.dtype != dtype:
+            raise TypeError(f"{what} must be {dtype}")
+        if t.numel() != numel or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous with {numel} elements")
+
+    def step(self, grads, grad_scale: torch.Tensor | None = None) -> None:
+        """One step from `grads`: per parameter a contiguous tensor of its size,
+        all float32 or all bfloat16, or None (the parameter and its moments
+        stay).  grad_scale: float32 device tensor of one element."""
+        grads = list(grads)
+        n = len(self.params)
+        if len(grads) != n:
+            raise ValueError(f"expected {n} gradients, got {len(grads)}")
+        dtype = next((g.dtype for g in grads if g is not None), torch.float32)
+        if dtype not in _GRAD:
+            raise TypeError("gradients must be float32 or bfloat16")
+        gp = (ctypes.c_void_p * n)()
+        pp = (ctypes.c_void_p * n)()
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            pp[i] = p.data_ptr()
+            if g is not None:
+                self._check(g, dtype, self._sizes[i], f"grads[{i}]")
+                gp[i] = g.data_ptr()
+        cp = None
+        if self.copies is not None:
+            cp = (ctypes.c_void_p * n)(*[None if c is None else c.data_ptr() for c in self.copies])
+        scale = None
+        if grad_scale is not None:
+            self._check(grad_scale, torch.float32, 1, "grad_scale")
+            scale = grad_scale.data_ptr()
+        cfg = capi.AdamWConfig(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
+                               self.state_bits, _GRAD[dtype])
+        with torch.cuda.device(self.device):
+            number = self.step_count + 1
+            at = None
+            if self._step_device is not None:
+                self._step_device.add_(1)
+                at = self._step_device.data_ptr()
+            capi.check(capi.lib().mgpt_adamw_step(
+                ctypes.byref(cfg), n, self._sizes, pp, gp, cp, self.state.data_ptr(), self.state.numel(),
+                number, at, scale, torch.cuda.current_stream().cuda_stream))
+        self.step_count = number
