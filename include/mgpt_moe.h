@@ -448,6 +448,42 @@ int mgpt_norm_backward(const mgpt_norm_config* cfg, const void* x, const void* h
                        void* dx, void* dh, float* dgamma_post, float* dgate, float* dgamma_pre,
                        int num_tokens, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The loss of a language model's head over its vocabulary, without keeping
+ * the logits z = x W^T + bias:
+ *   lse[n] = log(sum over v of exp(z[n][v])),  loss[n] = lse[n] - z[n][targets[n]]
+ * x [N,C], W [V,C] in dtype, row-major, bias [V] fp32 or null.  (The engine's
+ * lm_head keeps W transposed, [C,V].)  A target outside 0 .. V - 1 means that
+ * the row has none: its loss is 0 and it adds to no gradient.  Replaces
+ * lm_head's LinearLayer and CrossEntropyLossLayer. */
+typedef struct mgpt_lm_loss_config {
+  int embed_dim;    /* C: 1 .. 2^20 (multiples of 64 (bf16) or 32 (fp32) are read in place) */
+  int vocab_size;   /* V: 1 .. 2^24 */
+  int dtype;        /* MGPT_DTYPE_F32 or MGPT_DTYPE_BF16 */
+} mgpt_lm_loss_config;
+
+int mgpt_lm_loss_workspace_bytes(const mgpt_lm_loss_config* cfg, int num_tokens, size_t* bytes);
+int mgpt_lm_loss_backward_workspace_bytes(const mgpt_lm_loss_config* cfg, int num_tokens,
+                                          size_t* bytes);
+
+/* loss, lse: [N] fp32; mean (may be null): [2] fp32, the mean loss over the
+ * rows with a target (0 if there is none) and their number.  num_tokens up to
+ * 2^21.  workspace: 256-byte aligned. */
+int mgpt_lm_loss_forward(const mgpt_lm_loss_config* cfg, const void* x, const void* W,
+                         const float* bias, const int32_t* targets, float* loss, float* lse,
+                         float* mean, int num_tokens, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Gradients from the same x, W, bias and targets and the forward's lse, for
+ * the upstream gradient dloss [N] fp32 of each row's loss or, where dloss is
+ * null, dmean [1] of their mean (null: 1): dx [N,C], dW [V,C] in dtype, dbias
+ * [V] fp32, each written (not added to) where it is not null.  The logits are
+ * formed again, a piece of the vocabulary at a time.  Workspace: up to about 1
+ * GiB for a piece's gradients, and copies of x and of a piece of W. */
+int mgpt_lm_loss_backward(const mgpt_lm_loss_config* cfg, const void* x, const void* W,
+                          const float* bias, const int32_t* targets, const float* lse,
+                          const float* dloss, const float* dmean, void* dx, void* dW, float* dbias,
+                          int num_tokens, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Description of the last error on this host thread ("" if none). */
 const char* mgpt_moe_last_error(void);
 

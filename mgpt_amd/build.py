@@ -22,7 +22,7 @@ OBJ = os.path.join(HERE, "_build")
 HIP_SOURCES = ["router.hip", "dispatch.hip", "gemm.hip", "gemm_f32.hip", "gemm_dma.hip", "gemm_stream.hip",
                "gemm_decode.hip", "combine.hip",
                "pack.hip", "backward.hip", "wgrad.hip", "moe_capi.hip", "checkpoint.cpp",
-               "adamw.hip", "norm.hip"]
+               "adamw.hip", "norm.hip", "lm_loss.hip"]
 ARCH = os.environ.get("MGPT_OFFLOAD_ARCH", "gfx950")
 
 # -ffp-contract=off: the router must round every product and sum separately

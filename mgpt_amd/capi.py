@@ -63,6 +63,10 @@ class NormConfig(ctypes.Structure):
                 ("eps", ctypes.c_float), ("residual_scale", ctypes.c_float)]
 
 
+class LMLossConfig(ctypes.Structure):
+    _fields_ = [("embed_dim", ctypes.c_int), ("vocab_size", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
 class MoEError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"mgpt_moe status {status}: {message}")
@@ -116,6 +120,10 @@ def lib() -> ctypes.CDLL:
         "mgpt_moe_load_gpt_bin": [vp, ctypes.c_char_p, i, vp, vp],
         "mgpt_adamw_state_bytes": [i, vp, i, ctypes.POINTER(sz)],
         "mgpt_adamw_step": [ctypes.POINTER(AdamWConfig), i, vp, vp, vp, vp, vp, sz, i, vp, vp, vp],
+        "mgpt_lm_loss_workspace_bytes": [ctypes.POINTER(LMLossConfig), i, ctypes.POINTER(sz)],
+        "mgpt_lm_loss_backward_workspace_bytes": [ctypes.POINTER(LMLossConfig), i, ctypes.POINTER(sz)],
+        "mgpt_lm_loss_forward": [ctypes.POINTER(LMLossConfig)] + [vp] * 7 + [i, vp, sz, vp],
+        "mgpt_lm_loss_backward": [ctypes.POINTER(LMLossConfig)] + [vp] * 10 + [i, vp, sz, vp],
         "mgpt_norm_forward": [ctypes.POINTER(NormConfig)] + [vp] * 9 + [i, vp],
         "mgpt_norm_backward_workspace_bytes": [ctypes.POINTER(NormConfig), i, ctypes.POINTER(sz)],
         "mgpt_norm_backward": [ctypes.POINTER(NormConfig)] + [vp] * 14 + [i, vp, sz, vp],

@@ -1,0 +1,1053 @@
+// lm_loss.hip -- softmax cross entropy of a language model's head over its
+// vocabulary, and its gradients, without ever holding the logits.
+//
+// Reference: LinearLayer lm_head, then CrossEntropyLossLayer (layers/LinearLayer.cpp,
+// layers/CrossEntropyLossLayer.cpp), which keep logits, probabilities and their
+// gradients, three [N][V] arrays.  Here, with z = x W^T + b (x [N][C], W [V][C]):
+//   forward:  lse_n = log sum_v exp(z_nv),  loss_n = lse_n - z_n,t(n)
+//   backward: d_nv = (exp(z_nv - lse_n) - [v = t(n)]) g_n, with g_n row n's upstream
+//             gradient (0 where it has no target),
+//             dx = d W,  dW = d^T x,  db_v = sum_n d_nv
+//
+// Forward: one product whose epilogue reduces every 64 columns of a row to (max, sum of
+// exponentials) and picks the target's logit; join_kernel adds them up.
+// Backward, for a piece of the vocabulary at a time: the product again, whose epilogue
+// forms d, in the inputs' type, as rows [N][piece] and transposed [piece][N] (both
+// from registers, so that every product has both operands contiguous along its
+// contraction), and its column sums; then dx += d W_piece and dW_piece = d^T x.
+//
+// All four products are one kernel (ring_kernel): a persistent block per CU walks 256 x
+// 256 tiles, operands go HBM -> LDS by untracked 1 KB loads into a ring of 5 units (an
+// operand's 128-byte slabs of a tile), 8 waves of 64 columns x 128 rows run D = B . A^T
+// by v_mfma_f32_32x32x16_bf16 or, for fp32, v_mfma_f32_32x32x2_f32 on the same 16-byte
+// fragments (gemm_dma.hip describes the ring and its measurements).  Rows past an
+// operand's last re-read the last, so that nothing behind a caller's tensor is
+// touched.  Few tiles take 64 x 128 ones, two blocks of 4 waves a CU, and products of
+// few tiles (dx, dW) split their contraction, the parts added in order.
+//
+// What bounds it: the matrix rate, 2 N C V operations forward and 6 N C V backward (a
+// third of them to form the logits again), except for few rows, where reading W does.
+// Logits, sums and their logarithms are fp32.  With bf16 inputs d is rounded to bf16, as
+// the operand of two bf16 products; db is summed from d before that.
+#include <algorithm>
+#include <type_traits>
+
+#include "../../include/mgpt_moe.h"
+#include "capi_internal.hpp"
+#include "gemm_ring.hpp"
+
+namespace mgpt {
+
+template <typename T>
+hipError_t launch_copy_cols(const T*, int, T*, int, int, int, int, hipStream_t);   // pack.hip
+template <typename T>
+hipError_t launch_transpose_pad(const T*, int, int, size_t, T*, int, int, size_t, int,
+                                hipStream_t);                                     // backward.hip
+hipError_t launch_fill_zero(float* p, size_t n, hipStream_t stream);              // backward.hip
+
+namespace {
+
+enum LossEpilogue {
+  kLse,      // (max, sum of exponentials) per row and 64 columns, the target's logit
+  kDLogit,   // d and its transpose, its column sums
+  kPart,     // fp32 partial product, stored or added
+  kStore     // the product in the inputs' type
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct LossArgs {
+  const char *A, *B;     // A [M][lda], B [Nf][ldb], contiguous along the contraction
+  size_t lda, ldb;       // bytes; multiples of 16
+  int M, Nf, KT;         // rows, columns, 128-byte slabs of the contraction
+  int mt, nt, parts;     // tiles; parts of the contraction
+  // kLse and kDLogit: bias of the columns (or null), targets counted from column 0
+  const float* bias;
+  const int32_t* targets;
+  int target0;           // the piece's first column
+  float2* part_lse;      // [Nf / 64][ld_lse]
+  int ld_lse;
+  float* picked;         // [M]
+  const float *lse, *scale;
+  char *d, *dt;          // [M][ldd], [.][lddt] in T
+  size_t ldd, lddt;      // elements
+  int rows_t;            // rows that the transpose holds (zeros past M)
+  float* colsum;         // [2 mt][ldd] or null
+  // kPart: out [parts][M][ldo] fp32; kStore: out [M][ldo] in T
+  char* out;
+  size_t ldo;
+  int add, vec;
+};
+
+template <typename T> struct Frag;
+template <> struct Frag<bf16_t> { typedef bf16x8 type; };
+template <> struct Frag<float> { typedef f32x4 type; };
+
+__device__ __forceinline__ f32x16 contract(bf16x8 w, bf16x8 x, f32x16 acc) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, x, acc, 0, 0, 0);
+}
+// (k-step x pairs element x of the lane halves' vectors in both operands)
+__device__ __forceinline__ f32x16 contract(f32x4 w, f32x4 x, f32x16 acc) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(w[q], x[q], acc, 0, 0, 0);
+  return acc;
+}
+
+// A 1 KB direct-to-LDS load (see dma16) from a uniform base and a lane's offset.
+__device__ __forceinline__ void dma16_base(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+
+// A wave-uniform address, in scalar registers.
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t u = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return reinterpret_cast<const char*>((uintptr_t)(((uint64_t)hi << 32) | lo));
+}
+
+__device__ __forceinline__ float other_half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float other_half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Sum over the 32 lanes of each half, in its last lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_fadd(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  v = dpp_fadd<0x111, 0xf>(v);
+  v = dpp_fadd<0x112, 0xf>(v);
+  v = dpp_fadd<0x114, 0xf>(v);
+  v = dpp_fadd<0x118, 0xf>(v);
+  return dpp_fadd<0x142, 0xa>(v);
+}
+
+// Lane r of each four holds the 4 bf16 features of token r; afterwards it holds feature r
+// of the 4 tokens.
+__device__ __forceinline__ uint2 transpose4(uint2 u, int lane) {
+  const uint32_t p0 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, 0xB1, 0xf, 0xf, false);   // lane ^ 1
+  const uint32_t p1 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, 0xB1, 0xf, 0xf, false);
+  const bool odd = lane & 1, upper = lane & 2;
+  const uint32_t sel = odd ? 0x07060302u : 0x05040100u;
+  const uint32_t a0 = __builtin_amdgcn_perm(odd ? u.x : p0, odd ? p0 : u.x, sel);
+  const uint32_t a1 = __builtin_amdgcn_perm(odd ? u.y : p1, odd ? p1 : u.y, sel);
+  const uint32_t r = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(upper ? a0 : a1), 0x4E, 0xf, 0xf, false);   // lane ^ 2
+  return upper ? make_uint2(r, a1) : make_uint2(a0, r);
+}
+
+// Biases of a 32-column group's registers (column 8g + 4h + q, register 4g + q), -inf for
+// the columns past the last.
+__device__ __forceinline__ void load_bias(const LossArgs& g, int f0, int lhalf, float (&b)[16]) {
+  const bool whole = f0 + 32 <= g.Nf;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int f = f0 + 8 * k + 4 * lhalf + q;
+      float v = 0.0f;
+      if (g.bias) v = g.bias[whole ? f : min(f, g.Nf - 1)];
+      if (!whole && f >= g.Nf) v = -INFINITY;
+      b[4 * k + q] = v;
+    }
+}
+
+template <typename W>
+using Acc = f32x16[W::TN][W::TM];
+
+template <typename T, typename W>
+__device__ __forceinline__ void emit_lse(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow, int lhalf) {
+  if (fw >= g.Nf) return;
+  float b[W::TN][16];
+#pragma unroll
+  for (int j = 0; j < W::TN; ++j) load_bias(g, fw + 32 * j, lhalf, b[j]);
+#pragma unroll
+  for (int i = 0; i < W::TM; ++i) {
+    const int row = row0 + 32 * i + lrow;
+    const bool live = row < g.M;
+    const int t = live ? g.targets[row] : -1;
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < W::TN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        acc[j][i][v] += b[j][v];
+        m = fmaxf(m, acc[j][i][v]);
+      }
+    m = other_half_max(m);
+    // (differences before they are scaled: logits of the type's lowest value stay finite)
+    const float top = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < W::TN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s += __builtin_amdgcn_exp2f((acc[j][i][v] - top) * kLog2e);
+    s = other_half_sum(s);
+    if (live && lhalf == 0) g.part_lse[(size_t)(fw / 64) * g.ld_lse + row] = make_float2(m, s);
+    const int fl = t >= fw && t < min(fw + 64, g.Nf) ? t - fw : -1;
+    const bool mine = fl >= 0 && ((fl >> 2) & 1) == lhalf;
+    if (__ballot(mine)) {
+      float z = 0.0f;
+#pragma unroll
+      for (int j = 0; j < W::TN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (fl == 32 * j + 8 * (v / 4) + 4 * lhalf + v % 4) z = acc[j][i][v];
+      if (mine) g.picked[row] = z;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+template <typename T, typename W>
+__device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow, int lhalf,
+                                            int sum_row) {
+  float lse[W::TM], sc[W::TM];
+  int tg[W::TM];
+#pragma unroll
+  for (int i = 0; i < W::TM; ++i) {
+    const int row = row0 + 32 * i + lrow, r = min(row, g.M - 1);
+    lse[i] = g.lse[r];
+    sc[i] = row < g.M ? g.scale[r] : 0.0f;
+    tg[i] = g.targets[r] - g.target0;
+  }
+  T* dm = reinterpret_cast<T*>(g.d);
+  T* dt = reinterpret_cast<T*>(g.dt);
+#pragma unroll
+  for (int j = 0; j < W::TN; ++j) {
+    const int f0 = fw + 32 * j;
+    float b[16], cs[16];
+    load_bias(g, f0, lhalf, b);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) cs[v] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W::TM; ++i) {
+      const int row = row0 + 32 * i + lrow;
+      float d[16];
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int f = f0 + 8 * (v / 4) + 4 * lhalf + v % 4;
+        const float p = __builtin_amdgcn_exp2f((acc[j][i][v] + b[v] - lse[i]) * kLog2e);
+        d[v] = (f == tg[i] ? p - 1.0f : p) * sc[i];
+        d[v] = sc[i] == 0.0f ? 0.0f : d[v];
+        cs[v] += d[v];
+      }
+      if constexpr (sizeof(T) == 2) {
+        uint2 q[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = pack4_bf16(d[4 * k], d[4 * k + 1], d[4 * k + 2], d[4 * k + 3]);
+        store_group32(dm + (size_t)row * g.ldd + f0, q, lhalf, row < g.M);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint2 u = transpose4(q[k], lrow);
+          const int f = f0 + 8 * k + 4 * lhalf + (lrow & 3), r4 = row & ~3;
+          if (r4 < g.rows_t) *reinterpret_cast<uint2*>(dt + (size_t)f * g.lddt + r4) = u;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int f = f0 + 8 * k + 4 * lhalf;
+          if (row < g.M)
+            *reinterpret_cast<float4*>(dm + (size_t)row * g.ldd + f) =
+                make_float4(d[4 * k], d[4 * k + 1], d[4 * k + 2], d[4 * k + 3]);
+          if (row < g.rows_t) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) dt[(size_t)(f + q) * g.lddt + row] = d[4 * k + q];
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (g.colsum) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float s = half_sum(cs[v]);
+        if (lrow == 31) g.colsum[(size_t)sum_row * g.ldd + f0 + 8 * (v / 4) + 4 * lhalf + v % 4] = s;
+      }
+    }
+  }
+}
+
+template <typename W>
+__device__ __forceinline__ void emit_part(const LossArgs& g, Acc<W>& acc, int part, int row0, int fw, int lrow,
+                                          int lhalf) {
+  float* out = reinterpret_cast<float*>(g.out) + (size_t)part * g.M * g.ldo;
+#pragma unroll
+  for (int j = 0; j < W::TN; ++j) {
+    const int f0 = fw + 32 * j + 4 * lhalf;
+    if (fw + 32 * j >= g.Nf) continue;
+#pragma unroll
+    for (int i = 0; i < W::TM; ++i) {
+      const int row = row0 + 32 * i + lrow;
+      if (row < g.M) {
+        float4* o = reinterpret_cast<float4*>(out + (size_t)row * g.ldo + f0);   // (ldo covers whole tiles)
+        float4 old[4];
+        if (g.add) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) old[k] = o[2 * k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float4 r = make_float4(acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]);
+          if (g.add) {
+            r.x = old[k].x + r.x;
+            r.y = old[k].y + r.y;
+            r.z = old[k].z + r.z;
+            r.w = old[k].w + r.w;
+          }
+          o[2 * k] = r;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+template <typename T, typename W>
+__device__ __forceinline__ void emit_store(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow, int lhalf) {
+  T* out = reinterpret_cast<T*>(g.out);
+#pragma unroll
+  for (int j = 0; j < W::TN; ++j) {
+    const int f0 = fw + 32 * j;
+    if (f0 >= g.Nf) continue;
+    const bool vec = g.vec && f0 + 32 <= g.Nf;
+#pragma unroll
+    for (int i = 0; i < W::TM; ++i) {
+      const int row = row0 + 32 * i + lrow;
+      T* o = out + (size_t)row * g.ldo + f0;
+      if (vec) {
+        if constexpr (sizeof(T) == 2) {
+          uint2 q[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            q[k] = pack4_bf16(acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]);
+          store_group32(o, q, lhalf, row < g.M);
+        } else if (row < g.M) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4*>(o + 8 * k + 4 * lhalf) =
+                make_float4(acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]);
+        }
+      } else if (row < g.M) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int f = 8 * (v / 4) + 4 * lhalf + v % 4;
+          if (f0 + f < g.Nf) store_act(o + f, acc[j][i][v]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+struct Item {
+  int row0, n0, k0, k1, part;
+};
+
+template <int BM, int BN>
+__device__ __forceinline__ bool locate_item(const LossArgs& g, int v, Item* it) {
+  const int tiles = g.mt * g.nt;
+  if (v >= tiles * g.parts) return false;
+  const int part = v / tiles, u = v % tiles;
+  // groups of kGroupM row tiles x all column tiles, rows fastest (as locate_tile)
+  const int grp = u / (kGroupM * g.nt), gsize = min(kGroupM, g.mt - grp * kGroupM);
+  const int idx = u - grp * kGroupM * g.nt;
+  it->row0 = __builtin_amdgcn_readfirstlane((grp * kGroupM + idx % gsize) * BM);
+  it->n0 = __builtin_amdgcn_readfirstlane(idx / gsize * BN);
+  it->part = __builtin_amdgcn_readfirstlane(part);
+  // (parts <= 16 and KT < 2^17: no overflow)
+  it->k0 = __builtin_amdgcn_readfirstlane(part * g.KT / g.parts);
+  it->k1 = __builtin_amdgcn_readfirstlane((part + 1) * g.KT / g.parts);
+  return true;
+}
+
+// D[m][f] = sum_k A[m][k] B[f][k].  Ring, swizzle and schedule as gemm_ring5_kernel: units
+// A0 B0 A1 B1 .. of consecutive slabs, barrier s frees slab s - 1's two slots for the
+// weights of slab s + 1 and the rows of slab s + 2, whose loads go out in quarters
+// between the matrix instructions.
+template <typename T, int EPI, int BM, int BN, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
+  using W = Waves<NW, BM, BN>;
+  typedef typename Frag<T>::type F;
+  constexpr int kTN = W::TN, kTM = W::TM, kUnits = 5, kRow = 128;
+  constexpr int kSlot = (BM > BN ? BM : BN) * kRow;
+  constexpr int kDA = BM * kRow / 1024 / NW, kDB = BN * kRow / 1024 / NW;   // loads per wave and unit
+  __shared__ __attribute__((aligned(1024))) char smem[kUnits * kSlot];
+
+  const int G = gridDim.x, items = g.mt * g.nt * g.parts;
+  int t = blockIdx.x;
+  if (G % kNumXcd == 0) {   // each XCD a contiguous run of each round
+    const int run = (min(G, items) + kNumXcd - 1) / kNumXcd, in_xcd = (int)blockIdx.x / kNumXcd;
+    t = in_xcd < run ? (int)(blockIdx.x % kNumXcd) * run + in_xcd : items;
+  }
+  Item cur;
+  if (!locate_item<BM, BN>(g, t, &cur)) return;
+
+  const int tid = threadIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = lane_id();
+  const int wn = w % W::WN, wm = w / W::WN;
+  const int lrow = lane & 31, lhalf = lane >> 5;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)smem;
+  const uint32_t lds_a = lds0 + (uint32_t)(w * kDA * 1024), lds_b = lds0 + (uint32_t)(w * kDB * 1024);
+
+  // Cursors of the two operands, the rows' a slab ahead of the columns'.  Past the
+  // block's last slab they stay on it (in bounds, into a slot that is no longer read).
+  struct Cursor {
+    Item it;
+    int v, kt;
+    bool valid;
+  };
+  Cursor ca = {cur, t, cur.k0, true}, cb = ca;
+  uint32_t a_off[kDA], b_off[kDB];
+  const char *a_base, *b_base;
+  auto enter_a = [&]() __attribute__((always_inline)) {
+    a_base = g.A + (size_t)ca.it.row0 * g.lda;
+    const int last = g.M - 1 - ca.it.row0;
+#pragma unroll
+    for (int i = 0; i < kDA; ++i) {
+      const int r = (w * kDA + i) * 8 + lane / 8;
+      a_off[i] = (uint32_t)min(r, last) * (uint32_t)g.lda + (uint32_t)(((lane % 8) ^ ((r >> 1) & 7)) << 4);
+    }
+  };
+  auto enter_b = [&]() __attribute__((always_inline)) {
+    b_base = g.B + (size_t)cb.it.n0 * g.ldb;
+    const int last = g.Nf - 1 - cb.it.n0;
+#pragma unroll
+    for (int i = 0; i < kDB; ++i) {
+      const int r = (w * kDB + i) * 8 + lane / 8;
+      b_off[i] = (uint32_t)min(r, last) * (uint32_t)g.ldb + (uint32_t)(((lane % 8) ^ ((r >> 1) & 7)) << 4);
+    }
+  };
+  // moves a cursor past the slab that was just taken; true: to another item
+  auto advance = [&](Cursor& c) __attribute__((always_inline)) {
+    if (!c.valid || ++c.kt < c.it.k1) return false;
+    Item nx;
+    c.v += G;
+    c.valid = locate_item<BM, BN>(g, c.v, &nx);
+    if (!c.valid) {
+      --c.kt;
+      return false;
+    }
+    c.it = nx;
+    c.kt = nx.k0;
+    return true;
+  };
+  enter_a();
+  enter_b();
+  int dslot = 0;
+  bool fresh_a = false, fresh_b = false;   // the cursor's item has no offsets yet
+  const char *ua, *ub;
+  uint32_t da, db;
+  auto take_a = [&]() __attribute__((always_inline)) {
+    if (fresh_a) enter_a();
+    ua = uniform(a_base + (size_t)ca.kt * kRow);
+    da = lds_a + (uint32_t)(dslot * kSlot);
+    dslot = dslot + 1 == kUnits ? 0 : dslot + 1;
+    fresh_a = advance(ca);
+  };
+  auto take_b = [&]() __attribute__((always_inline)) {
+    if (fresh_b) enter_b();
+    ub = uniform(b_base + (size_t)cb.kt * kRow);
+    db = lds_b + (uint32_t)(dslot * kSlot);
+    dslot = dslot + 1 == kUnits ? 0 : dslot + 1;
+    fresh_b = advance(cb);
+  };
+  // loads d0 .. d1 - 1 of the taken units, the columns' first
+  auto issue = [&](int d0, int d1) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = d0; d < d1; ++d) {
+      if (d < kDB)
+        dma16_base(ub, b_off[d], db + d * 1024);
+      else
+        dma16_base(ua, a_off[d - kDB], da + (d - kDB) * 1024);
+    }
+  };
+  constexpr int kD = kDA + kDB;
+  auto quarter = [&](int q) __attribute__((always_inline)) { issue(q * kD / 4, (q + 1) * kD / 4); };
+  auto slab_wait = [&]() __attribute__((always_inline)) {
+    slab_barrier<kDA>();   // all but the rows of the slab after next
+    take_b();
+    take_a();
+  };
+
+  const int swz = (lrow >> 1) & 7;
+  const char* x_base = smem + (wm * W::WTM + lrow) * kRow;
+  const char* w_base = smem + (wn * W::WTN + lrow) * kRow;
+  F xf[2][kTM], wf[2][kTN];
+  auto frags = [&](int aslot, int ks, F (&xs)[kTM], F (&ws)[kTN]) __attribute__((always_inline)) {
+    const int bslot = aslot + 1 == kUnits ? 0 : aslot + 1;
+    const int cofs = (((ks * 2 + lhalf) ^ swz) << 4);
+#pragma unroll
+    for (int i = 0; i < kTM; ++i)
+      xs[i] = *reinterpret_cast<const F*>(x_base + aslot * kSlot + i * 32 * kRow + cofs);
+#pragma unroll
+    for (int j = 0; j < kTN; ++j)
+      ws[j] = *reinterpret_cast<const F*>(w_base + bslot * kSlot + j * 32 * kRow + cofs);
+  };
+
+  take_a();
+  issue(kDB, kD);
+  take_b();
+  issue(0, kDB);
+  take_a();
+  issue(kDB, kD);
+  slab_wait();
+  quarter(0);
+  frags(0, 0, xf[0], wf[0]);
+  int aslot = 0;
+
+  for (;;) {
+    f32x16 acc[kTN][kTM];
+#pragma unroll
+    for (int j = 0; j < kTN; ++j)
+#pragma unroll
+      for (int i = 0; i < kTM; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[j][i][v] = 0.0f;
+    for (int kt = cur.k0; kt < cur.k1; ++kt) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        if (ks + 1 < 4) {
+          quarter(ks + 1);
+          frags(aslot, ks + 1, xf[(ks + 1) & 1], wf[(ks + 1) & 1]);
+        } else {
+          aslot += 2;
+          if (aslot >= kUnits) aslot -= kUnits;
+          slab_wait();
+          quarter(0);
+          frags(aslot, 0, xf[0], wf[0]);
+        }
+#pragma unroll
+        for (int j = 0; j < kTN; ++j)
+#pragma unroll
+          for (int i = 0; i < kTM; ++i) acc[j][i] = contract(wf[ks & 1][j], xf[ks & 1][i], acc[j][i]);
+        constexpr int kReads = kTM + kTN, kMfma = kTN * kTM * (sizeof(T) == 4 ? 4 : 1);
+        constexpr int kPairs = kReads < kMfma ? kReads : kMfma;
+#pragma unroll
+        for (int q = 0; q < kPairs; ++q) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one MFMA
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // one LDS read
+        }
+        if constexpr (kMfma > kPairs) __builtin_amdgcn_sched_group_barrier(0x008, kMfma - kPairs, 0);
+        if constexpr (kReads > kPairs) __builtin_amdgcn_sched_group_barrier(0x100, kReads - kPairs, 0);
+      }
+    }
+    // (the lane formed again rather than kept live across the loop: the 256 x 256 tiles
+    // run at the register limit)
+    int lane_now;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane_now));
+    const int lr = lane_now & 31, lh = lane_now >> 5;
+    const int row0 = cur.row0 + wm * W::WTM, fw = cur.n0 + wn * W::WTN;
+    if constexpr (EPI == kLse)
+      emit_lse<T, W>(g, acc, row0, fw, lr, lh);
+    else if constexpr (EPI == kDLogit)
+      emit_dlogit<T, W>(g, acc, row0, fw, lr, lh, cur.row0 / BM * W::WM + wm);
+    else if constexpr (EPI == kPart)
+      emit_part<W>(g, acc, cur.part, row0, fw, lr, lh);
+    else
+      emit_store<T, W>(g, acc, row0, fw, lr, lh);
+    t += G;
+    if (!locate_item<BM, BN>(g, t, &cur)) break;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the repeated tail loads
+}
+
+// (max, sum) of two sets of exponentials, as one.
+__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
+  const float n = fmaxf(m, m2);
+  if (n == -INFINITY) return;   // both empty
+  s = s * __builtin_amdgcn_exp2f((m - n) * kLog2e) + s2 * __builtin_amdgcn_exp2f((m2 - n) * kLog2e);
+  m = n;
+}
+
+// 16 tokens a block, 64 threads each.
+__global__ __launch_bounds__(1024) void join_kernel(const float2* __restrict__ part, int P, int ld, int N, int V,
+                                                    const float* __restrict__ picked,
+                                                    const int32_t* __restrict__ targets, float* __restrict__ loss,
+                                                    float* __restrict__ lse) {
+  __shared__ float2 red[64][17];
+  const int tok = threadIdx.x % 16, slice = threadIdx.x / 16, n = blockIdx.x * 16 + tok;
+  float m = -INFINITY, s = 0.0f;
+  bool nan = false;
+  if (n < N) {
+    for (int p = slice; p < P; p += 64) {
+      const float2 v = part[(size_t)p * ld + n];
+      nan |= v.y != v.y;   // (the maximum passes over NaN)
+      merge(m, s, v.x, v.y);
+    }
+    if (nan) s = __uint_as_float(0x7FC00000u);
+  }
+  red[slice][tok] = make_float2(m, s);
+  __syncthreads();
+  for (int d = 32; d >= 1; d >>= 1) {
+    if (slice < d) {
+      const float2 o = red[slice + d][tok];
+      float2 v = red[slice][tok];
+      const bool bad = v.y != v.y || o.y != o.y;
+      merge(v.x, v.y, o.x, o.y);
+      if (bad) v.y = __uint_as_float(0x7FC00000u);
+      red[slice][tok] = v;
+    }
+    __syncthreads();
+  }
+  if (slice != 0 || n >= N) return;
+  const float2 v = red[0][tok];
+  const float l = v.x == -INFINITY && v.y == 0.0f ? -INFINITY : v.x + logf(v.y);
+  const int t = targets[n];
+  lse[n] = l;
+  loss[n] = t >= 0 && t < V ? l - picked[n] : 0.0f;
+}
+
+template <typename S>
+__device__ __forceinline__ S block_sum(S v, S* red) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, kWave);
+  if (lane_id() == 0) red[threadIdx.x / kWave] = v;
+  __syncthreads();
+  S t = 0;
+  for (int i = 0; i < 16; ++i) t += red[i];
+  __syncthreads();
+  return t;
+}
+
+// mean[0]: the mean over the rows with a target, 0 if there is none; mean[1]: their number.
+__global__ __launch_bounds__(1024) void mean_kernel(const float* __restrict__ loss, const int32_t* __restrict__ targets,
+                                                    int N, int V, float* __restrict__ mean) {
+  __shared__ double rs[16];
+  __shared__ int rc[16];
+  double s = 0.0;
+  int c = 0;
+  for (int n = threadIdx.x; n < N; n += 1024) {
+    const int t = targets[n];
+    if (t >= 0 && t < V) {
+      s += (double)loss[n];
+      ++c;
+    }
+  }
+  s = block_sum(s, rs);
+  c = block_sum(c, rc);
+  if (threadIdx.x == 0) {
+    mean[0] = c ? (float)(s / (double)c) : 0.0f;
+    mean[1] = (float)c;
+  }
+}
+
+// scale[n] = dloss[n], or dmean / (rows with a target), and 0 where row n has none.
+__global__ __launch_bounds__(1024) void scale_kernel(const int32_t* __restrict__ targets,
+                                                     const float* __restrict__ dloss, const float* __restrict__ dmean,
+                                                     int N, int V, float* __restrict__ scale) {
+  __shared__ int rc[16];
+  int c = 0;
+  if (!dloss) {
+    for (int n = threadIdx.x; n < N; n += 1024) {
+      const int t = targets[n];
+      c += t >= 0 && t < V;
+    }
+    c = block_sum(c, rc);
+  }
+  const float each = c ? (dmean ? *dmean : 1.0f) / (float)c : 0.0f;
+  const int n = blockIdx.x * 1024 + threadIdx.x;
+  if (n >= N) return;
+  const int t = targets[n];
+  scale[n] = t >= 0 && t < V ? (dloss ? dloss[n] : each) : 0.0f;
+}
+
+// out[m][c] = sum of part[.][m][c], in order; a quad of columns a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ part, int parts, int M, int C, size_t ld,
+                                                     T* __restrict__ out, int vec) {
+  const int quads = (C + 3) / 4;
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (size_t)M * quads) return;
+  const size_t m = i / quads;
+  const int c = (int)(i % quads) * 4;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int p = 0; p < parts; ++p) {
+    const float4 v = *reinterpret_cast<const float4*>(part + ((size_t)p * M + m) * ld + c);
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  T* o = out + m * C + c;
+  if (vec) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(o) = s;
+    else *reinterpret_cast<uint2*>(o) = pack4_bf16(s.x, s.y, s.z, s.w);
+  } else {
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (c + q < C) store_act(o + q, v[q]);
+  }
+}
+
+// db[f] = sum of the rows of colsum, 64 columns a block of 16 waves.
+__global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ src, int rows, size_t ld, int n,
+                                                      float* __restrict__ db) {
+  __shared__ float lds[16][kWave];
+  const int w = threadIdx.x / kWave, lane = lane_id(), f = blockIdx.x * kWave + lane;
+  float s = 0.0f;
+  if (f < n)
+    for (int r = w; r < rows; r += 16) s += src[(size_t)r * ld + f];
+  lds[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && f < n) {
+    float t = 0.0f;
+    for (int i = 0; i < 16; ++i) t += lds[i][lane];
+    db[f] = t;
+  }
+}
+
+int compute_units() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
+    return 256;
+  return n;
+}
+
+size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+int div_up(int a, int b) { return (a + b - 1) / b; }
+
+// Tile size and parts of a product of M rows, Nf columns, KT slabs.
+struct GemmPlan {
+  bool large;
+  int parts;
+};
+GemmPlan plan_gemm(int M, int Nf, int KT, bool split, int cus) {
+  const long tl = (long)div_up(M, 256) * div_up(Nf, 256), ts = (long)div_up(M, 64) * div_up(Nf, 128);
+  GemmPlan p{tl * 2 >= cus, 1};
+  if (split) {
+    const long want = p.large ? cus / tl : 2L * cus / ts;
+    p.parts = (int)std::max(1L, std::min({want, (long)KT / 8, 16L}));
+  }
+  return p;
+}
+
+template <typename T, int EPI>
+hipError_t launch_ring(LossArgs g, const GemmPlan& p, int cus, hipStream_t st) {
+  g.parts = std::min(p.parts, g.KT);   // (every part has a slab; a short last piece adds to fewer)
+  const int bm = p.large ? 256 : 64, bn = p.large ? 256 : 128;
+  g.mt = div_up(g.M, bm);
+  g.nt = div_up(g.Nf, bn);
+  const long items = (long)g.mt * g.nt * g.parts;
+  if (items > 0x3FFFFFFF || g.lda * 256 > 0xFFFFFFFFu || g.ldb * 256 > 0xFFFFFFFFu) return hipErrorInvalidValue;
+  const int grid = (int)std::min<long>((items + kNumXcd - 1) / kNumXcd * kNumXcd, p.large ? cus : 2 * cus);
+  if (p.large)
+    hipLaunchKernelGGL((ring_kernel<T, EPI, 256, 256, 8>), dim3(grid), dim3(512), 0, st, g);
+  else
+    hipLaunchKernelGGL((ring_kernel<T, EPI, 64, 128, 4>), dim3(grid), dim3(256), 0, st, g);
+  return hipGetLastError();
+}
+
+// The type's elements per 128-byte slab.
+template <typename T> constexpr int kSlab = 128 / (int)sizeof(T);
+
+struct LossLayout {
+  // forward
+  int ld_lse;
+  size_t part_lse, picked, xpad, wpad, total;
+  // backward
+  int piece, pieces, vpad, nk;   // columns a piece, pieces, columns of d, of its transpose
+  size_t scale, xt, wt, d, dt, colsum, dxp, dwp;
+  GemmPlan dl, dx, dw;
+  bool dx_part;
+  int ldx;   // columns of the fp32 partial products
+};
+
+constexpr size_t kPieceBytes = (size_t)1 << 30;
+
+template <typename T>
+LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
+  LossLayout l{};
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = off;
+    off = align_up(off + bytes, 256);
+    return o;
+  };
+  const int kp = (int)align_up((size_t)C, kSlab<T>);
+  if (!backward) {
+    l.ld_lse = (int)align_up((size_t)N, 64);
+    l.part_lse = take((size_t)div_up(V, 64) * l.ld_lse * sizeof(float2));
+    l.picked = take((size_t)N * 4);
+    l.xpad = take(pad ? (size_t)N * kp * sizeof(T) : 0);
+    l.wpad = take(pad ? (size_t)V * kp * sizeof(T) : 0);
+    l.total = off;
+    return l;
+  }
+  // d and its transpose within kPieceBytes, pieces of equal size
+  l.nk = (int)align_up((size_t)N, kSlab<T>);
+  const size_t most = std::max<size_t>(256, kPieceBytes / (2 * sizeof(T) * (size_t)l.nk) / 256 * 256);
+  l.pieces = (int)(((size_t)V + most - 1) / most);
+  l.piece = (int)align_up((size_t)div_up(V, l.pieces), 256);
+  l.pieces = div_up(V, l.piece);
+  l.vpad = l.piece;
+  l.ldx = (int)align_up((size_t)C, 256);
+  l.dl = plan_gemm(N, l.piece, kp / kSlab<T>, false, cus);
+  l.dx = plan_gemm(N, C, l.piece / kSlab<T>, true, cus);
+  l.dw = plan_gemm(std::min(V, l.piece), C, l.nk / kSlab<T>, true, cus);
+  l.dx_part = l.pieces > 1 || l.dx.parts > 1;
+  l.scale = take((size_t)N * 4);
+  l.xpad = take(pad ? (size_t)N * kp * sizeof(T) : 0);
+  l.wpad = take(pad ? (size_t)l.piece * kp * sizeof(T) : 0);
+  l.xt = take((size_t)C * l.nk * sizeof(T));
+  l.wt = take((size_t)C * l.vpad * sizeof(T));
+  l.d = take((size_t)N * l.vpad * sizeof(T));
+  l.dt = take((size_t)l.vpad * l.nk * sizeof(T));
+  l.colsum = take((size_t)div_up(N, l.dl.large ? 256 : 64) * 2 * l.vpad * 4);
+  l.dxp = take(l.dx_part ? (size_t)l.dx.parts * N * l.ldx * 4 : 0);
+  l.dwp = take(l.dw.parts > 1 ? (size_t)l.dw.parts * l.piece * l.ldx * 4 : 0);
+  l.total = off;
+  return l;
+}
+
+template <typename T>
+bool needs_pad(int C, const void* x, const void* W) {
+  return C % kSlab<T> != 0 || (((uintptr_t)x | (uintptr_t)W) & 15) != 0;
+}
+
+template <typename T>
+hipError_t forward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W, const float* bias,
+                        const int32_t* targets, int N, float* loss, float* lse, float* mean, char* ws, bool pad,
+                        const LossLayout& l, int cus, hipStream_t st) {
+  const int C = cfg->embed_dim, V = cfg->vocab_size, kp = (int)align_up((size_t)C, kSlab<T>);
+  hipError_t e;
+  if (pad) {
+    if ((e = launch_copy_cols<T>(x, C, (T*)(ws + l.xpad), kp, N, C, kp, st)) != hipSuccess) return e;
+    if ((e = launch_copy_cols<T>(W, C, (T*)(ws + l.wpad), kp, V, C, kp, st)) != hipSuccess) return e;
+    x = (const T*)(ws + l.xpad);
+    W = (const T*)(ws + l.wpad);
+  }
+  LossArgs g{};
+  g.A = (const char*)x;
+  g.B = (const char*)W;
+  g.lda = g.ldb = (size_t)kp * sizeof(T);
+  g.M = N;
+  g.Nf = V;
+  g.KT = kp / kSlab<T>;
+  g.bias = bias;
+  g.targets = targets;
+  g.part_lse = (float2*)(ws + l.part_lse);
+  g.ld_lse = l.ld_lse;
+  g.picked = (float*)(ws + l.picked);
+  if ((e = launch_ring<T, kLse>(g, plan_gemm(N, V, g.KT, false, cus), cus, st)) != hipSuccess) return e;
+  hipLaunchKernelGGL(join_kernel, dim3(div_up(N, 16)), dim3(1024), 0, st, g.part_lse, div_up(V, 64), l.ld_lse, N, V,
+                     g.picked, targets, loss, lse);
+  if (mean) hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(1024), 0, st, loss, targets, N, V, mean);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t reduce_parts(const float* part, int parts, int M, int C, int ld, T* out, hipStream_t st) {
+  const size_t n = (size_t)M * ((C + 3) / 4);
+  const int vec = C % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0;
+  if ((n + 255) / 256 > 0xFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(reduce_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, parts, M, C,
+                     (size_t)ld, out, vec);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W, const float* bias,
+                         const int32_t* targets, const float* lse, const float* dloss, const float* dmean, int N,
+                         T* dx, T* dW, float* db, char* ws, bool pad, const LossLayout& l, int cus,
+                         hipStream_t st) {
+  const int C = cfg->embed_dim, V = cfg->vocab_size, kp = (int)align_up((size_t)C, kSlab<T>);
+  hipError_t e;
+  float* scale = (float*)(ws + l.scale);
+  hipLaunchKernelGGL(scale_kernel, dim3(div_up(N, 1024)), dim3(1024), 0, st, targets, dloss, dmean, N, V, scale);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  const T* xk = x;
+  if (pad) {
+    if ((e = launch_copy_cols<T>(x, C, (T*)(ws + l.xpad), kp, N, C, kp, st)) != hipSuccess) return e;
+    xk = (const T*)(ws + l.xpad);
+  }
+  T *xt = (T*)(ws + l.xt), *wt = (T*)(ws + l.wt);
+  if (dW && (e = launch_transpose_pad<T>(x, N, C, 0, xt, C, l.nk, 0, 1, st)) != hipSuccess) return e;
+  for (int i = 0; i < l.pieces; ++i) {
+    const int v0 = i * l.piece, vn = std::min(l.piece, V - v0);
+    const T* wp = W + (size_t)v0 * C;
+    const T* wk = wp;
+    if (pad) {
+      if ((e = launch_copy_cols<T>(wp, C, (T*)(ws + l.wpad), kp, vn, C, kp, st)) != hipSuccess) return e;
+      wk = (const T*)(ws + l.wpad);
+    }
+    LossArgs g{};
+    g.A = (const char*)xk;
+    g.B = (const char*)wk;
+    g.lda = g.ldb = (size_t)kp * sizeof(T);
+    g.M = N;
+    g.Nf = vn;
+    g.KT = kp / kSlab<T>;
+    g.bias = bias ? bias + v0 : nullptr;
+    g.targets = targets;
+    g.target0 = v0;
+    g.lse = lse;
+    g.scale = scale;
+    g.d = ws + l.d;
+    g.ldd = l.vpad;
+    g.dt = ws + l.dt;
+    g.lddt = l.nk;
+    g.rows_t = l.nk;
+    g.colsum = db ? (float*)(ws + l.colsum) : nullptr;
+    if ((e = launch_ring<T, kDLogit>(g, l.dl, cus, st)) != hipSuccess) return e;
+    if (db) {
+      hipLaunchKernelGGL(colsum_kernel, dim3(div_up(vn, kWave)), dim3(1024), 0, st, g.colsum,
+                         div_up(N, l.dl.large ? 256 : 64) * 2, g.ldd, vn, db + v0);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if (dx) {
+      if ((e = launch_transpose_pad<T>(wp, vn, C, 0, wt, C, l.vpad, 0, 1, st)) != hipSuccess) return e;
+      LossArgs p{};
+      p.A = ws + l.d;
+      p.lda = (size_t)l.vpad * sizeof(T);
+      p.B = (const char*)wt;
+      p.ldb = (size_t)l.vpad * sizeof(T);
+      p.M = N;
+      p.Nf = C;
+      p.KT = div_up(vn, kSlab<T>);
+      p.out = l.dx_part ? ws + l.dxp : (char*)dx;
+      p.ldo = l.dx_part ? l.ldx : C;
+      p.add = i > 0;
+      p.vec = C % 8 == 0 && ((uintptr_t)dx & 15) == 0;
+      GemmPlan plan = l.dx;
+      if (l.dx_part)
+        e = launch_ring<T, kPart>(p, plan, cus, st);
+      else
+        e = launch_ring<T, kStore>(p, plan, cus, st);
+      if (e != hipSuccess) return e;
+    }
+    if (dW) {
+      LossArgs p{};
+      p.A = ws + l.dt;
+      p.lda = (size_t)l.nk * sizeof(T);
+      p.B = (const char*)xt;
+      p.ldb = (size_t)l.nk * sizeof(T);
+      p.M = vn;
+      p.Nf = C;
+      p.KT = l.nk / kSlab<T>;
+      T* out = dW + (size_t)v0 * C;
+      p.out = l.dw.parts > 1 ? ws + l.dwp : (char*)out;
+      p.ldo = l.dw.parts > 1 ? l.ldx : C;
+      p.vec = C % 8 == 0 && ((uintptr_t)out & 15) == 0;
+      if (l.dw.parts > 1) {
+        if ((e = launch_ring<T, kPart>(p, l.dw, cus, st)) != hipSuccess) return e;
+        e = reduce_parts<T>((const float*)(ws + l.dwp), l.dw.parts, vn, C, l.ldx, out, st);
+      } else {
+        e = launch_ring<T, kStore>(p, l.dw, cus, st);
+      }
+      if (e != hipSuccess) return e;
+    }
+  }
+  if (dx && l.dx_part) return reduce_parts<T>((const float*)(ws + l.dxp), l.dx.parts, N, C, l.ldx, dx, st);
+  return hipSuccess;
+}
+
+int check_loss(const mgpt_lm_loss_config* cfg, int N) {
+  if (!cfg) return fail(MGPT_ERR_INVALID_ARGUMENT, "config is null");
+  if (N < 0) return fail(MGPT_ERR_INVALID_ARGUMENT, "negative num_tokens");
+  if (cfg->embed_dim <= 0 || cfg->vocab_size <= 0)
+    return fail(MGPT_ERR_INVALID_ARGUMENT, "embed_dim %d, vocab_size %d", cfg->embed_dim, cfg->vocab_size);
+  if (cfg->dtype != MGPT_DTYPE_F32 && cfg->dtype != MGPT_DTYPE_BF16)
+    return fail(MGPT_ERR_UNSUPPORTED, "unsupported dtype %d", cfg->dtype);
+  // (row offsets within a tile are 32 bits, tile numbers too)
+  if (cfg->embed_dim > 1 << 20 || cfg->vocab_size > 1 << 24 || N > 1 << 21)
+    return fail(MGPT_ERR_UNSUPPORTED, "embed_dim %d > 2^20, vocab_size %d > 2^24 or num_tokens %d > 2^21",
+                cfg->embed_dim, cfg->vocab_size, N);
+  return MGPT_OK;
+}
+
+LossLayout layout_of(const mgpt_lm_loss_config* cfg, int N, bool backward, bool pad, int cus) {
+  return cfg->dtype == MGPT_DTYPE_F32
+             ? loss_layout<float>(N, cfg->embed_dim, cfg->vocab_size, backward, pad, cus)
+             : loss_layout<bf16_t>(N, cfg->embed_dim, cfg->vocab_size, backward, pad, cus);
+}
+
+int workspace(const mgpt_lm_loss_config* cfg, int N, bool backward, size_t* bytes) {
+  if (!bytes) return fail(MGPT_ERR_INVALID_ARGUMENT, "null bytes");
+  if (int rc = check_loss(cfg, N)) return rc;
+  // as if x or W were not 16-byte aligned, which no caller's size tells
+  *bytes = N == 0 ? 0 : layout_of(cfg, N, backward, true, compute_units()).total;
+  return MGPT_OK;
+}
+
+int check_workspace(const void* ws, size_t have, size_t need) {
+  if (!ws) return fail(MGPT_ERR_INVALID_ARGUMENT, "null workspace");
+  if ((uintptr_t)ws & 255) return fail(MGPT_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+  if (have < need) return fail(MGPT_ERR_WORKSPACE_TOO_SMALL, "workspace needs %zu bytes, got %zu", need, have);
+  return MGPT_OK;
+}
+
+}  // namespace
+}  // namespace mgpt
+
+using namespace mgpt;
+
+extern "C" {
+
+int mgpt_lm_loss_workspace_bytes(const mgpt_lm_loss_config* cfg, int num_tokens, size_t* bytes) {
+  return workspace(cfg, num_tokens, false, bytes);
+}
+
+int mgpt_lm_loss_backward_workspace_bytes(const mgpt_lm_loss_config* cfg, int num_tokens, size_t* bytes) {
+  return workspace(cfg, num_tokens, true, bytes);
+}
+
+int mgpt_lm_loss_forward(const mgpt_lm_loss_config* cfg, const void* x, const void* W, const float* bias,
+                         const int32_t* targets, float* loss, float* lse, float* mean, int num_tokens,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_loss(cfg, num_tokens)) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (num_tokens == 0) {
+    if (mean) HIP_TRY(launch_fill_zero(mean, 2, st));
+    return MGPT_OK;
+  }
+  if (!x || !W || !targets || !loss || !lse)
+    return fail(MGPT_ERR_INVALID_ARGUMENT, "null x, W, targets, loss or lse");
+  const int cus = compute_units();
+  const bool f32 = cfg->dtype == MGPT_DTYPE_F32;
+  const bool pad = f32 ? needs_pad<float>(cfg->embed_dim, x, W) : needs_pad<bf16_t>(cfg->embed_dim, x, W);
+  const LossLayout l = layout_of(cfg, num_tokens, false, pad, cus);
+  if (int rc = check_workspace(workspace, workspace_bytes, l.total)) return rc;
+  HIP_TRY(f32 ? forward_impl<float>(cfg, (const float*)x, (const float*)W, bias, targets, num_tokens, loss, lse,
+                                    mean, (char*)workspace, pad, l, cus, st)
+              : forward_impl<bf16_t>(cfg, (const bf16_t*)x, (const bf16_t*)W, bias, targets, num_tokens, loss, lse,
+                                     mean, (char*)workspace, pad, l, cus, st));
+  return MGPT_OK;
+}
+
+int mgpt_lm_loss_backward(const mgpt_lm_loss_config* cfg, const void* x, const void* W, const float* bias,
+                          const int32_t* targets, const float* lse, const float* dloss, const float* dmean,
+                          void* dx, void* dW, float* dbias, int num_tokens, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  if (int rc = check_loss(cfg, num_tokens)) return rc;
+  if (dloss && dmean) return fail(MGPT_ERR_INVALID_ARGUMENT, "dloss and dmean exclude each other");
+  hipStream_t st = (hipStream_t)stream;
+  const bool f32 = cfg->dtype == MGPT_DTYPE_F32;
+  const size_t C = cfg->embed_dim, V = cfg->vocab_size;
+  if (num_tokens == 0) {   // no token adds to the weights' gradients
+    if (dW && !f32 && ((uintptr_t)dW & 3)) return fail(MGPT_ERR_INVALID_ARGUMENT, "dW is not 4-byte aligned");
+    if (dW) HIP_TRY(launch_fill_zero((float*)dW, f32 ? V * C : V * C / 2, st));
+    if (dW && !f32 && (V * C) % 2)
+      HIP_TRY(launch_copy_cols<bf16_t>((const bf16_t*)dW, 0, (bf16_t*)dW + V * C - 1, 1, 1, 0, 1, st));
+    if (dbias) HIP_TRY(launch_fill_zero(dbias, V, st));
+    return MGPT_OK;
+  }
+  if (!x || !W || !targets || !lse) return fail(MGPT_ERR_INVALID_ARGUMENT, "null x, W, targets or lse");
+  if (!dx && !dW && !dbias) return MGPT_OK;
+  const int cus = compute_units();
+  const bool pad = f32 ? needs_pad<float>(cfg->embed_dim, x, W) : needs_pad<bf16_t>(cfg->embed_dim, x, W);
+  const LossLayout l = layout_of(cfg, num_tokens, true, pad, cus);
+  if (int rc = check_workspace(workspace, workspace_bytes, l.total)) return rc;
+  HIP_TRY(f32 ? backward_impl<float>(cfg, (const float*)x, (const float*)W, bias, targets, lse, dloss, dmean,
+                                     num_tokens, (float*)dx, (float*)dW, dbias, (char*)workspace, pad, l, cus, st)
+              : backward_impl<bf16_t>(cfg, (const bf16_t*)x, (const bf16_t*)W, bias, targets, lse, dloss, dmean,
+                                      num_tokens, (bf16_t*)dx, (bf16_t*)dW, dbias, (char*)workspace, pad, l, cus,
+                                      st));
+  return MGPT_OK;
+}
+
+}  // extern "C"
