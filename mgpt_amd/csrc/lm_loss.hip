@@ -77,6 +77,7 @@ struct LossArgs {
   char* out;
   size_t ldo;
   int add, vec;
+  const float* factor;   // kStore: of the product
 };
 
 template <typename T> struct Frag;
@@ -141,31 +142,65 @@ __device__ __forceinline__ uint2 transpose4(uint2 u, int lane) {
   return upper ? make_uint2(r, a1) : make_uint2(a0, r);
 }
 
-// Biases of a 32-column group's registers (column 8g + 4h + q, register 4g + q), -inf for
-// the columns past the last.
-__device__ __forceinline__ void load_bias(const LossArgs& g, int f0, int lhalf, float (&b)[16]) {
-  const bool whole = f0 + 32 <= g.Nf;
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int f = f0 + 8 * k + 4 * lhalf + q;
-      float v = 0.0f;
-      if (g.bias) v = g.bias[whole ? f : min(f, g.Nf - 1)];
-      if (!whole && f >= g.Nf) v = -INFINITY;
-      b[4 * k + q] = v;
-    }
-}
-
 template <typename W>
 using Acc = f32x16[W::TN][W::TM];
+
+// The accumulators of a wave's columns fw .. start from their biases (column 8k + 4h + q
+// of a group of 32 in register 4k + q) or, past the last column, from -inf: no
+// probability, no gradient.  Whole groups are read by scalar loads; a vector load would
+// wait for the ring's, which the compiler does not track.
+template <typename W>
+__device__ __forceinline__ void start_from_bias(const LossArgs& g, Acc<W>& acc, int fw, int lhalf) {
+#pragma unroll
+  for (int j = 0; j < W::TN; ++j) {
+    const int f0 = fw + 32 * j;
+    f32x16 b;
+    if (f0 + 32 <= g.Nf) {
+      if (g.bias) {
+        typedef const __attribute__((address_space(4))) float* cptr;
+        const cptr u = (cptr)(uintptr_t)(g.bias + f0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float lo = u[8 * k + q], hi = u[8 * k + 4 + q];
+            b[4 * k + q] = lhalf ? hi : lo;
+          }
+      } else {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) b[v] = 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int f = f0 + 8 * (v / 4) + 4 * lhalf + v % 4;
+        b[v] = g.bias ? g.bias[min(f, g.Nf - 1)] : 0.0f;
+        if (f >= g.Nf) b[v] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < W::TM; ++i) acc[j][i] = b;
+    __builtin_amdgcn_sched_barrier(0);   // one group at a time (scalar registers)
+  }
+}
+
+// exp(z - s) of a register: one fma into the hardware's exponential; `huge` (a lane's s
+// near the type's lowest or largest value, which times log2 e overflows): difference first.
+__device__ __forceinline__ float exp_less(float z, float s, float ns, bool huge) {
+  return __builtin_amdgcn_exp2f(huge ? (z - s) * kLog2e : __builtin_fmaf(z, kLog2e, ns));
+}
+constexpr float kHuge = 1e38f;
+
+// a * b, 0 where either is 0, whatever the other.
+__device__ __forceinline__ float mul_zero(float a, float b) {
+  float r;
+  asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
 
 template <typename T, typename W>
 __device__ __forceinline__ void emit_lse(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow, int lhalf) {
   if (fw >= g.Nf) return;
-  float b[W::TN][16];
-#pragma unroll
-  for (int j = 0; j < W::TN; ++j) load_bias(g, fw + 32 * j, lhalf, b[j]);
 #pragma unroll
   for (int i = 0; i < W::TM; ++i) {
     const int row = row0 + 32 * i + lrow;
@@ -175,18 +210,21 @@ __device__ __forceinline__ void emit_lse(const LossArgs& g, Acc<W>& acc, int row
 #pragma unroll
     for (int j = 0; j < W::TN; ++j)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        acc[j][i][v] += b[j][v];
-        m = fmaxf(m, acc[j][i][v]);
-      }
+      for (int v = 0; v < 16; v += 2) m = fmaxf(fmaxf(acc[j][i][v], acc[j][i][v + 1]), m);
     m = other_half_max(m);
-    // (differences before they are scaled: logits of the type's lowest value stay finite)
-    const float top = m == -INFINITY ? 0.0f : m;
+    const float top = m == -INFINITY ? 0.0f : m, ntop = -top * kLog2e;
     float s = 0.0f;
+    if (__ballot(!(fabsf(top) < kHuge))) {
 #pragma unroll
-    for (int j = 0; j < W::TN; ++j)
+      for (int j = 0; j < W::TN; ++j)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) s += __builtin_amdgcn_exp2f((acc[j][i][v] - top) * kLog2e);
+        for (int v = 0; v < 16; ++v) s += exp_less(acc[j][i][v], top, ntop, true);
+    } else {
+#pragma unroll
+      for (int j = 0; j < W::TN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s += exp_less(acc[j][i][v], top, ntop, false);
+    }
     s = other_half_sum(s);
     if (live && lhalf == 0) g.part_lse[(size_t)(fw / 64) * g.ld_lse + row] = make_float2(m, s);
     const int fl = t >= fw && t < min(fw + 64, g.Nf) ? t - fw : -1;
@@ -208,34 +246,49 @@ template <typename T, typename W>
 __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow, int lhalf,
                                             int sum_row) {
   float lse[W::TM], sc[W::TM];
-  int tg[W::TM];
+  int tl[W::TM];   // the target's column in the wave's 64
+  bool huge = false;
 #pragma unroll
   for (int i = 0; i < W::TM; ++i) {
     const int row = row0 + 32 * i + lrow, r = min(row, g.M - 1);
-    lse[i] = g.lse[r];
     sc[i] = row < g.M ? g.scale[r] : 0.0f;
-    tg[i] = g.targets[r] - g.target0;
+    lse[i] = sc[i] == 0.0f ? 0.0f : g.lse[r];
+    tl[i] = g.targets[r] - g.target0 - fw;
+    huge |= !(fabsf(lse[i]) < kHuge);
   }
+  const bool slow = __ballot(huge) != 0;
   T* dm = reinterpret_cast<T*>(g.d);
   T* dt = reinterpret_cast<T*>(g.dt);
 #pragma unroll
   for (int j = 0; j < W::TN; ++j) {
     const int f0 = fw + 32 * j;
-    float b[16], cs[16];
-    load_bias(g, f0, lhalf, b);
+    float cs[16];
 #pragma unroll
     for (int v = 0; v < 16; ++v) cs[v] = 0.0f;
 #pragma unroll
     for (int i = 0; i < W::TM; ++i) {
       const int row = row0 + 32 * i + lrow;
+      const float nl = -lse[i] * kLog2e;
       float d[16];
+      if (slow) {
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int f = f0 + 8 * (v / 4) + 4 * lhalf + v % 4;
-        const float p = __builtin_amdgcn_exp2f((acc[j][i][v] + b[v] - lse[i]) * kLog2e);
-        d[v] = (f == tg[i] ? p - 1.0f : p) * sc[i];
-        d[v] = sc[i] == 0.0f ? 0.0f : d[v];
-        cs[v] += d[v];
+        for (int v = 0; v < 16; ++v) d[v] = exp_less(acc[j][i][v], lse[i], nl, true);
+      } else {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) d[v] = exp_less(acc[j][i][v], lse[i], nl, false);
+      }
+      if (__ballot(tl[i] >= 32 * j && tl[i] < 32 * j + 32)) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (tl[i] == 32 * j + 8 * (v / 4) + 4 * lhalf + v % 4) d[v] -= 1.0f;
+      }
+      // (0 times anything is 0 here: a row without a target has no gradient even where its
+      // logits are not finite)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) d[v] = mul_zero(d[v], sc[i]);
+      if (g.colsum) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) cs[v] += d[v];
       }
       if constexpr (sizeof(T) == 2) {
         uint2 q[4];
@@ -311,6 +364,7 @@ __device__ __forceinline__ void emit_part(const LossArgs& g, Acc<W>& acc, int pa
 template <typename T, typename W>
 __device__ __forceinline__ void emit_store(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow, int lhalf) {
   T* out = reinterpret_cast<T*>(g.out);
+  const float factor = uniform_load(g.factor);
 #pragma unroll
   for (int j = 0; j < W::TN; ++j) {
     const int f0 = fw + 32 * j;
@@ -320,6 +374,8 @@ __device__ __forceinline__ void emit_store(const LossArgs& g, Acc<W>& acc, int r
     for (int i = 0; i < W::TM; ++i) {
       const int row = row0 + 32 * i + lrow;
       T* o = out + (size_t)row * g.ldo + f0;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[j][i][v] *= factor;
       if (vec) {
         if constexpr (sizeof(T) == 2) {
           uint2 q[4];
@@ -503,12 +559,16 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
 
   for (;;) {
     f32x16 acc[kTN][kTM];
+    if constexpr (EPI == kLse || EPI == kDLogit) {
+      start_from_bias<W>(g, acc, cur.n0 + wn * W::WTN, lhalf);
+    } else {
 #pragma unroll
-    for (int j = 0; j < kTN; ++j)
+      for (int j = 0; j < kTN; ++j)
 #pragma unroll
-      for (int i = 0; i < kTM; ++i)
+        for (int i = 0; i < kTM; ++i)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) acc[j][i][v] = 0.0f;
+          for (int v = 0; v < 16; ++v) acc[j][i][v] = 0.0f;
+    }
     for (int kt = cur.k0; kt < cur.k1; ++kt) {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
@@ -637,30 +697,49 @@ __global__ __launch_bounds__(1024) void mean_kernel(const float* __restrict__ lo
   }
 }
 
-// scale[n] = dloss[n], or dmean / (rows with a target), and 0 where row n has none.
+// The rows' upstream gradients as scale[n] times *factor: the largest magnitude (1 for
+// each row of a mean), so that d = (p - onehot) scale rounds to bf16 as p - onehot does;
+// one common odd factor within d would round all its targets' entries the same way, an
+// error that adds up over the rows.  0 where row n has no target.
 __global__ __launch_bounds__(1024) void scale_kernel(const int32_t* __restrict__ targets,
                                                      const float* __restrict__ dloss, const float* __restrict__ dmean,
-                                                     int N, int V, float* __restrict__ scale) {
+                                                     int N, int V, float* __restrict__ scale,
+                                                     float* __restrict__ factor) {
   __shared__ int rc[16];
+  __shared__ float rm[16];
   int c = 0;
-  if (!dloss) {
-    for (int n = threadIdx.x; n < N; n += 1024) {
-      const int t = targets[n];
-      c += t >= 0 && t < V;
+  float m = 0.0f;
+  for (int n = threadIdx.x; n < N; n += 1024) {
+    const int t = targets[n];
+    if (t >= 0 && t < V) {
+      ++c;
+      if (dloss) m = fmaxf(m, fabsf(dloss[n]));
     }
-    c = block_sum(c, rc);
   }
-  const float each = c ? (dmean ? *dmean : 1.0f) / (float)c : 0.0f;
+  float f;
+  if (dloss) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
+    if (lane_id() == 0) rm[threadIdx.x / kWave] = m;
+    __syncthreads();
+    f = 0.0f;
+    for (int i = 0; i < 16; ++i) f = fmaxf(f, rm[i]);
+    if (!(f > 1e-30f && f < 1e30f)) f = 1.0f;
+  } else {
+    c = block_sum(c, rc);
+    f = c ? (dmean ? *dmean : 1.0f) / (float)c : 0.0f;
+  }
   const int n = blockIdx.x * 1024 + threadIdx.x;
+  if (n == 0) *factor = f;
   if (n >= N) return;
   const int t = targets[n];
-  scale[n] = t >= 0 && t < V ? (dloss ? dloss[n] : each) : 0.0f;
+  scale[n] = t >= 0 && t < V ? (dloss ? dloss[n] / f : 1.0f) : 0.0f;
 }
 
-// out[m][c] = sum of part[.][m][c], in order; a quad of columns a thread.
+// out[m][c] = *factor times the sum of part[.][m][c], in order; a quad of columns a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ part, int parts, int M, int C, size_t ld,
-                                                     T* __restrict__ out, int vec) {
+                                                     const float* __restrict__ factor, T* __restrict__ out, int vec) {
   const int quads = (C + 3) / 4;
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (size_t)M * quads) return;
@@ -671,6 +750,8 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
     const float4 v = *reinterpret_cast<const float4*>(part + ((size_t)p * M + m) * ld + c);
     s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   }
+  const float f = *factor;
+  s.x *= f; s.y *= f; s.z *= f; s.w *= f;
   T* o = out + m * C + c;
   if (vec) {
     if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(o) = s;
@@ -683,9 +764,9 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
   }
 }
 
-// db[f] = sum of the rows of colsum, 64 columns a block of 16 waves.
+// db[f] = *factor times the sum of the rows of colsum, 64 columns a block of 16 waves.
 __global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ src, int rows, size_t ld, int n,
-                                                      float* __restrict__ db) {
+                                                      const float* __restrict__ factor, float* __restrict__ db) {
   __shared__ float lds[16][kWave];
   const int w = threadIdx.x / kWave, lane = lane_id(), f = blockIdx.x * kWave + lane;
   float s = 0.0f;
@@ -696,7 +777,7 @@ __global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ 
   if (w == 0 && f < n) {
     float t = 0.0f;
     for (int i = 0; i < 16; ++i) t += lds[i][lane];
-    db[f] = t;
+    db[f] = t * *factor;
   }
 }
 
@@ -751,7 +832,7 @@ struct LossLayout {
   size_t part_lse, picked, xpad, wpad, total;
   // backward
   int piece, pieces, vpad, nk;   // columns a piece, pieces, columns of d, of its transpose
-  size_t scale, xt, wt, d, dt, colsum, dxp, dwp;
+  size_t scale, factor, xt, wt, d, dt, colsum, dxp, dwp;
   GemmPlan dl, dx, dw;
   bool dx_part;
   int ldx;   // columns of the fp32 partial products
@@ -791,6 +872,7 @@ LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
   l.dw = plan_gemm(std::min(V, l.piece), C, l.nk / kSlab<T>, true, cus);
   l.dx_part = l.pieces > 1 || l.dx.parts > 1;
   l.scale = take((size_t)N * 4);
+  l.factor = take(4);
   l.xpad = take(pad ? (size_t)N * kp * sizeof(T) : 0);
   l.wpad = take(pad ? (size_t)l.piece * kp * sizeof(T) : 0);
   l.xt = take((size_t)C * l.nk * sizeof(T));
@@ -841,12 +923,13 @@ hipError_t forward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W, 
 }
 
 template <typename T>
-hipError_t reduce_parts(const float* part, int parts, int M, int C, int ld, T* out, hipStream_t st) {
+hipError_t reduce_parts(const float* part, int parts, int M, int C, int ld, const float* factor, T* out,
+                        hipStream_t st) {
   const size_t n = (size_t)M * ((C + 3) / 4);
   const int vec = C % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0;
   if ((n + 255) / 256 > 0xFFFFFF) return hipErrorInvalidValue;
   hipLaunchKernelGGL(reduce_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, parts, M, C,
-                     (size_t)ld, out, vec);
+                     (size_t)ld, factor, out, vec);
   return hipGetLastError();
 }
 
@@ -857,8 +940,9 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
                          hipStream_t st) {
   const int C = cfg->embed_dim, V = cfg->vocab_size, kp = (int)align_up((size_t)C, kSlab<T>);
   hipError_t e;
-  float* scale = (float*)(ws + l.scale);
-  hipLaunchKernelGGL(scale_kernel, dim3(div_up(N, 1024)), dim3(1024), 0, st, targets, dloss, dmean, N, V, scale);
+  float *scale = (float*)(ws + l.scale), *factor = (float*)(ws + l.factor);
+  hipLaunchKernelGGL(scale_kernel, dim3(div_up(N, 1024)), dim3(1024), 0, st, targets, dloss, dmean, N, V, scale,
+                     factor);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const T* xk = x;
   if (pad) {
@@ -896,7 +980,7 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
     if ((e = launch_ring<T, kDLogit>(g, l.dl, cus, st)) != hipSuccess) return e;
     if (db) {
       hipLaunchKernelGGL(colsum_kernel, dim3(div_up(vn, kWave)), dim3(1024), 0, st, g.colsum,
-                         div_up(N, l.dl.large ? 256 : 64) * 2, g.ldd, vn, db + v0);
+                         div_up(N, l.dl.large ? 256 : 64) * 2, g.ldd, vn, factor, db + v0);
       if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (dx) {
@@ -907,6 +991,7 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
       p.B = (const char*)wt;
       p.ldb = (size_t)l.vpad * sizeof(T);
       p.M = N;
+      p.factor = factor;
       p.Nf = C;
       p.KT = div_up(vn, kSlab<T>);
       p.out = l.dx_part ? ws + l.dxp : (char*)dx;
@@ -927,6 +1012,7 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
       p.B = (const char*)xt;
       p.ldb = (size_t)l.nk * sizeof(T);
       p.M = vn;
+      p.factor = factor;
       p.Nf = C;
       p.KT = l.nk / kSlab<T>;
       T* out = dW + (size_t)v0 * C;
@@ -935,14 +1021,14 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
       p.vec = C % 8 == 0 && ((uintptr_t)out & 15) == 0;
       if (l.dw.parts > 1) {
         if ((e = launch_ring<T, kPart>(p, l.dw, cus, st)) != hipSuccess) return e;
-        e = reduce_parts<T>((const float*)(ws + l.dwp), l.dw.parts, vn, C, l.ldx, out, st);
+        e = reduce_parts<T>((const float*)(ws + l.dwp), l.dw.parts, vn, C, l.ldx, factor, out, st);
       } else {
         e = launch_ring<T, kStore>(p, l.dw, cus, st);
       }
       if (e != hipSuccess) return e;
     }
   }
-  if (dx && l.dx_part) return reduce_parts<T>((const float*)(ws + l.dxp), l.dx.parts, N, C, l.ldx, dx, st);
+  if (dx && l.dx_part) return reduce_parts<T>((const float*)(ws + l.dxp), l.dx.parts, N, C, l.ldx, factor, dx, st);
   return hipSuccess;
 }
 
