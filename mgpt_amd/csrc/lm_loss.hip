@@ -80,18 +80,44 @@ struct LossArgs {
   const float* factor;   // kStore: of the product
 };
 
-template <typename T> struct Frag;
-template <> struct Frag<bf16_t> { typedef bf16x8 type; };
-template <> struct Frag<float> { typedef f32x4 type; };
-
+// fp32 operands as three bf16 numbers each, x = h + m + l exactly (8 of its 24 bits each,
+// rounded to nearest): six of the nine products keep all but 2^-24 of the whole, at 16
+// contracted columns an instruction of v_mfma_f32_32x32x16_bf16 for two of
+// v_mfma_f32_32x32x2_f32, of the same length.  (An infinity, or a magnitude above bf16's
+// largest, splits into NaN.)
+struct Split {
+  bf16x8 h, m, l;
+};
+__device__ __forceinline__ Split split(f32x4 a, f32x4 b) {
+  uint32_t w[3][4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float x = q < 2 ? a[2 * q] : b[2 * q - 4], y = q < 2 ? a[2 * q + 1] : b[2 * q - 3];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      w[p][q] = pack_bf16x2(x, y);
+      if (p < 2) {
+        x -= __uint_as_float(w[p][q] << 16);
+        y -= __uint_as_float(w[p][q] & 0xFFFF0000u);
+      }
+    }
+  }
+  Split s;
+  __builtin_memcpy(&s.h, w[0], 16);
+  __builtin_memcpy(&s.m, w[1], 16);
+  __builtin_memcpy(&s.l, w[2], 16);
+  return s;
+}
 __device__ __forceinline__ f32x16 contract(bf16x8 w, bf16x8 x, f32x16 acc) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, x, acc, 0, 0, 0);
 }
-// (k-step x pairs element x of the lane halves' vectors in both operands)
-__device__ __forceinline__ f32x16 contract(f32x4 w, f32x4 x, f32x16 acc) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(w[q], x[q], acc, 0, 0, 0);
-  return acc;
+__device__ __forceinline__ f32x16 contract(const Split& w, const Split& x, f32x16 acc) {
+  acc = contract(w.l, x.h, acc);   // the smallest first
+  acc = contract(w.m, x.m, acc);
+  acc = contract(w.h, x.l, acc);
+  acc = contract(w.m, x.h, acc);
+  acc = contract(w.h, x.m, acc);
+  return contract(w.h, x.h, acc);
 }
 
 // A 1 KB direct-to-LDS load (see dma16) from a uniform base and a lane's offset.
@@ -140,6 +166,14 @@ __device__ __forceinline__ uint2 transpose4(uint2 u, int lane) {
   const uint32_t a1 = __builtin_amdgcn_perm(odd ? u.y : p1, odd ? p1 : u.y, sel);
   const uint32_t r = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(upper ? a0 : a1), 0x4E, 0xf, 0xf, false);   // lane ^ 2
   return upper ? make_uint2(r, a1) : make_uint2(a0, r);
+}
+
+// The transpose's stores, past the caches: with d's own left in them, what both write a tile
+// (256 KB) drains sooner (16384 x 1024 x 16128: 695 us, so 637, d's too 685).
+__device__ __forceinline__ void store_through(bf16_t* p, uint2 v) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  const u32x2 u = {v.x, v.y};
+  __builtin_nontemporal_store(u, reinterpret_cast<u32x2*>(p));
 }
 
 template <typename W>
@@ -299,7 +333,7 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
         for (int k = 0; k < 4; ++k) {
           const uint2 u = transpose4(q[k], lrow);
           const int f = f0 + 8 * k + 4 * lhalf + (lrow & 3), r4 = row & ~3;
-          if (r4 < g.rows_t) *reinterpret_cast<uint2*>(dt + (size_t)f * g.lddt + r4) = u;
+          if (r4 < g.rows_t) store_through(dt + (size_t)f * g.lddt + r4, u);
         }
       } else {
 #pragma unroll
@@ -429,7 +463,6 @@ __device__ __forceinline__ bool locate_item(const LossArgs& g, int v, Item* it) 
 template <typename T, int EPI, int BM, int BN, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
   using W = Waves<NW, BM, BN>;
-  typedef typename Frag<T>::type F;
   constexpr int kTN = W::TN, kTM = W::TM, kUnits = 5, kRow = 128;
   constexpr int kSlot = (BM > BN ? BM : BN) * kRow;
   constexpr int kDA = BM * kRow / 1024 / NW, kDB = BN * kRow / 1024 / NW;   // loads per wave and unit
@@ -534,16 +567,24 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
   const int swz = (lrow >> 1) & 7;
   const char* x_base = smem + (wm * W::WTM + lrow) * kRow;
   const char* w_base = smem + (wn * W::WTN + lrow) * kRow;
-  F xf[2][kTM], wf[2][kTN];
-  auto frags = [&](int aslot, int ks, F (&xs)[kTM], F (&ws)[kTN]) __attribute__((always_inline)) {
+  // bf16: the fragments of a k-step (16 columns), a 16-byte vector a lane; fp32: of two (8
+  // vectors of 4 columns in the slab), which together contract 16 columns.
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr int kSteps = kF32 ? 2 : 4, kVec = kF32 ? 2 : 1;
+  typedef std::conditional_t<kF32, f32x4, bf16x8> F;
+  F xf[2][kTM][kVec], wf[2][kTN][kVec];
+  auto frags = [&](int aslot, int step, F (&xs)[kTM][kVec], F (&ws)[kTN][kVec]) __attribute__((always_inline)) {
     const int bslot = aslot + 1 == kUnits ? 0 : aslot + 1;
-    const int cofs = (((ks * 2 + lhalf) ^ swz) << 4);
 #pragma unroll
-    for (int i = 0; i < kTM; ++i)
-      xs[i] = *reinterpret_cast<const F*>(x_base + aslot * kSlot + i * 32 * kRow + cofs);
+    for (int c = 0; c < kVec; ++c) {
+      const int cofs = ((((step * kVec + c) * 2 + lhalf) ^ swz) << 4);
 #pragma unroll
-    for (int j = 0; j < kTN; ++j)
-      ws[j] = *reinterpret_cast<const F*>(w_base + bslot * kSlot + j * 32 * kRow + cofs);
+      for (int i = 0; i < kTM; ++i)
+        xs[i][c] = *reinterpret_cast<const F*>(x_base + aslot * kSlot + i * 32 * kRow + cofs);
+#pragma unroll
+      for (int j = 0; j < kTN; ++j)
+        ws[j][c] = *reinterpret_cast<const F*>(w_base + bslot * kSlot + j * 32 * kRow + cofs);
+    }
   };
 
   take_a();
@@ -571,9 +612,10 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
     }
     for (int kt = cur.k0; kt < cur.k1; ++kt) {
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        if (ks + 1 < 4) {
-          quarter(ks + 1);
+      for (int ks = 0; ks < kSteps; ++ks) {
+        if (ks + 1 < kSteps) {
+#pragma unroll
+          for (int q = ks * 3 / (kSteps - 1); q < (ks + 1) * 3 / (kSteps - 1); ++q) quarter(q + 1);
           frags(aslot, ks + 1, xf[(ks + 1) & 1], wf[(ks + 1) & 1]);
         } else {
           aslot += 2;
@@ -582,19 +624,33 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
           quarter(0);
           frags(aslot, 0, xf[0], wf[0]);
         }
+        auto& xs = xf[ks & 1];
+        auto& ws = wf[ks & 1];
+        if constexpr (kF32) {
+          Split sw[kTN];
 #pragma unroll
-        for (int j = 0; j < kTN; ++j)
+          for (int j = 0; j < kTN; ++j) sw[j] = split(ws[j][0], ws[j][1]);
 #pragma unroll
-          for (int i = 0; i < kTM; ++i) acc[j][i] = contract(wf[ks & 1][j], xf[ks & 1][i], acc[j][i]);
-        constexpr int kReads = kTM + kTN, kMfma = kTN * kTM * (sizeof(T) == 4 ? 4 : 1);
-        constexpr int kPairs = kReads < kMfma ? kReads : kMfma;
+          for (int i = 0; i < kTM; ++i) {
+            const Split sx = split(xs[i][0], xs[i][1]);
 #pragma unroll
-        for (int q = 0; q < kPairs; ++q) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one MFMA
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // one LDS read
+            for (int j = 0; j < kTN; ++j) acc[j][i] = contract(sw[j], sx, acc[j][i]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kTN; ++j)
+#pragma unroll
+            for (int i = 0; i < kTM; ++i) acc[j][i] = contract(ws[j][0], xs[i][0], acc[j][i]);
+          constexpr int kReads = kTM + kTN, kMfma = kTN * kTM;
+          constexpr int kPairs = kReads < kMfma ? kReads : kMfma;
+#pragma unroll
+          for (int q = 0; q < kPairs; ++q) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one MFMA
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // one LDS read
+          }
+          if constexpr (kMfma > kPairs) __builtin_amdgcn_sched_group_barrier(0x008, kMfma - kPairs, 0);
+          if constexpr (kReads > kPairs) __builtin_amdgcn_sched_group_barrier(0x100, kReads - kPairs, 0);
         }
-        if constexpr (kMfma > kPairs) __builtin_amdgcn_sched_group_barrier(0x008, kMfma - kPairs, 0);
-        if constexpr (kReads > kPairs) __builtin_amdgcn_sched_group_barrier(0x100, kReads - kPairs, 0);
       }
     }
     // (the lane formed again rather than kept live across the loop: the 256 x 256 tiles
@@ -793,15 +849,23 @@ size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 int div_up(int a, int b) { return (a + b - 1) / b; }
 
 // Tile size and parts of a product of M rows, Nf columns, KT slabs.
+enum TileSize { kSmall, kMid, kLarge };   // 64 x 128, 128 x 128 (two blocks a CU), 256 x 256
+int tile_rows(TileSize t) { return t == kLarge ? 256 : t == kMid ? 128 : 64; }
+int tile_cols(TileSize t) { return t == kLarge ? 256 : 128; }
 struct GemmPlan {
-  bool large;
+  TileSize tile;
   int parts;
 };
+template <typename T>
 GemmPlan plan_gemm(int M, int Nf, int KT, bool split, int cus) {
-  const long tl = (long)div_up(M, 256) * div_up(Nf, 256), ts = (long)div_up(M, 64) * div_up(Nf, 128);
-  GemmPlan p{tl * 2 >= cus, 1};
+  auto tiles = [&](TileSize t) { return (long)div_up(M, tile_rows(t)) * div_up(Nf, tile_cols(t)); };
+  GemmPlan p{kSmall, 1};
+  if (sizeof(T) == 2 && tiles(kLarge) * 2 >= cus)
+    p.tile = kLarge;
+  else if (tiles(kMid) >= cus)
+    p.tile = kMid;
   if (split) {
-    const long want = p.large ? cus / tl : 2L * cus / ts;
+    const long want = (p.tile == kLarge ? cus : 2L * cus) / tiles(p.tile);
     p.parts = (int)std::max(1L, std::min({want, (long)KT / 8, 16L}));
   }
   return p;
@@ -810,16 +874,25 @@ GemmPlan plan_gemm(int M, int Nf, int KT, bool split, int cus) {
 template <typename T, int EPI>
 hipError_t launch_ring(LossArgs g, const GemmPlan& p, int cus, hipStream_t st) {
   g.parts = std::min(p.parts, g.KT);   // (every part has a slab; a short last piece adds to fewer)
-  const int bm = p.large ? 256 : 64, bn = p.large ? 256 : 128;
-  g.mt = div_up(g.M, bm);
-  g.nt = div_up(g.Nf, bn);
+  g.mt = div_up(g.M, tile_rows(p.tile));
+  g.nt = div_up(g.Nf, tile_cols(p.tile));
   const long items = (long)g.mt * g.nt * g.parts;
   if (items > 0x3FFFFFFF || g.lda * 256 > 0xFFFFFFFFu || g.ldb * 256 > 0xFFFFFFFFu) return hipErrorInvalidValue;
-  const int grid = (int)std::min<long>((items + kNumXcd - 1) / kNumXcd * kNumXcd, p.large ? cus : 2 * cus);
-  if (p.large)
-    hipLaunchKernelGGL((ring_kernel<T, EPI, 256, 256, 8>), dim3(grid), dim3(512), 0, st, g);
-  else
-    hipLaunchKernelGGL((ring_kernel<T, EPI, 64, 128, 4>), dim3(grid), dim3(256), 0, st, g);
+  const int grid =
+      (int)std::min<long>((items + kNumXcd - 1) / kNumXcd * kNumXcd, p.tile == kLarge ? cus : 2 * cus);
+  auto go = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, g);
+  };
+  if (p.tile == kSmall) {
+    go(ring_kernel<T, EPI, 64, 128, 4>, 256);
+  } else if (p.tile == kMid) {
+    go(ring_kernel<T, EPI, 128, 128, 4>, 256);
+  } else {
+    if constexpr (sizeof(T) == 2)
+      go(ring_kernel<T, EPI, 256, 256, 8>, 512);
+    else
+      return hipErrorInvalidValue;   // (the split operands leave no registers for these)
+  }
   return hipGetLastError();
 }
 
@@ -867,9 +940,9 @@ LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
   l.pieces = div_up(V, l.piece);
   l.vpad = l.piece;
   l.ldx = (int)align_up((size_t)C, 256);
-  l.dl = plan_gemm(N, l.piece, kp / kSlab<T>, false, cus);
-  l.dx = plan_gemm(N, C, l.piece / kSlab<T>, true, cus);
-  l.dw = plan_gemm(std::min(V, l.piece), C, l.nk / kSlab<T>, true, cus);
+  l.dl = plan_gemm<T>(N, l.piece, kp / kSlab<T>, false, cus);
+  l.dx = plan_gemm<T>(N, C, l.piece / kSlab<T>, true, cus);
+  l.dw = plan_gemm<T>(std::min(V, l.piece), C, l.nk / kSlab<T>, true, cus);
   l.dx_part = l.pieces > 1 || l.dx.parts > 1;
   l.scale = take((size_t)N * 4);
   l.factor = take(4);
@@ -879,7 +952,7 @@ LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
   l.wt = take((size_t)C * l.vpad * sizeof(T));
   l.d = take((size_t)N * l.vpad * sizeof(T));
   l.dt = take((size_t)l.vpad * l.nk * sizeof(T));
-  l.colsum = take((size_t)div_up(N, l.dl.large ? 256 : 64) * 2 * l.vpad * 4);
+  l.colsum = take((size_t)div_up(N, tile_rows(l.dl.tile)) * 2 * l.vpad * 4);
   l.dxp = take(l.dx_part ? (size_t)l.dx.parts * N * l.ldx * 4 : 0);
   l.dwp = take(l.dw.parts > 1 ? (size_t)l.dw.parts * l.piece * l.ldx * 4 : 0);
   l.total = off;
@@ -915,7 +988,7 @@ hipError_t forward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W, 
   g.part_lse = (float2*)(ws + l.part_lse);
   g.ld_lse = l.ld_lse;
   g.picked = (float*)(ws + l.picked);
-  if ((e = launch_ring<T, kLse>(g, plan_gemm(N, V, g.KT, false, cus), cus, st)) != hipSuccess) return e;
+  if ((e = launch_ring<T, kLse>(g, plan_gemm<T>(N, V, g.KT, false, cus), cus, st)) != hipSuccess) return e;
   hipLaunchKernelGGL(join_kernel, dim3(div_up(N, 16)), dim3(1024), 0, st, g.part_lse, div_up(V, 64), l.ld_lse, N, V,
                      g.picked, targets, loss, lse);
   if (mean) hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(1024), 0, st, loss, targets, N, V, mean);
@@ -980,7 +1053,7 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
     if ((e = launch_ring<T, kDLogit>(g, l.dl, cus, st)) != hipSuccess) return e;
     if (db) {
       hipLaunchKernelGGL(colsum_kernel, dim3(div_up(vn, kWave)), dim3(1024), 0, st, g.colsum,
-                         div_up(N, l.dl.large ? 256 : 64) * 2, g.ldd, vn, factor, db + v0);
+                         div_up(N, tile_rows(l.dl.tile)) * 2, g.ldd, vn, factor, db + v0);
       if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (dx) {
