@@ -40,9 +40,6 @@ namespace mgpt {
 
 template <typename T>
 hipError_t launch_copy_cols(const T*, int, T*, int, int, int, int, hipStream_t);   // pack.hip
-template <typename T>
-hipError_t launch_transpose_pad(const T*, int, int, size_t, T*, int, int, size_t, int,
-                                hipStream_t);                                     // backward.hip
 hipError_t launch_fill_zero(float* p, size_t n, hipStream_t stream);              // backward.hip
 
 namespace {
@@ -68,6 +65,7 @@ struct LossArgs {
   float2* part_lse;      // [Nf / 64][ld_lse]
   int ld_lse;
   float* picked;         // [M]
+  int* counter;          // set to 0 for join_kernel's blocks
   const float *lse, *scale;
   char *d, *dt;          // [M][ldd], [.][lddt] in T
   size_t ldd, lddt;      // elements
@@ -478,6 +476,7 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
   if (!locate_item<BM, BN>(g, t, &cur)) return;
 
   const int tid = threadIdx.x;
+  if (EPI == kLse && blockIdx.x == 0 && tid == 0) *g.counter = 0;
   const int w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = lane_id();
   const int wn = w % W::WN, wm = w / W::WN;
   const int lrow = lane & 31, lhalf = lane >> 5;
@@ -681,20 +680,50 @@ __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
   m = n;
 }
 
-// 16 tokens a block, 64 threads each.
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
+  return v;
+}
+template <typename S>
+__device__ __forceinline__ S wave_total(S v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, kWave);
+  return v;
+}
+
+constexpr int kJoinTokens = 16;
+struct JoinSum {
+  double loss;
+  int count, pad;
+};
+
+// 16 tokens a block, 64 threads each.  mean[0]: the mean over the rows with a target, 0 if
+// there is none; mean[1]: their number; the last block to end adds the blocks' sums up,
+// in their order.
 __global__ __launch_bounds__(1024) void join_kernel(const float2* __restrict__ part, int P, int ld, int N, int V,
                                                     const float* __restrict__ picked,
                                                     const int32_t* __restrict__ targets, float* __restrict__ loss,
-                                                    float* __restrict__ lse) {
-  __shared__ float2 red[64][17];
-  const int tok = threadIdx.x % 16, slice = threadIdx.x / 16, n = blockIdx.x * 16 + tok;
+                                                    float* __restrict__ lse, float* __restrict__ mean,
+                                                    JoinSum* __restrict__ sums, int* counter) {
+  __shared__ float2 red[64][kJoinTokens + 1];
+  __shared__ JoinSum total[16];
+  __shared__ bool last;
+  const int tok = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens, n = blockIdx.x * kJoinTokens + tok;
   float m = -INFINITY, s = 0.0f;
   bool nan = false;
   if (n < N) {
-    for (int p = slice; p < P; p += 64) {
-      const float2 v = part[(size_t)p * ld + n];
-      nan |= v.y != v.y;   // (the maximum passes over NaN)
-      merge(m, s, v.x, v.y);
+    constexpr int kAhead = 4;   // loads in flight
+    for (int p0 = slice; p0 < P; p0 += 64 * kAhead) {
+      float2 v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        v[u] = p0 + 64 * u < P ? part[(size_t)(p0 + 64 * u) * ld + n] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        nan |= v[u].y != v[u].y;   // (the maximum passes over NaN)
+        merge(m, s, v[u].x, v[u].y);
+      }
     }
     if (nan) s = __uint_as_float(0x7FC00000u);
   }
@@ -711,85 +740,144 @@ __global__ __launch_bounds__(1024) void join_kernel(const float2* __restrict__ p
     }
     __syncthreads();
   }
-  if (slice != 0 || n >= N) return;
-  const float2 v = red[0][tok];
-  const float l = v.x == -INFINITY && v.y == 0.0f ? -INFINITY : v.x + logf(v.y);
-  const int t = targets[n];
-  lse[n] = l;
-  loss[n] = t >= 0 && t < V ? l - picked[n] : 0.0f;
-}
-
-template <typename S>
-__device__ __forceinline__ S block_sum(S v, S* red) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, kWave);
-  if (lane_id() == 0) red[threadIdx.x / kWave] = v;
-  __syncthreads();
-  S t = 0;
-  for (int i = 0; i < 16; ++i) t += red[i];
-  __syncthreads();
-  return t;
-}
-
-// mean[0]: the mean over the rows with a target, 0 if there is none; mean[1]: their number.
-__global__ __launch_bounds__(1024) void mean_kernel(const float* __restrict__ loss, const int32_t* __restrict__ targets,
-                                                    int N, int V, float* __restrict__ mean) {
-  __shared__ double rs[16];
-  __shared__ int rc[16];
-  double s = 0.0;
-  int c = 0;
-  for (int n = threadIdx.x; n < N; n += 1024) {
-    const int t = targets[n];
-    if (t >= 0 && t < V) {
-      s += (double)loss[n];
-      ++c;
+  if (threadIdx.x < kWave) {   // (the first 16 lanes have a token)
+    float l = 0.0f;
+    bool has = false;
+    if (slice == 0 && n < N) {
+      const float2 v = red[0][tok];
+      const float z = v.x == -INFINITY && v.y == 0.0f ? -INFINITY : v.x + logf(v.y);
+      const int t = targets[n];
+      has = t >= 0 && t < V;
+      l = has ? z - picked[n] : 0.0f;
+      lse[n] = z;
+      loss[n] = l;
+    }
+    if (mean) {
+      const double sum = wave_total((double)l);
+      const int count = wave_total(has ? 1 : 0);
+      if (threadIdx.x == 0) {
+        sums[blockIdx.x] = {sum, count, 0};
+        __threadfence();
+        last = atomicAdd(counter, 1) == (int)gridDim.x - 1;
+      }
     }
   }
-  s = block_sum(s, rs);
-  c = block_sum(c, rc);
+  if (!mean) return;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  JoinSum a = {0.0, 0, 0};
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += 1024) {
+    a.loss += sums[b].loss;
+    a.count += sums[b].count;
+  }
+  a.loss = wave_total(a.loss);
+  a.count = wave_total(a.count);
+  if (lane_id() == 0) total[threadIdx.x / kWave] = a;
+  __syncthreads();
   if (threadIdx.x == 0) {
-    mean[0] = c ? (float)(s / (double)c) : 0.0f;
-    mean[1] = (float)c;
+    for (int i = 1; i < 16; ++i) {
+      a.loss += total[i].loss;
+      a.count += total[i].count;
+    }
+    mean[0] = a.count ? (float)(a.loss / (double)a.count) : 0.0f;
+    mean[1] = (float)a.count;
   }
 }
 
-// The rows' upstream gradients as scale[n] times *factor: the largest magnitude (1 for
-// each row of a mean), so that d = (p - onehot) scale rounds to bf16 as p - onehot does;
-// one common odd factor within d would round all its targets' entries the same way, an
-// error that adds up over the rows.  0 where row n has no target.
-__global__ __launch_bounds__(1024) void scale_kernel(const int32_t* __restrict__ targets,
-                                                     const float* __restrict__ dloss, const float* __restrict__ dmean,
-                                                     int N, int V, float* __restrict__ scale,
-                                                     float* __restrict__ factor) {
-  __shared__ int rc[16];
-  __shared__ float rm[16];
-  int c = 0;
-  float m = 0.0f;
-  for (int n = threadIdx.x; n < N; n += 1024) {
-    const int t = targets[n];
-    if (t >= 0 && t < V) {
-      ++c;
-      if (dloss) m = fmaxf(m, fabsf(dloss[n]));
+// What a backward's products read, by ranges of blocks of 256 threads: the rows' upstream
+// gradients, and transposes of x and of the first piece of W (for a later piece that
+// alone), zeros past their rows, through 64 x 64 tiles.
+//
+// The upstream gradients as scale[n] times *factor, the largest magnitude (1 for each row
+// of a mean): so d = (p - onehot) scale rounds to bf16 as p - onehot does; one common odd
+// factor within d would round all its targets' entries the same way, an error that adds
+// up over the rows.  scale is 0 where row n has no target.
+template <typename T>
+struct PrepareArgs {
+  int scale_blocks, rows_per_block;
+  const int32_t* targets;
+  const float *dloss, *dmean;
+  int N, V;
+  float *scale, *factor;
+  struct {
+    const T* src;   // [rows][cols]
+    T* dst;         // [cols][ld]
+    int rows, cols, ld, blocks, vec;
+  } t[2];
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs<T> a) {
+  constexpr int kV = 16 / (int)sizeof(T);   // elements a vector
+  __shared__ __attribute__((aligned(16))) T tile[64][64 + kV];
+  __shared__ float rm[4];
+  __shared__ int rc[4];
+  int b = blockIdx.x;
+  if (b < a.scale_blocks) {
+    int c = 0;
+    float m = 0.0f;
+    for (int n = threadIdx.x; n < a.N; n += 256) {
+      const int t = a.targets[n];
+      if (t >= 0 && t < a.V) {
+        ++c;
+        if (a.dloss) m = fmaxf(m, fabsf(a.dloss[n]));
+      }
+    }
+    c = wave_total(c);
+    m = wave_max(m);
+    if (lane_id() == 0) {
+      rc[threadIdx.x / kWave] = c;
+      rm[threadIdx.x / kWave] = m;
+    }
+    __syncthreads();
+    c = rc[0] + rc[1] + rc[2] + rc[3];
+    m = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
+    float f;
+    if (a.dloss)
+      f = m > 1e-30f && m < 1e30f ? m : 1.0f;
+    else
+      f = c ? (a.dmean ? *a.dmean : 1.0f) / (float)c : 0.0f;
+    if (b == 0 && threadIdx.x == 0) *a.factor = f;
+    const int n1 = min(a.N, (b + 1) * a.rows_per_block);
+    for (int n = b * a.rows_per_block + threadIdx.x; n < n1; n += 256) {
+      const int t = a.targets[n];
+      a.scale[n] = t >= 0 && t < a.V ? (a.dloss ? a.dloss[n] / f : 1.0f) : 0.0f;
+    }
+    return;
+  }
+  b -= a.scale_blocks;
+  const int k = b < a.t[0].blocks ? 0 : 1;
+  if (k) b -= a.t[0].blocks;
+  const auto& t = a.t[k];
+  const int nx = (t.cols + 63) / 64;   // tiles across; columns fastest: whole rows of the source
+  const int c0 = b % nx * 64, r0 = b / nx * 64;
+  // rows r0 .. of src into the tile
+  for (int i = threadIdx.x; i < 64 * 64 / kV; i += 256) {
+    const int r = i / (64 / kV), c = i % (64 / kV) * kV;
+    const bool in = r0 + r < t.rows;
+    const T* p = t.src + (size_t)(r0 + r) * t.cols + c0 + c;
+    if (t.vec) {   // (cols % kV == 0: a vector is within the row or past it)
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (in && c0 + c < t.cols) v = *reinterpret_cast<const uint4*>(p);
+      *reinterpret_cast<uint4*>(&tile[r][c]) = v;
+    } else {
+#pragma unroll
+      for (int q = 0; q < kV; ++q) tile[r][c + q] = in && c0 + c + q < t.cols ? p[q] : T(0);
     }
   }
-  float f;
-  if (dloss) {
+  __syncthreads();
+  // (ld is a multiple of 64: every tile's columns of dst exist)
+  for (int i = threadIdx.x; i < 64 * 64 / kV; i += 256) {
+    const int c = i / (64 / kV), r = i % (64 / kV) * kV;
+    if (c0 + c >= t.cols) continue;
+    T v[kV];
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, kWave));
-    if (lane_id() == 0) rm[threadIdx.x / kWave] = m;
-    __syncthreads();
-    f = 0.0f;
-    for (int i = 0; i < 16; ++i) f = fmaxf(f, rm[i]);
-    if (!(f > 1e-30f && f < 1e30f)) f = 1.0f;
-  } else {
-    c = block_sum(c, rc);
-    f = c ? (dmean ? *dmean : 1.0f) / (float)c : 0.0f;
+    for (int q = 0; q < kV; ++q) v[q] = tile[r + q][c];
+    uint4 u;
+    __builtin_memcpy(&u, v, 16);
+    *reinterpret_cast<uint4*>(t.dst + (size_t)(c0 + c) * t.ld + r0 + r) = u;
   }
-  const int n = blockIdx.x * 1024 + threadIdx.x;
-  if (n == 0) *factor = f;
-  if (n >= N) return;
-  const int t = targets[n];
-  scale[n] = t >= 0 && t < V ? (dloss ? dloss[n] / f : 1.0f) : 0.0f;
 }
 
 // out[m][c] = *factor times the sum of part[.][m][c], in order; a quad of columns a thread.
@@ -848,7 +936,13 @@ int compute_units() {
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 int div_up(int a, int b) { return (a + b - 1) / b; }
 
-// Tile size and parts of a product of M rows, Nf columns, KT slabs.
+// Tile size and parts of a product of M rows, Nf columns, KT slabs: the least of the
+// estimated times over the sizes and, where the contraction may be split, 1 .. 16 parts of
+// at least 8 slabs.  A CU takes ceil(items / CUs) items one after the other (the
+// smaller tiles two at a time, at the same rate); a part costs its fp32 sums' way to memory and
+// back and a launch.  Rates: the large tile's, 1250 TFLOP/s in bf16 and 180 in fp32 over
+// 256 CUs, times what the smaller ones reach of it (16384 x 1024 x 16128, bf16, dW: 411 /
+// 524 / 769 us; 4096 x 512 x 8000, fp32, forward: 185 / 220 / 294).
 enum TileSize { kSmall, kMid, kLarge };   // 64 x 128, 128 x 128 (two blocks a CU), 256 x 256
 int tile_rows(TileSize t) { return t == kLarge ? 256 : t == kMid ? 128 : 64; }
 int tile_cols(TileSize t) { return t == kLarge ? 256 : 128; }
@@ -857,18 +951,27 @@ struct GemmPlan {
   int parts;
 };
 template <typename T>
-GemmPlan plan_gemm(int M, int Nf, int KT, bool split, int cus) {
-  auto tiles = [&](TileSize t) { return (long)div_up(M, tile_rows(t)) * div_up(Nf, tile_cols(t)); };
-  GemmPlan p{kSmall, 1};
-  if (sizeof(T) == 2 && tiles(kLarge) * 2 >= cus)
-    p.tile = kLarge;
-  else if (tiles(kMid) >= cus)
-    p.tile = kMid;
-  if (split) {
-    const long want = (p.tile == kLarge ? cus : 2L * cus) / tiles(p.tile);
-    p.parts = (int)std::max(1L, std::min({want, (long)KT / 8, 16L}));
+GemmPlan plan_gemm(int M, int Nf, int KT, bool split, TileSize most, int cus) {
+  const double rate = (sizeof(T) == 2 ? 1250e6 : 180e6) / 256;   // operations a us and CU
+  GemmPlan best{kSmall, 1};
+  double least = 1e300;
+  for (int t = kSmall; t <= most; ++t) {
+    const TileSize tile = (TileSize)t;
+    const double reach = tile == kLarge ? 1.0 : tile == kMid ? 0.82 : 0.6;
+    const long tiles = (long)div_up(M, tile_rows(tile)) * div_up(Nf, tile_cols(tile));
+    const double one = 2.0 * tile_rows(tile) * tile_cols(tile) * KT * (128 / sizeof(T)) / (rate * reach);
+    for (int p = 1; p <= (split ? std::max(1, std::min(16, KT / 8)) : 1); ++p) {
+      const long rounds = (tiles * p + cus - 1) / cus;
+      double us = (double)rounds * one / p;
+      if (rounds == 1 && tile != kLarge) us *= 1.35;   // a block alone does not cover its waits
+      if (p > 1) us += p * (double)M * Nf * 8 / 5e6 + 4;
+      if (us < least) {
+        least = us;
+        best = {tile, p};
+      }
+    }
   }
-  return p;
+  return best;
 }
 
 template <typename T, int EPI>
@@ -888,10 +991,10 @@ hipError_t launch_ring(LossArgs g, const GemmPlan& p, int cus, hipStream_t st) {
   } else if (p.tile == kMid) {
     go(ring_kernel<T, EPI, 128, 128, 4>, 256);
   } else {
-    if constexpr (sizeof(T) == 2)
+    if constexpr (!(sizeof(T) == 4 && EPI == kDLogit))
       go(ring_kernel<T, EPI, 256, 256, 8>, 512);
     else
-      return hipErrorInvalidValue;   // (the split operands leave no registers for these)
+      return hipErrorInvalidValue;   // (its epilogue beside the split operands spills registers)
   }
   return hipGetLastError();
 }
@@ -902,7 +1005,7 @@ template <typename T> constexpr int kSlab = 128 / (int)sizeof(T);
 struct LossLayout {
   // forward
   int ld_lse;
-  size_t part_lse, picked, xpad, wpad, total;
+  size_t part_lse, picked, sums, counter, xpad, wpad, total;
   // backward
   int piece, pieces, vpad, nk;   // columns a piece, pieces, columns of d, of its transpose
   size_t scale, factor, xt, wt, d, dt, colsum, dxp, dwp;
@@ -927,22 +1030,24 @@ LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
     l.ld_lse = (int)align_up((size_t)N, 64);
     l.part_lse = take((size_t)div_up(V, 64) * l.ld_lse * sizeof(float2));
     l.picked = take((size_t)N * 4);
+    l.sums = take((size_t)div_up(N, kJoinTokens) * sizeof(JoinSum));
+    l.counter = take(4);
     l.xpad = take(pad ? (size_t)N * kp * sizeof(T) : 0);
     l.wpad = take(pad ? (size_t)V * kp * sizeof(T) : 0);
     l.total = off;
     return l;
   }
   // d and its transpose within kPieceBytes, pieces of equal size
-  l.nk = (int)align_up((size_t)N, kSlab<T>);
+  l.nk = (int)align_up((size_t)N, 64);
   const size_t most = std::max<size_t>(256, kPieceBytes / (2 * sizeof(T) * (size_t)l.nk) / 256 * 256);
   l.pieces = (int)(((size_t)V + most - 1) / most);
   l.piece = (int)align_up((size_t)div_up(V, l.pieces), 256);
   l.pieces = div_up(V, l.piece);
   l.vpad = l.piece;
   l.ldx = (int)align_up((size_t)C, 256);
-  l.dl = plan_gemm<T>(N, l.piece, kp / kSlab<T>, false, cus);
-  l.dx = plan_gemm<T>(N, C, l.piece / kSlab<T>, true, cus);
-  l.dw = plan_gemm<T>(std::min(V, l.piece), C, l.nk / kSlab<T>, true, cus);
+  l.dl = plan_gemm<T>(N, l.piece, kp / kSlab<T>, false, sizeof(T) == 4 ? kMid : kLarge, cus);
+  l.dx = plan_gemm<T>(N, C, l.piece / kSlab<T>, true, kLarge, cus);
+  l.dw = plan_gemm<T>(std::min(V, l.piece), C, l.nk / kSlab<T>, true, kLarge, cus);
   l.dx_part = l.pieces > 1 || l.dx.parts > 1;
   l.scale = take((size_t)N * 4);
   l.factor = take(4);
@@ -988,10 +1093,10 @@ hipError_t forward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W, 
   g.part_lse = (float2*)(ws + l.part_lse);
   g.ld_lse = l.ld_lse;
   g.picked = (float*)(ws + l.picked);
-  if ((e = launch_ring<T, kLse>(g, plan_gemm<T>(N, V, g.KT, false, cus), cus, st)) != hipSuccess) return e;
-  hipLaunchKernelGGL(join_kernel, dim3(div_up(N, 16)), dim3(1024), 0, st, g.part_lse, div_up(V, 64), l.ld_lse, N, V,
-                     g.picked, targets, loss, lse);
-  if (mean) hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(1024), 0, st, loss, targets, N, V, mean);
+  g.counter = (int*)(ws + l.counter);
+  if ((e = launch_ring<T, kLse>(g, plan_gemm<T>(N, V, g.KT, false, kLarge, cus), cus, st)) != hipSuccess) return e;
+  hipLaunchKernelGGL(join_kernel, dim3(div_up(N, kJoinTokens)), dim3(1024), 0, st, g.part_lse, div_up(V, 64),
+                     l.ld_lse, N, V, g.picked, targets, loss, lse, mean, (JoinSum*)(ws + l.sums), g.counter);
   return hipGetLastError();
 }
 
@@ -1014,18 +1119,40 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
   const int C = cfg->embed_dim, V = cfg->vocab_size, kp = (int)align_up((size_t)C, kSlab<T>);
   hipError_t e;
   float *scale = (float*)(ws + l.scale), *factor = (float*)(ws + l.factor);
-  hipLaunchKernelGGL(scale_kernel, dim3(div_up(N, 1024)), dim3(1024), 0, st, targets, dloss, dmean, N, V, scale,
-                     factor);
-  if ((e = hipGetLastError()) != hipSuccess) return e;
   const T* xk = x;
   if (pad) {
     if ((e = launch_copy_cols<T>(x, C, (T*)(ws + l.xpad), kp, N, C, kp, st)) != hipSuccess) return e;
     xk = (const T*)(ws + l.xpad);
   }
   T *xt = (T*)(ws + l.xt), *wt = (T*)(ws + l.wt);
-  if (dW && (e = launch_transpose_pad<T>(x, N, C, 0, xt, C, l.nk, 0, 1, st)) != hipSuccess) return e;
+  auto prepare = [&](int piece) -> hipError_t {
+    PrepareArgs<T> a{};
+    auto transpose = [&](int k, const T* src, int rows, T* dst, int ld) {
+      a.t[k] = {src, dst, rows, C, ld, div_up(C, 64) * (ld / 64), C % (16 / (int)sizeof(T)) == 0 && ((uintptr_t)src & 15) == 0};
+    };
+    if (piece == 0) {
+      a.rows_per_block = std::max(256, div_up(N, 64));
+      a.scale_blocks = div_up(N, a.rows_per_block);
+      a.targets = targets;
+      a.dloss = dloss;
+      a.dmean = dmean;
+      a.N = N;
+      a.V = V;
+      a.scale = scale;
+      a.factor = factor;
+      if (dW) transpose(0, x, N, xt, l.nk);
+    }
+    const int v0 = piece * l.piece;
+    if (dx) transpose(1, W + (size_t)v0 * C, std::min(l.piece, V - v0), wt, l.vpad);
+    const long blocks = (long)a.scale_blocks + a.t[0].blocks + a.t[1].blocks;
+    if (blocks == 0) return hipSuccess;
+    if (blocks > 0xFFFFFF) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(prepare_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+    return hipGetLastError();
+  };
   for (int i = 0; i < l.pieces; ++i) {
     const int v0 = i * l.piece, vn = std::min(l.piece, V - v0);
+    if ((e = prepare(i)) != hipSuccess) return e;
     const T* wp = W + (size_t)v0 * C;
     const T* wk = wp;
     if (pad) {
@@ -1057,7 +1184,6 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
       if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (dx) {
-      if ((e = launch_transpose_pad<T>(wp, vn, C, 0, wt, C, l.vpad, 0, 1, st)) != hipSuccess) return e;
       LossArgs p{};
       p.A = ws + l.d;
       p.lda = (size_t)l.vpad * sizeof(T);

@@ -9,12 +9,16 @@ tensors a MoELayer loads, with the gradients of MoELayer.get_gradients().
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
 from . import capi
 
 _GRAD = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16}
+_dtype = operator.attrgetter("dtype")
+_numel, _is_contiguous = torch.Tensor.numel, torch.Tensor.is_contiguous
+_get_device, _data_ptr = torch.Tensor.get_device, torch.Tensor.data_ptr
 
 
 class AdamW:
@@ -41,7 +45,8 @@ class AdamW:
                 self._check(self.copies[i], torch.bfloat16, p.numel(), f"copies[{i}]")
         self.step_count = 0
         n = len(self.params)
-        self._sizes = (ctypes.c_int64 * n)(*[p.numel() for p in self.params])
+        self._numels = [p.numel() for p in self.params]
+        self._sizes = (ctypes.c_int64 * n)(*self._numels)
         need = ctypes.c_size_t()
         capi.check(capi.lib().mgpt_adamw_state_bytes(n, self._sizes, state_bits, ctypes.byref(need)))
         self.state = torch.zeros(need.value, dtype=torch.uint8, device=self.device)
@@ -71,25 +76,31 @@ class AdamW:
         n = len(self.params)
         if len(grads) != n:
             raise ValueError(f"expected {n} gradients, got {len(grads)}")
-        dtype = next((g.dtype for g in grads if g is not None), torch.float32)
-        if dtype not in _GRAD:
-            raise TypeError("gradients must be float32 or bfloat16")
-        gp = (ctypes.c_void_p * n)()
-        pp = (ctypes.c_void_p * n)()
-        for i, (p, g) in enumerate(zip(self.params, grads)):
-            pp[i] = p.data_ptr()
-            if g is not None:
-                self._check(g, dtype, self._sizes[i], f"grads[{i}]")
-                gp[i] = g.data_ptr()
-        cp = None
+        # (attribute by attribute over all tensors: a model has hundreds, and their
+        # checks one by one would take longer than the step)
+        some = [g for g in grads if g is not None]
+        dtypes = set(map(_dtype, some)) or {torch.float32}
+        if len(dtypes) != 1 or not dtypes <= _GRAD.keys():
+            raise TypeError("gradients must be all float32 or all bfloat16")
+        sizes = self._numels if len(some) == n else [k for k, g in zip(self._numels, grads) if g is not None]
+        if list(map(_numel, some)) != sizes or not all(map(_is_contiguous, some)):
+            raise ValueError("gradients must be contiguous and have their parameters' sizes")
+        if not set(map(_get_device, some)) <= {self.device.index}:
+            raise ValueError(f"gradients must be CUDA tensors on {self.device}")
+        ptrs = list(map(_data_ptr, some))
+        if len(some) != n:
+            at = iter(ptrs)
+            ptrs = [None if g is None else next(at) for g in grads]
+        array = ctypes.c_void_p * n
+        copies = None
         if self.copies is not None:
-            cp = (ctypes.c_void_p * n)(*[None if c is None else c.data_ptr() for c in self.copies])
+            copies = array(*[None if c is None else c.data_ptr() for c in self.copies])
         scale = None
         if grad_scale is not None:
             self._check(grad_scale, torch.float32, 1, "grad_scale")
             scale = grad_scale.data_ptr()
         cfg = capi.AdamWConfig(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
-                               self.state_bits, _GRAD[dtype])
+                               self.state_bits, _GRAD[dtypes.pop()])
         with torch.cuda.device(self.device):
             number = self.step_count + 1
             at = None
@@ -97,6 +108,7 @@ class AdamW:
                 self._step_device.add_(1)
                 at = self._step_device.data_ptr()
             capi.check(capi.lib().mgpt_adamw_step(
-                ctypes.byref(cfg), n, self._sizes, pp, gp, cp, self.state.data_ptr(), self.state.numel(),
-                number, at, scale, torch.cuda.current_stream().cuda_stream))
+                ctypes.byref(cfg), n, self._sizes, array(*map(_data_ptr, self.params)), array(*ptrs), copies,
+                self.state.data_ptr(), self.state.numel(), number, at, scale,
+                torch.cuda.current_stream().cuda_stream))
         self.step_count = number
