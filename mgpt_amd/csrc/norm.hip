@@ -264,7 +264,7 @@ __device__ __forceinline__ void block_columns(const float (&acc)[NV][8], float* 
 
 // sum_part: a block's T_g (parts > 0) or its part of dgamma_post (whole groups); pre_part:
 // its part of dgamma_pre, each [blocks][C].
-template <typename T, int W, int NV>
+template <typename T, int W, int NV, bool WHOLE>
 __global__ __launch_bounds__(W <= 4 ? 256 : W * 64) void norm_backward_kernel(
     NormArgs a, const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ dout,
     const T* __restrict__ dy, T* __restrict__ dx, T* __restrict__ dh, float* __restrict__ dgate,
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64) void norm_backward_kernel(
     }
     if (W > 1 && !(a.post && a.pre)) __syncthreads();   // (as in the forward)
   };
-  if (a.parts > 0) {
+  if constexpr (!WHOLE) {
     const int g = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     const int r1 = g * R + min(R, (part + 1) * a.chunk);
     load_gate(g);
@@ -453,10 +453,11 @@ int compute_units() {
   return n;
 }
 
-// Waves and vectors of a row: 1024 columns a wave at most (its gains and a row's values
-// fill the registers).
-void row_layout(int C, int* W, int* NV) {
-  *NV = C <= 512 ? 1 : 2;
+// Waves and vectors of a row.  Forward: 1024 columns a wave, whose gains then serve more
+// of a row (16384 x 1024: 22.4 us, with 512 24.5; 32768 x 2048: 95 / 110).  Backward: 512,
+// for twice the waves on a CU (below).
+void row_layout(int C, bool backward, int* W, int* NV) {
+  *NV = C <= (backward ? 8192 : 512) ? 1 : 2;
   int w = 1;
   while (w * *NV * 512 < C) w *= 2;
   *W = w;
@@ -464,10 +465,10 @@ void row_layout(int C, int* W, int* NV) {
 
 NormPlan plan_backward(int N, int C, int G) {
   NormPlan p{};
-  row_layout(C, &p.W, &p.NV);
+  row_layout(C, true, &p.W, &p.NV);
   const int S = p.W <= 4 ? 4 / p.W : 1, R = N / G;
   // enough blocks for the chip, few enough that their column sums cost little
-  const int target = p.W <= 4 ? 512 : 256;
+  const int target = p.W <= 4 ? 1024 : 256;
   if (R < 8 || G >= target * S) {
     const int per = (G + target - 1) / target;
     p.per_block = (per + S - 1) / S * S;
@@ -495,16 +496,16 @@ NormLayout norm_layout(const NormPlan& p, int C, int G) {
 
 template <typename F>
 hipError_t for_layout(int W, int NV, F&& f) {
-  if (NV == 1) {
-    f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-    return hipGetLastError();
-  }
+  auto nv = [&](auto w) {
+    if (NV == 1) f(w, std::integral_constant<int, 1>{});
+    else f(w, std::integral_constant<int, 2>{});
+  };
   switch (W) {
-    case 1: f(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}); break;
-    case 2: f(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}); break;
-    case 4: f(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{}); break;
-    case 8: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{}); break;
-    default: f(std::integral_constant<int, 16>{}, std::integral_constant<int, 2>{}); break;
+    case 1: nv(std::integral_constant<int, 1>{}); break;
+    case 2: nv(std::integral_constant<int, 2>{}); break;
+    case 4: nv(std::integral_constant<int, 4>{}); break;
+    case 8: nv(std::integral_constant<int, 8>{}); break;
+    default: nv(std::integral_constant<int, 16>{}); break;
   }
   return hipGetLastError();
 }
@@ -562,7 +563,7 @@ int mgpt_norm_forward(const mgpt_norm_config* cfg, const void* x, const void* h,
   const NormArgs a = norm_args(cfg, num_tokens, gamma_post, gate, gamma_pre, rstd_post, rstd_pre,
                                {x, h, out, gamma_pre ? y : nullptr, gamma_post, gate, gamma_pre});
   int W, NV;
-  row_layout(a.C, &W, &NV);
+  row_layout(a.C, false, &W, &NV);
   const int S = W <= 4 ? 4 / W : 1, rows = (num_tokens + S - 1) / S;
   const int grid = std::min(rows, compute_units() * (W <= 4 ? 4 : 16 / W));
   auto go = [&](auto t) {
@@ -628,9 +629,12 @@ int mgpt_norm_backward(const mgpt_norm_config* cfg, const void* x, const void* h
     using T = decltype(t);
     return for_layout(p.W, p.NV, [&](auto w, auto nv) {
       constexpr int kW = decltype(w)::value, kNV = decltype(nv)::value;
-      hipLaunchKernelGGL((norm_backward_kernel<T, kW, kNV>), dim3(p.blocks), dim3(kW <= 4 ? 256 : kW * 64), 0,
-                         st, a, (const T*)x, (const T*)h, (const T*)dout, (const T*)dy, (T*)dx, (T*)dh, dgate,
-                         sums, pres);
+      auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(p.blocks), dim3(kW <= 4 ? 256 : kW * 64), 0, st, a, (const T*)x,
+                           (const T*)h, (const T*)dout, (const T*)dy, (T*)dx, (T*)dh, dgate, sums, pres);
+      };
+      if (p.parts > 0) launch(norm_backward_kernel<T, kW, kNV, false>);
+      else launch(norm_backward_kernel<T, kW, kNV, true>);
     });
   };
   HIP_TRY(cfg->dtype == MGPT_DTYPE_F32 ? go(float{}) : go(bf16_t{}));
