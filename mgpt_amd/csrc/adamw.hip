@@ -113,10 +113,10 @@ template <> struct Held<32> { float4 m, v; };
 template <> struct Held<8> { uint32_t m, v; int me, ve; };
 
 __device__ __forceinline__ Held<32> load_held32(const AdamwArgs& a, size_t at) {
-  return {*reinterpret_cast<const float4*>(a.m + 4 * at), *reinterpret_cast<const float4*>(a.v + 4 * at)};
+  return {load_once(reinterpret_cast<const float4*>(a.m + 4 * at)), load_once(reinterpret_cast<const float4*>(a.v + 4 * at))};
 }
 __device__ __forceinline__ Held<8> load_held8(const AdamwArgs& a, size_t at, size_t block) {
-  return {*reinterpret_cast<const uint32_t*>(a.m + at), *reinterpret_cast<const uint32_t*>(a.v + at),
+  return {load_once(reinterpret_cast<const uint32_t*>(a.m + at)), load_once(reinterpret_cast<const uint32_t*>(a.v + at)),
           a.me[block], a.ve[block]};
 }
 template <int BITS>
@@ -145,8 +145,8 @@ __device__ __forceinline__ void decode(const Held<8>& h, float (&m)[4], float (&
 
 __device__ __forceinline__ void store_held(const AdamwArgs& a, size_t at, size_t, uint32_t,
                                            const float (&m)[4], const float (&v)[4], IntTag<32>) {
-  *reinterpret_cast<float4*>(a.m + 4 * at) = make_float4(m[0], m[1], m[2], m[3]);
-  *reinterpret_cast<float4*>(a.v + 4 * at) = make_float4(v[0], v[1], v[2], v[3]);
+  store_once(reinterpret_cast<float4*>(a.m + 4 * at), make_float4(m[0], m[1], m[2], m[3]));
+  store_once(reinterpret_cast<float4*>(a.v + 4 * at), make_float4(v[0], v[1], v[2], v[3]));
 }
 __device__ __forceinline__ void store_held(const AdamwArgs& a, size_t at, size_t block, uint32_t step,
                                            const float (&m)[4], const float (&v)[4], IntTag<8>) {
@@ -179,8 +179,8 @@ __device__ __forceinline__ void store_held(const AdamwArgs& a, size_t at, size_t
     c = u == 0 ? 0 : u < 0x7F800000u ? c : 255;
     cv |= (uint32_t)c << (8 * q);
   }
-  *reinterpret_cast<uint32_t*>(a.m + at) = (uint32_t)cm;
-  *reinterpret_cast<uint32_t*>(a.v + at) = cv;
+  store_once(reinterpret_cast<uint32_t*>(a.m + at), (uint32_t)cm);
+  store_once(reinterpret_cast<uint32_t*>(a.v + at), cv);
   if (lane_id() == 0) {
     a.me[block] = (uint8_t)me;
     a.ve[block] = (uint8_t)ve;
@@ -188,11 +188,11 @@ __device__ __forceinline__ void store_held(const AdamwArgs& a, size_t at, size_t
 }
 
 __device__ __forceinline__ void load_grad4(const float* g, float (&o)[4]) {
-  const float4 x = *reinterpret_cast<const float4*>(g);
+  const float4 x = load_once(reinterpret_cast<const float4*>(g));
   o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
 }
 __device__ __forceinline__ void load_grad4(const bf16_t* g, float (&o)[4]) {
-  const uint2 x = *reinterpret_cast<const uint2*>(g);
+  const uint2 x = load_once(reinterpret_cast<const uint2*>(g));
   o[0] = __uint_as_float(x.x << 16); o[1] = __uint_as_float(x.x & 0xFFFF0000u);
   o[2] = __uint_as_float(x.y << 16); o[3] = __uint_as_float(x.y & 0xFFFF0000u);
 }
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwTensors ts, AdamwArgs a
     for (int i = 0; i < kIters; ++i) {
       const int b = 4 * i + w;
       const int64_t e = first + b * kBlock + 4 * lane;
-      pv[i] = *reinterpret_cast<const float4*>(p + e);
+      pv[i] = load_once(reinterpret_cast<const float4*>(p + e));
       load_grad4(g + e, gv[i]);
       held[i] = load_held<BITS>(a, (block0 + b) * kBlock + 4 * lane, block0 + b);
     }
@@ -250,10 +250,10 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwTensors ts, AdamwArgs a
       decode(held[i], m, v);
 #pragma unroll
       for (int q = 0; q < 4; ++q) update(x[q], gv[i][q], m[q], v[q]);
-      *reinterpret_cast<float4*>(p + e) = make_float4(x[0], x[1], x[2], x[3]);
+      store_once(reinterpret_cast<float4*>(p + e), make_float4(x[0], x[1], x[2], x[3]));
       store_held(a, (block0 + b) * kBlock + 4 * lane, block0 + b, step, m, v, IntTag<BITS>{});
       if (copy)
-        *reinterpret_cast<uint2*>(copy + e) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+        store_once(reinterpret_cast<uint2*>(copy + e), make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])));
     }
     return;
   }

@@ -112,6 +112,32 @@ __device__ __forceinline__ float to_f32(bf16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ void store_act(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_act(bf16_t* p, float v) { *p = f32_to_bf16(v); }
 
+// Loads and stores that do not stay in the caches (data passed once).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void store_once(float4* p, float4 v) {
+  const f32x4 x = {v.x, v.y, v.z, v.w};
+  __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(p));
+}
+__device__ __forceinline__ void store_once(uint4* p, uint4 v) {
+  const u32x4 x = {v.x, v.y, v.z, v.w};
+  __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(p));
+}
+__device__ __forceinline__ void store_once(uint2* p, uint2 v) {
+  const u32x2 x = {v.x, v.y};
+  __builtin_nontemporal_store(x, reinterpret_cast<u32x2*>(p));
+}
+__device__ __forceinline__ void store_once(uint32_t* p, uint32_t v) { __builtin_nontemporal_store(v, p); }
+__device__ __forceinline__ float4 load_once(const float4* p) {
+  const f32x4 x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
+  return make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ uint2 load_once(const uint2* p) {
+  const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+  return make_uint2(x[0], x[1]);
+}
+__device__ __forceinline__ uint32_t load_once(const uint32_t* p) { return __builtin_nontemporal_load(p); }
+
 __device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & (kWave - 1)); }
 
 // Inclusive prefix sum over the 64 lanes of a wave (every lane active), by

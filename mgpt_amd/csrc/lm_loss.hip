@@ -166,14 +166,6 @@ __device__ __forceinline__ uint2 transpose4(uint2 u, int lane) {
   return upper ? make_uint2(r, a1) : make_uint2(a0, r);
 }
 
-// The transpose's stores, past the caches: with d's own left in them, what both write a tile
-// (256 KB) drains sooner (16384 x 1024 x 16128: 695 us, so 637, d's too 685).
-__device__ __forceinline__ void store_through(bf16_t* p, uint2 v) {
-  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-  const u32x2 u = {v.x, v.y};
-  __builtin_nontemporal_store(u, reinterpret_cast<u32x2*>(p));
-}
-
 template <typename W>
 using Acc = f32x16[W::TN][W::TM];
 
@@ -331,7 +323,9 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
         for (int k = 0; k < 4; ++k) {
           const uint2 u = transpose4(q[k], lrow);
           const int f = f0 + 8 * k + 4 * lhalf + (lrow & 3), r4 = row & ~3;
-          if (r4 < g.rows_t) store_through(dt + (size_t)f * g.lddt + r4, u);
+          // (past the caches: 695 -> 637 us at 16384 x 1024 x 16128, where both write 256 KB a
+          // tile; d's own stores too: 685)
+          if (r4 < g.rows_t) store_once(reinterpret_cast<uint2*>(dt + (size_t)f * g.lddt + r4), u);
         }
       } else {
 #pragma unroll
