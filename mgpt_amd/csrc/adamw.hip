@@ -26,7 +26,7 @@
 // What bounds it: memory.  Per element 28 bytes in 32 bits with fp32 gradients, 14 in 8
 // bits with bf16 ones (+2 with a bf16 copy).  A block of threads takes 4096 elements of
 // one tensor (found by a search of the tensors' table, which is a kernel argument: any
-// set of tensors in one launch per 96), every load of a lane requested before the first
+// set of tensors in one launch per 116), every load of a lane requested before the first
 // use.
 #include <hip/hip_runtime.h>
 
@@ -45,13 +45,13 @@ constexpr int kTile = 4 * kIters * kBlock;   // elements per workgroup
 constexpr uint64_t kMaxTiles = 1u << 23;     // per launch (2^31 threads)
 
 struct AdamwTensors {
-  static constexpr int kMax = 96;   // keeps the argument block under 4 KB
+  static constexpr int kMax = 116;   // keeps the argument block under 4 KB
   float* p[kMax];
   const void* g[kMax];
   bf16_t* copy[kMax];
-  int64_t size[kMax];
-  uint32_t block0[kMax];   // first state block
-  uint32_t tile0[kMax];    // first workgroup
+  uint32_t block0[kMax];      // first state block
+  uint32_t tile0[kMax + 1];   // first workgroup; past the last tensor: all of them
+  uint16_t tail[kMax];        // elements of the last workgroup's tile, 1 .. kTile
   int n;
 };
 
@@ -206,11 +206,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwTensors ts, AdamwArgs a
     if (ts.tile0[mid] <= blockIdx.x) lo = mid;
     else hi = mid;
   }
-  const int64_t size = ts.size[lo];
   float* __restrict__ p = ts.p[lo];
   const GT* __restrict__ g = static_cast<const GT*>(ts.g[lo]);
   bf16_t* __restrict__ copy = ts.copy[lo];
   const uint32_t tile = blockIdx.x - ts.tile0[lo];
+  const int left = blockIdx.x + 1 == ts.tile0[lo + 1] ? ts.tail[lo] : kTile;   // elements of this tile
   uint32_t step = a.step;
   if (a.step_device) {
     step = (uint32_t)max(*a.step_device, 1);
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwTensors ts, AdamwArgs a
   };
   const bool aligned = ((reinterpret_cast<uintptr_t>(p) & 15) | (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(GT) - 1)) |
                         (reinterpret_cast<uintptr_t>(copy) & 7)) == 0;
-  if (aligned && first + kTile <= size) {
+  if (aligned && left == kTile) {
     float4 pv[kIters];
     float gv[kIters][4];
     Held<BITS> held[kIters];
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwTensors ts, AdamwArgs a
   // the end are zeros throughout (the state has room for whole blocks).
   for (int i = 0; i < kIters; ++i) {
     const int b = 4 * i + w;
-    if (first + b * kBlock >= size) return;
+    if (b * kBlock >= left) return;
     const int64_t e = first + b * kBlock + 4 * lane;
     const size_t at = (block0 + b) * kBlock + 4 * lane;
     float m[4], v[4], x[4];
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwTensors ts, AdamwArgs a
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       x[q] = 0.0f;
-      if (e + q < size) {
+      if (b * kBlock + 4 * lane + q < left) {
         x[q] = p[e + q];
         update(x[q], to_f32(g[e + q]), m[q], v[q]);
         p[e + q] = x[q];
@@ -365,6 +365,7 @@ int mgpt_adamw_step(const mgpt_adamw_config* cfg, int num_tensors, const int64_t
   auto flush = [&]() -> hipError_t {
     if (ts.n == 0) return hipSuccess;
     auto go = [&](auto kernel) {
+      ts.tile0[ts.n] = (uint32_t)tiles;
       hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), 0, (hipStream_t)stream, ts, a);
     };
     const bool f32 = cfg->grad_dtype == MGPT_DTYPE_F32;
@@ -388,7 +389,7 @@ int mgpt_adamw_step(const mgpt_adamw_config* cfg, int num_tensors, const int64_t
       ts.p[ts.n] = params[i];
       ts.g[ts.n] = grads[i];
       ts.copy[ts.n] = copies ? (bf16_t*)copies[i] : nullptr;
-      ts.size[ts.n] = size;
+      ts.tail[ts.n] = (uint16_t)(size - (int64_t)(t - 1) * kTile);
       ts.block0[ts.n] = (uint32_t)block;
       ts.tile0[ts.n] = (uint32_t)tiles;
       ++ts.n;

@@ -1,4 +1,4 @@
-"""AdamW: one step over all tensors of a model in one launch per 96 of them.
+"""AdamW: one step over all tensors of a model in one launch per 116 of them.
 
 Mirrors the engine's AdamWOptimizer
 (/root/reference/src/main/neuralnetwork/optimisers/AdamWOptimiser.h:13-97)

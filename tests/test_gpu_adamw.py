@@ -86,7 +86,7 @@ def gradients(rng, sizes, bf16):
     return gs, t
 
 
-SIZES = [[1], [256], [257, 1, 0, 255, 4096], [5000, 3, 70001, 4097], [17] * 203]
+SIZES = [[1], [256], [257, 1, 0, 255, 4096], [5000, 3, 70001, 4097], [17] * 233]
 
 
 @pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{max(s)}")
