@@ -401,8 +401,8 @@ int mgpt_adamw_state_bytes(int num_tensors, const int64_t* sizes, int state_bits
 
 /* params[i]: fp32, updated in place; grads[i]: grad_dtype, read; copies (may
  * be null, or hold nulls): bf16 copies of the updated params.  All device
- * memory, aligned to their elements (16-byte aligned ones are faster), while
- * the arrays of pointers and sizes are host memory, read during the call.  A
+ * memory, aligned to their elements (16-byte aligned ones are faster) and
+ * without overlaps, while the arrays of pointers and sizes are host memory, read during the call.  A
  * tensor whose grads[i] is null is left as it is, its moments too.  step: 1
  * for the first; if step_device is not null the device reads the number
  * there instead (a captured step that is replayed; below 1 counts as 1).
@@ -453,8 +453,11 @@ int mgpt_norm_backward(const mgpt_norm_config* cfg, const void* x, const void* h
  *   lse[n] = log(sum over v of exp(z[n][v])),  loss[n] = lse[n] - z[n][targets[n]]
  * x [N,C], W [V,C] in dtype, row-major, bias [V] fp32 or null.  (The engine's
  * lm_head keeps W transposed, [C,V].)  A target outside 0 .. V - 1 means that
- * the row has none: its loss is 0 and it adds to no gradient.  Replaces
- * lm_head's LinearLayer and CrossEntropyLossLayer. */
+ * the row has none: its loss is 0 and it adds to no gradient, whatever it
+ * holds.  fp32 products are formed from three bf16 parts of each operand, six
+ * of nine products, to fp32's accuracy (magnitudes up to 3.38e38; beyond, and
+ * for infinities, NaN).  Replaces lm_head's LinearLayer and
+ * CrossEntropyLossLayer. */
 typedef struct mgpt_lm_loss_config {
   int embed_dim;    /* C: 1 .. 2^20 (multiples of 64 (bf16) or 32 (fp32) are read in place) */
   int vocab_size;   /* V: 1 .. 2^24 */
@@ -478,7 +481,8 @@ int mgpt_lm_loss_forward(const mgpt_lm_loss_config* cfg, const void* x, const vo
  * null, dmean [1] of their mean (null: 1): dx [N,C], dW [V,C] in dtype, dbias
  * [V] fp32, each written (not added to) where it is not null.  The logits are
  * formed again, a piece of the vocabulary at a time.  Workspace: up to about 1
- * GiB for a piece's gradients, and copies of x and of a piece of W. */
+ * GiB for a piece's gradients (more where 256 columns take more), and copies
+ * of x and of a piece of W. */
 int mgpt_lm_loss_backward(const mgpt_lm_loss_config* cfg, const void* x, const void* W,
                           const float* bias, const int32_t* targets, const float* lse,
                           const float* dloss, const float* dmean, void* dx, void* dW, float* dbias,

@@ -6,6 +6,7 @@ loudly if the HIP library has not been built: there is no fallback path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -141,3 +142,13 @@ def lib() -> ctypes.CDLL:
 def check(status: int) -> None:
     if status != MGPT_OK:
         raise MoEError(status, lib().mgpt_moe_last_error().decode())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """A context in which `device` (a torch.device with an index) is the current
+    one; nothing to enter where it is already."""
+    import torch
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)

@@ -46,7 +46,8 @@ namespace {
 
 enum LossEpilogue {
   kLse,      // (max, sum of exponentials) per row and 64 columns, the target's logit
-  kDLogit,   // d and its transpose, its column sums
+  kDLogit,   // d and its transpose
+  kDLogitSum,   // and d's column sums
   kPart,     // fp32 partial product, stored or added
   kStore     // the product in the inputs' type
 };
@@ -70,7 +71,7 @@ struct LossArgs {
   char *d, *dt;          // [M][ldd], [.][lddt] in T
   size_t ldd, lddt;      // elements
   int rows_t;            // rows that the transpose holds (zeros past M)
-  float* colsum;         // [2 mt][ldd] or null
+  float* colsum;         // [2 mt][ldd]
   // kPart: out [parts][M][ldo] fp32; kStore: out [M][ldo] in T
   char* out;
   size_t ldo;
@@ -210,6 +211,7 @@ __device__ __forceinline__ void start_from_bias(const LossArgs& g, Acc<W>& acc, 
 
 // exp(z - s) of a register: one fma into the hardware's exponential; `huge` (a lane's s
 // near the type's lowest or largest value, which times log2 e overflows): difference first.
+// (By lane: a row's bits do not depend on its neighbours.)
 __device__ __forceinline__ float exp_less(float z, float s, float ns, bool huge) {
   return __builtin_amdgcn_exp2f(huge ? (z - s) * kLog2e : __builtin_fmaf(z, kLog2e, ns));
 }
@@ -238,11 +240,12 @@ __device__ __forceinline__ void emit_lse(const LossArgs& g, Acc<W>& acc, int row
     m = other_half_max(m);
     const float top = m == -INFINITY ? 0.0f : m, ntop = -top * kLog2e;
     float s = 0.0f;
-    if (__ballot(!(fabsf(top) < kHuge))) {
+    const bool huge = !(fabsf(top) < kHuge);
+    if (__ballot(huge)) {
 #pragma unroll
       for (int j = 0; j < W::TN; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) s += exp_less(acc[j][i][v], top, ntop, true);
+        for (int v = 0; v < 16; ++v) s += exp_less(acc[j][i][v], top, ntop, huge);
     } else {
 #pragma unroll
       for (int j = 0; j < W::TN; ++j)
@@ -266,7 +269,7 @@ __device__ __forceinline__ void emit_lse(const LossArgs& g, Acc<W>& acc, int row
   }
 }
 
-template <typename T, typename W>
+template <typename T, typename W, bool SUM>
 __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow, int lhalf,
                                             int sum_row) {
   float lse[W::TM], sc[W::TM];
@@ -296,7 +299,7 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
       float d[16];
       if (slow) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v) d[v] = exp_less(acc[j][i][v], lse[i], nl, true);
+        for (int v = 0; v < 16; ++v) d[v] = exp_less(acc[j][i][v], lse[i], nl, !(fabsf(lse[i]) < kHuge));
       } else {
 #pragma unroll
         for (int v = 0; v < 16; ++v) d[v] = exp_less(acc[j][i][v], lse[i], nl, false);
@@ -310,7 +313,7 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
       // logits are not finite)
 #pragma unroll
       for (int v = 0; v < 16; ++v) d[v] = mul_zero(d[v], sc[i]);
-      if (g.colsum) {
+      if constexpr (SUM) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) cs[v] += d[v];
       }
@@ -342,7 +345,7 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (g.colsum) {
+    if constexpr (SUM) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         const float s = half_sum(cs[v]);
@@ -593,7 +596,7 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
 
   for (;;) {
     f32x16 acc[kTN][kTM];
-    if constexpr (EPI == kLse || EPI == kDLogit) {
+    if constexpr (EPI == kLse || EPI == kDLogit || EPI == kDLogitSum) {
       start_from_bias<W>(g, acc, cur.n0 + wn * W::WTN, lhalf);
     } else {
 #pragma unroll
@@ -654,8 +657,8 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
     const int row0 = cur.row0 + wm * W::WTM, fw = cur.n0 + wn * W::WTN;
     if constexpr (EPI == kLse)
       emit_lse<T, W>(g, acc, row0, fw, lr, lh);
-    else if constexpr (EPI == kDLogit)
-      emit_dlogit<T, W>(g, acc, row0, fw, lr, lh, cur.row0 / BM * W::WM + wm);
+    else if constexpr (EPI == kDLogit || EPI == kDLogitSum)
+      emit_dlogit<T, W, EPI == kDLogitSum>(g, acc, row0, fw, lr, lh, cur.row0 / BM * W::WM + wm);
     else if constexpr (EPI == kPart)
       emit_part<W>(g, acc, cur.part, row0, fw, lr, lh);
     else
@@ -846,10 +849,15 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs<T> a) {
   const auto& t = a.t[k];
   const int nx = (t.cols + 63) / 64;   // tiles across; columns fastest: whole rows of the source
   const int c0 = b % nx * 64, r0 = b / nx * 64;
-  // rows r0 .. of src into the tile
+  // rows r0 .. of src into the tile; a row of x without a target as zeros, whatever it
+  // holds (its d is 0, and 0 times what is not finite would not be)
   for (int i = threadIdx.x; i < 64 * 64 / kV; i += 256) {
     const int r = i / (64 / kV), c = i % (64 / kV) * kV;
-    const bool in = r0 + r < t.rows;
+    bool in = r0 + r < t.rows;
+    if (k == 0 && in) {
+      const int target = a.targets[r0 + r];
+      in = target >= 0 && target < a.V;
+    }
     const T* p = t.src + (size_t)(r0 + r) * t.cols + c0 + c;
     if (t.vec) {   // (cols % kV == 0: a vector is within the row or past it)
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -985,7 +993,7 @@ hipError_t launch_ring(LossArgs g, const GemmPlan& p, int cus, hipStream_t st) {
   } else if (p.tile == kMid) {
     go(ring_kernel<T, EPI, 128, 128, 4>, 256);
   } else {
-    if constexpr (!(sizeof(T) == 4 && EPI == kDLogit))
+    if constexpr (!(sizeof(T) == 4 && (EPI == kDLogit || EPI == kDLogitSum)))
       go(ring_kernel<T, EPI, 256, 256, 8>, 512);
     else
       return hipErrorInvalidValue;   // (its epilogue beside the split operands spills registers)
@@ -1171,7 +1179,8 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
     g.lddt = l.nk;
     g.rows_t = l.nk;
     g.colsum = db ? (float*)(ws + l.colsum) : nullptr;
-    if ((e = launch_ring<T, kDLogit>(g, l.dl, cus, st)) != hipSuccess) return e;
+    e = db ? launch_ring<T, kDLogitSum>(g, l.dl, cus, st) : launch_ring<T, kDLogit>(g, l.dl, cus, st);
+    if (e != hipSuccess) return e;
     if (db) {
       hipLaunchKernelGGL(colsum_kernel, dim3(div_up(vn, kWave)), dim3(1024), 0, st, g.colsum,
                          div_up(N, tile_rows(l.dl.tile)) * 2, g.ldd, vn, factor, db + v0);

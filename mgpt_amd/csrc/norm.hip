@@ -532,7 +532,7 @@ hipError_t for_layout(int W, int NV, F&& f) {
   return hipGetLastError();
 }
 
-int check_norm(const mgpt_norm_config* cfg, int N) {
+int check_norm(const mgpt_norm_config* cfg, int N, bool gated) {
   if (!cfg) return fail(MGPT_ERR_INVALID_ARGUMENT, "config is null");
   if (N < 0) return fail(MGPT_ERR_INVALID_ARGUMENT, "negative num_tokens");
   if (cfg->embed_dim <= 0) return fail(MGPT_ERR_INVALID_ARGUMENT, "embed_dim %d", cfg->embed_dim);
@@ -542,7 +542,7 @@ int check_norm(const mgpt_norm_config* cfg, int N) {
     return fail(MGPT_ERR_UNSUPPORTED, "unsupported dtype %d", cfg->dtype);
   if (!(cfg->eps >= 0.0f) || !std::isfinite(cfg->residual_scale))
     return fail(MGPT_ERR_INVALID_ARGUMENT, "eps must be >= 0 and residual_scale finite");
-  if (cfg->gate_rows < 1 || (N > 0 && N % cfg->gate_rows != 0))
+  if (cfg->gate_rows < 1 || (gated && N % cfg->gate_rows != 0))
     return fail(MGPT_ERR_INVALID_ARGUMENT, "gate_rows %d must divide num_tokens %d", cfg->gate_rows, N);
   return MGPT_OK;
 }
@@ -577,7 +577,7 @@ extern "C" {
 int mgpt_norm_forward(const mgpt_norm_config* cfg, const void* x, const void* h, const float* gamma_post,
                       const float* gate, const float* gamma_pre, void* out, void* y, float* rstd_post,
                       float* rstd_pre, int num_tokens, void* stream) {
-  if (int rc = check_norm(cfg, num_tokens)) return rc;
+  if (int rc = check_norm(cfg, num_tokens, gate != nullptr)) return rc;
   if (num_tokens == 0) return MGPT_OK;
   if (!x || !h || !out) return fail(MGPT_ERR_INVALID_ARGUMENT, "null x, h or out");
   if ((gamma_pre && (!y || !rstd_pre)) || (gamma_post && !rstd_post))
@@ -602,11 +602,11 @@ int mgpt_norm_forward(const mgpt_norm_config* cfg, const void* x, const void* h,
 
 int mgpt_norm_backward_workspace_bytes(const mgpt_norm_config* cfg, int num_tokens, size_t* bytes) {
   if (!bytes) return fail(MGPT_ERR_INVALID_ARGUMENT, "null bytes");
-  if (int rc = check_norm(cfg, num_tokens)) return rc;
+  if (int rc = check_norm(cfg, num_tokens, false)) return rc;
   *bytes = 0;
   if (num_tokens == 0) return MGPT_OK;
   // with and without a gate (whose rows decide the blocks)
-  const int C = cfg->embed_dim, G = cfg->gate_rows;
+  const int C = cfg->embed_dim, G = num_tokens % cfg->gate_rows == 0 ? cfg->gate_rows : 1;
   *bytes = std::max(norm_layout(plan_backward(num_tokens, C, G), C, G).total,
                     norm_layout(plan_backward(num_tokens, C, 1), C, 1).total);
   return MGPT_OK;
@@ -617,7 +617,7 @@ int mgpt_norm_backward(const mgpt_norm_config* cfg, const void* x, const void* h
                        const float* rstd_pre, const void* dout, const void* dy, void* dx, void* dh,
                        float* dgamma_post, float* dgate, float* dgamma_pre, int num_tokens, void* workspace,
                        size_t workspace_bytes, void* stream) {
-  if (int rc = check_norm(cfg, num_tokens)) return rc;
+  if (int rc = check_norm(cfg, num_tokens, gate != nullptr)) return rc;
   if ((dgamma_post && !gamma_post) || (dgate && !gate) || (dgamma_pre && !gamma_pre))
     return fail(MGPT_ERR_INVALID_ARGUMENT, "a gradient of a gain that is null");
   const int C = cfg->embed_dim;

@@ -58,7 +58,7 @@ class LMLoss:
         log-sum-exp, float32 in the shape of targets, and float32 [2], the mean
         loss over the tokens with a target and their number."""
         n, ptrs = self._inputs(x, weight, targets, bias)
-        with torch.cuda.device(x.device):
+        with capi.on_device(x.device):
             loss = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
             lse = torch.empty_like(loss)
             mean = torch.empty(2, dtype=torch.float32, device=x.device)
@@ -82,7 +82,7 @@ class LMLoss:
         if dmean is not None and dmean.numel() != 1:
             raise ValueError("dmean must have one element")
         ptrs.append(None if dmean is None else self._check(dmean, torch.float32, tuple(dmean.shape), dev, "dmean"))
-        with torch.cuda.device(dev):
+        with capi.on_device(dev):
             dx = torch.empty_like(x) if need[0] else None
             dw = torch.empty_like(weight) if need[1] else None
             db = torch.empty_like(bias) if need[2] and bias is not None else None

@@ -64,7 +64,7 @@ class ResidualNorm:
         cfg, n, gains = self._gains(x, gamma_post, gate, gamma_pre)
         xp = self._rows(x, x.shape, x.device, "x")
         hp = self._rows(h, x.shape, x.device, "h")
-        with torch.cuda.device(x.device):
+        with capi.on_device(x.device):
             out = torch.empty_like(x)
             y = torch.empty_like(x) if gamma_pre is not None else None
             rh = torch.empty(n, dtype=torch.float32, device=x.device) if gamma_post is not None else None
@@ -95,7 +95,7 @@ class ResidualNorm:
             raise ValueError("dout is needed without gamma_pre")
         up = [None if dout is None else self._rows(dout, x.shape, x.device, "dout"),
               None if gamma_pre is None else self._rows(dy, x.shape, x.device, "dy")]
-        with torch.cuda.device(x.device):
+        with capi.on_device(x.device):
             dx, dh = torch.empty_like(x), torch.empty_like(x)
             grads = [None if g is None else torch.empty_like(g) for g in (gamma_post, gate, gamma_pre)]
             need = ctypes.c_size_t()

@@ -43,6 +43,10 @@ class AdamW:
             self._check(p, torch.float32, p.numel(), f"params[{i}]")
             if self.copies is not None and self.copies[i] is not None:
                 self._check(self.copies[i], torch.bfloat16, p.numel(), f"copies[{i}]")
+        written = self.params + [c for c in self.copies or [] if c is not None]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written if t.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("params and copies must not overlap")
         self.step_count = 0
         n = len(self.params)
         self._numels = [p.numel() for p in self.params]
@@ -101,7 +105,7 @@ class AdamW:
             scale = grad_scale.data_ptr()
         cfg = capi.AdamWConfig(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
                                self.state_bits, _GRAD[dtypes.pop()])
-        with torch.cuda.device(self.device):
+        with capi.on_device(self.device):
             number = self.step_count + 1
             at = None
             if self._step_device is not None:

@@ -185,23 +185,37 @@ def test_every_logit_at_the_lowest_value():
     assert (got["loss"] == 0).all()
 
 
-def test_a_row_that_is_not_finite_stays_alone():
-    """A NaN row makes its own loss NaN, and as a row without a target no
-    gradient of the others."""
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_row_without_a_target_may_hold_anything(act, value):
+    """Padding that is not finite changes no gradient and no other row."""
+    x, W, b, t = inputs(100, 64, 300, act)
+    t[17], t[99] = -1, 300
+    clean = run(x, W, b, t, act)
+    x2 = x.clone()
+    x2[17, 5] = value
+    x2[99] = value
+    got = run(x2, W, b, t, act)
+    assert not torch.isfinite(got["lse"][17]) and got["loss"][17] == 0 and got["loss"][99] == 0
+    rows = torch.ones(100, dtype=torch.bool, device="cuda")
+    rows[17] = rows[99] = False
+    for k in ("loss", "lse", "dx"):
+        assert torch.equal(got[k][rows], clean[k][rows]), k
+    for k in ("mean", "dW", "db"):
+        assert torch.equal(got[k], clean[k]), k
+    assert not got["dx"][~rows].any()
+
+
+def test_a_row_with_a_target_that_is_not_finite():
+    """Its loss is NaN, the others' are as before."""
     x, W, b, t = inputs(100, 64, 300, "bf16")
-    t[17] = -1
     clean = run(x, W, b, t, "bf16")
     x2 = x.clone()
     x2[17, 5] = float("nan")
     got = run(x2, W, b, t, "bf16")
-    assert torch.isnan(got["lse"][17]) and got["loss"][17] == 0
     rows = torch.arange(100, device="cuda") != 17
-    for k in ("loss", "lse", "dx"):
-        assert torch.equal(got[k][rows], clean[k][rows]), k
-    assert torch.equal(got["db"], clean["db"]) and not got["dx"][17].any()
-    # (dW contracts over the rows: 0 times NaN is NaN in column 5)
-    cols = torch.arange(64, device="cuda") != 5
-    assert torch.equal(got["dW"][:, cols], clean["dW"][:, cols])
+    assert torch.isnan(got["loss"][17]) and torch.equal(got["loss"][rows], clean["loss"][rows])
+    assert torch.equal(got["dx"][rows], clean["dx"][rows])
 
 
 def test_gradients_are_the_losses_differences():
