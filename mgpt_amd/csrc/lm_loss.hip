@@ -49,7 +49,8 @@ enum LossEpilogue {
   kDLogit,   // d and its transpose
   kDLogitSum,   // and d's column sums
   kPart,     // fp32 partial product, stored or added
-  kStore     // the product in the inputs' type
+  kStore,    // the product in the inputs' type, rows as 16-byte vectors
+  kStoreOdd  // the same for rows that are not: a lane has a column, so that a row's neighbours are stored together
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -72,11 +73,11 @@ struct LossArgs {
   size_t ldd, lddt;      // elements
   int rows_t;            // rows that the transpose holds (zeros past M)
   float* colsum;         // [2 mt][ldd]
-  // kPart: out [parts][M][ldo] fp32; kStore: out [M][ldo] in T
+  // kPart: out [parts][M][ldo] fp32; kStore, kStoreOdd: out [M][ldo] in T
   char* out;
   size_t ldo;
-  int add, vec;
-  const float* factor;   // kStore: of the product
+  int add;
+  const float* factor;   // kStore, kStoreOdd: of the product
 };
 
 // fp32 operands as three bf16 numbers each, x = h + m + l exactly (8 of its 24 bits each,
@@ -398,32 +399,53 @@ __device__ __forceinline__ void emit_store(const LossArgs& g, Acc<W>& acc, int r
   for (int j = 0; j < W::TN; ++j) {
     const int f0 = fw + 32 * j;
     if (f0 >= g.Nf) continue;
-    const bool vec = g.vec && f0 + 32 <= g.Nf;
+    const bool whole = f0 + 32 <= g.Nf;
 #pragma unroll
     for (int i = 0; i < W::TM; ++i) {
       const int row = row0 + 32 * i + lrow;
       T* o = out + (size_t)row * g.ldo + f0;
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[j][i][v] *= factor;
-      if (vec) {
-        if constexpr (sizeof(T) == 2) {
-          uint2 q[4];
+      if (whole && sizeof(T) == 2) {
+        uint2 q[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            q[k] = pack4_bf16(acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]);
-          store_group32(o, q, lhalf, row < g.M);
-        } else if (row < g.M) {
+        for (int k = 0; k < 4; ++k)
+          q[k] = pack4_bf16(acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]);
+        store_group32(reinterpret_cast<bf16_t*>(o), q, lhalf, row < g.M);
+      } else if (row < g.M) {   // (a row is a multiple of 8 columns: quads are whole)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<float4*>(o + 8 * k + 4 * lhalf) =
+        for (int k = 0; k < 4; ++k) {
+          const int f = 8 * k + 4 * lhalf;
+          if (f0 + f >= g.Nf) continue;
+          if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint2*>(o + f) =
+                pack4_bf16(acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]);
+          else
+            *reinterpret_cast<float4*>(o + f) =
                 make_float4(acc[j][i][4 * k], acc[j][i][4 * k + 1], acc[j][i][4 * k + 2], acc[j][i][4 * k + 3]);
         }
-      } else if (row < g.M) {
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// Accumulators of A . B^T: register v of a tile holds row 8 (v / 4) + 4 h + v % 4, column
+// lane % 32.
+template <typename T, typename W>
+__device__ __forceinline__ void emit_store_odd(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow,
+                                               int lhalf) {
+  T* out = reinterpret_cast<T*>(g.out);
+  const float factor = uniform_load(g.factor);
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int f = 8 * (v / 4) + 4 * lhalf + v % 4;
-          if (f0 + f < g.Nf) store_act(o + f, acc[j][i][v]);
-        }
+  for (int j = 0; j < W::TN; ++j) {
+    const int f = fw + 32 * j + lrow;
+#pragma unroll
+    for (int i = 0; i < W::TM; ++i) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int row = row0 + 32 * i + 8 * (v / 4) + 4 * lhalf + v % 4;
+        if (f < g.Nf && row < g.M) store_act(out + (size_t)row * g.ldo + f, acc[j][i][v] * factor);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -445,20 +467,23 @@ __device__ __forceinline__ bool locate_item(const LossArgs& g, int v, Item* it) 
   it->row0 = __builtin_amdgcn_readfirstlane((grp * kGroupM + idx % gsize) * BM);
   it->n0 = __builtin_amdgcn_readfirstlane(idx / gsize * BN);
   it->part = __builtin_amdgcn_readfirstlane(part);
-  // (parts <= 16 and KT < 2^17: no overflow)
+  // (parts <= 128 and KT < 2^17: no overflow)
   it->k0 = __builtin_amdgcn_readfirstlane(part * g.KT / g.parts);
   it->k1 = __builtin_amdgcn_readfirstlane((part + 1) * g.KT / g.parts);
   return true;
 }
 
 // D[m][f] = sum_k A[m][k] B[f][k].  Ring, swizzle and schedule as gemm_ring5_kernel: units
-// A0 B0 A1 B1 .. of consecutive slabs, barrier s frees slab s - 1's two slots for the
-// weights of slab s + 1 and the rows of slab s + 2, whose loads go out in quarters
-// between the matrix instructions.
-template <typename T, int EPI, int BM, int BN, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
+// A0 B0 A1 B1 .. of consecutive slabs in UNITS slots; barrier s frees slab s - 1's two for
+// the columns of slab s + (UNITS - 3) / 2 and the rows of the one after, whose loads go
+// out in quarters between the matrix instructions.  Five slots; nine where a block is
+// alone on its CU anyway, whose slabs are then requested early enough for the memory's
+// latency.
+template <typename T, int EPI, int BM, int BN, int NW, int UNITS>
+__global__ __launch_bounds__(NW * 64, NW == 8 || UNITS == 5 ? 2 : 1) void ring_kernel(LossArgs g) {
   using W = Waves<NW, BM, BN>;
-  constexpr int kTN = W::TN, kTM = W::TM, kUnits = 5, kRow = 128;
+  constexpr int kTN = W::TN, kTM = W::TM, kUnits = UNITS, kRow = 128;
+  static_assert(kUnits % 2 == 1 && kUnits >= 5, "rows one slab further ahead than columns");
   constexpr int kSlot = (BM > BN ? BM : BN) * kRow;
   constexpr int kDA = BM * kRow / 1024 / NW, kDB = BN * kRow / 1024 / NW;   // loads per wave and unit
   __shared__ __attribute__((aligned(1024))) char smem[kUnits * kSlot];
@@ -555,7 +580,7 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
   constexpr int kD = kDA + kDB;
   auto quarter = [&](int q) __attribute__((always_inline)) { issue(q * kD / 4, (q + 1) * kD / 4); };
   auto slab_wait = [&]() __attribute__((always_inline)) {
-    slab_barrier<kDA>();   // all but the rows of the slab after next
+    slab_barrier<(kUnits - 3) / 2 * kDA + (kUnits - 5) / 2 * kDB>();   // all but the slabs after the next one's columns
     take_b();
     take_a();
   };
@@ -565,7 +590,7 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
   const char* w_base = smem + (wn * W::WTN + lrow) * kRow;
   // bf16: the fragments of a k-step (16 columns), a 16-byte vector a lane; fp32: of two (8
   // vectors of 4 columns in the slab), which together contract 16 columns.
-  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr bool kF32 = sizeof(T) == 4, kRowsFirst = EPI == kStoreOdd;
   constexpr int kSteps = kF32 ? 2 : 4, kVec = kF32 ? 2 : 1;
   typedef std::conditional_t<kF32, f32x4, bf16x8> F;
   F xf[2][kTM][kVec], wf[2][kTN][kVec];
@@ -585,10 +610,13 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
 
   take_a();
   issue(kDB, kD);
-  take_b();
-  issue(0, kDB);
-  take_a();
-  issue(kDB, kD);
+#pragma unroll
+  for (int u = 1; u < kUnits - 2; u += 2) {
+    take_b();
+    issue(0, kDB);
+    take_a();
+    issue(kDB, kD);
+  }
   slab_wait();
   quarter(0);
   frags(0, 0, xf[0], wf[0]);
@@ -630,13 +658,15 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
           for (int i = 0; i < kTM; ++i) {
             const Split sx = split(xs[i][0], xs[i][1]);
 #pragma unroll
-            for (int j = 0; j < kTN; ++j) acc[j][i] = contract(sw[j], sx, acc[j][i]);
+            for (int j = 0; j < kTN; ++j)
+              acc[j][i] = kRowsFirst ? contract(sx, sw[j], acc[j][i]) : contract(sw[j], sx, acc[j][i]);
           }
         } else {
 #pragma unroll
           for (int j = 0; j < kTN; ++j)
 #pragma unroll
-            for (int i = 0; i < kTM; ++i) acc[j][i] = contract(ws[j][0], xs[i][0], acc[j][i]);
+            for (int i = 0; i < kTM; ++i)
+              acc[j][i] = kRowsFirst ? contract(xs[i][0], ws[j][0], acc[j][i]) : contract(ws[j][0], xs[i][0], acc[j][i]);
           constexpr int kReads = kTM + kTN, kMfma = kTN * kTM;
           constexpr int kPairs = kReads < kMfma ? kReads : kMfma;
 #pragma unroll
@@ -661,8 +691,10 @@ __global__ __launch_bounds__(NW * 64, 2) void ring_kernel(LossArgs g) {
       emit_dlogit<T, W, EPI == kDLogitSum>(g, acc, row0, fw, lr, lh, cur.row0 / BM * W::WM + wm);
     else if constexpr (EPI == kPart)
       emit_part<W>(g, acc, cur.part, row0, fw, lr, lh);
-    else
+    else if constexpr (EPI == kStore)
       emit_store<T, W>(g, acc, row0, fw, lr, lh);
+    else
+      emit_store_odd<T, W>(g, acc, row0, fw, lr, lh);
     t += G;
     if (!locate_item<BM, BN>(g, t, &cur)) break;
   }
@@ -689,33 +721,35 @@ __device__ __forceinline__ S wave_total(S v) {
   return v;
 }
 
-constexpr int kJoinTokens = 16;
 struct JoinSum {
   double loss;
   int count, pad;
 };
 
-// 16 tokens a block, 64 threads each.  mean[0]: the mean over the rows with a target, 0 if
+// TOK tokens a block, SLICES threads each (64 where few rows or many columns leave much to
+// add up per row, 4 where not).  mean[0]: the mean over the rows with a target, 0 if
 // there is none; mean[1]: their number; the last block to end adds the blocks' sums up,
 // in their order.
-__global__ __launch_bounds__(1024) void join_kernel(const float2* __restrict__ part, int P, int ld, int N, int V,
+template <int TOK, int SLICES>
+__global__ __launch_bounds__(TOK * SLICES) void join_kernel(const float2* __restrict__ part, int P, int ld, int N, int V,
                                                     const float* __restrict__ picked,
                                                     const int32_t* __restrict__ targets, float* __restrict__ loss,
                                                     float* __restrict__ lse, float* __restrict__ mean,
                                                     JoinSum* __restrict__ sums, int* counter) {
-  __shared__ float2 red[64][kJoinTokens + 1];
-  __shared__ JoinSum total[16];
+  constexpr int kThreads = TOK * SLICES;
+  __shared__ float2 red[SLICES][TOK + 1];
+  __shared__ JoinSum total[kThreads / kWave];
   __shared__ bool last;
-  const int tok = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens, n = blockIdx.x * kJoinTokens + tok;
+  const int tok = threadIdx.x % TOK, slice = threadIdx.x / TOK, n = blockIdx.x * TOK + tok;
   float m = -INFINITY, s = 0.0f;
   bool nan = false;
   if (n < N) {
     constexpr int kAhead = 4;   // loads in flight
-    for (int p0 = slice; p0 < P; p0 += 64 * kAhead) {
+    for (int p0 = slice; p0 < P; p0 += SLICES * kAhead) {
       float2 v[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        v[u] = p0 + 64 * u < P ? part[(size_t)(p0 + 64 * u) * ld + n] : make_float2(-INFINITY, 0.0f);
+        v[u] = p0 + SLICES * u < P ? part[(size_t)(p0 + SLICES * u) * ld + n] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         nan |= v[u].y != v[u].y;   // (the maximum passes over NaN)
@@ -726,7 +760,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const float2* __restrict__ p
   }
   red[slice][tok] = make_float2(m, s);
   __syncthreads();
-  for (int d = 32; d >= 1; d >>= 1) {
+  for (int d = SLICES / 2; d >= 1; d >>= 1) {
     if (slice < d) {
       const float2 o = red[slice + d][tok];
       float2 v = red[slice][tok];
@@ -737,7 +771,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const float2* __restrict__ p
     }
     __syncthreads();
   }
-  if (threadIdx.x < kWave) {   // (the first 16 lanes have a token)
+  if (threadIdx.x < kWave) {   // (the first TOK lanes have a token)
     float l = 0.0f;
     bool has = false;
     if (slice == 0 && n < N) {
@@ -764,7 +798,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const float2* __restrict__ p
   if (!last) return;
   __threadfence();
   JoinSum a = {0.0, 0, 0};
-  for (int b = threadIdx.x; b < (int)gridDim.x; b += 1024) {
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += kThreads) {
     a.loss += sums[b].loss;
     a.count += sums[b].count;
   }
@@ -773,7 +807,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const float2* __restrict__ p
   if (lane_id() == 0) total[threadIdx.x / kWave] = a;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; ++i) {
+    for (int i = 1; i < kThreads / kWave; ++i) {
       a.loss += total[i].loss;
       a.count += total[i].count;
     }
@@ -803,6 +837,49 @@ struct PrepareArgs {
     int rows, cols, ld, blocks, vec;
   } t[2];
 };
+
+// The kV elements p[0 .. kV - 1] of a row, those from the n-th on as zeros, for a row that
+// starts anywhere: by dwords where all that they hold is the row's own.
+template <typename T>
+__device__ __forceinline__ uint4 load_odd(const T* p, int n, bool before) {
+  constexpr int kV = 16 / (int)sizeof(T);
+  struct __attribute__((packed, aligned(4))) Words {
+    uint32_t w[4];
+  };
+  if (((uintptr_t)p & 3) == 0 && n >= kV) {
+    const Words d = *reinterpret_cast<const Words*>(p);
+    return make_uint4(d.w[0], d.w[1], d.w[2], d.w[3]);
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (before && n > kV) {   // (an odd row: the elements from -1 to kV, shifted)
+      const Words d = *reinterpret_cast<const Words*>(p - 1);
+      const uint32_t last = *reinterpret_cast<const uint32_t*>(p + 7);
+      return make_uint4(__builtin_amdgcn_alignbyte(d.w[1], d.w[0], 2), __builtin_amdgcn_alignbyte(d.w[2], d.w[1], 2),
+                        __builtin_amdgcn_alignbyte(d.w[3], d.w[2], 2), __builtin_amdgcn_alignbyte(last, d.w[3], 2));
+    }
+  }
+  T v[kV];
+#pragma unroll
+  for (int q = 0; q < kV; ++q) v[q] = q < n ? p[q] : T(0);
+  uint4 u;
+  __builtin_memcpy(&u, v, 16);
+  return u;
+}
+
+// dst [rows][ld] = src [rows][cols], zeros past a row; ld a multiple of a 16-byte vector.
+template <typename T>
+__global__ __launch_bounds__(256) void pad_kernel(const T* __restrict__ src, int rows, int cols,
+                                                  T* __restrict__ dst, int ld) {
+  constexpr int kV = 16 / (int)sizeof(T);
+  const int per = ld / kV;
+  const size_t total = (size_t)rows * per;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+    const size_t r = i / per;
+    const int c = (int)(i % per) * kV;
+    const uint4 u = c < cols ? load_odd(src + r * cols + c, cols - c, c > 0) : make_uint4(0u, 0u, 0u, 0u);
+    *reinterpret_cast<uint4*>(dst + i * kV) = u;
+  }
+}
 
 template <typename T>
 __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs<T> a) {
@@ -859,14 +936,12 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs<T> a) {
       in = target >= 0 && target < a.V;
     }
     const T* p = t.src + (size_t)(r0 + r) * t.cols + c0 + c;
-    if (t.vec) {   // (cols % kV == 0: a vector is within the row or past it)
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (in && c0 + c < t.cols) v = *reinterpret_cast<const uint4*>(p);
-      *reinterpret_cast<uint4*>(&tile[r][c]) = v;
-    } else {
-#pragma unroll
-      for (int q = 0; q < kV; ++q) tile[r][c + q] = in && c0 + c + q < t.cols ? p[q] : T(0);
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (in && c0 + c < t.cols) {
+      if (t.vec) v = *reinterpret_cast<const uint4*>(p);   // (a vector is within the row or past it)
+      else v = load_odd(p, t.cols - c0 - c, c0 + c > 0);
     }
+    *reinterpret_cast<uint4*>(&tile[r][c]) = v;
   }
   __syncthreads();
   // (ld is a multiple of 64: every tile's columns of dst exist)
@@ -939,7 +1014,7 @@ size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 int div_up(int a, int b) { return (a + b - 1) / b; }
 
 // Tile size and parts of a product of M rows, Nf columns, KT slabs: the least of the
-// estimated times over the sizes and, where the contraction may be split, 1 .. 16 parts of
+// estimated times over the sizes and, where the contraction may be split, 1 .. 128 parts of
 // at least 8 slabs.  A CU takes ceil(items / CUs) items one after the other (the
 // smaller tiles two at a time, at the same rate); a part costs its fp32 sums' way to memory and
 // back and a launch.  Rates: the large tile's, 1250 TFLOP/s in bf16 and 180 in fp32 over
@@ -962,7 +1037,7 @@ GemmPlan plan_gemm(int M, int Nf, int KT, bool split, TileSize most, int cus) {
     const double reach = tile == kLarge ? 1.0 : tile == kMid ? 0.82 : 0.6;
     const long tiles = (long)div_up(M, tile_rows(tile)) * div_up(Nf, tile_cols(tile));
     const double one = 2.0 * tile_rows(tile) * tile_cols(tile) * KT * (128 / sizeof(T)) / (rate * reach);
-    for (int p = 1; p <= (split ? std::max(1, std::min(16, KT / 8)) : 1); ++p) {
+    for (int p = 1; p <= (split ? std::max(1, std::min(128, KT / 8)) : 1); ++p) {
       const long rounds = (tiles * p + cus - 1) / cus;
       double us = (double)rounds * one / p;
       if (rounds == 1 && tile != kLarge) us *= 1.35;   // a block alone does not cover its waits
@@ -988,17 +1063,26 @@ hipError_t launch_ring(LossArgs g, const GemmPlan& p, int cus, hipStream_t st) {
   auto go = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, g);
   };
+  const bool alone = items <= cus;
   if (p.tile == kSmall) {
-    go(ring_kernel<T, EPI, 64, 128, 4>, 256);
+    if (alone) go(ring_kernel<T, EPI, 64, 128, 4, 9>, 256);
+    else go(ring_kernel<T, EPI, 64, 128, 4, 5>, 256);
   } else if (p.tile == kMid) {
-    go(ring_kernel<T, EPI, 128, 128, 4>, 256);
+    if (alone) go(ring_kernel<T, EPI, 128, 128, 4, 9>, 256);
+    else go(ring_kernel<T, EPI, 128, 128, 4, 5>, 256);
   } else {
     if constexpr (!(sizeof(T) == 4 && (EPI == kDLogit || EPI == kDLogitSum)))
-      go(ring_kernel<T, EPI, 256, 256, 8>, 512);
+      go(ring_kernel<T, EPI, 256, 256, 8, 5>, 512);
     else
       return hipErrorInvalidValue;   // (its epilogue beside the split operands spills registers)
   }
   return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_store(const LossArgs& g, const GemmPlan& p, int cus, hipStream_t st) {
+  const bool vec = g.Nf % 8 == 0 && ((uintptr_t)g.out & 15) == 0;
+  return vec ? launch_ring<T, kStore>(g, p, cus, st) : launch_ring<T, kStoreOdd>(g, p, cus, st);
 }
 
 // The type's elements per 128-byte slab.
@@ -1032,7 +1116,7 @@ LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
     l.ld_lse = (int)align_up((size_t)N, 64);
     l.part_lse = take((size_t)div_up(V, 64) * l.ld_lse * sizeof(float2));
     l.picked = take((size_t)N * 4);
-    l.sums = take((size_t)div_up(N, kJoinTokens) * sizeof(JoinSum));
+    l.sums = take((size_t)div_up(N, 16) * sizeof(JoinSum));
     l.counter = take(4);
     l.xpad = take(pad ? (size_t)N * kp * sizeof(T) : 0);
     l.wpad = take(pad ? (size_t)V * kp * sizeof(T) : 0);
@@ -1072,14 +1156,22 @@ bool needs_pad(int C, const void* x, const void* W) {
 }
 
 template <typename T>
+hipError_t launch_pad(const T* src, int rows, int cols, T* dst, int ld, hipStream_t st) {
+  const size_t blocks = ((size_t)rows * (ld / (16 / sizeof(T))) + 255) / 256;
+  hipLaunchKernelGGL(pad_kernel<T>, dim3((unsigned)std::min<size_t>(blocks, 1 << 16)), dim3(256), 0, st, src, rows,
+                     cols, dst, ld);
+  return hipGetLastError();
+}
+
+template <typename T>
 hipError_t forward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W, const float* bias,
                         const int32_t* targets, int N, float* loss, float* lse, float* mean, char* ws, bool pad,
                         const LossLayout& l, int cus, hipStream_t st) {
   const int C = cfg->embed_dim, V = cfg->vocab_size, kp = (int)align_up((size_t)C, kSlab<T>);
   hipError_t e;
   if (pad) {
-    if ((e = launch_copy_cols<T>(x, C, (T*)(ws + l.xpad), kp, N, C, kp, st)) != hipSuccess) return e;
-    if ((e = launch_copy_cols<T>(W, C, (T*)(ws + l.wpad), kp, V, C, kp, st)) != hipSuccess) return e;
+    if ((e = launch_pad<T>(x, N, C, (T*)(ws + l.xpad), kp, st)) != hipSuccess) return e;
+    if ((e = launch_pad<T>(W, V, C, (T*)(ws + l.wpad), kp, st)) != hipSuccess) return e;
     x = (const T*)(ws + l.xpad);
     W = (const T*)(ws + l.wpad);
   }
@@ -1097,8 +1189,12 @@ hipError_t forward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W, 
   g.picked = (float*)(ws + l.picked);
   g.counter = (int*)(ws + l.counter);
   if ((e = launch_ring<T, kLse>(g, plan_gemm<T>(N, V, g.KT, false, kLarge, cus), cus, st)) != hipSuccess) return e;
-  hipLaunchKernelGGL(join_kernel, dim3(div_up(N, kJoinTokens)), dim3(1024), 0, st, g.part_lse, div_up(V, 64),
-                     l.ld_lse, N, V, g.picked, targets, loss, lse, mean, (JoinSum*)(ws + l.sums), g.counter);
+  auto join = [&](auto kernel, int tokens, int threads) {
+    hipLaunchKernelGGL(kernel, dim3(div_up(N, tokens)), dim3(threads), 0, st, g.part_lse, div_up(V, 64), l.ld_lse, N,
+                       V, g.picked, targets, loss, lse, mean, (JoinSum*)(ws + l.sums), g.counter);
+  };
+  if (N >= 4096 && V <= 64 * 64) join(join_kernel<64, 4>, 64, 256);
+  else join(join_kernel<16, 64>, 16, 1024);
   return hipGetLastError();
 }
 
@@ -1123,7 +1219,7 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
   float *scale = (float*)(ws + l.scale), *factor = (float*)(ws + l.factor);
   const T* xk = x;
   if (pad) {
-    if ((e = launch_copy_cols<T>(x, C, (T*)(ws + l.xpad), kp, N, C, kp, st)) != hipSuccess) return e;
+    if ((e = launch_pad<T>(x, N, C, (T*)(ws + l.xpad), kp, st)) != hipSuccess) return e;
     xk = (const T*)(ws + l.xpad);
   }
   T *xt = (T*)(ws + l.xt), *wt = (T*)(ws + l.wt);
@@ -1158,7 +1254,7 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
     const T* wp = W + (size_t)v0 * C;
     const T* wk = wp;
     if (pad) {
-      if ((e = launch_copy_cols<T>(wp, C, (T*)(ws + l.wpad), kp, vn, C, kp, st)) != hipSuccess) return e;
+      if ((e = launch_pad<T>(wp, vn, C, (T*)(ws + l.wpad), kp, st)) != hipSuccess) return e;
       wk = (const T*)(ws + l.wpad);
     }
     LossArgs g{};
@@ -1199,12 +1295,11 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
       p.out = l.dx_part ? ws + l.dxp : (char*)dx;
       p.ldo = l.dx_part ? l.ldx : C;
       p.add = i > 0;
-      p.vec = C % 8 == 0 && ((uintptr_t)dx & 15) == 0;
       GemmPlan plan = l.dx;
       if (l.dx_part)
         e = launch_ring<T, kPart>(p, plan, cus, st);
       else
-        e = launch_ring<T, kStore>(p, plan, cus, st);
+        e = launch_store<T>(p, plan, cus, st);
       if (e != hipSuccess) return e;
     }
     if (dW) {
@@ -1220,12 +1315,11 @@ hipError_t backward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W,
       T* out = dW + (size_t)v0 * C;
       p.out = l.dw.parts > 1 ? ws + l.dwp : (char*)out;
       p.ldo = l.dw.parts > 1 ? l.ldx : C;
-      p.vec = C % 8 == 0 && ((uintptr_t)out & 15) == 0;
       if (l.dw.parts > 1) {
         if ((e = launch_ring<T, kPart>(p, l.dw, cus, st)) != hipSuccess) return e;
         e = reduce_parts<T>((const float*)(ws + l.dwp), l.dw.parts, vn, C, l.ldx, factor, out, st);
       } else {
-        e = launch_ring<T, kStore>(p, l.dw, cus, st);
+        e = launch_store<T>(p, l.dw, cus, st);
       }
       if (e != hipSuccess) return e;
     }

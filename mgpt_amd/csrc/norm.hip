@@ -72,8 +72,14 @@ __device__ __forceinline__ float stream_sum(float v, float (*red)[16], int w, in
   return v;
 }
 
-// 8 columns c .. c + 7 of a row of C; vec: the row is 16-byte aligned and C a multiple
-// of 8.  Columns past the row are zeros and not written.
+// A lane's 8 columns of a row of C, from c on: neighbours where the row is 16-byte aligned
+// and C a multiple of 8 (vec), else every 64th, so that a wave's are neighbours.  Columns
+// past the row are zeros and not written.
+__device__ __forceinline__ int first_column(int wave, int lane, bool vec) {
+  return vec ? (wave * kWave + lane) * 8 : wave * 512 + lane;
+}
+__device__ __forceinline__ int column(int c, int q, bool vec) { return c + (vec ? q : q * kWave); }
+
 template <typename T>
 __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int C, bool vec, float (&o)[8]) {
   if (vec) {
@@ -96,7 +102,7 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int c, int C, b
     }
   } else {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) o[q] = c + q < C ? to_f32(row[c + q]) : 0.0f;
+    for (int q = 0; q < 8; ++q) o[q] = c + q * kWave < C ? to_f32(row[c + q * kWave]) : 0.0f;
   }
 }
 
@@ -125,7 +131,7 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int c, int C, bool v
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
-      if (c + q < C) store_act(row + c + q, o[q]);
+      if (c + q * kWave < C) store_act(row + c + q * kWave, o[q]);
   }
 }
 
@@ -164,7 +170,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64) void norm_forward_kernel(
   __shared__ float red[2][16];
   constexpr int S = W <= 4 ? 4 / W : 1;   // streams of a block
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), lane = lane_id();
-  const int col = ((w % W) * kWave + lane) * 8;   // vector v: columns col + v W 512 ..
+  const int col = first_column(w % W, lane, a.vec);   // vector v: from col + v W 512 on
   float post[NV][8], gate[NV][8], pre[NV][8];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -237,9 +243,9 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64) void norm_forward_kernel(
 // Column sums of a block's streams added in stream order, written by the first.
 template <int W, int NV>
 __device__ __forceinline__ void block_columns(const float (&acc)[NV][8], float* lds, int w, int lane, int C,
-                                              float* __restrict__ dst) {
+                                              bool vec, float* __restrict__ dst) {
   constexpr int S = W <= 4 ? 4 / W : 1;
-  const int col = ((w % W) * kWave + lane) * 8, s = w / W;
+  const int col = first_column(w % W, lane, vec), s = w / W;
   float t[NV][8];
 #pragma unroll
   for (int v = 0; v < NV; ++v)
@@ -268,7 +274,7 @@ __device__ __forceinline__ void block_columns(const float (&acc)[NV][8], float* 
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const int c = col + v * W * 512 + q;
+        const int c = column(col + v * W * 512, q, vec);
         if (c < C) dst[c] = t[v][q];
       }
   }
@@ -285,7 +291,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64) void norm_backward_kernel(
   __shared__ float red[2][16];
   __shared__ float lds[S > 1 ? S * W * kWave * NV * 8 : 1];
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), lane = lane_id();
-  const int col = ((w % W) * kWave + lane) * 8, s = w / W;
+  const int col = first_column(w % W, lane, a.vec), s = w / W;
   const int R = a.N / a.G;
   const float inv = 1.0f / (float)a.C;
   float post[NV][8], gate[NV][8], pre[NV][8], t_acc[NV][8], pre_acc[NV][8];
@@ -373,7 +379,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64) void norm_backward_kernel(
     const int r1 = g * R + min(R, part * a.chunk + a.span);
     load_gate(g);
     for (int r0 = g * R + part * a.chunk; r0 < r1; r0 += a.step) do_row(min(r0 + s, r1 - 1), r0 + s < r1);
-    block_columns<W, NV>(t_acc, lds, w, lane, a.C, sum_part + (size_t)blockIdx.x * a.C);
+    block_columns<W, NV>(t_acc, lds, w, lane, a.C, a.vec, sum_part + (size_t)blockIdx.x * a.C);
   } else {
     float post_acc[NV][8];
 #pragma unroll
@@ -390,15 +396,15 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64) void norm_backward_kernel(
       for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const int c = col + v * W * 512 + q;
+          const int c = column(col + v * W * 512, q, a.vec);
           if (dgate && live && c < a.C) dgate[(size_t)g * a.C + c] = t_acc[v][q] * post[v][q];
           post_acc[v][q] += t_acc[v][q] * gate[v][q];
           t_acc[v][q] = 0.0f;
         }
     }
-    block_columns<W, NV>(post_acc, lds, w, lane, a.C, sum_part + (size_t)blockIdx.x * a.C);
+    block_columns<W, NV>(post_acc, lds, w, lane, a.C, a.vec, sum_part + (size_t)blockIdx.x * a.C);
   }
-  if (a.pre) block_columns<W, NV>(pre_acc, lds, w, lane, a.C, pre_part + (size_t)blockIdx.x * a.C);
+  if (a.pre) block_columns<W, NV>(pre_acc, lds, w, lane, a.C, a.vec, pre_part + (size_t)blockIdx.x * a.C);
 }
 
 // Sums rows r0 .. r1 - 1 of src [.][C] at 64 columns by 16 waves, in a fixed order; the
