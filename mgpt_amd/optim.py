@@ -8,6 +8,7 @@ tensors a MoELayer loads, with the gradients of MoELayer.get_gradients().
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import operator
 
@@ -19,6 +20,16 @@ _GRAD = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16}
 _dtype = operator.attrgetter("dtype")
 _numel, _is_contiguous = torch.Tensor.numel, torch.Tensor.is_contiguous
 _get_device, _data_ptr = torch.Tensor.get_device, torch.Tensor.data_ptr
+
+
+def _addresses(tensors, some):
+    """The tensors' addresses, 0 for None, as the C ABI takes them; some: those
+    that are not None."""
+    ptrs = list(map(_data_ptr, some))
+    if len(some) != len(tensors):
+        at = iter(ptrs)
+        ptrs = [0 if t is None else next(at) for t in tensors]
+    return array.array("Q", ptrs)
 
 
 class AdamW:
@@ -91,14 +102,9 @@ class AdamW:
             raise ValueError("gradients must be contiguous and have their parameters' sizes")
         if not set(map(_get_device, some)) <= {self.device.index}:
             raise ValueError(f"gradients must be CUDA tensors on {self.device}")
-        ptrs = list(map(_data_ptr, some))
-        if len(some) != n:
-            at = iter(ptrs)
-            ptrs = [None if g is None else next(at) for g in grads]
-        array = ctypes.c_void_p * n
-        copies = None
+        gp, pp, cp = _addresses(grads, some), _addresses(self.params, self.params), None
         if self.copies is not None:
-            copies = array(*[None if c is None else c.data_ptr() for c in self.copies])
+            cp = _addresses(self.copies, [c for c in self.copies if c is not None])
         scale = None
         if grad_scale is not None:
             self._check(grad_scale, torch.float32, 1, "grad_scale")
@@ -112,7 +118,7 @@ class AdamW:
                 self._step_device.add_(1)
                 at = self._step_device.data_ptr()
             capi.check(capi.lib().mgpt_adamw_step(
-                ctypes.byref(cfg), n, self._sizes, array(*map(_data_ptr, self.params)), array(*ptrs), copies,
-                self.state.data_ptr(), self.state.numel(), number, at, scale,
-                torch.cuda.current_stream().cuda_stream))
+                ctypes.byref(cfg), n, self._sizes, pp.buffer_info()[0], gp.buffer_info()[0],
+                None if cp is None else cp.buffer_info()[0], self.state.data_ptr(), self.state.numel(), number, at,
+                scale, torch.cuda.current_stream().cuda_stream))
         self.step_count = number
