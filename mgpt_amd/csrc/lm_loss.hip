@@ -962,26 +962,26 @@ template <typename T>
 __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ part, int parts, int M, int C, size_t ld,
                                                      const float* __restrict__ factor, T* __restrict__ out, int vec) {
   const int quads = (C + 3) / 4;
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (size_t)M * quads) return;
-  const size_t m = i / quads;
-  const int c = (int)(i % quads) * 4;
-  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int p = 0; p < parts; ++p) {
-    const float4 v = *reinterpret_cast<const float4*>(part + ((size_t)p * M + m) * ld + c);
-    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-  }
   const float f = *factor;
-  s.x *= f; s.y *= f; s.z *= f; s.w *= f;
-  T* o = out + m * C + c;
-  if (vec) {
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(o) = s;
-    else *reinterpret_cast<uint2*>(o) = pack4_bf16(s.x, s.y, s.z, s.w);
-  } else {
-    const float v[4] = {s.x, s.y, s.z, s.w};
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)M * quads; i += (size_t)gridDim.x * 256) {
+    const size_t m = i / quads;
+    const int c = (int)(i % quads) * 4;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = 0; p < parts; ++p) {
+      const float4 v = *reinterpret_cast<const float4*>(part + ((size_t)p * M + m) * ld + c);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    s.x *= f; s.y *= f; s.z *= f; s.w *= f;
+    T* o = out + m * C + c;
+    if (vec) {
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(o) = s;
+      else *reinterpret_cast<uint2*>(o) = pack4_bf16(s.x, s.y, s.z, s.w);
+    } else {
+      const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (c + q < C) store_act(o + q, v[q]);
+      for (int q = 0; q < 4; ++q)
+        if (c + q < C) store_act(o + q, v[q]);
+    }
   }
 }
 
@@ -1203,9 +1203,8 @@ hipError_t reduce_parts(const float* part, int parts, int M, int C, int ld, cons
                         hipStream_t st) {
   const size_t n = (size_t)M * ((C + 3) / 4);
   const int vec = C % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0;
-  if ((n + 255) / 256 > 0xFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(reduce_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, parts, M, C,
-                     (size_t)ld, factor, out, vec);
+  hipLaunchKernelGGL(reduce_kernel<T>, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, st,
+                     part, parts, M, C, (size_t)ld, factor, out, vec);
   return hipGetLastError();
 }
 

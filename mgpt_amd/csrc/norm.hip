@@ -541,6 +541,7 @@ hipError_t for_layout(int W, int NV, F&& f) {
 int check_norm(const mgpt_norm_config* cfg, int N, bool gated) {
   if (!cfg) return fail(MGPT_ERR_INVALID_ARGUMENT, "config is null");
   if (N < 0) return fail(MGPT_ERR_INVALID_ARGUMENT, "negative num_tokens");
+  if (N > 1 << 30) return fail(MGPT_ERR_UNSUPPORTED, "num_tokens %d > 2^30", N);
   if (cfg->embed_dim <= 0) return fail(MGPT_ERR_INVALID_ARGUMENT, "embed_dim %d", cfg->embed_dim);
   if (cfg->embed_dim > kMaxC)
     return fail(MGPT_ERR_UNSUPPORTED, "embed_dim %d > %d", cfg->embed_dim, kMaxC);

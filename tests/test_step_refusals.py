@@ -101,6 +101,7 @@ def test_norm_refuses_arguments():
     cfg = capi.NormConfig(64, 0, 4, 1e-5, 1.0)
     refused(norm_forward(None), INV)
     refused(norm_forward(cfg, n=-4), INV)
+    refused(norm_forward(cfg, n=(1 << 30) + 4), UNS)
     for k in ("x", "h", "out", "y", "rh", "ro"):
         refused(norm_forward(cfg, **{k: None}), INV)
     for k in ("x", "h", "dy", "dx", "dh", "rh", "ro", "ws"):
