@@ -17,8 +17,9 @@
 //
 // What bounds it: memory; forward x, h in, o, y out, backward x, h, dout, dy in, dx, dh
 // out.  A row stays in the registers of its W waves (8 columns a lane and vector, NV
-// vectors), so that everything is read once; the gains sit in registers across a
-// stream's rows.  A stream is W waves that take rows in turn.  Column sums are kept per
+// vectors), so that everything is read once; the gains sit in registers (or LDS) across
+// a stream's rows.  A stream is W waves that take rows in turn.  MI355X: forward 16384 x
+// 1024 bf16 22 us (134 MB, 6.1 TB/s), 32768 x 2048 92 us (537 MB, 5.8 TB/s).  Column sums are kept per
 // lane over a stream's rows, added over a block's streams through LDS, and over the blocks
 // by norm_reduce_kernel, in a fixed order: the same call gives the same bits.
 // All arithmetic is fp32; out, y, dx and dh are rounded once.
@@ -407,6 +408,140 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64) void norm_backward_kernel(
   if (a.pre) block_columns<W, NV>(pre_acc, lds, w, lane, a.C, a.vec, pre_part + (size_t)blockIdx.x * a.C);
 }
 
+// 8 columns as they are in memory: a row that is requested while another is worked on.
+template <typename T> struct Raw;
+template <> struct Raw<bf16_t> { uint4 u; };
+template <> struct Raw<float> { float4 a, b; };
+__device__ __forceinline__ void widen(const Raw<float>& r, float (&o)[8]) {
+  o[0] = r.a.x; o[1] = r.a.y; o[2] = r.a.z; o[3] = r.a.w;
+  o[4] = r.b.x; o[5] = r.b.y; o[6] = r.b.z; o[7] = r.b.w;
+}
+__device__ __forceinline__ void widen(const Raw<bf16_t>& r, float (&o)[8]) {
+  const uint32_t wv[4] = {r.u.x, r.u.y, r.u.z, r.u.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    o[2 * q] = __uint_as_float(wv[q] << 16);
+    o[2 * q + 1] = __uint_as_float(wv[q] & 0xFFFF0000u);
+  }
+}
+
+// norm_backward_kernel for the case that training has: both norms and dout there, rows of
+// 16-byte vectors up to 512 W columns, groups split over blocks.  Nothing in a row's
+// course depends on what is there, so that the compiler can count loads and stores: a
+// row's stores need not have ended for the next row's values, which were requested
+// before them, to be used (memory operations of a wave end in order).  The gains are in
+// LDS, which leaves the registers to that second row.  A stream without a row of its own
+// in a turn repeats the group's last one, whose results it stores once more, and adds
+// nothing to the column sums.
+// MI355X, us against norm_backward_kernel: 16384 x 1024 bf16 41.6 -> 36.4, 32768 x 2048 190
+// -> 175 (805 MB, 4.6 TB/s), 20000 x 512 23.4 -> 22.3; 4096 x 4096 fp32 75 -> 78, 8000 x 8192
+// 187 -> 190.  Memory bounds it: without the sums over a row it takes as long, without one of
+// the two stores 30 us less at 32768 x 2048, without two of the four loads 60.
+template <typename T, int W, bool ONCE>
+__global__ __launch_bounds__(W <= 4 ? 256 : W * 64, 4) void norm_backward_full_kernel(
+    NormArgs a, const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ dout,
+    const T* __restrict__ dy, T* __restrict__ dx, T* __restrict__ dh, float* __restrict__ sum_part,
+    float* __restrict__ pre_part) {
+  constexpr int S = W <= 4 ? 4 / W : 1;
+  __shared__ float red[2][16];
+  __shared__ float lds[S > 1 ? S * W * kWave * 8 : 1];
+  __shared__ __attribute__((aligned(16))) float gains[3][W * 512];
+  const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), lane = lane_id();
+  const int col = first_column(w % W, lane, true), s = w / W;
+  const int R = a.N / a.G, g = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  const float inv = 1.0f / (float)a.C;
+  for (int c = threadIdx.x; c < W * 512; c += blockDim.x) {
+    const bool in = c < a.C;
+    gains[0][c] = in ? a.post[c] : 0.0f;
+    gains[1][c] = in ? a.pre[c] : 0.0f;
+    gains[2][c] = !in ? 0.0f : a.gate ? a.gate[(size_t)g * a.C + c] : 1.0f;
+  }
+  __syncthreads();
+  auto gain = [&](int k, float (&o)[8]) __attribute__((always_inline)) {
+    const float4* p = reinterpret_cast<const float4*>(&gains[k][col]);
+    const float4 u = p[0], v = p[1];
+    o[0] = u.x; o[1] = u.y; o[2] = u.z; o[3] = u.w;
+    o[4] = v.x; o[5] = v.y; o[6] = v.z; o[7] = v.w;
+  };
+  // (lanes past the row read its first columns, against gains of 0, and store nothing)
+  const bool in_row = col < a.C;
+  const int from = in_row ? col : 0;
+  Raw<T> nx, nh, nd, ny;
+  float nrh, nro;
+  auto request = [&](int row) __attribute__((always_inline)) {
+    const size_t at = (size_t)row * a.C + from;
+    nx = *reinterpret_cast<const Raw<T>*>(x + at);
+    nh = *reinterpret_cast<const Raw<T>*>(h + at);
+    nd = *reinterpret_cast<const Raw<T>*>(dout + at);
+    ny = *reinterpret_cast<const Raw<T>*>(dy + at);
+    nrh = a.rh[row];
+    nro = a.ro[row];
+  };
+  float t_acc[8], pre_acc[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) t_acc[q] = pre_acc[q] = 0.0f;
+  const int r1 = g * R + min(R, part * a.chunk + a.span);
+  int r0 = g * R + part * a.chunk;
+  request(min(r0 + s, r1 - 1));
+  for (; r0 < r1; r0 += a.step) {
+    const int row = min(r0 + s, r1 - 1);
+    const float live = r0 + s < r1 ? 1.0f : 0.0f;
+    float o[8], n[8], d[8], z[8];
+    widen(nx, o);
+    widen(nh, n);
+    widen(nd, d);
+    widen(ny, z);
+    const float rh = nrh, ro = nro;
+    request(min(r0 + a.step + s, r1 - 1));
+    float s1 = 0.0f;
+    {
+      float post[8], gate[8], pre[8];
+      gain(0, post);
+      gain(2, gate);
+      gain(1, pre);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        n[q] *= rh;
+        o[q] = __builtin_fmaf(a.scale, o[q], gate[q] * (n[q] * post[q])) * ro;
+        const float k = z[q] * pre[q];
+        s1 = __builtin_fmaf(k, o[q], s1);
+        pre_acc[q] = __builtin_fmaf(z[q] * live, o[q], pre_acc[q]);
+        z[q] = k;
+      }
+    }
+    s1 = stream_sum<W>(s1, red, w, 0) * inv;
+    float s2 = 0.0f;
+    {
+      float post[8], gate[8];
+      gain(0, post);
+      gain(2, gate);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        d[q] = __builtin_fmaf(ro, __builtin_fmaf(-o[q], s1, z[q]), d[q]);
+        t_acc[q] = __builtin_fmaf(d[q] * live, n[q], t_acc[q]);
+        z[q] = d[q] * gate[q] * post[q];
+        s2 = __builtin_fmaf(z[q], n[q], s2);
+        d[q] *= a.scale;
+      }
+    }
+    s2 = stream_sum<W>(s2, red, w, 1) * inv;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) z[q] = rh * __builtin_fmaf(-n[q], s2, z[q]);
+    if (in_row) {
+      store8(dx + (size_t)row * a.C, col, a.C, true, d, ONCE);
+      store8(dh + (size_t)row * a.C, col, a.C, true, z, ONCE);
+    }
+  }
+  float t[1][8], p[1][8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    t[0][q] = t_acc[q];
+    p[0][q] = pre_acc[q];
+  }
+  block_columns<W, 1>(t, lds, w, lane, a.C, true, sum_part + (size_t)blockIdx.x * a.C);
+  block_columns<W, 1>(p, lds, w, lane, a.C, true, pre_part + (size_t)blockIdx.x * a.C);
+}
+
 // Sums rows r0 .. r1 - 1 of src [.][C] at 64 columns by 16 waves, in a fixed order; the
 // first wave has them.
 __device__ __forceinline__ float column_sum(const float* __restrict__ src, int r0, int r1, int C, int c,
@@ -473,7 +608,8 @@ int compute_units() {
 
 // Waves and vectors of a row.  Forward: 1024 columns a wave, whose gains then serve more
 // of a row (16384 x 1024: 22.4 us, with 512 24.5; 32768 x 2048: 95 / 110).  Backward: 512,
-// for twice the waves on a CU (below).
+// for twice the waves on a CU (norm_backward_kernel, us with 1024 / 512: 16384 x 1024 53 /
+// 44, 32768 x 2048 259 / 199).
 void row_layout(int C, bool backward, int* W, int* NV) {
   *NV = C <= (backward ? 8192 : 512) ? 1 : 2;
   int w = 1;
@@ -481,20 +617,22 @@ void row_layout(int C, bool backward, int* W, int* NV) {
   *W = w;
 }
 
-NormPlan plan_backward(int N, int C, int G) {
+NormPlan plan_backward(int N, int C, int G, bool full) {
   NormPlan p{};
   row_layout(C, true, &p.W, &p.NV);
   const int S = p.W <= 4 ? 4 / p.W : 1, R = N / G;
-  // enough blocks for the chip, few enough that their column sums cost little
-  const int target = p.W <= 4 ? 1024 : 256;
+  // Enough blocks for the chip, few enough that their column sums cost little; half as many
+  // where a wave has two rows in flight (us with 512 / 1024 blocks: 16384 x 1024 36.4 /
+  // 41.8, 32768 x 2048 175 / 185; norm_backward_kernel, one row in flight, 59 / 44).
+  const int target = p.W > 4 ? 256 : full ? 512 : 1024;
   if (R < 8 || G >= target * S) {
     const int per = (G + target - 1) / target;
     p.per_block = (per + S - 1) / S * S;
     p.blocks = (G + p.per_block - 1) / p.per_block;
   } else {
     // A block's own run of rows, or rows in turn with the group's other blocks, whose rows in
-    // flight then are neighbours (us, run / in turn: 20000 x 512 23.8 / 25.3, 32768 x 2048
-    // 198 / 191, 8000 x 8192 206 / 189).
+    // flight then are neighbours (us of norm_backward_kernel, run / in turn: 20000 x 512 23.8 /
+    // 25.3, 32768 x 2048 198 / 191, 8000 x 8192 206 / 189).
     p.parts = std::max(1, std::min((target + G - 1) / G, (R + S - 1) / S));
     if (p.W == 1) {
       p.chunk = p.span = ((R + p.parts - 1) / p.parts + S - 1) / S * S;
@@ -614,8 +752,9 @@ int mgpt_norm_backward_workspace_bytes(const mgpt_norm_config* cfg, int num_toke
   if (num_tokens == 0) return MGPT_OK;
   // with and without a gate (whose rows decide the blocks)
   const int C = cfg->embed_dim, G = num_tokens % cfg->gate_rows == 0 ? cfg->gate_rows : 1;
-  *bytes = std::max(norm_layout(plan_backward(num_tokens, C, G), C, G).total,
-                    norm_layout(plan_backward(num_tokens, C, 1), C, 1).total);
+  for (const int g : {G, 1})
+    for (const bool full : {false, true})
+      *bytes = std::max(*bytes, norm_layout(plan_backward(num_tokens, C, g, full), C, g).total);
   return MGPT_OK;
 }
 
@@ -643,7 +782,8 @@ int mgpt_norm_backward(const mgpt_norm_config* cfg, const void* x, const void* h
   NormArgs a = norm_args(cfg, num_tokens, gamma_post, gate, gamma_pre, const_cast<float*>(rstd_post),
                          const_cast<float*>(rstd_pre),
                          {x, h, dout, gamma_pre ? dy : nullptr, dx, dh, gamma_post, gate, gamma_pre});
-  const NormPlan p = plan_backward(a.N, C, a.G);
+  const bool all = a.vec && a.post && a.pre && dout && C <= 8192;   // what norm_backward_full_kernel takes
+  const NormPlan p = plan_backward(a.N, C, a.G, all);
   const NormLayout l = norm_layout(p, C, a.G);
   if (workspace_bytes < l.total)
     return fail(MGPT_ERR_WORKSPACE_TOO_SMALL, "workspace needs %zu bytes, got %zu", l.total, workspace_bytes);
@@ -667,6 +807,17 @@ int mgpt_norm_backward(const mgpt_norm_config* cfg, const void* x, const void* h
         hipLaunchKernelGGL(kernel, dim3(p.blocks), dim3(kW <= 4 ? 256 : kW * 64), 0, st, a, (const T*)x,
                            (const T*)h, (const T*)dout, (const T*)dy, (T*)dx, (T*)dh, dgate, sums, pres);
       };
+      if constexpr (kNV == 1) {
+        if (p.parts > 0 && all) {
+          auto full = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(p.blocks), dim3(kW <= 4 ? 256 : kW * 64), 0, st, a, (const T*)x,
+                               (const T*)h, (const T*)dout, (const T*)dy, (T*)dx, (T*)dh, sums, pres);
+          };
+          if (a.once) full(norm_backward_full_kernel<T, kW, true>);
+          else full(norm_backward_full_kernel<T, kW, false>);
+          return;
+        }
+      }
       if (p.parts > 0) launch(norm_backward_kernel<T, kW, kNV, false>);
       else launch(norm_backward_kernel<T, kW, kNV, true>);
     });
