@@ -18,15 +18,21 @@
 //
 // All four products are one kernel (ring_kernel): a persistent block per CU walks 256 x
 // 256 tiles, operands go HBM -> LDS by untracked 1 KB loads into a ring of 5 units (an
-// operand's 128-byte slabs of a tile), 8 waves of 64 columns x 128 rows run D = B . A^T
-// by v_mfma_f32_32x32x16_bf16 or, for fp32, v_mfma_f32_32x32x2_f32 on the same 16-byte
-// fragments (gemm_dma.hip describes the ring and its measurements).  Rows past an
-// operand's last re-read the last, so that nothing behind a caller's tensor is
-// touched.  Few tiles take 64 x 128 ones, two blocks of 4 waves a CU, and products of
-// few tiles (dx, dW) split their contraction, the parts added in order.
+// operand's 128-byte slabs of a tile), 8 waves of 64 columns x 128 rows run D = B . A^T by
+// v_mfma_f32_32x32x16_bf16 (gemm_dma.hip describes the ring and its measurements); fp32
+// operands are split in registers into three bf16 numbers (Split).  Rows past an operand's
+// last re-read the last, so that nothing behind a caller's tensor is touched.  Few tiles
+// take 128 x 128 or 64 x 128 ones, two blocks of 4 waves a CU, and products of few tiles
+// (dx, dW) split their contraction, the parts added in order (plan_gemm).
 //
 // What bounds it: the matrix rate, 2 N C V operations forward and 6 N C V backward (a
 // third of them to form the logits again), except for few rows, where reading W does.
+// MI355X, kernel times: 16384 x 1024 x 32000 bf16 (1.07 T operations a product): logits
+// forward 939 us, again with d's epilogue 1275, dx 842, dW 822 (1140, 840, 1275, 1305
+// TFLOP/s; a library product of 8192^3 1373).  The logits' epilogues are what those lack:
+// an exponential per logit on the vector unit, and for d 2 GB of stores, which a wave's
+// next loads wait behind.  64 rows x 2048 x 50257: 33 us (206 MB, 6.1 TB/s from the
+// last-level cache).
 // Logits, sums and their logarithms are fp32.  With bf16 inputs d is rounded to bf16, as
 // the operand of two bf16 products; db is summed from d before that.
 #include <algorithm>
@@ -80,11 +86,13 @@ struct LossArgs {
   const float* factor;   // kStore, kStoreOdd: of the product
 };
 
-// fp32 operands as three bf16 numbers each, x = h + m + l exactly (8 of its 24 bits each,
-// rounded to nearest): six of the nine products keep all but 2^-24 of the whole, at 16
-// contracted columns an instruction of v_mfma_f32_32x32x16_bf16 for two of
-// v_mfma_f32_32x32x2_f32, of the same length.  (An infinity, or a magnitude above bf16's
-// largest, splits into NaN.)
+// fp32 operands as three bf16 numbers each, x = h + m + l exactly (rounded to nearest, 8 of
+// its 24 bits each): six of the nine products keep all but some 2^-24 of the factors'
+// magnitudes.  Six v_mfma_f32_32x32x16_bf16 of 32 cycles contract 16 columns, where
+// v_mfma_f32_32x32x2_f32 takes eight of 64; the splitting, 5.5 vector instructions a value,
+// then runs beside them (999 x 500 x 8003: products of 73 to 143 us became 57 to 67; the
+// error against 64 bits fell from 5.7e-7 to 2.7e-7).  An infinity, or a magnitude above
+// bf16's largest, splits into NaN.
 struct Split {
   bf16x8 h, m, l;
 };
@@ -726,8 +734,8 @@ struct JoinSum {
   int count, pad;
 };
 
-// TOK tokens a block, SLICES threads each (64 where few rows or many columns leave much to
-// add up per row, 4 where not).  mean[0]: the mean over the rows with a target, 0 if
+// TOK tokens a block, SLICES threads each: 64, or 4 where many rows have little to add up
+// (13895 rows of 282 columns 26 us with 64; 64 rows of 50257 columns 9 with 64 or 256).  mean[0]: the mean over the rows with a target, 0 if
 // there is none; mean[1]: their number; the last block to end adds the blocks' sums up,
 // in their order.
 template <int TOK, int SLICES>
