@@ -168,10 +168,10 @@ __device__ __forceinline__ float half_sum(float v) {
 __device__ __forceinline__ uint2 transpose4(uint2 u, int lane) {
   const uint32_t p0 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, 0xB1, 0xf, 0xf, false);   // lane ^ 1
   const uint32_t p1 = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, 0xB1, 0xf, 0xf, false);
-  const bool odd = lane & 1, upper = lane & 2;
-  const uint32_t sel = odd ? 0x07060302u : 0x05040100u;
-  const uint32_t a0 = __builtin_amdgcn_perm(odd ? u.x : p0, odd ? p0 : u.x, sel);
-  const uint32_t a1 = __builtin_amdgcn_perm(odd ? u.y : p1, odd ? p1 : u.y, sel);
+  // even lanes: both lanes' first feature of the pair; odd ones: their second
+  const uint32_t sel = lane & 1 ? 0x07060302u : 0x01000504u;
+  const uint32_t a0 = __builtin_amdgcn_perm(u.x, p0, sel), a1 = __builtin_amdgcn_perm(u.y, p1, sel);
+  const bool upper = lane & 2;
   const uint32_t r = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(upper ? a0 : a1), 0x4E, 0xf, 0xf, false);   // lane ^ 2
   return upper ? make_uint2(r, a1) : make_uint2(a0, r);
 }
@@ -293,8 +293,15 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
     huge |= !(fabsf(lse[i]) < kHuge);
   }
   const bool slow = __ballot(huge) != 0;
-  T* dm = reinterpret_cast<T*>(g.d);
-  T* dt = reinterpret_cast<T*>(g.dt);
+  // (uniform addresses and a lane's 32-bit offsets: a tile's rows are within 4 GB, as
+  // launch_ring checks)
+  const uint32_t d_off = ((uint32_t)lrow * (uint32_t)g.ldd + 4 * lhalf) * (uint32_t)sizeof(T);
+  uint32_t t_off[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    t_off[k] = sizeof(T) == 2
+                   ? ((uint32_t)(8 * k + 4 * lhalf + (lrow & 3)) * (uint32_t)g.lddt + (uint32_t)(lrow & ~3)) * 2
+                   : ((uint32_t)(8 * k + 4 * lhalf) * (uint32_t)g.lddt + (uint32_t)lrow) * 4;
 #pragma unroll
   for (int j = 0; j < W::TN; ++j) {
     const int f0 = fw + 32 * j;
@@ -326,30 +333,32 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
 #pragma unroll
         for (int v = 0; v < 16; ++v) cs[v] += d[v];
       }
+      char* dm = g.d + ((size_t)(row0 + 32 * i) * g.ldd + f0) * sizeof(T);
+      char* dt = g.dt + ((size_t)f0 * g.lddt + (row0 + 32 * i)) * sizeof(T);
       if constexpr (sizeof(T) == 2) {
         uint2 q[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) q[k] = pack4_bf16(d[4 * k], d[4 * k + 1], d[4 * k + 2], d[4 * k + 3]);
-        store_group32(dm + (size_t)row * g.ldd + f0, q, lhalf, row < g.M);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint2 u = transpose4(q[k], lrow);
-          const int f = f0 + 8 * k + 4 * lhalf + (lrow & 3), r4 = row & ~3;
+        store_group32(reinterpret_cast<bf16_t*>(dm + (d_off - 8 * lhalf)), q, lhalf, row < g.M);
+        if ((row & ~3) < g.rows_t) {
           // (past the caches: 695 -> 637 us at 16384 x 1024 x 16128, where both write 256 KB a
           // tile; d's own stores too: 685)
-          if (r4 < g.rows_t) store_once(reinterpret_cast<uint2*>(dt + (size_t)f * g.lddt + r4), u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) store_once(reinterpret_cast<uint2*>(dt + t_off[k]), transpose4(q[k], lrow));
         }
       } else {
+        if (row < g.M) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int f = f0 + 8 * k + 4 * lhalf;
-          if (row < g.M)
-            *reinterpret_cast<float4*>(dm + (size_t)row * g.ldd + f) =
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4*>(dm + d_off + 32 * k) =
                 make_float4(d[4 * k], d[4 * k + 1], d[4 * k + 2], d[4 * k + 3]);
-          if (row < g.rows_t) {
+        }
+        if (row < g.rows_t) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) dt[(size_t)(f + q) * g.lddt + row] = d[4 * k + q];
-          }
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<float*>(dt + (size_t)q * g.lddt * 4 + t_off[k]) = d[4 * k + q];
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -1065,7 +1074,9 @@ hipError_t launch_ring(LossArgs g, const GemmPlan& p, int cus, hipStream_t st) {
   g.mt = div_up(g.M, tile_rows(p.tile));
   g.nt = div_up(g.Nf, tile_cols(p.tile));
   const long items = (long)g.mt * g.nt * g.parts;
-  if (items > 0x3FFFFFFF || g.lda * 256 > 0xFFFFFFFFu || g.ldb * 256 > 0xFFFFFFFFu) return hipErrorInvalidValue;
+  if (items > 0x3FFFFFFF || std::max(g.lda, g.ldb) * 256 > 0xFFFFFFFFu ||
+      std::max(g.ldd, g.lddt) * 32 * sizeof(T) > 0xFFFFFFFFu)
+    return hipErrorInvalidValue;
   const int grid =
       (int)std::min<long>((items + kNumXcd - 1) / kNumXcd * kNumXcd, p.tile == kLarge ? cus : 2 * cus);
   auto go = [&](auto kernel, int threads) {
