@@ -409,15 +409,17 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64) void norm_backward_kernel(
 }
 
 // 8 columns as they are in memory: a row that is requested while another is worked on.
+// widen: as fp32, or zeros.
 template <typename T> struct Raw;
 template <> struct Raw<bf16_t> { uint4 u; };
 template <> struct Raw<float> { float4 a, b; };
-__device__ __forceinline__ void widen(const Raw<float>& r, float (&o)[8]) {
-  o[0] = r.a.x; o[1] = r.a.y; o[2] = r.a.z; o[3] = r.a.w;
-  o[4] = r.b.x; o[5] = r.b.y; o[6] = r.b.z; o[7] = r.b.w;
+__device__ __forceinline__ void widen(const Raw<float>& r, bool in, float (&o)[8]) {
+  const float v[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+  for (int q = 0; q < 8; ++q) o[q] = in ? v[q] : 0.0f;
 }
-__device__ __forceinline__ void widen(const Raw<bf16_t>& r, float (&o)[8]) {
-  const uint32_t wv[4] = {r.u.x, r.u.y, r.u.z, r.u.w};
+__device__ __forceinline__ void widen(const Raw<bf16_t>& r, bool in, float (&o)[8]) {
+  const uint32_t wv[4] = {in ? r.u.x : 0u, in ? r.u.y : 0u, in ? r.u.z : 0u, in ? r.u.w : 0u};
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     o[2 * q] = __uint_as_float(wv[q] << 16);
@@ -463,7 +465,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64, 4) void norm_backward_full_k
     o[0] = u.x; o[1] = u.y; o[2] = u.z; o[3] = u.w;
     o[4] = v.x; o[5] = v.y; o[6] = v.z; o[7] = v.w;
   };
-  // (lanes past the row read its first columns, against gains of 0, and store nothing)
+  // (lanes past the row read its first columns, take them as zeros, and store nothing)
   const bool in_row = col < a.C;
   const int from = in_row ? col : 0;
   Raw<T> nx, nh, nd, ny;
@@ -485,12 +487,12 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64, 4) void norm_backward_full_k
   request(min(r0 + s, r1 - 1));
   for (; r0 < r1; r0 += a.step) {
     const int row = min(r0 + s, r1 - 1);
-    const float live = r0 + s < r1 ? 1.0f : 0.0f;
+    const bool live = r0 + s < r1;
     float o[8], n[8], d[8], z[8];
-    widen(nx, o);
-    widen(nh, n);
-    widen(nd, d);
-    widen(ny, z);
+    widen(nx, in_row, o);
+    widen(nh, in_row, n);
+    widen(nd, in_row, d);
+    widen(ny, in_row, z);
     const float rh = nrh, ro = nro;
     request(min(r0 + a.step + s, r1 - 1));
     float s1 = 0.0f;
@@ -505,7 +507,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64, 4) void norm_backward_full_k
         o[q] = __builtin_fmaf(a.scale, o[q], gate[q] * (n[q] * post[q])) * ro;
         const float k = z[q] * pre[q];
         s1 = __builtin_fmaf(k, o[q], s1);
-        pre_acc[q] = __builtin_fmaf(z[q] * live, o[q], pre_acc[q]);
+        pre_acc[q] = live ? __builtin_fmaf(z[q], o[q], pre_acc[q]) : pre_acc[q];
         z[q] = k;
       }
     }
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : W * 64, 4) void norm_backward_full_k
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         d[q] = __builtin_fmaf(ro, __builtin_fmaf(-o[q], s1, z[q]), d[q]);
-        t_acc[q] = __builtin_fmaf(d[q] * live, n[q], t_acc[q]);
+        t_acc[q] = live ? __builtin_fmaf(d[q], n[q], t_acc[q]) : t_acc[q];
         z[q] = d[q] * gate[q] * post[q];
         s2 = __builtin_fmaf(z[q], n[q], s2);
         d[q] *= a.scale;

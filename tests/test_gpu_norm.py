@@ -203,3 +203,23 @@ def test_no_tokens():
     dx, dh, *gr = op.backward(e, e, e, e, rh, ro, **g)
     assert out.shape == (0, 32) and dx.shape == (0, 32)
     assert all((t == 0).all() for t in gr)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("N,C,G", [(9, 72, 1), (13, 1032, 1), (66, 520, 2)])
+def test_an_infinity_stays_where_the_formulas_put_it(N, C, G, act):
+    """An infinite dy in a group's last row: dgamma_pre is infinite in its column
+    alone, dx of the row infinite (NaN in that column: inf - inf) and every other
+    row's results are those without it."""
+    rows, gains = inputs(N, C, G, act)
+    clean = run(rows, gains, G, 0.7, ALL, act)
+    rows["dy"][N - 1, 3] = float("inf")
+    got = run(rows, gains, G, 0.7, ALL, act)
+    last = torch.arange(N) == N - 1
+    for k in ("dx", "dh"):
+        assert torch.equal(got[k].reshape(N, C).cpu()[~last], clean[k].reshape(N, C).cpu()[~last]), k
+    column = torch.arange(C) == 3
+    dpre = got["dpre"].cpu().flatten()
+    assert dpre[3].isinf() and torch.equal(dpre[~column], clean["dpre"].cpu().flatten()[~column])
+    dx = got["dx"].reshape(N, C).cpu()[N - 1]
+    assert dx[3].isnan() and dx[~column].isinf().all()
