@@ -33,9 +33,9 @@ def _addresses(tensors, some):
 
 
 class AdamW:
-    """params: contiguous float32 CUDA tensors of one device.  copies: None, or
-    per parameter a bfloat16 tensor of its size (or None) that every step
-    refreshes.  state_bits: 32 or 8.  device_step: keep the step's number on
+    """params: contiguous float32 CUDA tensors of one device, which keep their
+    memory.  copies: None, or per parameter a bfloat16 tensor of its size (or
+    None) that every step refreshes.  state_bits: 32 or 8.  device_step: keep the step's number on
     the device, so that a step captured into a HIP graph counts on when it is
     replayed (step_count then stays where it was)."""
 
@@ -58,6 +58,10 @@ class AdamW:
         spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written if t.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("params and copies must not overlap")
+        # aliases: as long as a parameter is still at its address, the memory there is
+        # the one that was checked, whatever has been assigned to its .data since
+        self._held = [t.detach() for t in written]
+        self._at = self._written()
         self.step_count = 0
         n = len(self.params)
         self._numels = [p.numel() for p in self.params]
@@ -83,6 +87,13 @@ class AdamW:
         if t.numel() != numel or not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous with {numel} elements")
 
+    def _written(self):
+        """The addresses of the parameters and of their copies (None: no copies)."""
+        if self.copies is None:
+            return _addresses(self.params, self.params), None
+        return (_addresses(self.params, self.params),
+                _addresses(self.copies, [c for c in self.copies if c is not None]))
+
     def step(self, grads, grad_scale: torch.Tensor | None = None) -> None:
         """One step from `grads`: per parameter a contiguous tensor of its size,
         all float32 or all bfloat16, or None (the parameter and its moments
@@ -102,9 +113,9 @@ class AdamW:
             raise ValueError("gradients must be contiguous and have their parameters' sizes")
         if not set(map(_get_device, some)) <= {self.device.index}:
             raise ValueError(f"gradients must be CUDA tensors on {self.device}")
-        gp, pp, cp = _addresses(grads, some), _addresses(self.params, self.params), None
-        if self.copies is not None:
-            cp = _addresses(self.copies, [c for c in self.copies if c is not None])
+        if self._written() != self._at:
+            raise ValueError("a parameter or a copy no longer has the memory it was given with")
+        gp, (pp, cp) = _addresses(grads, some), self._at
         scale = None
         if grad_scale is not None:
             self._check(grad_scale, torch.float32, 1, "grad_scale")
@@ -117,8 +128,11 @@ class AdamW:
             if self._step_device is not None:
                 self._step_device.add_(1)
                 at = self._step_device.data_ptr()
-            capi.check(capi.lib().mgpt_adamw_step(
+            status = capi.lib().mgpt_adamw_step(
                 ctypes.byref(cfg), n, self._sizes, pp.buffer_info()[0], gp.buffer_info()[0],
                 None if cp is None else cp.buffer_info()[0], self.state.data_ptr(), self.state.numel(), number, at,
-                scale, torch.cuda.current_stream().cuda_stream))
+                scale, torch.cuda.current_stream().cuda_stream)
+            if status != capi.MGPT_OK and at is not None:
+                self._step_device.sub_(1)   # a refused step is none
+            capi.check(status)
         self.step_count = number

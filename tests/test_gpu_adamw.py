@@ -318,3 +318,37 @@ def test_captured_step_counts_on(bits):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(p, ref) and torch.equal(a.state, b.state)
+
+
+def test_parameters_keep_their_memory():
+    """Memory assigned to a parameter later may have any size, type or device:
+    refused, and nothing is written."""
+    p = torch.nn.Parameter(torch.ones(600, device="cuda"), requires_grad=False)
+    c = torch.zeros(600, dtype=torch.bfloat16, device="cuda")
+    opt = make([p], copies=[c])
+    g = torch.ones(600, device="cuda")
+    opt.step([g])
+    was, held = p.data, p.clone()
+    for other in (p.data.clone(), p.data.bfloat16(), p.data[1:], p.data.cpu()):
+        p.data = other
+        with pytest.raises(ValueError, match="memory"):
+            opt.step([g])
+    p.data = was
+    assert torch.equal(p, held) and opt.step_count == 1
+    opt.step([g])
+    assert not torch.equal(p, held) and torch.equal(c, p.bfloat16())
+
+
+def test_a_refused_step_is_not_counted():
+    from mgpt_amd.capi import MoEError
+    p = torch.ones(300, device="cuda")
+    ref = p.clone()
+    a, b = make([ref]), make([p], device_step=True)
+    g = torch.ones(300, device="cuda")
+    lr, b.lr = b.lr, float("nan")
+    with pytest.raises(MoEError):
+        b.step([g])
+    b.lr = lr
+    a.step([g])
+    b.step([g])
+    assert torch.equal(p, ref) and b.step_count == 1
