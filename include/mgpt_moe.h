@@ -402,8 +402,8 @@ int mgpt_adamw_state_bytes(int num_tensors, const int64_t* sizes, int state_bits
 /* params[i]: fp32, updated in place; grads[i]: grad_dtype, read; copies (may
  * be null, or hold nulls): bf16 copies of the updated params.  All device
  * memory, aligned to their elements (16-byte aligned ones are faster) and
- * without overlaps, while the arrays of pointers and sizes are host memory, read during the call.  A
- * tensor whose grads[i] is null is left as it is, its moments too.  step: 1
+ * without overlaps; the arrays of pointers and sizes are host memory, read
+ * during the call.  A tensor whose grads[i] is null is left as it is, its moments too.  step: 1
  * for the first; if step_device is not null the device reads the number
  * there instead (a captured step that is replayed; below 1 counts as 1).
  * grad_scale: device float, or null for 1 (a clip coefficient). */

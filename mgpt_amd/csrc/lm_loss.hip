@@ -744,9 +744,9 @@ struct JoinSum {
 };
 
 // TOK tokens a block, SLICES threads each: 64, or 4 where many rows have little to add up
-// (13895 rows of 282 columns 26 us with 64; 64 rows of 50257 columns 9 with 64 or 256).  mean[0]: the mean over the rows with a target, 0 if
-// there is none; mean[1]: their number; the last block to end adds the blocks' sums up,
-// in their order.
+// (13895 rows of 282 columns 26 us with 64; 64 rows of 50257 columns 9 with 64 or 256).
+// mean[0]: the mean over the rows with a target, 0 if there is none; mean[1]: their
+// number; the last block to end adds the blocks' sums up, in their order.
 template <int TOK, int SLICES>
 __global__ __launch_bounds__(TOK * SLICES) void join_kernel(const float2* __restrict__ part, int P, int ld, int N, int V,
                                                     const float* __restrict__ picked,
