@@ -22,8 +22,8 @@
 // v_mfma_f32_32x32x16_bf16 (gemm_dma.hip describes the ring and its measurements); fp32
 // operands are split in registers into three bf16 numbers (Split).  Rows past an operand's
 // last re-read the last, so that nothing behind a caller's tensor is touched.  Few tiles
-// take 128 x 128 or 64 x 128 ones, two blocks of 4 waves a CU, and products of few tiles
-// (dx, dW) split their contraction, the parts added in order (plan_gemm).
+// take 128 x 128 or 64 x 128 ones, two blocks of 4 waves a CU, or 64 x 64 ones, and products
+// of few tiles (dx, dW) split their contraction, the parts added in order (plan_gemm).
 //
 // What bounds it: the matrix rate, 2 N C V operations forward and 6 N C V backward (a
 // third of them to form the logits again), except for few rows, where reading W does.
@@ -70,7 +70,7 @@ struct LossArgs {
   const float* bias;
   const int32_t* targets;
   int target0;           // the piece's first column
-  float2* part_lse;      // [Nf / 64][ld_lse]
+  float2* part_lse;      // [columns of a wave][ld_lse]
   int ld_lse;
   float* picked;         // [M]
   int* counter;          // set to 0 for join_kernel's blocks
@@ -262,8 +262,8 @@ __device__ __forceinline__ void emit_lse(const LossArgs& g, Acc<W>& acc, int row
         for (int v = 0; v < 16; ++v) s += exp_less(acc[j][i][v], top, ntop, false);
     }
     s = other_half_sum(s);
-    if (live && lhalf == 0) g.part_lse[(size_t)(fw / 64) * g.ld_lse + row] = make_float2(m, s);
-    const int fl = t >= fw && t < min(fw + 64, g.Nf) ? t - fw : -1;
+    if (live && lhalf == 0) g.part_lse[(size_t)(fw / W::WTN) * g.ld_lse + row] = make_float2(m, s);
+    const int fl = t >= fw && t < min(fw + W::WTN, g.Nf) ? t - fw : -1;
     const bool mine = fl >= 0 && ((fl >> 2) & 1) == lhalf;
     if (__ballot(mine)) {
       float z = 0.0f;
@@ -282,7 +282,7 @@ template <typename T, typename W, bool SUM>
 __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow, int lhalf,
                                             int sum_row) {
   float lse[W::TM], sc[W::TM];
-  int tl[W::TM];   // the target's column in the wave's 64
+  int tl[W::TM];   // the target's column in the wave's
   bool huge = false;
 #pragma unroll
   for (int i = 0; i < W::TM; ++i) {
@@ -743,8 +743,8 @@ struct JoinSum {
   int count, pad;
 };
 
-// TOK tokens a block, SLICES threads each: 64, or 4 where many rows have little to add up
-// (13895 rows of 282 columns 26 us with 64; 64 rows of 50257 columns 9 with 64 or 256).
+// TOK tokens a block, SLICES threads each: 64, or 4 where a row has up to 64 sums to add up
+// (us, 64 / 4: 1024 rows of 8 sums 8.5 / 5.2; 64 rows of 50257 columns 9 with 64 or 256).
 // mean[0]: the mean over the rows with a target, 0 if there is none; mean[1]: their
 // number; the last block to end adds the blocks' sums up, in their order.
 template <int TOK, int SLICES>
@@ -984,6 +984,7 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
     const size_t m = i / quads;
     const int c = (int)(i % quads) * 4;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
     for (int p = 0; p < parts; ++p) {
       const float4 v = *reinterpret_cast<const float4*>(part + ((size_t)p * M + m) * ld + c);
       s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
@@ -1032,14 +1033,18 @@ int div_up(int a, int b) { return (a + b - 1) / b; }
 
 // Tile size and parts of a product of M rows, Nf columns, KT slabs: the least of the
 // estimated times over the sizes and, where the contraction may be split, 1 .. 128 parts of
-// at least 8 slabs.  A CU takes ceil(items / CUs) items one after the other (the
+// at least 4 slabs.  A CU takes ceil(items / CUs) items one after the other (the
 // smaller tiles two at a time, at the same rate); a part costs its fp32 sums' way to memory and
-// back and a launch.  Rates: the large tile's, 1250 TFLOP/s in bf16 and 180 in fp32 over
+// back, all of them a launch.  Rates: the large tile's, 1250 TFLOP/s in bf16 and 180 in fp32 over
 // 256 CUs, times what the smaller ones reach of it (16384 x 1024 x 16128, bf16, dW: 411 /
-// 524 / 769 us; 4096 x 512 x 8000, fp32, forward: 185 / 220 / 294).
-enum TileSize { kSmall, kMid, kLarge };   // 64 x 128, 128 x 128 (two blocks a CU), 256 x 256
+// 524 / 769 us; 4096 x 512 x 8000, fp32, forward: 185 / 220 / 294).  The smallest tile is
+// for products that leave CUs without one, whose waves then do half as much each: 1024 x
+// 128 x 256 fp32, the forward 10.3 us with 64 x 128 tiles, 8.2 with 64 x 64, d 13.2 / 10.3,
+// dx 12.9 / 10.2.
+enum TileSize { kTiny, kSmall, kMid, kLarge };   // 64 x 64, 64 x 128, 128 x 128 (two blocks a CU), 256 x 256
 int tile_rows(TileSize t) { return t == kLarge ? 256 : t == kMid ? 128 : 64; }
-int tile_cols(TileSize t) { return t == kLarge ? 256 : 128; }
+int tile_cols(TileSize t) { return t == kLarge ? 256 : t == kTiny ? 64 : 128; }
+int wave_cols(TileSize t) { return t == kTiny ? 32 : 64; }
 struct GemmPlan {
   TileSize tile;
   int parts;
@@ -1049,16 +1054,17 @@ GemmPlan plan_gemm(int M, int Nf, int KT, bool split, TileSize most, int cus) {
   const double rate = (sizeof(T) == 2 ? 1250e6 : 180e6) / 256;   // operations a us and CU
   GemmPlan best{kSmall, 1};
   double least = 1e300;
-  for (int t = kSmall; t <= most; ++t) {
+  for (int t = kTiny; t <= most; ++t) {
     const TileSize tile = (TileSize)t;
-    const double reach = tile == kLarge ? 1.0 : tile == kMid ? 0.82 : 0.6;
+    const double reach = tile == kLarge ? 1.0 : tile == kMid ? 0.82 : tile == kSmall ? 0.6 : 0.5;
     const long tiles = (long)div_up(M, tile_rows(tile)) * div_up(Nf, tile_cols(tile));
     const double one = 2.0 * tile_rows(tile) * tile_cols(tile) * KT * (128 / sizeof(T)) / (rate * reach);
-    for (int p = 1; p <= (split ? std::max(1, std::min(128, KT / 8)) : 1); ++p) {
+    for (int p = 1; p <= (split ? std::max(1, std::min(128, KT / 4)) : 1); ++p) {
       const long rounds = (tiles * p + cus - 1) / cus;
+      if (rounds > 1 && tile == kTiny) break;
       double us = (double)rounds * one / p;
       if (rounds == 1 && tile != kLarge) us *= 1.35;   // a block alone does not cover its waits
-      if (p > 1) us += p * (double)M * Nf * 8 / 5e6 + 4;
+      if (p > 1) us += p * ((double)M * Nf * 8 / 5e6 + 0.25) + 4;
       if (us < least) {
         least = us;
         best = {tile, p};
@@ -1083,7 +1089,9 @@ hipError_t launch_ring(LossArgs g, const GemmPlan& p, int cus, hipStream_t st) {
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, g);
   };
   const bool alone = items <= cus;
-  if (p.tile == kSmall) {
+  if (p.tile == kTiny) {
+    go(ring_kernel<T, EPI, 64, 64, 4, 9>, 256);
+  } else if (p.tile == kSmall) {
     if (alone) go(ring_kernel<T, EPI, 64, 128, 4, 9>, 256);
     else go(ring_kernel<T, EPI, 64, 128, 4, 5>, 256);
   } else if (p.tile == kMid) {
@@ -1133,7 +1141,8 @@ LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
   const int kp = (int)align_up((size_t)C, kSlab<T>);
   if (!backward) {
     l.ld_lse = (int)align_up((size_t)N, 64);
-    l.part_lse = take((size_t)div_up(V, 64) * l.ld_lse * sizeof(float2));
+    l.dl = plan_gemm<T>(N, V, kp / kSlab<T>, false, kLarge, cus);
+    l.part_lse = take((size_t)div_up(V, wave_cols(l.dl.tile)) * l.ld_lse * sizeof(float2));
     l.picked = take((size_t)N * 4);
     l.sums = take((size_t)div_up(N, 16) * sizeof(JoinSum));
     l.counter = take(4);
@@ -1151,7 +1160,7 @@ LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
   l.vpad = l.piece;
   l.ldx = (int)align_up((size_t)C, 256);
   l.dl = plan_gemm<T>(N, l.piece, kp / kSlab<T>, false, sizeof(T) == 4 ? kMid : kLarge, cus);
-  l.dx = plan_gemm<T>(N, C, l.piece / kSlab<T>, true, kLarge, cus);
+  l.dx = plan_gemm<T>(N, C, div_up(std::min(V, l.piece), kSlab<T>), true, kLarge, cus);
   l.dw = plan_gemm<T>(std::min(V, l.piece), C, l.nk / kSlab<T>, true, kLarge, cus);
   l.dx_part = l.pieces > 1 || l.dx.parts > 1;
   l.scale = take((size_t)N * 4);
@@ -1207,12 +1216,13 @@ hipError_t forward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W, 
   g.ld_lse = l.ld_lse;
   g.picked = (float*)(ws + l.picked);
   g.counter = (int*)(ws + l.counter);
-  if ((e = launch_ring<T, kLse>(g, plan_gemm<T>(N, V, g.KT, false, kLarge, cus), cus, st)) != hipSuccess) return e;
+  if ((e = launch_ring<T, kLse>(g, l.dl, cus, st)) != hipSuccess) return e;
+  const int P = div_up(V, wave_cols(l.dl.tile));
   auto join = [&](auto kernel, int tokens, int threads) {
-    hipLaunchKernelGGL(kernel, dim3(div_up(N, tokens)), dim3(threads), 0, st, g.part_lse, div_up(V, 64), l.ld_lse, N,
-                       V, g.picked, targets, loss, lse, mean, (JoinSum*)(ws + l.sums), g.counter);
+    hipLaunchKernelGGL(kernel, dim3(div_up(N, tokens)), dim3(threads), 0, st, g.part_lse, P, l.ld_lse, N, V,
+                        g.picked, targets, loss, lse, mean, (JoinSum*)(ws + l.sums), g.counter);
   };
-  if (N >= 4096 && V <= 64 * 64) join(join_kernel<64, 4>, 64, 256);
+  if (P <= 64) join(join_kernel<64, 4>, 64, 256);
   else join(join_kernel<16, 64>, 16, 1024);
   return hipGetLastError();
 }

@@ -124,6 +124,23 @@ def test_large_tiles_and_split_contractions(N, C, V, act):
     check(run(x, W, b, t, act), reference(x, W, b, t))
 
 
+# Shapes of few tiles: every tile size with one tile a CU and with several, the gradients
+# stored whole, by odd rows and in parts.
+TILES = [(1, 8, 34875), (4327, 8, 2), (17916, 8, 2), (69, 8, 43707), (132, 8, 51576), (1, 1496, 1636), (5377, 1496, 3),
+         (1065, 3600, 4), (1, 88, 8874), (1, 136, 53557), (1, 400, 27252), (1, 118, 8818), (2, 1572, 2468),
+         (1, 12, 20526), (1, 131, 56687), (1, 75, 9109), (7, 3673, 1039), (1, 177, 58058), (1, 3280, 1272),
+         (1, 3222, 2031), (1, 3348, 5455), (1, 3589, 11708), (943, 3385, 73), (216, 8, 16491), (17706, 135, 381),
+         (4535, 72, 3396), (4435, 152, 11982), (40, 32, 30), (500, 64, 32)]
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("N,C,V", TILES)
+def test_tile_sizes(N, C, V, act):
+    print(N, C, V, act, flush=True)
+    x, W, b, t = inputs(N, C, V, act, bias=(N + C + V) % 2 == 1)
+    check(run(x, W, b, t, act), reference(x, W, b, t))
+
+
 @pytest.mark.parametrize("N,V,act", [(70000, 4200, "bf16"), (70001, 2100, "f32")])
 def test_several_pieces_of_the_vocabulary(N, V, act):
     """More rows than one piece of the vocabulary has room for: the pieces'
