@@ -152,3 +152,11 @@ def on_device(device):
     one; nothing to enter where it is already."""
     import torch
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def stream(device):
+    """The current stream of `device`, as the C ABI takes it.  (The call that
+    torch.cuda.current_stream ends in: 0.1 us, where making its Stream object
+    takes 2.7.)"""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)

@@ -65,7 +65,7 @@ class LMLoss:
             ws = self._workspace(capi.lib().mgpt_lm_loss_workspace_bytes, n, x.device)
             capi.check(capi.lib().mgpt_lm_loss_forward(
                 ctypes.byref(self._cfg), *ptrs, loss.data_ptr(), lse.data_ptr(), mean.data_ptr(), n, ws.data_ptr(),
-                ws.numel(), torch.cuda.current_stream().cuda_stream))
+                ws.numel(), capi.stream(x.device)))
         return loss, lse, mean
 
     def backward(self, x, weight, targets, lse, bias=None, dloss=None, dmean=None, need=(True, True, True)):
@@ -89,5 +89,5 @@ class LMLoss:
             ws = self._workspace(capi.lib().mgpt_lm_loss_backward_workspace_bytes, n, dev)
             capi.check(capi.lib().mgpt_lm_loss_backward(
                 ctypes.byref(self._cfg), *ptrs, *[None if t is None else t.data_ptr() for t in (dx, dw, db)], n,
-                ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+                ws.data_ptr(), ws.numel(), capi.stream(x.device)))
         return dx, dw, db

@@ -72,7 +72,7 @@ class ResidualNorm:
             capi.check(capi.lib().mgpt_norm_forward(
                 ctypes.byref(cfg), xp, hp, *gains, out.data_ptr(), None if y is None else y.data_ptr(),
                 None if rh is None else rh.data_ptr(), None if ro is None else ro.data_ptr(), n,
-                torch.cuda.current_stream().cuda_stream))
+                capi.stream(x.device)))
         return out, y, rh, ro
 
     def backward(self, x, h, dout, dy, rstd_post, rstd_pre, gamma_post=None, gate=None, gamma_pre=None):
@@ -104,5 +104,5 @@ class ResidualNorm:
             capi.check(capi.lib().mgpt_norm_backward(
                 ctypes.byref(cfg), *ptrs, *gains, *up, dx.data_ptr(), dh.data_ptr(),
                 *[None if g is None else g.data_ptr() for g in grads], n, ws.data_ptr() if need.value else None,
-                need.value, torch.cuda.current_stream().cuda_stream))
+                need.value, capi.stream(x.device)))
         return dx, dh, *grads

@@ -131,7 +131,7 @@ class AdamW:
             status = capi.lib().mgpt_adamw_step(
                 ctypes.byref(cfg), n, self._sizes, pp.buffer_info()[0], gp.buffer_info()[0],
                 None if cp is None else cp.buffer_info()[0], self.state.data_ptr(), self.state.numel(), number, at,
-                scale, torch.cuda.current_stream().cuda_stream)
+                scale, capi.stream(self.device))
             if status != capi.MGPT_OK and at is not None:
                 self._step_device.sub_(1)   # a refused step is none
             capi.check(status)
