@@ -31,8 +31,8 @@
 // forward 939 us, again with d's epilogue 1275, dx 842, dW 822 (1140, 840, 1275, 1305
 // TFLOP/s; a library product of 8192^3 1373).  The logits' epilogues are what those lack:
 // an exponential per logit on the vector unit, and for d 2 GB of stores, which a wave's
-// next loads wait behind.  64 rows x 2048 x 50257: 33 us (206 MB, 6.1 TB/s from the
-// last-level cache).
+// next loads wait behind.  64 rows x 2048 x 50257: 47 us from memory
+// (206 MB, 4.4 TB/s; a library's sum reads 3.8), 33 from the last-level cache (6.1).
 // Logits, sums and their logarithms are fp32.  With bf16 inputs d is rounded to bf16, as
 // the operand of two bf16 products; db is summed from d before that.
 #include <algorithm>
@@ -66,6 +66,7 @@ struct LossArgs {
   size_t lda, ldb;       // bytes; multiples of 16
   int M, Nf, KT;         // rows, columns, 128-byte slabs of the contraction
   int mt, nt, parts;     // tiles; parts of the contraction
+  int turn, once;        // UNITS even: a power of 2 up to a part's slabs, less 1 (see slab_of); B past the caches
   // kLse and kDLogit: bias of the columns (or null), targets counted from column 0
   const float* bias;
   const int32_t* targets;
@@ -131,6 +132,11 @@ __device__ __forceinline__ f32x16 contract(const Split& w, const Split& x, f32x1
 // A 1 KB direct-to-LDS load (see dma16) from a uniform base and a lane's offset.
 __device__ __forceinline__ void dma16_base(const char* base, uint32_t off, uint32_t lds) {
   asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+
+// The same past the caches.
+__device__ __forceinline__ void dma16_once(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("global_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
 
 // A wave-uniform address, in scalar registers.
@@ -490,20 +496,40 @@ __device__ __forceinline__ bool locate_item(const LossArgs& g, int v, Item* it) 
   return true;
 }
 
+// The slab in memory of an item's slab kt, with neighbouring tiles a slab apart.
+template <int BN>
+__device__ __forceinline__ int slab_of(const LossArgs& g, const Item& it, int kt) {
+  const int k = kt + ((it.n0 / BN) & g.turn);
+  return k < it.k1 ? k : k - (it.k1 - it.k0);
+}
+
 // D[m][f] = sum_k A[m][k] B[f][k].  Ring, swizzle and schedule as gemm_ring5_kernel: units
 // A0 B0 A1 B1 .. of consecutive slabs in UNITS slots; barrier s frees slab s - 1's two for
 // the columns of slab s + (UNITS - 3) / 2 and the rows of the one after, whose loads go
 // out in quarters between the matrix instructions.  Five slots; nine where a block is
 // alone on its CU anyway, whose slabs are then requested early enough for the memory's
 // latency.
+//
+// UNITS even: for one row of tiles, where reading B, once, is what takes the time.  Slots of
+// the units' own sizes, so that three slabs fit (six where a block is alone on its CU), and
+// barrier s frees slab s - 1's for both units of slab s + UNITS / 2 - 1.  Neighbouring
+// tiles start a slab apart: in step, all blocks read the same few columns of every row,
+// which memory has on a few of its channels.  B that no cache could hold for its next
+// use is read past them.  W from memory, the forward's us with 5 or 9 units / these: 64 x 2048
+// x 50257 62 / 55, 64 x 4096 x 32000 (262 MB) 68 / 56, 64 x 2048 x 32000 44 / 38; past the caches
+// where they could hold it, 64 x 2048 x 50257 takes 52, but 55 and not 46 from the caches.
 template <typename T, int EPI, int BM, int BN, int NW, int UNITS>
-__global__ __launch_bounds__(NW * 64, NW == 8 || UNITS == 5 ? 2 : 1) void ring_kernel(LossArgs g) {
+__global__ __launch_bounds__(NW * 64, NW == 8 || UNITS <= 6 ? 2 : 1) void ring_kernel(LossArgs g) {
   using W = Waves<NW, BM, BN>;
   constexpr int kTN = W::TN, kTM = W::TM, kUnits = UNITS, kRow = 128;
-  static_assert(kUnits % 2 == 1 && kUnits >= 5, "rows one slab further ahead than columns");
+  constexpr bool kOdd = kUnits % 2 == 1;
+  static_assert(kUnits >= 5, "a slab worked on, the next one on its way");
   constexpr int kSlot = (BM > BN ? BM : BN) * kRow;
   constexpr int kDA = BM * kRow / 1024 / NW, kDB = BN * kRow / 1024 / NW;   // loads per wave and unit
-  __shared__ __attribute__((aligned(1024))) char smem[kUnits * kSlot];
+  auto slot_at = [](int slot) __attribute__((always_inline)) {
+    return kOdd ? slot * kSlot : (slot / 2 * (BM + BN) + (slot & 1) * BM) * kRow;
+  };
+  __shared__ __attribute__((aligned(1024))) char smem[kOdd ? kUnits * kSlot : kUnits / 2 * (BM + BN) * kRow];
 
   const int G = gridDim.x, items = g.mt * g.nt * g.parts;
   int t = blockIdx.x;
@@ -522,7 +548,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || UNITS == 5 ? 2 : 1) void ring_k
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char*)smem;
   const uint32_t lds_a = lds0 + (uint32_t)(w * kDA * 1024), lds_b = lds0 + (uint32_t)(w * kDB * 1024);
 
-  // Cursors of the two operands, the rows' a slab ahead of the columns'.  Past the
+  // Cursors of the two operands (UNITS odd: the rows' a slab ahead of the columns').  Past the
   // block's last slab they stay on it (in bounds, into a slot that is no longer read).
   struct Cursor {
     Item it;
@@ -572,15 +598,15 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || UNITS == 5 ? 2 : 1) void ring_k
   uint32_t da, db;
   auto take_a = [&]() __attribute__((always_inline)) {
     if (fresh_a) enter_a();
-    ua = uniform(a_base + (size_t)ca.kt * kRow);
-    da = lds_a + (uint32_t)(dslot * kSlot);
+    ua = uniform(a_base + (size_t)(kOdd ? ca.kt : slab_of<BN>(g, ca.it, ca.kt)) * kRow);
+    da = lds_a + (uint32_t)slot_at(dslot);
     dslot = dslot + 1 == kUnits ? 0 : dslot + 1;
     fresh_a = advance(ca);
   };
   auto take_b = [&]() __attribute__((always_inline)) {
     if (fresh_b) enter_b();
-    ub = uniform(b_base + (size_t)cb.kt * kRow);
-    db = lds_b + (uint32_t)(dslot * kSlot);
+    ub = uniform(b_base + (size_t)(kOdd ? cb.kt : slab_of<BN>(g, cb.it, cb.kt)) * kRow);
+    db = lds_b + (uint32_t)slot_at(dslot);
     dslot = dslot + 1 == kUnits ? 0 : dslot + 1;
     fresh_b = advance(cb);
   };
@@ -588,7 +614,9 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || UNITS == 5 ? 2 : 1) void ring_k
   auto issue = [&](int d0, int d1) __attribute__((always_inline)) {
 #pragma unroll
     for (int d = d0; d < d1; ++d) {
-      if (d < kDB)
+      if (d < kDB && !kOdd && g.once)
+        dma16_once(ub, b_off[d], db + d * 1024);
+      else if (d < kDB)
         dma16_base(ub, b_off[d], db + d * 1024);
       else
         dma16_base(ua, a_off[d - kDB], da + (d - kDB) * 1024);
@@ -597,9 +625,15 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || UNITS == 5 ? 2 : 1) void ring_k
   constexpr int kD = kDA + kDB;
   auto quarter = [&](int q) __attribute__((always_inline)) { issue(q * kD / 4, (q + 1) * kD / 4); };
   auto slab_wait = [&]() __attribute__((always_inline)) {
-    slab_barrier<(kUnits - 3) / 2 * kDA + (kUnits - 5) / 2 * kDB>();   // all but the slabs after the next one's columns
-    take_b();
-    take_a();
+    if constexpr (kOdd) {
+      slab_barrier<(kUnits - 3) / 2 * kDA + (kUnits - 5) / 2 * kDB>();   // all but the slabs after the next one's columns
+      take_b();
+      take_a();
+    } else {
+      slab_barrier<(kUnits / 2 - 2) * kD>();
+      take_a();
+      take_b();
+    }
   };
 
   const int swz = (lrow >> 1) & 7;
@@ -618,21 +652,30 @@ __global__ __launch_bounds__(NW * 64, NW == 8 || UNITS == 5 ? 2 : 1) void ring_k
       const int cofs = ((((step * kVec + c) * 2 + lhalf) ^ swz) << 4);
 #pragma unroll
       for (int i = 0; i < kTM; ++i)
-        xs[i][c] = *reinterpret_cast<const F*>(x_base + aslot * kSlot + i * 32 * kRow + cofs);
+        xs[i][c] = *reinterpret_cast<const F*>(x_base + slot_at(aslot) + i * 32 * kRow + cofs);
 #pragma unroll
       for (int j = 0; j < kTN; ++j)
-        ws[j][c] = *reinterpret_cast<const F*>(w_base + bslot * kSlot + j * 32 * kRow + cofs);
+        ws[j][c] = *reinterpret_cast<const F*>(w_base + slot_at(bslot) + j * 32 * kRow + cofs);
     }
   };
 
-  take_a();
-  issue(kDB, kD);
-#pragma unroll
-  for (int u = 1; u < kUnits - 2; u += 2) {
-    take_b();
-    issue(0, kDB);
+  if constexpr (kOdd) {
     take_a();
     issue(kDB, kD);
+#pragma unroll
+    for (int u = 1; u < kUnits - 2; u += 2) {
+      take_b();
+      issue(0, kDB);
+      take_a();
+      issue(kDB, kD);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kUnits - 2; u += 2) {
+      take_a();
+      take_b();
+      issue(0, kD);
+    }
   }
   slab_wait();
   quarter(0);
@@ -743,8 +786,9 @@ struct JoinSum {
   int count, pad;
 };
 
-// TOK tokens a block, SLICES threads each: 64, or 4 where a row has up to 64 sums to add up
-// (us, 64 / 4: 1024 rows of 8 sums 8.5 / 5.2; 64 rows of 50257 columns 9 with 64 or 256).
+// TOK tokens a block, SLICES threads each: 16 and 64; 64 and 4 where a row has up to 64 sums to
+// add up (1024 rows of 8 sums 8.5 -> 5.2 us); 4 and 64, with more loads in flight, for few
+// rows (64 rows of 786 sums 9 -> 7 us, but 2000 rows of 470 12 -> 21).
 // mean[0]: the mean over the rows with a target, 0 if there is none; mean[1]: their
 // number; the last block to end adds the blocks' sums up, in their order.
 template <int TOK, int SLICES>
@@ -761,7 +805,7 @@ __global__ __launch_bounds__(TOK * SLICES) void join_kernel(const float2* __rest
   float m = -INFINITY, s = 0.0f;
   bool nan = false;
   if (n < N) {
-    constexpr int kAhead = 4;   // loads in flight
+    constexpr int kAhead = TOK == 4 ? 16 : 4;   // loads in flight
     for (int p0 = slice; p0 < P; p0 += SLICES * kAhead) {
       float2 v[kAhead];
 #pragma unroll
@@ -1079,6 +1123,9 @@ hipError_t launch_ring(LossArgs g, const GemmPlan& p, int cus, hipStream_t st) {
   g.parts = std::min(p.parts, g.KT);   // (every part has a slab; a short last piece adds to fewer)
   g.mt = div_up(g.M, tile_rows(p.tile));
   g.nt = div_up(g.Nf, tile_cols(p.tile));
+  for (g.turn = 1; 2 * g.turn <= g.KT / g.parts;) g.turn *= 2;
+  --g.turn;
+  g.once = (size_t)g.Nf * g.ldb >= (size_t)256 << 20;   // (what the last-level cache has no room for)
   const long items = (long)g.mt * g.nt * g.parts;
   if (items > 0x3FFFFFFF || std::max(g.lda, g.ldb) * 256 > 0xFFFFFFFFu ||
       std::max(g.ldd, g.lddt) * 32 * sizeof(T) > 0xFFFFFFFFu)
@@ -1092,7 +1139,9 @@ hipError_t launch_ring(LossArgs g, const GemmPlan& p, int cus, hipStream_t st) {
   if (p.tile == kTiny) {
     go(ring_kernel<T, EPI, 64, 64, 4, 9>, 256);
   } else if (p.tile == kSmall) {
-    if (alone) go(ring_kernel<T, EPI, 64, 128, 4, 9>, 256);
+    if (g.mt == 1 && alone) go(ring_kernel<T, EPI, 64, 128, 4, 12>, 256);
+    else if (g.mt == 1) go(ring_kernel<T, EPI, 64, 128, 4, 6>, 256);
+    else if (alone) go(ring_kernel<T, EPI, 64, 128, 4, 9>, 256);
     else go(ring_kernel<T, EPI, 64, 128, 4, 5>, 256);
   } else if (p.tile == kMid) {
     if (alone) go(ring_kernel<T, EPI, 128, 128, 4, 9>, 256);
@@ -1144,7 +1193,7 @@ LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
     l.dl = plan_gemm<T>(N, V, kp / kSlab<T>, false, kLarge, cus);
     l.part_lse = take((size_t)div_up(V, wave_cols(l.dl.tile)) * l.ld_lse * sizeof(float2));
     l.picked = take((size_t)N * 4);
-    l.sums = take((size_t)div_up(N, 16) * sizeof(JoinSum));
+    l.sums = take((size_t)std::max(32, div_up(N, 16)) * sizeof(JoinSum));
     l.counter = take(4);
     l.xpad = take(pad ? (size_t)N * kp * sizeof(T) : 0);
     l.wpad = take(pad ? (size_t)V * kp * sizeof(T) : 0);
@@ -1223,6 +1272,7 @@ hipError_t forward_impl(const mgpt_lm_loss_config* cfg, const T* x, const T* W, 
                         g.picked, targets, loss, lse, mean, (JoinSum*)(ws + l.sums), g.counter);
   };
   if (P <= 64) join(join_kernel<64, 4>, 64, 256);
+  else if (N <= 128) join(join_kernel<4, 64>, 4, 256);
   else join(join_kernel<16, 64>, 16, 1024);
   return hipGetLastError();
 }
