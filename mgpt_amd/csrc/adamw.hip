@@ -27,7 +27,9 @@
 // bits with bf16 ones (+2 with a bf16 copy).  A block of threads takes 4096 elements of
 // one tensor (found by a search of the tensors' table, which is a kernel argument: any
 // set of tensors in one launch per 116), every load of a lane requested before the first
-// use.
+// use, all of it past the caches, which would hold none of it for the next step.  MI355X,
+// 98 tensors of 139M elements: 665 to 684 us in 32 bits (5.7 to 5.9 TB/s; through the
+// caches 741), 365 to 374 in 8 with bf16 gradients and copies (16 bytes an element, 5.9 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <cmath>

@@ -19,9 +19,10 @@
 // out.  A row stays in the registers of its W waves (8 columns a lane and vector, NV
 // vectors), so that everything is read once; the gains sit in registers (or LDS) across
 // a stream's rows.  A stream is W waves that take rows in turn.  MI355X: forward 16384 x
-// 1024 bf16 22 us (134 MB, 6.1 TB/s), 32768 x 2048 92 us (537 MB, 5.8 TB/s).  Column sums are kept per
-// lane over a stream's rows, added over a block's streams through LDS, and over the blocks
-// by norm_reduce_kernel, in a fixed order: the same call gives the same bits.
+// 1024 bf16 22 us (134 MB, 6.1 TB/s), 32768 x 2048 97 us (537 MB, 5.5 TB/s); stores past
+// the caches 23 and 103.  Column sums are kept per lane over a stream's rows, added over a
+// block's streams through LDS, and over the blocks by norm_reduce_kernel, in a fixed
+// order: the same call gives the same bits.
 // All arithmetic is fp32; out, y, dx and dh are rounded once.
 #include <hip/hip_runtime.h>
 
