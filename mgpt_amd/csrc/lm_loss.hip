@@ -1210,7 +1210,9 @@ LossLayout loss_layout(int N, int C, int V, bool backward, bool pad, int cus) {
   l.ldx = (int)align_up((size_t)C, 256);
   l.dl = plan_gemm<T>(N, l.piece, kp / kSlab<T>, false, sizeof(T) == 4 ? kMid : kLarge, cus);
   l.dx = plan_gemm<T>(N, C, div_up(std::min(V, l.piece), kSlab<T>), true, kLarge, cus);
-  l.dw = plan_gemm<T>(std::min(V, l.piece), C, l.nk / kSlab<T>, true, kLarge, cus);
+  // (few rows: little but dW's stores, which two blocks a CU overlap; with gradients, 1 x 1024 x
+  // 100000 341 -> 327 us, 64 x 4096 x 20000 280 -> 266)
+  l.dw = plan_gemm<T>(std::min(V, l.piece), C, l.nk / kSlab<T>, true, l.nk / kSlab<T> <= 2 ? kMid : kLarge, cus);
   l.dx_part = l.pieces > 1 || l.dx.parts > 1;
   l.scale = take((size_t)N * 4);
   l.factor = take(4);

@@ -130,7 +130,8 @@ TILES = [(1, 8, 34875), (4327, 8, 2), (17916, 8, 2), (69, 8, 43707), (132, 8, 51
          (1065, 3600, 4), (1, 88, 8874), (1, 136, 53557), (1, 400, 27252), (1, 118, 8818), (2, 1572, 2468),
          (1, 12, 20526), (1, 131, 56687), (1, 75, 9109), (7, 3673, 1039), (1, 177, 58058), (1, 3280, 1272),
          (1, 3222, 2031), (1, 3348, 5455), (1, 3589, 11708), (943, 3385, 73), (216, 8, 16491), (17706, 135, 381),
-         (4535, 72, 3396), (4435, 152, 11982), (40, 32, 30), (500, 64, 32)]
+         (4535, 72, 3396), (4435, 152, 11982), (40, 32, 30), (500, 64, 32), (4119, 3024, 2), (3302, 3783, 2),
+         (3458, 3536, 2), (12841, 897, 2), (300, 1024, 20000), (300, 1025, 20000)]
 
 
 @pytest.mark.parametrize("act", ["f32", "bf16"])
