@@ -232,6 +232,13 @@ __device__ __forceinline__ float exp_less(float z, float s, float ns, bool huge)
 }
 constexpr float kHuge = 1e38f;
 
+// What exp_less's ns = -s log2 e lost to rounding, as the factor that all exponentials of
+// the row lack: half a step of 1.44 |s|, 5e-6 of them for an s near 100.  (The fma is
+// exact.)  It goes to the row's sum or upstream gradient, so no exponential costs more.
+__device__ __forceinline__ float lost_in_product(float s, float ns, bool huge) {
+  return huge ? 1.0f : __builtin_amdgcn_exp2f(-__builtin_fmaf(s, kLog2e, ns));
+}
+
 // a * b, 0 where either is 0, whatever the other.
 __device__ __forceinline__ float mul_zero(float a, float b) {
   float r;
@@ -267,7 +274,7 @@ __device__ __forceinline__ void emit_lse(const LossArgs& g, Acc<W>& acc, int row
 #pragma unroll
         for (int v = 0; v < 16; ++v) s += exp_less(acc[j][i][v], top, ntop, false);
     }
-    s = other_half_sum(s);
+    s = other_half_sum(s) * lost_in_product(top, ntop, huge);
     if (live && lhalf == 0) g.part_lse[(size_t)(fw / W::WTN) * g.ld_lse + row] = make_float2(m, s);
     const int fl = t >= fw && t < min(fw + W::WTN, g.Nf) ? t - fw : -1;
     const bool mine = fl >= 0 && ((fl >> 2) & 1) == lhalf;
@@ -287,7 +294,7 @@ __device__ __forceinline__ void emit_lse(const LossArgs& g, Acc<W>& acc, int row
 template <typename T, typename W, bool SUM>
 __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int row0, int fw, int lrow, int lhalf,
                                             int sum_row) {
-  float lse[W::TM], sc[W::TM];
+  float lse[W::TM], sc[W::TM], psc[W::TM];   // psc: of the probabilities
   int tl[W::TM];   // the target's column in the wave's
   bool huge = false;
 #pragma unroll
@@ -295,6 +302,7 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
     const int row = row0 + 32 * i + lrow, r = min(row, g.M - 1);
     sc[i] = row < g.M ? g.scale[r] : 0.0f;
     lse[i] = sc[i] == 0.0f ? 0.0f : g.lse[r];
+    psc[i] = sc[i] * lost_in_product(lse[i], -lse[i] * kLog2e, !(fabsf(lse[i]) < kHuge));
     tl[i] = g.targets[r] - g.target0 - fw;
     huge |= !(fabsf(lse[i]) < kHuge);
   }
@@ -326,15 +334,15 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
 #pragma unroll
         for (int v = 0; v < 16; ++v) d[v] = exp_less(acc[j][i][v], lse[i], nl, false);
       }
-      if (__ballot(tl[i] >= 32 * j && tl[i] < 32 * j + 32)) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (tl[i] == 32 * j + 8 * (v / 4) + 4 * lhalf + v % 4) d[v] -= 1.0f;
-      }
       // (0 times anything is 0 here: a row without a target has no gradient even where its
       // logits are not finite)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) d[v] = mul_zero(d[v], sc[i]);
+      for (int v = 0; v < 16; ++v) d[v] = mul_zero(d[v], psc[i]);
+      if (__ballot(tl[i] >= 32 * j && tl[i] < 32 * j + 32)) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (tl[i] == 32 * j + 8 * (v / 4) + 4 * lhalf + v % 4) d[v] -= sc[i];
+      }
       if constexpr (SUM) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) cs[v] += d[v];
