@@ -35,9 +35,11 @@ def _addresses(tensors, some):
 class AdamW:
     """params: contiguous float32 CUDA tensors of one device, which keep their
     memory.  copies: None, or per parameter a bfloat16 tensor of its size (or
-    None) that every step refreshes.  state_bits: 32 or 8.  device_step: keep the step's number on
-    the device, so that a step captured into a HIP graph counts on when it is
-    replayed (step_count then stays where it was)."""
+    None) that every step refreshes.  state_bits: 32 or 8.  device_step: keep the
+    step's number on the device, so that a step captured into a HIP graph counts
+    on when it is replayed; without it a replayed step repeats the number that
+    it was captured with.  To go on from a saved run, copy its state into
+    `state` and set step_count."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, state_bits: int = 32, copies=None, device_step: bool = False):
@@ -62,7 +64,6 @@ class AdamW:
         # the one that was checked, whatever has been assigned to its .data since
         self._held = [t.detach() for t in written]
         self._at = self._written()
-        self.step_count = 0
         n = len(self.params)
         self._numels = [p.numel() for p in self.params]
         self._sizes = (ctypes.c_int64 * n)(*self._numels)
@@ -70,6 +71,7 @@ class AdamW:
         capi.check(capi.lib().mgpt_adamw_state_bytes(n, self._sizes, state_bits, ctypes.byref(need)))
         self.state = torch.zeros(need.value, dtype=torch.uint8, device=self.device)
         self._step_device = (torch.zeros(1, dtype=torch.int32, device=self.device) if device_step else None)
+        self._steps = 0   # where the number is not on the device
         blocks = sum((p.numel() + 255) // 256 for p in self.params)
         held = blocks * 256 * state_bits // 8
         kinds = (torch.float32, torch.float32) if state_bits == 32 else (torch.float8_e4m3fn, torch.uint8)
@@ -78,6 +80,19 @@ class AdamW:
         self.v = self.state[held:2 * held].view(kinds[1])
         self.m_exp = self.state[2 * held:2 * held + blocks] if state_bits == 8 else None
         self.v_exp = self.state[2 * held + blocks:] if state_bits == 8 else None
+
+    @property
+    def step_count(self) -> int:
+        """The steps taken; the next is one more.  With device_step it is read
+        from the device, which waits for the steps before, and set there."""
+        return self._steps if self._step_device is None else int(self._step_device.item())
+
+    @step_count.setter
+    def step_count(self, count: int) -> None:
+        if self._step_device is None:
+            self._steps = count
+        else:
+            self._step_device.fill_(count)
 
     def _check(self, t, dtype, numel, what):
         if t.device != self.device or not t.is_cuda:
@@ -123,7 +138,7 @@ class AdamW:
         cfg = capi.AdamWConfig(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
                                self.state_bits, _GRAD[dtypes.pop()])
         with capi.on_device(self.device):
-            number = self.step_count + 1
+            number = self._steps + 1
             at = None
             if self._step_device is not None:
                 self._step_device.add_(1)
@@ -135,4 +150,5 @@ class AdamW:
             if status != capi.MGPT_OK and at is not None:
                 self._step_device.sub_(1)   # a refused step is none
             capi.check(status)
-        self.step_count = number
+        if at is None:
+            self._steps = number
