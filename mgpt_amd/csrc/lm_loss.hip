@@ -46,7 +46,7 @@ namespace mgpt {
 
 template <typename T>
 hipError_t launch_copy_cols(const T*, int, T*, int, int, int, int, hipStream_t);   // pack.hip
-hipError_t launch_fill_zero(float* p, size_t n, hipStream_t stream);              // backward.hip
+hipError_t launch_fill_zero(float* p, size_t n, hipStream_t stream);              // wgrad.hip
 
 namespace {
 
@@ -1499,10 +1499,9 @@ int mgpt_lm_loss_backward(const mgpt_lm_loss_config* cfg, const void* x, const v
   const bool f32 = cfg->dtype == MGPT_DTYPE_F32;
   const size_t C = cfg->embed_dim, V = cfg->vocab_size;
   if (num_tokens == 0) {   // no token adds to the weights' gradients
-    if (dW && !f32 && ((uintptr_t)dW & 3)) return fail(MGPT_ERR_INVALID_ARGUMENT, "dW is not 4-byte aligned");
-    if (dW) HIP_TRY(launch_fill_zero((float*)dW, f32 ? V * C : V * C / 2, st));
-    if (dW && !f32 && (V * C) % 2)
-      HIP_TRY(launch_copy_cols<bf16_t>((const bf16_t*)dW, 0, (bf16_t*)dW + V * C - 1, 1, 1, 0, 1, st));
+    if (dW && f32) HIP_TRY(launch_fill_zero((float*)dW, V * C, st));
+    if (dW && !f32)
+      HIP_TRY(launch_copy_cols<bf16_t>((const bf16_t*)dW, 0, (bf16_t*)dW, (int)C, (int)V, 0, (int)C, st));
     if (dbias) HIP_TRY(launch_fill_zero(dbias, V, st));
     return MGPT_OK;
   }

@@ -568,26 +568,26 @@ __global__ __launch_bounds__(256) void zero_idle_experts_kernel(const int32_t* _
   }
 }
 
-// n floats of p (16-byte aligned) set to zero: a kernel, so that a HIP graph
-// captures a kernel node and not a memset node.
-__global__ __launch_bounds__(256) void fill_zero_kernel(float4* __restrict__ p, size_t n4,
-                                                        float* __restrict__ tail, int ntail) {
-  const size_t t0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+// n floats of p set to zero, by float4 from the first that is 16-byte aligned, `head`
+// floats on: a kernel, so that a HIP graph captures a kernel node and not a memset node.
+__global__ __launch_bounds__(256) void fill_zero_kernel(float* __restrict__ p, size_t n, int head) {
+  const size_t t0 = (size_t)blockIdx.x * blockDim.x + threadIdx.x, n4 = (n - head) / 4;
+  float4* body = reinterpret_cast<float4*>(p + head);
   for (size_t i = t0; i < n4; i += (size_t)gridDim.x * blockDim.x)
-    p[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (t0 < (size_t)ntail) tail[t0] = 0.0f;
+    body[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (t0 < (size_t)head) p[t0] = 0.0f;
+  if (head + 4 * n4 + t0 < n) p[head + 4 * n4 + t0] = 0.0f;   // (fewer than 4)
 }
 
 }  // namespace
 
 hipError_t launch_fill_zero(float* p, size_t n, hipStream_t stream) {
   if (n == 0) return hipSuccess;
-  if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return hipErrorInvalidValue;
-  const size_t n4 = n / 4;
-  const size_t want = (n4 + 255) / 256;
+  if ((reinterpret_cast<uintptr_t>(p) & 3) != 0) return hipErrorInvalidValue;
+  const size_t head = std::min<size_t>(n, (16 - (reinterpret_cast<uintptr_t>(p) & 15)) / 4 % 4);
+  const size_t want = (n / 4 + 255) / 256;
   const int blocks = (int)std::max<size_t>(1, std::min<size_t>(want, 2048));
-  hipLaunchKernelGGL(fill_zero_kernel, dim3(blocks), dim3(256), 0, stream,
-                     reinterpret_cast<float4*>(p), n4, p + 4 * n4, (int)(n - 4 * n4));
+  hipLaunchKernelGGL(fill_zero_kernel, dim3(blocks), dim3(256), 0, stream, p, n, (int)head);
   return hipGetLastError();
 }
 
