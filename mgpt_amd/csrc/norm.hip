@@ -37,7 +37,7 @@
 
 namespace mgpt {
 
-hipError_t launch_fill_zero(float* p, size_t n, hipStream_t stream);   // backward.hip
+hipError_t launch_fill_zero(float* p, size_t n, hipStream_t stream);   // wgrad.hip
 
 namespace {
 
@@ -663,18 +663,26 @@ NormLayout norm_layout(const NormPlan& p, int C, int G) {
   return l;
 }
 
-template <typename F>
+// f(waves, vectors) of row_layout's rows: one vector, or two forward past 512 columns and
+// backward past 8192, where it is 16 waves.
+template <bool BACKWARD, typename F>
 hipError_t for_layout(int W, int NV, F&& f) {
-  auto nv = [&](auto w) {
-    if (NV == 1) f(w, std::integral_constant<int, 1>{});
-    else f(w, std::integral_constant<int, 2>{});
-  };
-  switch (W) {
-    case 1: nv(std::integral_constant<int, 1>{}); break;
-    case 2: nv(std::integral_constant<int, 2>{}); break;
-    case 4: nv(std::integral_constant<int, 4>{}); break;
-    case 8: nv(std::integral_constant<int, 8>{}); break;
-    default: nv(std::integral_constant<int, 16>{}); break;
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, 2> two;
+  constexpr std::integral_constant<int, 16> most;
+  if (BACKWARD && NV == 2) {
+    f(most, two);
+  } else if (!BACKWARD && NV == 1) {
+    f(one, one);
+  } else {
+    constexpr std::integral_constant<int, BACKWARD ? 1 : 2> nv;
+    switch (W) {
+      case 1: f(one, nv); break;
+      case 2: f(two, nv); break;
+      case 4: f(std::integral_constant<int, 4>{}, nv); break;
+      case 8: f(std::integral_constant<int, 8>{}, nv); break;
+      default: f(most, nv); break;
+    }
   }
   return hipGetLastError();
 }
@@ -738,7 +746,7 @@ int mgpt_norm_forward(const mgpt_norm_config* cfg, const void* x, const void* h,
   const int grid = std::min(rows, compute_units() * (W <= 4 ? 4 : 16 / W));
   auto go = [&](auto t) {
     using T = decltype(t);
-    return for_layout(W, NV, [&](auto w, auto nv) {
+    return for_layout<false>(W, NV, [&](auto w, auto nv) {
       constexpr int kW = decltype(w)::value, kNV = decltype(nv)::value;
       hipLaunchKernelGGL((norm_forward_kernel<T, kW, kNV>), dim3(grid), dim3(kW <= 4 ? 256 : kW * 64), 0,
                          (hipStream_t)stream, a, (const T*)x, (const T*)h, (T*)out, (T*)y);
@@ -804,7 +812,7 @@ int mgpt_norm_backward(const mgpt_norm_config* cfg, const void* x, const void* h
   hipStream_t st = (hipStream_t)stream;
   auto go = [&](auto t) {
     using T = decltype(t);
-    return for_layout(p.W, p.NV, [&](auto w, auto nv) {
+    return for_layout<true>(p.W, p.NV, [&](auto w, auto nv) {
       constexpr int kW = decltype(w)::value, kNV = decltype(nv)::value;
       auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(p.blocks), dim3(kW <= 4 ? 256 : kW * 64), 0, st, a, (const T*)x,
