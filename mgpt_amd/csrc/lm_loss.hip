@@ -334,14 +334,23 @@ __device__ __forceinline__ void emit_dlogit(const LossArgs& g, Acc<W>& acc, int 
 #pragma unroll
         for (int v = 0; v < 16; ++v) d[v] = exp_less(acc[j][i][v], lse[i], nl, false);
       }
+      // the target's entry apart: (p - 1) times the upstream gradient, which may be infinite
+      const bool hit = __ballot(tl[i] >= 32 * j && tl[i] < 32 * j + 32) != 0;
+      float at = 0.0f;
+      if (hit) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (tl[i] == 32 * j + 8 * (v / 4) + 4 * lhalf + v % 4) at = d[v];
+        at = mul_zero(at * lost_in_product(lse[i], nl, !(fabsf(lse[i]) < kHuge)) - 1.0f, sc[i]);
+      }
       // (0 times anything is 0 here: a row without a target has no gradient even where its
       // logits are not finite)
 #pragma unroll
       for (int v = 0; v < 16; ++v) d[v] = mul_zero(d[v], psc[i]);
-      if (__ballot(tl[i] >= 32 * j && tl[i] < 32 * j + 32)) {
+      if (hit) {
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          if (tl[i] == 32 * j + 8 * (v / 4) + 4 * lhalf + v % 4) d[v] -= sc[i];
+          if (tl[i] == 32 * j + 8 * (v / 4) + 4 * lhalf + v % 4) d[v] = at;
       }
       if constexpr (SUM) {
 #pragma unroll

@@ -85,3 +85,19 @@ def test_gradient_of_the_bias_of_one_row(act):
     got = torch.stack([op.backward(x[n:n + 1], W, t[n:n + 1], lse[n:n + 1], bias=b)[2] for n in range(N)])
     err = (got.double() - want).abs()
     assert (err <= tol).all(), (float((err / tol).max()), int((err > tol).sum()))
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_an_infinite_upstream_gradient(act):
+    """(p - [v = t]) times it: infinite, and of the sign of the difference."""
+    from mgpt_amd.loss import LMLoss
+    x, W, b, t, z = exact_logits(act)
+    lse = torch.logsumexp(z, 1).float()
+    op = LMLoss(C, V, act=act)
+    for g in (float("inf"), float("-inf")):
+        for n in (0, 5, 69):
+            dloss = torch.full((1,), g, device="cuda")
+            _, _, db = op.backward(x[n:n + 1], W, t[n:n + 1], lse[n:n + 1], bias=b, dloss=dloss)
+            want = torch.full((V,), g, device="cuda")
+            want[int(t[n])] = -g
+            assert torch.equal(db, want), (g, n, db)
