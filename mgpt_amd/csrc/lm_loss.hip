@@ -224,13 +224,13 @@ __device__ __forceinline__ void start_from_bias(const LossArgs& g, Acc<W>& acc, 
   }
 }
 
-// exp(z - s) of a register: one fma into the hardware's exponential; `huge` (a lane's s
-// near the type's lowest or largest value, which times log2 e overflows): difference first.
-// (By lane: a row's bits do not depend on its neighbours.)
+// exp(z - s) of a register: one fma into the hardware's exponential; `huge` (a lane's s at
+// kHuge and beyond, where the rounding of s log2 e would be some and at last all of the
+// exponent): difference first.  (By lane: a row's bits do not depend on its neighbours.)
 __device__ __forceinline__ float exp_less(float z, float s, float ns, bool huge) {
   return __builtin_amdgcn_exp2f(huge ? (z - s) * kLog2e : __builtin_fmaf(z, kLog2e, ns));
 }
-constexpr float kHuge = 1e38f;
+constexpr float kHuge = 0x1p20f;   // (half a step of 1.44 kHuge is 1/16)
 
 // What exp_less's ns = -s log2 e lost to rounding, as the factor that all exponentials of
 // the row lack: half a step of 1.44 |s|, 5e-6 of them for an s near 100.  (The fma is

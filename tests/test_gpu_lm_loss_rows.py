@@ -101,3 +101,34 @@ def test_an_infinite_upstream_gradient(act):
             want = torch.full((V,), g, device="cuda")
             want[int(t[n])] = -g
             assert torch.equal(db, want), (g, n, db)
+
+
+FAR = [1e4, 3e6, 1e9, 1e10, 1e20, 1e30, 3e38]
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_rows_of_far_logits(act, sign):
+    """Rows whose logits are all one number, up to the largest and down to the lowest
+    (masked ones): lse is within its rounding of it, and the probabilities from a
+    given lse are those of its difference from the logits."""
+    from mgpt_amd.loss import LMLoss
+    dt = torch.float32 if act == "f32" else torch.bfloat16
+    n = len(FAR)
+    x, W = torch.zeros(n, C, dtype=dt, device="cuda"), torch.zeros(V, C, dtype=dt, device="cuda")
+    x[:, 0] = sign * torch.tensor(FAR)
+    W[:, 0] = 1
+    a = x[:, 0].to(torch.bfloat16)   # a single part of a split product
+    x[:, 0] = a
+    t = torch.arange(n, dtype=torch.int32, device="cuda")
+    b = torch.zeros(V, device="cuda")
+    z = a.double()[:, None].expand(n, V)
+    op = LMLoss(C, V, act=act)
+    loss, lse, mean = op.forward(x, W, t, bias=b)
+    want = torch.logsumexp(z, 1)
+    assert ((lse.double() - want).abs() <= U * want.abs() + 21 * U).all(), lse
+    assert ((loss.double() - want + z[:, 0]).abs() <= U * want.abs() + 22 * U).all(), loss
+    given = want.float()
+    d, tol = reference(z, given, t)
+    got = torch.stack([op.backward(x[i:i + 1], W, t[i:i + 1], given[i:i + 1], bias=b)[2] for i in range(n)])
+    assert ((got.double() - d).abs() <= tol).all(), got
