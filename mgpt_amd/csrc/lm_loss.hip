@@ -987,7 +987,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(PrepareArgs<T> a) {
     m = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
     float f;
     if (a.dloss)
-      f = m > 1e-30f && m < 1e30f ? m : 1.0f;
+      f = m > 0.0f && m < INFINITY ? m : 1.0f;
     else
       f = c ? (a.dmean ? *a.dmean : 1.0f) / (float)c : 0.0f;
     if (b == 0 && threadIdx.x == 0) *a.factor = f;
