@@ -455,9 +455,10 @@ int mgpt_norm_backward(const mgpt_norm_config* cfg, const void* x, const void* h
  * lm_head keeps W transposed, [C,V].)  A target outside 0 .. V - 1 means that
  * the row has none: its loss is 0 and it adds to no gradient, whatever it
  * holds.  fp32 products are formed from three bf16 parts of each operand, six
- * of nine products, to fp32's accuracy (magnitudes up to 3.38e38; beyond, and
- * for infinities, NaN).  Replaces lm_head's LinearLayer and
- * CrossEntropyLossLayer. */
+ * of nine products, to fp32's accuracy (magnitudes of 2^-110 to 3.38e38; of
+ * smaller ones the parts below 2^-133 are lost; beyond, and for infinities,
+ * NaN).  A row with a logit of +infinity has NaN as its lse and loss, as one
+ * with a NaN.  Replaces lm_head's LinearLayer and CrossEntropyLossLayer. */
 typedef struct mgpt_lm_loss_config {
   int embed_dim;    /* C: 1 .. 2^20 (multiples of 64 (bf16) or 32 (fp32) are read in place) */
   int vocab_size;   /* V: 1 .. 2^24 */
@@ -480,7 +481,12 @@ int mgpt_lm_loss_forward(const mgpt_lm_loss_config* cfg, const void* x, const vo
  * the upstream gradient dloss [N] fp32 of each row's loss or, where dloss is
  * null, dmean [1] of their mean (null: 1): dx [N,C], dW [V,C] in dtype, dbias
  * [V] fp32, each written (not added to) where it is not null.  The logits are
- * formed again, a piece of the vocabulary at a time.  Workspace: up to about 1
+ * formed again, a piece of the vocabulary at a time.  With bf16 inputs their
+ * gradients are rounded to bf16 before the products for dx and dW (not for
+ * dbias): where the probabilities are not all near 0 or 1, dx and dW are off by
+ * about 1.25 times what rounding the results alone gives.  A row whose upstream
+ * gradient is below 2^-110 of the largest loses bits of its gradients.
+ * Workspace: up to about 1
  * GiB for a piece's gradients (more where 256 columns take more), and copies
  * of x and of a piece of W. */
 int mgpt_lm_loss_backward(const mgpt_lm_loss_config* cfg, const void* x, const void* W,

@@ -17,7 +17,7 @@
 //    one is left for rounding up.  v moves by (1 - b2) = 0.001 a step, far less than
 //    half of a code's step (6%), so rounding to nearest would hold it for good: it is
 //    rounded up with the probability of what is cut off, 16 bits of a counter hash
-//    (Wells' lowbias32 over the element pair and the step: the same call gives the same
+//    (Wellons' lowbias32 over the element pair and the step: the same call gives the same
 //    bits).  v > 0 is never held as 0, which m / (sqrt(0) + eps) would blow up.
 //  * A moment that is not finite is held as NaN (e4m3's, code 255) and does not
 //    enter the block's power of two, so it stays where it arose.
@@ -29,7 +29,8 @@
 // set of tensors in one launch per 116), every load of a lane requested before the first
 // use, all of it past the caches, which would hold none of it for the next step.  MI355X,
 // 98 tensors of 139M elements: 665 to 684 us in 32 bits (5.7 to 5.9 TB/s; through the
-// caches 741), 365 to 374 in 8 with bf16 gradients and copies (16 bytes an element, 5.9 TB/s).
+// caches 741), 367 to 380 in 8 with bf16 gradients and copies (16 bytes an element, 5.9
+// TB/s; the first sixty launches after a pause take up to 520).
 #include <hip/hip_runtime.h>
 
 #include <cmath>

@@ -438,8 +438,10 @@ __device__ __forceinline__ void widen(const Raw<bf16_t>& r, bool in, float (&o)[
 // nothing to the column sums.
 // MI355X, us against norm_backward_kernel: 16384 x 1024 bf16 41.6 -> 36.4, 32768 x 2048 190
 // -> 175 (805 MB, 4.6 TB/s), 20000 x 512 23.4 -> 22.3; 4096 x 4096 fp32 75 -> 78, 8000 x 8192
-// 187 -> 190.  Memory bounds it: without the sums over a row it takes as long, without one of
-// the two stores 30 us less at 32768 x 2048, without two of the four loads 60.
+// 187 -> 190.  A gain or dout less keeps norm_backward_kernel: 16384 x 1024 38 with gamma_pre
+// alone, 37 without dout, 32768 x 2048 182.  Memory bounds it: without the sums over a row it
+// takes as long, without one of the two stores 30 us less at 32768 x 2048, without two of the
+// four loads 60.
 template <typename T, int W, bool ONCE>
 __global__ __launch_bounds__(W <= 4 ? 256 : W * 64, 4) void norm_backward_full_kernel(
     NormArgs a, const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ dout,

@@ -72,7 +72,9 @@ class LMLoss:
         """(dx, dweight, dbias) from forward's inputs and its lse, for the
         upstream gradient dloss (float32, per token) or dmean (float32, one
         element; None: 1) of the mean loss.  need: which of the three are
-        wanted; one that is not, and dbias without a bias, is None."""
+        wanted; one that is not, and dbias without a bias, is None.  In bf16
+        dx and dweight are products of logits' gradients rounded to bf16,
+        dbias is their sum before that."""
         n, ptrs = self._inputs(x, weight, targets, bias)
         dev = x.device
         ptrs.append(self._check(lse, torch.float32, tuple(targets.shape), dev, "lse"))
