@@ -285,7 +285,7 @@ def _own_route(s):
     idx, w = s["op"].forward(s["l"], bias=s["b"])
     out = {"idx": idx, "w": w}
     if s["case"]["op"] == "route_grad":
-        out["dl"] = s["op"].backward(s["l"], idx, s["dw"], bias=s["b"], dscores=s["ds"])
+        out["dl"] = s["op"].backward(s["l"], idx, w, s["dw"], dscores=s["ds"])
     return out
 
 
