@@ -494,6 +494,54 @@ int mgpt_lm_loss_backward(const mgpt_lm_loss_config* cfg, const void* x, const v
                           const float* dloss, const float* dmean, void* dx, void* dW, float* dbias,
                           int num_tokens, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The choice of experts from a router's logits [N,E], in dtype:
+ *   s = softmax(l) or 1 / (1 + exp(-l)),  key = l, or s + bias with a bias
+ * An expert whose logit is -infinity or NaN, or whose key is, takes no part;
+ * logits of +infinity count as the largest float.  With groups > 1 (expert e
+ * in group e / (E / groups)) a group's size is the sum of the scores (with the
+ * bias) of its best group_best experts, and the top_groups largest take part.
+ * idx [N,k]: the k largest keys, descending, the lower id first where equal;
+ * where fewer take part the lowest other ids follow, with weight 0.  weights [N,k] fp32:
+ * scale s_j / (sum of the k's s + 1e-20) if renormalise is not 0, else scale
+ * s_j.  Keys with a bias and the groups' sizes are compared as 64 bits hold
+ * them.  The layer's own router (mgpt_moe_forward) is the engine's; see
+ * mgpt_moe_set_routing. */
+typedef enum mgpt_score {
+  MGPT_SCORE_SOFTMAX = 0,
+  MGPT_SCORE_SIGMOID = 1
+} mgpt_score;
+
+typedef struct mgpt_route_config {
+  int num_experts;   /* E: 1 .. 512 */
+  int top_k;         /* 1 .. 8 */
+  int score;         /* mgpt_score */
+  int groups;        /* divides E; 1 .. 64 */
+  int top_groups;    /* 1 .. groups */
+  int group_best;    /* 1 or 2 */
+  int renormalise;
+  float scale;       /* finite, not 0 */
+  int dtype;         /* of the logits: MGPT_DTYPE_F32 or MGPT_DTYPE_BF16 */
+} mgpt_route_config;
+
+/* bias: [E] fp32 or null; it decides the choice only, not the weights.
+ * counts (may be null): int32 [E], to which each expert's number of tokens is
+ * added.  num_tokens up to 2^28. */
+int mgpt_route_forward(const mgpt_route_config* cfg, const void* logits, const float* bias,
+                       int32_t* idx, float* weights, int32_t* counts, int num_tokens, void* stream);
+
+/* dlogits [N,E] in dtype, for the upstream gradients dweights [N,k] fp32 and,
+ * where not null, dscores [E] fp32: the gradient of expert e's score in every
+ * token (a balance loss on the scores' means).  idx and weights are the
+ * forward's; the choice is taken as given.  An expert whose logit is -infinity
+ * or NaN has gradient 0. */
+int mgpt_route_backward(const mgpt_route_config* cfg, const void* logits, const int32_t* idx,
+                        const float* weights, const float* dweights, const float* dscores,
+                        void* dlogits, int num_tokens, void* stream);
+
+/* bias[e] += rate where counts[e] is below the counts' mean, -= rate above it. */
+int mgpt_route_balance(int num_experts, const int32_t* counts, float rate, float* bias,
+                       void* stream);
+
 /* Description of the last error on this host thread ("" if none). */
 const char* mgpt_moe_last_error(void);
 

@@ -25,6 +25,7 @@ MGPT_ERR_NOT_READY = 4
 MGPT_ERR_HIP = 5
 MGPT_ERR_OUT_OF_MEMORY = 6
 
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 DTYPE_F32, DTYPE_BF16, DTYPE_FP8_E4M3 = 0, 1, 2
 NUM_STAGES = 5
 STAGE_NAMES = ["router_topk", "permute", "gemm_gateup", "gemm_down", "combine"]
@@ -66,6 +67,12 @@ class NormConfig(ctypes.Structure):
 
 class LMLossConfig(ctypes.Structure):
     _fields_ = [("embed_dim", ctypes.c_int), ("vocab_size", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
+class RouteConfig(ctypes.Structure):
+    _fields_ = [("num_experts", ctypes.c_int), ("top_k", ctypes.c_int), ("score", ctypes.c_int),
+                ("groups", ctypes.c_int), ("top_groups", ctypes.c_int), ("group_best", ctypes.c_int),
+                ("renormalise", ctypes.c_int), ("scale", ctypes.c_float), ("dtype", ctypes.c_int)]
 
 
 class MoEError(RuntimeError):
@@ -128,6 +135,9 @@ def lib() -> ctypes.CDLL:
         "mgpt_norm_forward": [ctypes.POINTER(NormConfig)] + [vp] * 9 + [i, vp],
         "mgpt_norm_backward_workspace_bytes": [ctypes.POINTER(NormConfig), i, ctypes.POINTER(sz)],
         "mgpt_norm_backward": [ctypes.POINTER(NormConfig)] + [vp] * 14 + [i, vp, sz, vp],
+        "mgpt_route_forward": [ctypes.POINTER(RouteConfig)] + [vp] * 5 + [i, vp],
+        "mgpt_route_backward": [ctypes.POINTER(RouteConfig)] + [vp] * 6 + [i, vp],
+        "mgpt_route_balance": [i, vp, ctypes.c_float, vp, vp],
     }
     for name, args in sig.items():
         f = getattr(L, name)
