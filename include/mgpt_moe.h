@@ -542,6 +542,33 @@ int mgpt_route_backward(const mgpt_route_config* cfg, const void* logits, const 
 int mgpt_route_balance(int num_experts, const int32_t* counts, float rate, float* bias,
                        void* stream);
 
+/* A linear layer in 8-bit integers with a scale for each token and each output:
+ *   sx[n] = max|x[n]| / 127,  q = rint(x 127 / max|x[n]|),
+ *   y[n][m] = (sum over k of q[n][k] w[m][k]) sx[n] scales[m] + bias[m]
+ * x [N,K], y [N,M] in dtype; the weight is kept as the kernels read it, packed once
+ * from int8 [M,K] with scales of the caller's or from float rows by the same rule.
+ * The integer sums are exact.  A token with an infinity or a NaN has NaN in
+ * all its outputs. */
+typedef struct mgpt_i8_config {
+  int in_features;    /* K: 1 .. 2^17 */
+  int out_features;   /* M: 1 .. 2^24 */
+  int dtype;          /* of x and y: MGPT_DTYPE_F32 or MGPT_DTYPE_BF16 */
+} mgpt_i8_config;
+
+/* Size of the packed weight (256-byte aligned device memory of the caller's). */
+int mgpt_i8_weight_bytes(const mgpt_i8_config* cfg, size_t* bytes);
+/* weight: [M,K] in weight_dtype (fp32 or bf16); scales: [M] fp32, written. */
+int mgpt_i8_pack_weight(const mgpt_i8_config* cfg, const void* weight, int weight_dtype, void* packed,
+                        float* scales, void* stream);
+/* weight: [M,K] int8, row-major. */
+int mgpt_i8_pack_quantized(const mgpt_i8_config* cfg, const int8_t* weight, void* packed, void* stream);
+
+int mgpt_i8_linear_workspace_bytes(const mgpt_i8_config* cfg, int num_tokens, size_t* bytes);
+/* bias: [M] fp32 or null.  num_tokens up to 2^21.  workspace: 256-byte aligned. */
+int mgpt_i8_linear_forward(const mgpt_i8_config* cfg, const void* x, const void* packed,
+                           const float* scales, const float* bias, void* y, int num_tokens,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* Description of the last error on this host thread ("" if none). */
 const char* mgpt_moe_last_error(void);
 

@@ -75,6 +75,10 @@ class RouteConfig(ctypes.Structure):
                 ("renormalise", ctypes.c_int), ("scale", ctypes.c_float), ("dtype", ctypes.c_int)]
 
 
+class I8Config(ctypes.Structure):
+    _fields_ = [("in_features", ctypes.c_int), ("out_features", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
 class MoEError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"mgpt_moe status {status}: {message}")
@@ -138,6 +142,11 @@ def lib() -> ctypes.CDLL:
         "mgpt_route_forward": [ctypes.POINTER(RouteConfig)] + [vp] * 5 + [i, vp],
         "mgpt_route_backward": [ctypes.POINTER(RouteConfig)] + [vp] * 6 + [i, vp],
         "mgpt_route_balance": [i, vp, ctypes.c_float, vp, vp],
+        "mgpt_i8_weight_bytes": [ctypes.POINTER(I8Config), ctypes.POINTER(sz)],
+        "mgpt_i8_pack_weight": [ctypes.POINTER(I8Config), vp, i, vp, vp, vp],
+        "mgpt_i8_pack_quantized": [ctypes.POINTER(I8Config), vp, vp, vp],
+        "mgpt_i8_linear_workspace_bytes": [ctypes.POINTER(I8Config), i, ctypes.POINTER(sz)],
+        "mgpt_i8_linear_forward": [ctypes.POINTER(I8Config)] + [vp] * 5 + [i, vp, sz, vp],
     }
     for name, args in sig.items():
         f = getattr(L, name)
