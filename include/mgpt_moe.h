@@ -44,7 +44,8 @@ typedef enum mgpt_status {
 typedef enum mgpt_dtype {
   MGPT_DTYPE_F32 = 0,
   MGPT_DTYPE_BF16 = 1,
-  MGPT_DTYPE_FP8_E4M3 = 2          /* OCP E4M3FN, per-output-channel fp32 scale */
+  MGPT_DTYPE_FP8_E4M3 = 2,         /* OCP E4M3FN, per-output-channel fp32 scale */
+  MGPT_DTYPE_I8 = 3                /* 8-bit integers, a fp32 scale for each output channel and row */
 } mgpt_dtype;
 
 /* Shape and precision of one MoE block.  Replaces the constructor arguments
@@ -60,10 +61,13 @@ typedef struct mgpt_moe_config {
                         gradients) */
   int top_k;         /* k: 1..min(E, 8) */
   int act_dtype;     /* x and y: MGPT_DTYPE_F32 or MGPT_DTYPE_BF16 */
-  int weight_dtype;  /* F32 (act F32 only), BF16 or FP8_E4M3.  With act F32
+  int weight_dtype;  /* F32 (act F32 only), BF16, FP8_E4M3 or I8.  With act F32
                         and BF16 / FP8 weights the caller's tensors stay fp32:
                         routing on the fp32 rows, expert products in bf16,
-                        fp32 outputs (inference only) */
+                        fp32 outputs (inference only).  I8 (inference only):
+                        the experts' rows and hidden units are quantised with a
+                        scale each (as mgpt_i8_linear_forward's) and both
+                        products run in integers */
 } mgpt_moe_config;
 
 typedef struct mgpt_moe mgpt_moe;   /* opaque handle; owns packed weights */
@@ -537,6 +541,22 @@ int mgpt_route_forward(const mgpt_route_config* cfg, const void* logits, const f
 int mgpt_route_backward(const mgpt_route_config* cfg, const void* logits, const int32_t* idx,
                         const float* weights, const float* dweights, const float* dscores,
                         void* dlogits, int num_tokens, void* stream);
+
+/* Runs the layer with this rule instead of the engine's, or (cfg null) with the engine's again:
+ * forward, block and training entry points alike.  The layer's logits are those of its router weights in fp32
+ * (cfg->dtype: F32; num_experts and top_k the layer's).  bias: device [E] fp32 or null, read by
+ * every forward from then on (it may be updated in place; the caller keeps it alive).  balance >= 0: the factor of
+ * the load-balance loss whose gradient the backward adds to every token's
+ * scores, balance E (counts[e] / N) / N (the engine's router: 0.01).  Workspaces grow with it: query them
+ * again.  A backward needs a training forward under the same setting. */
+int mgpt_moe_set_routing(mgpt_moe* h, const mgpt_route_config* cfg, const float* bias, float balance);
+
+/* mgpt_moe_forward with a routing that is given: idx, weights [N,k] device memory, y[t] = the sum of
+ * weights[t][j] expert(idx[t][j])(x[t]).  An idx outside 0 .. E - 1 counts as expert 0 with weight 0; the
+ * same expert may come twice.  Inference only. */
+int mgpt_moe_forward_routed(mgpt_moe* h, const void* x, const int32_t* idx, const float* weights,
+                            void* y, int num_tokens, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 /* bias[e] += rate where counts[e] is below the counts' mean, -= rate above it. */
 int mgpt_route_balance(int num_experts, const int32_t* counts, float rate, float* bias,

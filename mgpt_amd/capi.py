@@ -26,7 +26,7 @@ MGPT_ERR_HIP = 5
 MGPT_ERR_OUT_OF_MEMORY = 6
 
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
-DTYPE_F32, DTYPE_BF16, DTYPE_FP8_E4M3 = 0, 1, 2
+DTYPE_F32, DTYPE_BF16, DTYPE_FP8_E4M3, DTYPE_I8 = 0, 1, 2, 3
 NUM_STAGES = 5
 STAGE_NAMES = ["router_topk", "permute", "gemm_gateup", "gemm_down", "combine"]
 NUM_BWD_STAGES = 7
@@ -139,6 +139,8 @@ def lib() -> ctypes.CDLL:
         "mgpt_norm_forward": [ctypes.POINTER(NormConfig)] + [vp] * 9 + [i, vp],
         "mgpt_norm_backward_workspace_bytes": [ctypes.POINTER(NormConfig), i, ctypes.POINTER(sz)],
         "mgpt_norm_backward": [ctypes.POINTER(NormConfig)] + [vp] * 14 + [i, vp, sz, vp],
+        "mgpt_moe_set_routing": [vp, ctypes.POINTER(RouteConfig), vp, ctypes.c_float],
+        "mgpt_moe_forward_routed": [vp, vp, vp, vp, vp, i, vp, sz, vp],
         "mgpt_route_forward": [ctypes.POINTER(RouteConfig)] + [vp] * 5 + [i, vp],
         "mgpt_route_backward": [ctypes.POINTER(RouteConfig)] + [vp] * 6 + [i, vp],
         "mgpt_route_balance": [i, vp, ctypes.c_float, vp, vp],

@@ -476,6 +476,25 @@ hipError_t launch_scatter_bwd(const ActT* dy, const ActT* ye, const int32_t* per
   return hipGetLastError();
 }
 
+// dx from the logits' gradients dL.
+template <typename ActT>
+hipError_t launch_token_dx(const ActT* dxe, const int32_t* slot_of, const float* dL, const float* wrt, int N, int C,
+                           int E, int k, ActT* dx, hipStream_t stream) {
+  if (N <= 0) return hipSuccess;
+  if (E > kMaxExpertsWide || k > kMaxTopK || C % 8) return hipErrorInvalidValue;
+  const dim3 gdx((N + kDxTokens - 1) / kDxTokens, (C + 511) / 512);
+  if (E > 256)
+    hipLaunchKernelGGL((token_dx_kernel<ActT, kMaxExpertsWide>), gdx, dim3(64), 0, stream, dxe,
+                       slot_of, dL, wrt, N, C, E, k, dx);
+  else if (E > kMaxExperts)
+    hipLaunchKernelGGL((token_dx_kernel<ActT, 256>), gdx, dim3(64), 0, stream, dxe,
+                       slot_of, dL, wrt, N, C, E, k, dx);
+  else
+    hipLaunchKernelGGL((token_dx_kernel<ActT, kMaxExperts>), gdx, dim3(64), 0, stream, dxe,
+                       slot_of, dL, wrt, N, C, E, k, dx);
+  return hipGetLastError();
+}
+
 template <typename ActT>
 hipError_t launch_token_bwd(const ActT* dxe, const int32_t* slot_of, const int32_t* topk_idx,
                             const float* dtp, const float* probs, const int32_t* counts,
@@ -498,17 +517,7 @@ hipError_t launch_token_bwd(const ActT* dxe, const int32_t* slot_of, const int32
   else
     hipLaunchKernelGGL(token_dl_kernel<64>, dim3((N + 3) / 4), dim3(256), 0, stream, topk_idx,
                        dtp, probs, counts, N, E, k, dL);
-  const dim3 gdx((N + kDxTokens - 1) / kDxTokens, (C + 511) / 512);
-  if (E > 256)
-    hipLaunchKernelGGL((token_dx_kernel<ActT, kMaxExpertsWide>), gdx, dim3(64), 0, stream, dxe,
-                       slot_of, dL, wrt, N, C, E, k, dx);
-  else if (E > kMaxExperts)
-    hipLaunchKernelGGL((token_dx_kernel<ActT, 256>), gdx, dim3(64), 0, stream, dxe,
-                       slot_of, dL, wrt, N, C, E, k, dx);
-  else
-    hipLaunchKernelGGL((token_dx_kernel<ActT, kMaxExperts>), gdx, dim3(64), 0, stream, dxe,
-                       slot_of, dL, wrt, N, C, E, k, dx);
-  return hipGetLastError();
+  return launch_token_dx<ActT>(dxe, slot_of, dL, wrt, N, C, E, k, dx, stream);
 }
 
 int router_wgrad_chunks(int N) { return (N + kRwChunk - 1) / kRwChunk; }
@@ -838,6 +847,8 @@ hipError_t launch_transpose_pad(const T* src, int src_rows, int src_cols, size_t
                                           const float*, const float*, const int32_t*,          \
                                           const float*, int, int, int, int, T*, float*,        \
                                           hipStream_t);                                        \
+  template hipError_t launch_token_dx<T>(const T*, const int32_t*, const float*, const float*, \
+                                         int, int, int, int, T*, hipStream_t);                 \
   template hipError_t launch_router_wgrad<T>(const T*, const float*, int, int, int, float*,    \
                                              float*, float*, float*, bool, const float*,       \
                                              const float*, hipStream_t);                       \

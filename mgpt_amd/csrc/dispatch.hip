@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256) void permute_kernel(
   const int qf = q0 + tid % W;
   // The rows do not depend on the slots: the first batch is loaded before
   // the ranking, so its latency overlaps the histogram and id loads.
-  const bool have_pre = rr < R && qf < q1 && rr < ntok;
+  const bool have_pre = xg && rr < R && qf < q1 && rr < ntok;
   Chunk pre[U];
   if (have_pre) {
 #pragma unroll
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256) void permute_kernel(
   }
   __syncthreads();
   // Row copy (a narrow slice still keeps nearly every lane busy).
-  if (rr < R) {
+  if (xg && rr < R) {
     for (int q = qf; q < q1; q += W) {
       for (int r0 = rr; r0 < ntok; r0 += R * U) {
         Chunk in[U];
@@ -346,7 +346,8 @@ __global__ __launch_bounds__(256) void permute_kernel(
 
 // rstd / gamma (both null, or both set): the fused block gathers
 // (x * rstd[t]) * gamma instead of x.  InT: the caller's rows (fp32 rows may
-// feed a bf16 gather); ActT: the gathered rows.
+// feed a bf16 gather); ActT: the gathered rows.  xg null: no row is copied (the
+// 8-bit integer experts quantise them as they gather).
 template <typename InT, typename ActT>
 hipError_t launch_permute(const InT* x, const int32_t* topk_idx, const int32_t* hist,
                           int32_t* base, int N, int C, int E, int k, int32_t* counts,
@@ -363,7 +364,7 @@ hipError_t launch_permute(const InT* x, const int32_t* topk_idx, const int32_t* 
   // Column slices: enough blocks for ~512 in all, each slice >= 8 chunks
   // (128 bytes of a row).
   const int chunks = C * (int)sizeof(ActT) / 16;
-  const int slices = max(1, min(chunks / 8, (512 + nb - 1) / nb));
+  const int slices = xg ? max(1, min(chunks / 8, (512 + nb - 1) / nb)) : 1;
   hipLaunchKernelGGL((permute_kernel<InT, ActT>), dim3(nb, slices), dim3(256), 0, stream, x, topk_idx,
                      hist, fold ? nullptr : base, nb, N, C, E, k, counts, perm, slot_of, xg, rstd,
                      gamma);

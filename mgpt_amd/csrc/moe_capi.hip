@@ -20,6 +20,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <mutex>
 #include <cstdio>
@@ -33,6 +34,8 @@
 #include "../../include/mgpt_moe.h"
 #include "capi_internal.hpp"
 #include "common.hpp"
+#include "i8.hpp"
+#include "route.hpp"
 
 namespace mgpt {
 // kernels (router.hip, dispatch.hip, combine.hip, pack.hip and the gemm_*.hip)
@@ -40,6 +43,9 @@ template <typename ActT>
 hipError_t launch_router(const ActT*, const float*, const float*, const float*, const float*, int,
                          int, int, int, int32_t*, float*, int32_t*, float*, float*, const float*,
                          float, int, float*, float*, hipStream_t);
+template <typename ActT>
+hipError_t launch_router_logits(const ActT*, const float*, const float*, const float*, int, int, int, float*,
+                                const float*, float, int, float*, float*, hipStream_t);
 hipError_t launch_expf_probe(const float*, float*, int, hipStream_t);
 template <typename InT, typename ActT>
 hipError_t launch_permute(const InT*, const int32_t*, const int32_t*, int32_t*, int, int, int,
@@ -91,6 +97,9 @@ template <typename ActT>
 hipError_t launch_token_bwd(const ActT*, const int32_t*, const int32_t*, const float*,
                             const float*, const int32_t*, const float*, int, int, int, int, ActT*,
                             float*, hipStream_t);
+template <typename ActT>
+hipError_t launch_token_dx(const ActT*, const int32_t*, const float*, const float*, int, int, int, int, ActT*,
+                           hipStream_t);
 int router_wgrad_chunks(int N);
 template <typename ActT>
 hipError_t launch_router_wgrad(const ActT*, const float*, int, int, int, float*, float*, float*,
@@ -160,6 +169,12 @@ struct Layout {
   size_t wg_part2;
   size_t dypad, dxpad;   // padded width: dy and dx at width C
   size_t nrm_part;       // fused block backward: ln2 scale-gradient partials
+  // 8-bit integer experts: the gathered rows and the hidden units as row blocks with their
+  // scales, and the hidden units' exponents
+  size_t xq, xs, hq, hs, hexp;
+  // a routing of the caller's rule: logits [N][E], and the scores' gradients [E]; last, so
+  // that the other regions lie where they do without it
+  size_t rlogits, dscore;
   size_t total;
 };
 
@@ -222,8 +237,8 @@ struct mgpt_moe {
   // [E][Npad/256][K/128][256][128] (null when the shape does not tile)
   void* wgu_t = nullptr;
   void* wd_t = nullptr;
-  float* sgu = nullptr;    // fp8 scales [E][2Hp] (packed-row order)
-  float* sd = nullptr;     // fp8 scales [E][Cp]
+  float* sgu = nullptr;    // fp8 and int8 scales [E][2Hp] (packed-row order)
+  float* sd = nullptr;     // fp8 and int8 scales [E][Cp]
   float* bg = nullptr;     // [E][Hp]
   float* bu = nullptr;     // [E][Hp]
   float* bd = nullptr;     // [E][Cp]
@@ -278,6 +293,13 @@ struct mgpt_moe {
   int dact_cus = 0;   // persistent blocks of the d(act) product when forked
   int dx_cus = 0;     // persistent blocks of the dX product beside the gate/up weight gradient (0: serial)
   const int32_t* last_counts = nullptr;
+  // mgpt_moe_set_routing: the rule in place of the engine's, its bias and balance loss, how
+  // often it was set and its number at the last training forward
+  bool routed = false;
+  mgpt_route_config route{};
+  const float* route_bias = nullptr;
+  float route_balance = 0.0f;
+  unsigned route_set = 0, route_trained = 0;
 
   size_t act_bytes() const { return act == MGPT_DTYPE_BF16 ? 2 : 4; }
   size_t io_bytes() const { return io == MGPT_DTYPE_BF16 ? 2 : 4; }
@@ -309,7 +331,15 @@ struct mgpt_moe {
   // 200, 62 rows 226 / 200; 222 / 209.  E = 64, C = 2048, H = 1408: 44 rows 239 /
   // 243; 233 / 253, 62 rows 279 / 254; 282 / 272.
   bool fp8_decode(int N) const { return wgu_t && !wide() && (size_t)N * k < (size_t)64 * E; }
-  size_t w_bytes() const { return wdt == MGPT_DTYPE_FP8_E4M3 ? 1 : (wdt == MGPT_DTYPE_BF16 ? 2 : 4); }
+  size_t w_bytes() const {
+    return wdt == MGPT_DTYPE_FP8_E4M3 || wdt == MGPT_DTYPE_I8 ? 1 : (wdt == MGPT_DTYPE_BF16 ? 2 : 4);
+  }
+  bool i8() const { return wdt == MGPT_DTYPE_I8; }
+  // row blocks that A rows of E experts make up at most
+  size_t row_blocks(size_t A) const { return A / kI8Rows + std::min((size_t)E, A); }
+  // bytes of an expert's gate/up and down operands in 8-bit integers
+  size_t i8_gu_bytes() const { return (size_t)(2 * Hp / kI8Rows) * i8_row_block_bytes(C); }
+  size_t i8_d_bytes() const { return (size_t)(Cp / kI8Rows) * i8_row_block_bytes(Hp); }
   // h (SwiGLU output) is kept in the activation dtype.
   Layout layout(int N, bool train = false) const {
     Layout L{};
@@ -333,7 +363,7 @@ struct mgpt_moe {
     // never shrinks as N grows past 4095 (every N when E > 64: the wide
     // forward always routes through the logits)
     L.logits = take(E > 16 ? (size_t)(wide() ? N : std::min(N, 4095)) * E * 4 : 0);
-    L.xg = take((A + kRowPad) * C * act_bytes());
+    L.xg = take(i8() ? 0 : (A + kRowPad) * C * act_bytes());
     L.hbuf = take((A + kRowPad) * Hp * act_bytes());
     L.obuf = take((A + kRowPad) * C * act_bytes());
     // fp32 partial tiles of the large-M GEMMs' split last round (one per CU)
@@ -358,6 +388,18 @@ struct mgpt_moe {
       L.dxpad = take(pad_rows);
       L.nrm_part = take((size_t)rmsnorm_bwd_blocks(N) * C * 4);
     }
+    if (i8()) {
+      const size_t blocks = row_blocks(A);
+      L.xq = take(blocks * i8_row_block_bytes(C));
+      L.xs = take(blocks * kI8Rows * 4);
+      L.hq = take(blocks * i8_row_block_bytes(Hp));
+      L.hs = take(blocks * kI8Rows * 4);
+      L.hexp = take(A * (Hp / 32));
+    }
+    if (routed) {
+      L.rlogits = take((size_t)N * E * 4);
+      L.dscore = take((size_t)E * 4);
+    }
     L.total = off;
     return L;
   }
@@ -380,7 +422,8 @@ int check_config(const mgpt_moe_config* c) {
   // fp32 activations with bf16 / fp8 weights: the caller's tensors stay
   // fp32 (routing on the fp32 rows), the expert products run in bf16.
   const bool f32 = c->act_dtype == MGPT_DTYPE_F32 && c->weight_dtype == MGPT_DTYPE_F32;
-  const bool lowp_w = c->weight_dtype == MGPT_DTYPE_BF16 || c->weight_dtype == MGPT_DTYPE_FP8_E4M3;
+  const bool lowp_w = c->weight_dtype == MGPT_DTYPE_BF16 || c->weight_dtype == MGPT_DTYPE_FP8_E4M3 ||
+                      c->weight_dtype == MGPT_DTYPE_I8;
   const bool bf = (c->act_dtype == MGPT_DTYPE_BF16 || c->act_dtype == MGPT_DTYPE_F32) && lowp_w;
   if (!f32 && !bf)
     return fail(MGPT_ERR_UNSUPPORTED, "unsupported dtype pair act=%d weight=%d", c->act_dtype,
@@ -400,8 +443,8 @@ void free_weights(mgpt_moe* h) {
   h->bwd_ready = h->bwd_filled = h->bwd_used = false;
 }
 
-// Training is built for bf16 x bf16 and fp32 x fp32 handles (fp8 weights
-// are an inference format here, and fp32 tensors over bf16 products an
+// Training is built for bf16 x bf16 and fp32 x fp32 handles (fp8 and int8
+// weights are inference formats here, and fp32 tensors over bf16 products an
 // inference option).
 bool trainable(const mgpt_moe* h) { return h->wdt == h->act && h->io == h->act; }
 
@@ -589,7 +632,7 @@ int mgpt_moe_load_parameters(mgpt_moe* h, const float* const* params, int num_pa
   HIP_TRY(hipSetDevice(h->device));
   const int C = h->C, Cx = h->Cx, H = h->H, E = h->E, Hp = h->Hp, Cp = h->Cp;
   const size_t wb = h->w_bytes();
-  const bool fp8 = h->wdt == MGPT_DTYPE_FP8_E4M3;
+  const bool fp8 = h->wdt == MGPT_DTYPE_FP8_E4M3, i8 = h->i8(), q8 = fp8 || i8;
   const bool bf = h->wdt == MGPT_DTYPE_BF16;
   const int RE = router_experts_per_wave(E);
   // The packed buffers depend only on the handle's shape: the first load
@@ -609,14 +652,19 @@ int mgpt_moe_load_parameters(mgpt_moe* h, const float* const* params, int num_pa
     HIP_TRY(hipMalloc(&h->bg, sizeof(float) * E * Hp));
     HIP_TRY(hipMalloc(&h->bu, sizeof(float) * E * Hp));
     HIP_TRY(hipMalloc(&h->bd, sizeof(float) * E * Cp));
-    if (fp8) {
+    if (q8) {
       HIP_TRY(hipMalloc(&h->sgu, sizeof(float) * E * 2 * Hp));
       HIP_TRY(hipMalloc(&h->sd, sizeof(float) * E * Cp));
     }
-    HIP_TRY(hipMalloc(&h->wd, wb * E * Cp * Hp));
-    HIP_TRY(hipMemsetAsync(h->wd, 0, wb * E * Cp * Hp, st));
-    HIP_TRY(hipMalloc(&h->wgu, wb * E * 2 * Hp * C));
-    HIP_TRY(hipMemsetAsync(h->wgu, 0, wb * E * 2 * Hp * C, st));
+    if (i8) {   // (every byte is written by the packs)
+      HIP_TRY(hipMalloc(&h->wd, E * h->i8_d_bytes()));
+      HIP_TRY(hipMalloc(&h->wgu, E * h->i8_gu_bytes()));
+    } else {
+      HIP_TRY(hipMalloc(&h->wd, wb * E * Cp * Hp));
+      HIP_TRY(hipMemsetAsync(h->wd, 0, wb * E * Cp * Hp, st));
+      HIP_TRY(hipMalloc(&h->wgu, wb * E * 2 * Hp * C));
+      HIP_TRY(hipMemsetAsync(h->wgu, 0, wb * E * 2 * Hp * C, st));
+    }
   }
 
   // Host parameters are staged through one device buffer, the router's two
@@ -626,10 +674,10 @@ int mgpt_moe_load_parameters(mgpt_moe* h, const float* const* params, int num_pa
   const size_t sizes[6] = {CH, (size_t)H, CH, (size_t)H, CH, (size_t)Cx};
   const size_t stage_elems = std::max(up4((size_t)Cx * E) + up4(E), 3 * up4(CH) + 2 * up4(H) + up4(Cx));
   if (!params_on_device && !h->stage) HIP_TRY(hipMalloc(&h->stage, sizeof(float) * stage_elems));
-  if (fp8 && !h->stage_tmp)
+  if (q8 && !h->stage_tmp)
     HIP_TRY(hipMalloc(&h->stage_tmp,
                       sizeof(float) * std::max<size_t>((size_t)2 * Hp * C, (size_t)Cp * Hp)));
-  float* fp32tmp = h->stage_tmp;   // fp8: packed fp32 before quantisation
+  float* fp32tmp = h->stage_tmp;   // fp8, int8: packed fp32 before quantisation
   int rc = MGPT_OK;
   // Device addresses of parameters i0 .. i0+n-1 (sizes sz) in p.
   auto fetch = [&](int i0, int n, const size_t* sz, const float** p) -> bool {
@@ -672,7 +720,7 @@ int mgpt_moe_load_parameters(mgpt_moe* h, const float* const* params, int num_pa
       break;
     }
     if (!staged()) break;
-    if (!fp8) {
+    if (!q8) {
       // one launch per group of experts; host sources go expert by expert
       const int step = params_on_device ? kMaxExperts : 1;
       for (int e0 = 0; e0 < E && rc == MGPT_OK; e0 += step) {
@@ -700,28 +748,48 @@ int mgpt_moe_load_parameters(mgpt_moe* h, const float* const* params, int num_pa
       }
       break;
     }
+    // int8 rows, as row blocks
+    auto quantize = [&](int rows, int K, char* q, float* scale) {
+      QuantizeArgs a{};
+      a.src = fp32tmp;
+      a.ld = K;
+      a.N = rows;
+      a.K = K;
+      a.q = q;
+      a.scale = scale;
+      return launch_i8_quantize(kRowsF32, a, rows / kI8Rows, st);
+    };
+    auto clear = [&](size_t n) {   // (a captured load takes no memset)
+      return i8 ? launch_fill_zero(fp32tmp, n, st) : hipMemsetAsync(fp32tmp, 0, sizeof(float) * n, st);
+    };
     for (int e = 0; e < E && rc == MGPT_OK; ++e) {
       const float* s[6];
       if (!fetch(2 + 6 * e, 6, sizes, s)) break;
       const size_t gu_off = (size_t)e * 2 * Hp * C;
       const size_t d_off = (size_t)e * Cp * Hp;
-      HIP_TRY(hipMemsetAsync(fp32tmp, 0, sizeof(float) * 2 * Hp * C, st));
+      HIP_TRY(clear((size_t)2 * Hp * C));
       for (int which = 0; which < 2; ++which) {   // gate, up
         // [Cx][H] -> rows of the packed [2Hp][C]: columns past Cx stay zero
         HIP_TRY(launch_pack_transpose(s[2 * which], Cx, H, fp32tmp, C, 1, 32 * which, st));
         HIP_TRY(launch_pad_row(s[2 * which + 1], H, (which ? h->bu : h->bg) + (size_t)e * Hp, Hp, st));
       }
-      HIP_TRY(launch_quantize_rows(fp32tmp, 2 * Hp, C, (uint8_t*)h->wgu + gu_off,
-                                   h->sgu + (size_t)e * 2 * Hp, st));
+      if (i8)
+        HIP_TRY(quantize(2 * Hp, C, (char*)h->wgu + e * h->i8_gu_bytes(), h->sgu + (size_t)e * 2 * Hp));
+      else
+        HIP_TRY(launch_quantize_rows(fp32tmp, 2 * Hp, C, (uint8_t*)h->wgu + gu_off,
+                                     h->sgu + (size_t)e * 2 * Hp, st));
       // [H][Cx] -> rows 0..Cx of the packed [Cp][Hp]; the rest stay zero
-      HIP_TRY(hipMemsetAsync(fp32tmp, 0, sizeof(float) * Cp * Hp, st));
+      HIP_TRY(clear((size_t)Cp * Hp));
       HIP_TRY(launch_pack_transpose(s[4], H, Cx, fp32tmp, Hp, 0, 0, st));
-      HIP_TRY(launch_quantize_rows(fp32tmp, Cp, Hp, (uint8_t*)h->wd + d_off,
-                                   h->sd + (size_t)e * Cp, st));
+      if (i8)
+        HIP_TRY(quantize(Cp, Hp, (char*)h->wd + e * h->i8_d_bytes(), h->sd + (size_t)e * Cp));
+      else
+        HIP_TRY(launch_quantize_rows(fp32tmp, Cp, Hp, (uint8_t*)h->wd + d_off,
+                                     h->sd + (size_t)e * Cp, st));
       HIP_TRY(launch_pad_row(s[5], Cx, h->bd + (size_t)e * Cp, Cp, st));
       if (!staged()) break;
     }
-    if (rc == MGPT_OK && C % 128 == 0 && Hp % 128 == 0 && Cp % 256 == 0) {
+    if (rc == MGPT_OK && fp8 && C % 128 == 0 && Hp % 128 == 0 && Cp % 256 == 0) {
       // the decode stream's contiguous 32 KB stage tiles (a second copy)
       if (!h->wgu_t) HIP_TRY(hipMalloc(&h->wgu_t, (size_t)E * 2 * Hp * C));
       if (!h->wd_t) HIP_TRY(hipMalloc(&h->wd_t, (size_t)E * Cp * Hp));
@@ -802,7 +870,77 @@ namespace {
 struct BlockArgs {
   const float* gamma = nullptr;
   float eps = 0.0f;
+  // a routing that is given: idx and weights [N][k]
+  const int32_t* idx = nullptr;
+  const float* weights = nullptr;
 };
+
+// The experts in 8-bit integers: rows of x (normalised, with gamma) quantised as they are gathered,
+// gate/up with SwiGLU, the hidden units quantised in turn, down.
+template <typename IoT, typename Mark>
+int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, const float* gamma, size_t A,
+               const int32_t* counts, const int32_t* perm, char* ws, hipStream_t st, Mark mark) {
+  const int C = h->C, Hp = h->Hp, Cp = h->Cp, E = h->E;
+  const int blocks = (int)h->row_blocks(A);
+  const HiddenRows hidden{(int16_t*)(ws + L.hbuf), (uint8_t*)(ws + L.hexp), Hp};
+  QuantizeArgs q{};
+  q.src = x;
+  q.ld = C;
+  q.K = C;
+  q.counts = counts;
+  q.perm = perm;
+  q.E = E;
+  q.k = h->k;
+  q.rstd = rstd;
+  q.gamma = gamma;
+  q.q = ws + L.xq;
+  q.scale = (float*)(ws + L.xs);
+  HIP_TRY(launch_i8_quantize(sizeof(IoT) == 4 ? kRowsF32 : kRowsBf16, q, blocks, st));
+  I8Args g{};
+  g.A = ws + L.xq;
+  g.sa = (const float*)(ws + L.xs);
+  g.B = (const char*)h->wgu;
+  g.sb = h->sgu;
+  g.b_expert = h->i8_gu_bytes();
+  g.ldsb = 2 * Hp;
+  g.KT = (C + kI8Slab - 1) / kI8Slab;
+  g.Nf = 2 * Hp;
+  g.b_blocks = 2 * Hp / kI8Rows;
+  g.bias0 = h->bg;
+  g.bias1 = h->bu;
+  g.bias_ld = Hp;
+  g.counts = counts;
+  g.E = E;
+  g.N = (int)A;
+  g.h = hidden;
+  HIP_TRY(launch_i8_gemm(kI8GateUp, g, h->num_cus, st));
+  HIP_TRY(mark(3));
+  QuantizeArgs qh{};
+  qh.h = hidden;
+  qh.K = Hp;
+  qh.counts = counts;
+  qh.E = E;
+  qh.k = h->k;
+  qh.q = ws + L.hq;
+  qh.scale = (float*)(ws + L.hs);
+  HIP_TRY(launch_i8_quantize(kRowsHidden, qh, blocks, st));
+  g.A = ws + L.hq;
+  g.sa = (const float*)(ws + L.hs);
+  g.B = (const char*)h->wd;
+  g.sb = h->sd;
+  g.b_expert = h->i8_d_bytes();
+  g.ldsb = Cp;
+  g.KT = Hp / kI8Slab;
+  g.Nf = C;
+  g.b_blocks = Cp / kI8Rows;
+  g.bias0 = h->bd;
+  g.bias1 = nullptr;
+  g.bias_ld = Cp;
+  g.out = ws + L.obuf;
+  g.ldo = C;
+  HIP_TRY(launch_i8_gemm(kI8Bf16, g, h->num_cus, st));
+  return MGPT_OK;
+}
 
 // IoT: the caller's x and y; ActT: the gathered rows, h and expert outputs.
 template <typename IoT, typename ActT>
@@ -861,9 +999,25 @@ int forward_impl(mgpt_moe* h, const IoT* x, IoT* y, int N, char* ws, bool train,
   float* rstd = gamma ? (float*)(ws + L.rstd) : nullptr;
   // the router's normalised fp32 rows, where the permuted rows and h come later
   float* xn = gamma && (size_t)N * C * 4 <= L.obuf - L.xg ? (float*)(ws + L.xg) : nullptr;
-  HIP_TRY(launch_router<IoT>(xi, h->wr_g, h->wr1, h->wr4, h->br, N, C, E,
-                             k, idx, topp, hist, logits,
-                             probs, gamma, blk.eps, Cx, rstd, xn, st));
+  int32_t* block_hist = N <= kPermuteCountTokens ? nullptr : hist;
+  if (blk.idx) {
+    HIP_TRY(launch_route_take(blk.idx, blk.weights, N, E, k, idx, topp, block_hist, st));
+  } else if (h->routed) {
+    float* rl = (float*)(ws + L.rlogits);
+    HIP_TRY(launch_router_logits<IoT>(xi, h->wr1, h->wr4, h->br, N, C, E, rl, gamma, blk.eps, Cx, rstd, xn, st));
+    RouteArgs ra = route_args(&h->route, rl, nullptr, N);
+    ra.bias = h->route_bias;
+    ra.idx = idx;
+    ra.weights = topp;
+    HIP_TRY(launch_route(&h->route, ra, false, st));
+    if (block_hist) HIP_TRY(launch_route_take(nullptr, nullptr, N, E, k, idx, topp, block_hist, st));
+    if (train) h->route_trained = h->route_set;
+  } else {
+    HIP_TRY(launch_router<IoT>(xi, h->wr_g, h->wr1, h->wr4, h->br, N, C, E,
+                               k, idx, topp, hist, logits,
+                               probs, gamma, blk.eps, Cx, rstd, xn, st));
+    if (train) h->route_trained = h->route_set;
+  }
   HIP_TRY(mark(1));
   // A decode step of at most 512 flat ids (N * k) with fp8 weights (no
   // training caches): the gate/up weight-streaming GEMM routes the ids
@@ -872,10 +1026,12 @@ int forward_impl(mgpt_moe* h, const IoT* x, IoT* y, int N, char* ws, bool train,
   const bool gather_decode = !train && !gamma && h->fp8_decode(N) &&
                              A <= (size_t)kRouterTokens * kMaxTopK;
   if (!gather_decode)
-    HIP_TRY((launch_permute<IoT, ActT>(xi, idx, N <= kPermuteCountTokens ? nullptr : hist, base, N,
-                                       C, E, k, counts, perm, slot_of, xg, rstd, gamma, st)));
+    HIP_TRY((launch_permute<IoT, ActT>(xi, idx, block_hist, base, N, C, E, k, counts, perm, slot_of,
+                                       h->i8() ? nullptr : xg, rstd, gamma, st)));
   HIP_TRY(mark(2));
-  if constexpr (sizeof(ActT) == 4) {
+  if (h->i8()) {
+    if (int rc = i8_experts<IoT>(h, L, xi, rstd, gamma, A, counts, perm, ws, st, mark)) return rc;
+  } else if constexpr (sizeof(ActT) == 4) {
     HIP_TRY(launch_gemm_f32<kEpiGateUp>(xg, (const float*)h->wgu, h->bg, h->bu, counts, E, C, 2 * Hp,
                                         2 * Hp, Hp, hb, Hp, A, gu, 2 * Hp, h->num_cus, st));
     HIP_TRY(mark(3));
@@ -1143,8 +1299,21 @@ int backward_impl(mgpt_moe* h, const ActT* x, const ActT* dy, ActT* dx, int N, c
   if (!gateup_done)
     if (int rc = gateup_wgrad(wpart, st)) return rc;
   HIP_TRY(mark(5));
-  HIP_TRY(launch_token_bwd<ActT>(ob, slot_of, idx, dtp, probs, counts, h->wrt, N, C, E, k, dx,
-                                 dlog, st));
+  if (h->routed) {
+    float* dscore = h->route_balance != 0.0f ? (float*)(ws + L.dscore) : nullptr;
+    if (dscore) HIP_TRY(launch_route_dscore(counts, E, N, h->route_balance, dscore, st));
+    RouteArgs ra = route_args(&h->route, ws + L.rlogits, dlog, N);
+    ra.bidx = idx;
+    ra.bw = topp;
+    ra.dw = dtp;
+    ra.dscore = dscore;
+    ra.dlogits = dlog;
+    HIP_TRY(launch_route(&h->route, ra, true, st));
+    HIP_TRY(launch_token_dx<ActT>(ob, slot_of, dlog, h->wrt, N, C, E, k, dx, st));
+  } else {
+    HIP_TRY(launch_token_bwd<ActT>(ob, slot_of, idx, dtp, probs, counts, h->wrt, N, C, E, k, dx,
+                                   dlog, st));
+  }
   HIP_TRY(mark(6));
   HIP_TRY(launch_router_wgrad<ActT>(x, dlog, N, C, E, (float*)(ws + L.rw_part),
                                     (float*)(ws + L.rw_part_b), g + h->g_off[0], g + h->g_off[1],
@@ -1279,6 +1448,39 @@ int mgpt_moe_forward_block(mgpt_moe* h, const void* x, const float* gamma, float
   return dispatch_forward(h, x, out, num_tokens, (char*)workspace, false, st, blk);
 }
 
+int mgpt_moe_set_routing(mgpt_moe* h, const mgpt_route_config* cfg, const float* bias, float balance) {
+  if (!h) return fail(MGPT_ERR_INVALID_ARGUMENT, "null handle");
+  if (cfg) {
+    if (int rc = check_route(cfg, 0)) return rc;
+    if (cfg->num_experts != h->E || cfg->top_k != h->k)
+      return fail(MGPT_ERR_INVALID_ARGUMENT, "the routing takes %d of %d experts, the layer %d of %d", cfg->top_k,
+                  cfg->num_experts, h->k, h->E);
+    if (cfg->dtype != MGPT_DTYPE_F32)
+      return fail(MGPT_ERR_UNSUPPORTED, "the layer's logits are fp32, not dtype %d", cfg->dtype);
+    if (!(balance >= 0.0f) || !std::isfinite(balance))
+      return fail(MGPT_ERR_INVALID_ARGUMENT, "balance must be finite and >= 0");
+    h->route = *cfg;
+  }
+  h->routed = cfg != nullptr;
+  h->route_bias = cfg ? bias : nullptr;
+  h->route_balance = cfg ? balance : 0.0f;
+  ++h->route_set;
+  return MGPT_OK;
+}
+
+int mgpt_moe_forward_routed(mgpt_moe* h, const void* x, const int32_t* idx, const float* weights, void* y,
+                            int num_tokens, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_forward_args(h, x, y, num_tokens, workspace, workspace_bytes, false))
+    return rc;
+  if (num_tokens == 0) return MGPT_OK;
+  if (!idx || !weights) return fail(MGPT_ERR_INVALID_ARGUMENT, "null idx or weights");
+  HIP_TRY(hipSetDevice(h->device));
+  BlockArgs blk;
+  blk.idx = idx;
+  blk.weights = weights;
+  return dispatch_forward(h, x, y, num_tokens, (char*)workspace, false, (hipStream_t)stream, blk);
+}
+
 int mgpt_moe_get_rstd(const mgpt_moe* h, int num_tokens, void* workspace, float** rstd) {
   if (!h || !workspace || !rstd || num_tokens < 0)
     return fail(MGPT_ERR_INVALID_ARGUMENT, "null argument or negative num_tokens");
@@ -1333,6 +1535,8 @@ int backward_entry(mgpt_moe* h, const void* x, const void* dy, void* dx, int num
   };
   if (overlap(dx, dy) || overlap(dx, x))
     return fail(MGPT_ERR_INVALID_ARGUMENT, "dx must not overlap x or dy");
+  if (h->route_trained != h->route_set)
+    return fail(MGPT_ERR_NOT_READY, "the routing was set after the last training forward");
   HIP_TRY(hipSetDevice(h->device));
   hipStream_t st = (hipStream_t)stream;
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;

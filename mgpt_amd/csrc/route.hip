@@ -25,26 +25,10 @@
 #include <cmath>
 #include <type_traits>
 
-#include "../../include/mgpt_moe.h"
 #include "capi_internal.hpp"
-#include "common.hpp"
+#include "route.hpp"
 
 namespace mgpt {
-
-struct RouteArgs {
-  const void* logits;    // [N][E]
-  const float* bias;     // [E] or null
-  int32_t* idx;          // [N][k]
-  float* weights;        // [N][k]
-  int32_t* counts;       // [E], added to, or null
-  // backward
-  const int32_t* bidx;
-  const float *bw, *dw, *dscore;   // dscore [E] or null
-  void* dlogits;
-  int N, E, k, G, S, top_groups, best;   // S = E / G
-  float scale;
-  int renorm, vec;
-};
 
 namespace {
 
@@ -495,6 +479,64 @@ __global__ __launch_bounds__(512) void route_balance_kernel(const int32_t* __res
   if (e < E && c * E != sum) bias[e] += c * E < sum ? rate : -rate;
 }
 
+// (a block: 64 tokens)
+__global__ __launch_bounds__(256) void route_take_kernel(const int32_t* from, const float* from_w, int N, int E, int k,
+                                                         int32_t* idx, float* w, int32_t* hist, int nb) {
+  __shared__ int s_hist[kMaxExpertsWide];
+  for (int e = threadIdx.x; e < E; e += 256) s_hist[e] = 0;
+  __syncthreads();
+  const size_t f0 = (size_t)blockIdx.x * kRouterTokens * k;
+  const int n = min(kRouterTokens, N - (int)blockIdx.x * kRouterTokens) * k;
+  for (int f = threadIdx.x; f < n; f += 256) {
+    int e;
+    if (from) {
+      e = from[f0 + f];
+      const bool in = (unsigned)e < (unsigned)E;
+      w[f0 + f] = in ? from_w[f0 + f] : 0.0f;
+      e = in ? e : 0;
+      idx[f0 + f] = e;
+    } else {
+      e = idx[f0 + f];
+    }
+    if (hist) atomicAdd(&s_hist[e], 1);
+  }
+  if (!hist) return;
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += 256) hist[(size_t)e * nb + blockIdx.x] = s_hist[e];
+}
+
+__global__ __launch_bounds__(512) void route_dscore_kernel(const int32_t* __restrict__ counts, int E, int N,
+                                                           float alpha, float* __restrict__ dscore) {
+  const int e = threadIdx.x;
+  if (e < E) dscore[e] = (alpha * (float)E * ((float)counts[e] / (float)N)) / (float)N;
+}
+
+int compute_units() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
+    return 256;
+  return n;
+}
+
+// Calls go(lanes per token, experts per lane, softmax) for the config.
+template <typename Go>
+hipError_t for_route(const mgpt_route_config* cfg, Go go) {
+  auto with = [&](auto lp, auto v) {
+    cfg->score == MGPT_SCORE_SOFTMAX ? go(lp, v, std::true_type{}) : go(lp, v, std::false_type{});
+  };
+  const int E = cfg->num_experts;
+  if (E <= 16) with(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+  else if (E <= 32) with(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
+  else if (E <= 64) with(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+  else if (E <= 128) with(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+  else if (E <= 256) with(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+  else with(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+  return hipGetLastError();
+}
+
+}  // namespace
+
 int check_route(const mgpt_route_config* cfg, int N) {
   if (!cfg) return fail(MGPT_ERR_INVALID_ARGUMENT, "config is null");
   if (N < 0) return fail(MGPT_ERR_INVALID_ARGUMENT, "negative num_tokens");
@@ -536,31 +578,20 @@ RouteArgs route_args(const mgpt_route_config* cfg, const void* logits, const voi
   return g;
 }
 
-int compute_units() {
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-    return 256;
-  return n;
-}
-
-// Calls go(lanes per token, experts per lane, softmax) for the config.
-template <typename Go>
-hipError_t for_route(const mgpt_route_config* cfg, Go go) {
-  auto with = [&](auto lp, auto v) {
-    cfg->score == MGPT_SCORE_SOFTMAX ? go(lp, v, std::true_type{}) : go(lp, v, std::false_type{});
-  };
-  const int E = cfg->num_experts;
-  if (E <= 16) with(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-  else if (E <= 32) with(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
-  else if (E <= 64) with(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
-  else if (E <= 128) with(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
-  else if (E <= 256) with(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-  else with(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+hipError_t launch_route_take(const int32_t* from, const float* from_w, int N, int E, int k, int32_t* idx, float* w,
+                             int32_t* hist, hipStream_t st) {
+  const int nb = (N + kRouterTokens - 1) / kRouterTokens;
+  if (nb <= 0) return hipSuccess;
+  if (E > kMaxExpertsWide) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(route_take_kernel, dim3(nb), dim3(256), 0, st, from, from_w, N, E, k, idx, w, hist, nb);
   return hipGetLastError();
 }
 
-}  // namespace
+hipError_t launch_route_dscore(const int32_t* counts, int E, int N, float alpha, float* dscore, hipStream_t st) {
+  if (E > kMaxExpertsWide) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(route_dscore_kernel, dim3(1), dim3(512), 0, st, counts, E, N, alpha, dscore);
+  return hipGetLastError();
+}
 
 hipError_t launch_route(const mgpt_route_config* cfg, const RouteArgs& g, bool backward, hipStream_t st) {
   return for_route(cfg, [&](auto lp, auto v, auto softmax) {

@@ -1598,6 +1598,47 @@ hipError_t launch_router(const ActT* x, const float* wr_g, const float* wr1, con
   return hipGetLastError();
 }
 
+// The logits [N][E] alone, for a routing of the caller's rule (route.hip); arguments as
+// launch_router's.  A wave for every 64 experts of one to four tokens from about one wave per SIMD on,
+// product and chain waves below.  With gamma the rows are normalised first where xn has room.
+template <typename ActT>
+hipError_t launch_router_logits(const ActT* x, const float* wr1, const float* wr4, const float* br, int N, int C,
+                                int E, float* logits, const float* gamma, float eps, int cn, float* rstd, float* xn,
+                                hipStream_t stream) {
+  const int nb = (N + kRT - 1) / kRT;
+  if (nb == 0) return hipSuccess;
+  if (E > kMaxExpertsWide || !logits) return hipErrorInvalidValue;
+  if (gamma) {
+    const RowNorm nrm{gamma, eps, cn};
+    if (xn && C <= kRowNormMaxC) {
+      hipLaunchKernelGGL(router_rownorm_kernel<ActT>, dim3((N + 3) / 4), dim3(256), (size_t)C * 16, stream, x, N, C,
+                         nrm, rstd, xn);
+      return launch_router_logits<float>(xn, wr1, wr4, br, N, C, E, logits, nullptr, 0.0f, C, nullptr, nullptr, stream);
+    }
+    hipLaunchKernelGGL((router_logits_kernel<ActT>), dim3(nb, (E + kSplitExperts - 1) / kSplitExperts),
+                       dim3(kSplitExperts * kWave), 0, stream, x, wr1, br, N, C, E, logits, nrm, rstd);
+    return hipGetLastError();
+  }
+  const int eg = (E + kMaxExperts - 1) / kMaxExperts;
+  const long pairs = (long)N * eg;
+  if (wr4 && pairs >= 1024) {
+    auto go = [&](auto kernel, int T) {
+      hipLaunchKernelGGL(kernel, dim3((N + 4 * T - 1) / (4 * T), eg), dim3(256), 0, stream, x,
+                         reinterpret_cast<const float4*>(wr4), br, N, C, E, logits);
+    };
+    if (pairs <= 2048) go(router_logits_lane_kernel<ActT, 1>, 1);
+    else if (pairs <= 6144 || (sizeof(ActT) == 4 && eg == 1)) go(router_logits_lane_kernel<ActT, 2>, 2);
+    else go(router_logits_lane_kernel<ActT, 4>, 4);
+  } else {
+    hipLaunchKernelGGL((router_logits_pc_kernel<ActT>), dim3(nb, E), dim3(256), 0, stream, x, wr1, br, N, C, E, logits);
+  }
+  return hipGetLastError();
+}
+template hipError_t launch_router_logits<float>(const float*, const float*, const float*, const float*, int, int, int,
+                                                float*, const float*, float, int, float*, float*, hipStream_t);
+template hipError_t launch_router_logits<bf16_t>(const bf16_t*, const float*, const float*, const float*, int, int, int,
+                                                 float*, const float*, float, int, float*, float*, hipStream_t);
+
 template hipError_t launch_router<float>(const float*, const float*, const float*, const float*,
                                          const float*, int, int, int, int, int32_t*, float*,
                                          int32_t*, float*, float*, const float*, float, int,

@@ -21,7 +21,7 @@ import torch
 from . import capi
 
 _ACT = {"f32": capi.DTYPE_F32, "bf16": capi.DTYPE_BF16}
-_W = {"f32": capi.DTYPE_F32, "bf16": capi.DTYPE_BF16, "fp8": capi.DTYPE_FP8_E4M3}
+_W = {"f32": capi.DTYPE_F32, "bf16": capi.DTYPE_BF16, "fp8": capi.DTYPE_FP8_E4M3, "i8": capi.DTYPE_I8}
 _TORCH = {"f32": torch.float32, "bf16": torch.bfloat16}
 
 
@@ -45,6 +45,7 @@ class MoELayer:
         self._loaded = False
         self._train_x = None   # input of the last training forward (cached_input)
         self._train_block = None   # (x, gamma) of the last training forward_block
+        self._route_bias = None    # the device reads it in every forward
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -149,6 +150,43 @@ class MoELayer:
     def forward(self, x: torch.Tensor, train: bool = False) -> torch.Tensor:
         out = torch.empty_like(x)
         self.forward_into(x, out, train)
+        return out
+
+    def set_routing(self, routing, bias: torch.Tensor | None = None, balance: float = 0.0) -> None:
+        """Runs the layer with `routing` (mgpt_amd.routing.ExpertRouting of its
+        experts and top_k, act "f32") in place of the engine's router, or with
+        that again (None).  bias: float32 device [E], read by every forward
+        from then on; balance: the load-balance loss' factor in backwards."""
+        if routing is None:
+            capi.check(capi.lib().mgpt_moe_set_routing(self._h, None, None, 0.0))
+            self._route_bias = None
+            return
+        if bias is not None and (not bias.is_cuda or bias.dtype != torch.float32 or tuple(bias.shape) != (self.E,)
+                                 or not bias.is_contiguous()):
+            raise ValueError(f"bias must be a contiguous float32 CUDA tensor of {self.E} elements")
+        capi.check(capi.lib().mgpt_moe_set_routing(self._h, ctypes.byref(routing.config),
+                                                   None if bias is None else bias.data_ptr(), float(balance)))
+        self._route_bias = bias
+
+    def forward_routed(self, x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
+        """The layer with a routing that is given: the sum over j of weights[..., j]
+        (float32) times expert idx[..., j] (int32) of x; an idx outside 0 .. E - 1
+        counts for nothing.  Inference only."""
+        if not x.is_cuda or x.dtype != self.dtype or x.shape[-1] != self.C or not x.is_contiguous():
+            raise ValueError("x must be a contiguous device tensor [..., C] of the layer's dtype")
+        shape = (*x.shape[:-1], self.k)
+        for t, dt, what in ((idx, torch.int32, "idx"), (weights, torch.float32, "weights")):
+            if t.device != x.device or t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"{what} must be a contiguous {dt} tensor of shape {list(shape)} on the device of x")
+        out = torch.empty_like(x)
+        n = x.numel() // self.C
+        ws = self._workspace(n, x.device)
+        capi.check(capi.lib().mgpt_moe_forward_routed(self._h, x.data_ptr(), idx.data_ptr(), weights.data_ptr(),
+                                                      out.data_ptr(), n, ws.data_ptr(), ws.numel(),
+                                                      capi.stream(x.device)))
+        self._last_n = n
+        self._train_x = None
+        self._train_block = None
         return out
 
     def forward_block(self, x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
