@@ -589,6 +589,34 @@ int mgpt_i8_linear_forward(const mgpt_i8_config* cfg, const void* x, const void*
                            const float* scales, const float* bias, void* y, int num_tokens,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/* A token for each row of logits [B,V] from a given random number.  With a row's
+ * logits l (NaN as -infinity, each at most the largest float) in the order of (l
+ * descending, id ascending):
+ *   w_i = rint(2^40 exp((l_i - max l) / temperature))
+ * the first top_k are kept (<= 0: all), of those the ones before which less than
+ * top_p of their sum lies (>= 1: all), of those the ones with w_i >= min_p 2^40,
+ * and always the first.  The token is the first, by id, at which the running
+ * sum of the kept w exceeds u times their sum.  temperature 0 takes the largest
+ * logit.  A row of nothing but -infinity has token -1.  Replaces the Generator's
+ * sampling on the host (pipeline/Generator.cpp:13-36). */
+typedef struct mgpt_sample_config {
+  int vocab_size;      /* V: 1 .. 2^20 */
+  int dtype;           /* of the logits: MGPT_DTYPE_F32 or MGPT_DTYPE_BF16 */
+  float temperature;   /* >= 0; these four hold where the array of the rows' own is null */
+  int top_k;
+  float top_p;         /* >= 0 */
+  float min_p;         /* >= 0 */
+} mgpt_sample_config;
+
+/* u: [B] fp32, each in [0, 1); temperature, top_p, min_p: [B] fp32 or null; top_k: [B] int32 or null;
+ * token: [B] int32; logp: [B] fp32 or null, the logarithm of the token's
+ * probability among the kept ones (0 at temperature 0, -infinity for token -1).
+ * All device memory.  The arrays' values are not checked: what is not a number
+ * counts as 0 in temperature and u, and as no restriction in top_p. */
+int mgpt_sample(const mgpt_sample_config* cfg, const void* logits, const float* u,
+                const float* temperature, const int32_t* top_k, const float* top_p,
+                const float* min_p, int32_t* token, float* logp, int num_rows, void* stream);
+
 /* Description of the last error on this host thread ("" if none). */
 const char* mgpt_moe_last_error(void);
 

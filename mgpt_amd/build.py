@@ -23,7 +23,7 @@ HIP_SOURCES = ["router.hip", "dispatch.hip", "gemm.hip", "gemm_f32.hip", "gemm_d
                "gemm_decode.hip", "combine.hip",
                "pack.hip", "backward.hip", "wgrad.hip", "moe_capi.hip", "checkpoint.cpp",
                "adamw.hip", "norm.hip", "lm_loss.hip", "route.hip",
-               "i8_quantize.hip", "i8_gemm.hip"]
+               "i8_quantize.hip", "i8_gemm.hip", "sample.hip"]
 ARCH = os.environ.get("MGPT_OFFLOAD_ARCH", "gfx950")
 
 # -ffp-contract=off: the router must round every product and sum separately

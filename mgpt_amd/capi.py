@@ -79,6 +79,11 @@ class I8Config(ctypes.Structure):
     _fields_ = [("in_features", ctypes.c_int), ("out_features", ctypes.c_int), ("dtype", ctypes.c_int)]
 
 
+class SampleConfig(ctypes.Structure):
+    _fields_ = [("vocab_size", ctypes.c_int), ("dtype", ctypes.c_int), ("temperature", ctypes.c_float),
+                ("top_k", ctypes.c_int), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float)]
+
+
 class MoEError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"mgpt_moe status {status}: {message}")
@@ -144,6 +149,7 @@ def lib() -> ctypes.CDLL:
         "mgpt_route_forward": [ctypes.POINTER(RouteConfig)] + [vp] * 5 + [i, vp],
         "mgpt_route_backward": [ctypes.POINTER(RouteConfig)] + [vp] * 6 + [i, vp],
         "mgpt_route_balance": [i, vp, ctypes.c_float, vp, vp],
+        "mgpt_sample": [ctypes.POINTER(SampleConfig)] + [vp] * 8 + [i, vp],
         "mgpt_i8_weight_bytes": [ctypes.POINTER(I8Config), ctypes.POINTER(sz)],
         "mgpt_i8_pack_weight": [ctypes.POINTER(I8Config), vp, i, vp, vp, vp],
         "mgpt_i8_pack_quantized": [ctypes.POINTER(I8Config), vp, vp, vp],

@@ -1,0 +1,61 @@
+"""Sampler: a token for each row of logits from a given random number.
+
+Temperature, top-k, top-p and min-p, for all rows or for each its own, over the
+C ABI (mgpt_sample): the sampling of the engine's Generator
+(/root/reference/src/main/pipeline/Generator.cpp:13-36) on the device, so
+that a decode step needs no copy to the host and can be captured whole.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import capi
+
+_DT = {"f32": (torch.float32, capi.DTYPE_F32), "bf16": (torch.bfloat16, capi.DTYPE_BF16)}
+
+
+class Sampler:
+    """Logits are [..., V] in `act`'s type."""
+
+    def __init__(self, vocab_size: int, act: str = "f32"):
+        self.V = vocab_size
+        self.dtype, self._dt = _DT[act]
+
+    @staticmethod
+    def _check(t, dtype, shape, device, what):
+        if not t.is_cuda or t.device != device:
+            raise ValueError(f"{what} must be a CUDA tensor on the device of logits")
+        if t.dtype != dtype:
+            raise TypeError(f"{what} must be {dtype}")
+        if tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous with shape {list(shape)}")
+        return t.data_ptr()
+
+    def forward(self, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """(token, logp): int32 and float32 [...], one per row.  u: float32 [...] in
+        [0, 1).  temperature (0: the largest logit), top_k (0: all), top_p
+        and min_p: numbers, or tensors [...] (int32 for top_k, else float32).
+        logp is the token's log-probability among those kept; a row of
+        nothing but -inf has token -1."""
+        if logits.dim() < 1 or logits.shape[-1] != self.V:
+            raise ValueError(f"logits must have {self.V} columns")
+        dev, shape = logits.device, tuple(logits.shape[:-1])
+        ptr = self._check(logits, self.dtype, tuple(logits.shape), dev, "logits")
+        up = self._check(u, torch.float32, shape, dev, "u")
+        cfg = capi.SampleConfig(self.V, self._dt, 1.0, 0, 1.0, 0.0)
+        ptrs = []
+        for name, v, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                            ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+            if isinstance(v, torch.Tensor):
+                ptrs.append(self._check(v, dt, shape, dev, name))
+            else:
+                setattr(cfg, name, v)
+                ptrs.append(None)
+        with capi.on_device(dev):
+            token = torch.empty(shape, dtype=torch.int32, device=dev)
+            logp = torch.empty(shape, dtype=torch.float32, device=dev)
+            capi.check(capi.lib().mgpt_sample(ctypes.byref(cfg), ptr, up, *ptrs, token.data_ptr(), logp.data_ptr(),
+                                              token.numel(), capi.stream(dev)))
+        return token, logp
