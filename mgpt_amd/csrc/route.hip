@@ -14,12 +14,18 @@
 //   sigmoid: dl = ds s (1 - s),   softmax: dl = s (ds - sum_e ds_e s_e)
 //
 // A token's experts lie in LP lanes of a wave, V neighbouring ones in each, so that 64 / LP tokens
-// share a wave, and stay in registers; the token's own LDS holds what lanes look up by expert (scores
-// for the groups, the gradient's scatter).  A choice is k rounds of a maximum over V registers and LP lanes.
+// share a wave, and stay in registers; the token's own LDS holds what lanes look up by expert (logits, the
+// gradient's scatter) and pass between groups.
 //
-// Keys with a bias, and sizes of groups, are those of 64 bits: fp32 ones, 2^-20 of a score off at
-// most, decide where the values that are compared are further apart than that, and otherwise the
-// wave does the token again in 64 bits.
+// The choice: keys as whole numbers, (key - the largest) in a fixed unit, with the expert's id below them, so that
+// no two are equal.  Every lane sorts its own by a network of minima and maxima; k rounds then take the largest of the
+// lanes' first ones, by moves within rows of 16 lanes, and pop it.
+//
+// Keys with a bias, and sizes of groups, are those of 64 bits, and logits may have the same number without being equal:
+// where what is compared is not further apart than its rounding, the wave does its tokens again in 64 bits (one in
+// thousands), in rolled loops through LDS: code that a wave comes to once, by itself, costs its fetches.  At 32768 x 256
+// (8 groups, a bias), us: 64 bits throughout 52, a wave to a token that searches for each maximum 57, again in
+// 64 bits by unrolled code 64, so 43 (17 of them the waves' mean).
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -42,13 +48,18 @@ __device__ __forceinline__ float exp_full(float x) {
   return y > -INFINITY && y < 128.0f ? __builtin_fmaf(e, r * 0.693147180559945f, e) : e;
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
-}
+// (bounds as the hardware's zeros, so that the move folds into the operation; every lane has a source)
 template <int CTRL>
 __device__ __forceinline__ int dpp(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false);
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)dpp<CTRL>((int)v);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(dpp<CTRL>(__float_as_int(v)));
 }
 template <int CTRL>
 __device__ __forceinline__ double dpp(double v) {
@@ -66,6 +77,8 @@ __device__ __forceinline__ int partner32(int v) {
   const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return (lane_id() & 32) ? r[0] : r[1];
 }
+__device__ __forceinline__ uint32_t partner16(uint32_t v) { return (uint32_t)partner16((int)v); }
+__device__ __forceinline__ uint32_t partner32(uint32_t v) { return (uint32_t)partner32((int)v); }
 __device__ __forceinline__ float partner16(float v) { return __int_as_float(partner16(__float_as_int(v))); }
 __device__ __forceinline__ float partner32(float v) { return __int_as_float(partner32(__float_as_int(v))); }
 __device__ __forceinline__ double partner16(double v) {
@@ -93,14 +106,7 @@ __device__ __forceinline__ T across(T v, Op op) {
   if constexpr (L > 32) v = op(v, partner<32>(v));
   return v;
 }
-__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
-__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
-__device__ __forceinline__ double smaller(double a, double b) { return fmin(a, b); }
-__device__ __forceinline__ float exp_of(float x) { return exp_full(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
-__device__ __forceinline__ float inverse(float x) { return 1.0f / x; }
-__device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
+__device__ __forceinline__ float inverse(float x) { return __builtin_amdgcn_rcpf(x); }   // 1 ulp
 
 // Orders a wave's own LDS accesses across its lanes.
 __device__ __forceinline__ void wave_sync() {
@@ -138,220 +144,524 @@ __device__ __forceinline__ void load_logits(const RouteArgs& g, size_t t, int e0
 }
 
 // An infinity or a NaN among the logits, out of the way.
-__device__ __forceinline__ float clean(float l) { return l != l ? kNone : fminf(l, FLT_MAX); }
+// (The hardware's median of three with a NaN is their minimum; the compiler would make a minimum of two of it.)
+__device__ __forceinline__ float clean(float l) {
+  float r;
+  asm("v_med3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(l), "v"(kNone), "v"(FLT_MAX));
+  return r;
+}
 
-template <int LP, int V, bool SOFTMAX, typename K>
-__device__ __forceinline__ void scores_of(const float (&l)[V], K (&s)[V]) {
-  if constexpr (SOFTMAX) {
-    float m = l[0];
+// A maximum of numbers that are none a signalling NaN (fmaxf would first make sure of that).
+__device__ __forceinline__ float max32(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
+template <int LP, int V>
+__device__ __forceinline__ float largest(const float (&l)[V]) {
+  float m = l[0];
 #pragma unroll
-    for (int v = 1; v < V; ++v) m = fmaxf(m, l[v]);
-    m = across<LP>(m, [](float a, float b) { return fmaxf(a, b); });
-    m = fmaxf(m, -FLT_MAX);   // a row without experts
-    K z = 0;
+  for (int v = 1; v < V; ++v) m = max32(m, l[v]);
+  return max32(across<LP>(m, [](float a, float b) { return max32(a, b); }), -FLT_MAX);   // (a row without experts)
+}
+
+// Scores to some 2^-22.
+template <int LP, int V, bool SOFTMAX>
+__device__ __forceinline__ void scores_of(const float (&l)[V], float (&s)[V]) {
+  if constexpr (SOFTMAX) {
+    const float m = largest<LP, V>(l);
+    float z = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      s[v] = exp_of((K)l[v] - (K)m);
+      s[v] = exp_full(l[v] - m);
       z += s[v];
     }
-    z = across<LP>(z, [](K a, K b) { return a + b; });
-    const K r = z > 0 ? inverse(z) : (K)0;
+    z = across<LP>(z, [](float a, float b) { return a + b; });
+    const float r = z > 0.0f ? inverse(z) : 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) s[v] *= r;
   } else {
 #pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = inverse((K)1 + exp_of(-(K)l[v]));
+    for (int v = 0; v < V; ++v) s[v] = inverse(1.0f + exp_full(-l[v]));
   }
 }
 
-// What a wave keeps in LDS: for each of its tokens the scores (or gradients) by expert, the sizes of the
-// groups, and the chosen experts with their scores.
+// exp(x) in 64 bits to 2^-51, x up to 700 in magnitude (beyond: as there): 2^t by its whole part and a polynomial of degree 10 on
+// [-1/2, 1/2] (least maximum relative error, 2^-52).
+__device__ __forceinline__ double exp64(double x) {
+  const double t = fmin(fmax(x * 1.4426950408889634, -1000.0), 1000.0);
+  const double n = (t + 0x1.8p52) - 0x1.8p52, f = t - n;
+  double q = 0x1.e3992178bd0ddp-28;
+  q = __builtin_fma(q, f, 0x1.b6740fb0785eap-24);
+  q = __builtin_fma(q, f, 0x1.62c157ec7ee12p-20);
+  q = __builtin_fma(q, f, 0x1.ffcb55e844f93p-17);
+  q = __builtin_fma(q, f, 0x1.43091260573e4p-13);
+  q = __builtin_fma(q, f, 0x1.5d87fe9cc5ce9p-10);
+  q = __builtin_fma(q, f, 0x1.3b2ab6fbde0f3p-7);
+  q = __builtin_fma(q, f, 0x1.c6b08d703d48ap-5);
+  q = __builtin_fma(q, f, 0x1.ebfbdff82c3b9p-3);
+  q = __builtin_fma(q, f, 0x1.62e42fefa3a17p-1);
+  q = __builtin_fma(q, f, 1.0);
+  return __builtin_ldexp(q, (int)n);
+}
+// 1 / x to 2^-52: the hardware's and two Newton steps.
+__device__ __forceinline__ double inverse64(double x) {
+  double r = __builtin_amdgcn_rcp(x);
+  r = __builtin_fma(r, __builtin_fma(-x, r, 1.0), r);
+  return __builtin_fma(r, __builtin_fma(-x, r, 1.0), r);
+}
+
+__device__ __forceinline__ void order2(uint32_t& a, uint32_t& b) {
+  const uint32_t x = max(a, b);
+  b = min(a, b);
+  a = x;
+}
+// The largest min(V, 8) of V numbers, descending.
+template <int V>
+__device__ __forceinline__ void sort_lane(const uint32_t* x, uint32_t* y) {
+  if constexpr (V == 16) {
+    uint32_t z[8];
+    sort_lane<8>(x, y);
+    sort_lane<8>(x + 8, z);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = max(y[i], z[7 - i]);   // the 8 largest, up and down
+#pragma unroll
+    for (int d = 4; d >= 1; d /= 2)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(i & d)) order2(y[i], y[i + d]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = x[i];
+    // odd-even merges
+    constexpr int kNet8[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6},
+                                  {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+    constexpr int kNet4[5][2] = {{0, 1}, {2, 3}, {0, 2}, {1, 3}, {1, 2}};
+    if constexpr (V == 8) {
+#pragma unroll
+      for (int i = 0; i < 19; ++i) order2(y[kNet8[i][0]], y[kNet8[i][1]]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) order2(y[kNet4[i][0]], y[kNet4[i][1]]);
+    }
+  }
+}
+
+// What a wave keeps in LDS: for each of its tokens the logits (32 bits) or keys (64) by expert, the sizes
+// of the groups, and the chosen experts, as packed numbers or (64 bits) ids.
 template <int LP, int V>
 struct Space {
   static constexpr int kTokens = kWave / LP;
   static constexpr int kGroups = LP * V < kMaxExperts ? LP * V : kMaxExperts;
   double key[kWave * V];
-  double size[kTokens][kGroups + 2];
-  int on[kTokens][kGroups];
-  int id[kTokens][kMaxTopK];
-  float score[kTokens][kMaxTopK];
+  double size[kTokens][kGroups];
+  uint8_t on[kTokens][kGroups];
+  uint32_t pick[kTokens][kMaxTopK + 2];
 };
 
-// The groups that take part, in sp.on; returns whether the last of them and the first that does
-// not are further apart than `tol`.
-template <int LP, int V, typename K>
-__device__ __forceinline__ bool choose_groups(const RouteArgs& g, const K (&key)[V], int e0, int tok, int lp, K tol,
-                                              Space<LP, V>& sp) {
-  K* keys = reinterpret_cast<K*>(sp.key) + tok * LP * V;
-  K* sizes = reinterpret_cast<K*>(sp.size[tok]);
-#pragma unroll
-  for (int v = 0; v < V; ++v) keys[e0 + v] = key[v];
-  wave_sync();
-  // P lanes to a group, a power of two
-  int P = 1;
-  while (2 * P * g.G <= LP) P *= 2;
-  const K none = -INFINITY;
-  for (int gr0 = 0; gr0 < g.G; gr0 += LP / P) {
-    const int gr = gr0 + lp / P;
-    K a = none, b = none;
-    if (gr < g.G)
-      for (int i = lp % P; i < g.S; i += P) {
-        const K x = keys[gr * g.S + i];
-        b = larger(b, smaller(a, x));
-        a = larger(a, x);
-      }
-    auto join = [&](K a2, K b2) {
-      b = larger(smaller(a, a2), larger(b, b2));
-      a = larger(a, a2);
-    };
-    if (P > 1) join(partner<1>(a), partner<1>(b));
-    if (P > 2) join(partner<2>(a), partner<2>(b));
-    if (P > 4) join(partner<4>(a), partner<4>(b));
-    if (P > 8) join(partner<8>(a), partner<8>(b));
-    if constexpr (LP > 16)
-      if (P > 16) join(partner<16>(a), partner<16>(b));
-    if (gr < g.G && lp % P == 0) sizes[gr] = g.best > 1 && b > none ? a + b : a;
-  }
-  if (lp == 0) sizes[g.G] = sizes[g.G + 1] = none;
-  wave_sync();
-  for (int gr = lp; gr < g.G; gr += LP) {
-    const K x = sizes[gr];
-    int rank = 0;
-    for (int o = 0; o < g.G; ++o) rank += sizes[o] > x || (sizes[o] == x && o < gr);
-    sp.on[tok][gr] = rank < g.top_groups;
-    // (a lane of another group reads only the first G)
-    if (rank == g.top_groups - 1) sizes[g.G] = x;
-    if (rank == g.top_groups) sizes[g.G + 1] = x;
-  }
-  wave_sync();
-  const K last = sizes[g.G], next = sizes[g.G + 1];
-  return next == none || last - next > tol;
-}
+constexpr double kOut = -1e300;   // in 64 bits: takes no part; places past E are below
 
-// k rounds over the keys; the chosen ids and scores into sp.  Returns whether neighbours
-// in the order, the first that was not chosen among them, are further apart than `tol`
-// (tol < 0: whether equal ones are in order is known).
-template <int LP, int V, typename K>
-__device__ __forceinline__ bool choose(const RouteArgs& g, K (&key)[V], const float (&s)[V], unsigned taken, int e0,
-                                       int tok, int lp, K tol, Space<LP, V>& sp) {
-  const K none = -INFINITY;
-  bool sure = true;
-  K last = INFINITY;
-  const int rounds = tol >= 0 ? g.k + 1 : g.k;
-  for (int j = 0; j < rounds; ++j) {
-    K m = none;
+// The groups that take part, in 32 bits: the keys of the others become -infinity.  Returns whether the last of them and
+// the first that does not are further apart than tol.
+template <int LP, int V>
+__device__ __forceinline__ bool choose_groups(const RouteArgs& g, float (&key)[V], int e0, int tok, int lp, float tol,
+                                              Space<LP, V>& sp) {
+  float* sizes = reinterpret_cast<float*>(sp.size[tok]);
+  float a = kNone, b = kNone;
+  auto take = [&](float x) {
+    b = __builtin_amdgcn_fmed3f(a, b, x);   // (a >= b)
+    a = max32(a, x);
+  };
+  auto join = [&](float a2, float b2) {
+    b = __builtin_amdgcn_fmed3f(a, a2, max32(b, b2));   // (the larger second is under both firsts, or between them)
+    a = max32(a, a2);
+  };
+  const int lanes = g.S / V;
+  const bool whole = g.S % V == 0 && (lanes & (lanes - 1)) == 0 && lanes <= 16;
+  int mine = lp;   // the lane's group, or of a loop's first turn
+  if (whole) {
+    // a group fills whole lanes, a power of two of them: by those themselves
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (!(taken >> v & 1)) m = larger(m, key[v]);
-    m = across<LP>(m, [](K a, K b) { return larger(a, b); });
-    if (tol >= 0 && j > 0) sure &= m == none || last - m > tol;
-    last = m;
-    if (j == g.k) break;
-    int e = INT_MAX;
+    for (int v = 0; v < V; ++v) take(key[v]);
+    if (lanes > 1) join(partner<1>(a), partner<1>(b));
+    if (lanes > 2) join(partner<2>(a), partner<2>(b));
+    if (lanes > 4) join(partner<4>(a), partner<4>(b));
+    if (lanes > 8) join(partner<8>(a), partner<8>(b));
+    mine = lp / lanes;
+    if (lp % lanes == 0 && mine < g.G) sizes[mine] = g.best > 1 && b > kNone ? a + b : a;
+  } else {
+    float* keys = reinterpret_cast<float*>(sp.key) + tok * LP * V;
 #pragma unroll
-    for (int v = V - 1; v >= 0; --v)
-      if (!(taken >> v & 1) && key[v] == m) e = e0 + v;
-    const int mine = e;
-    e = across<LP>(e, [](int a, int b) { return min(a, b); });
-    if (mine == e) {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (e == e0 + v) {
-          taken |= 1u << v;
-          sp.id[tok][j] = e;
-          sp.score[tok][j] = m > none ? s[v] : -1.0f;   // (-1: takes no part)
-        }
+    for (int v = 0; v < V; v += 4)
+      *reinterpret_cast<float4*>(keys + e0 + v) = make_float4(key[v], key[v + 1], key[v + 2], key[v + 3]);
+    wave_sync();
+    // P lanes to a group, a power of two (at most 16)
+    int P = 1;
+    while (2 * P * g.G <= LP && P < 16) P *= 2;
+    for (int gr0 = 0; gr0 < g.G; gr0 += LP / P) {
+      const int gr = gr0 + lp / P;
+      a = b = kNone;
+      if (gr < g.G)
+        for (int i = lp % P; i < g.S; i += P) take(keys[gr * g.S + i]);
+      if (P > 1) join(partner<1>(a), partner<1>(b));
+      if (P > 2) join(partner<2>(a), partner<2>(b));
+      if (P > 4) join(partner<4>(a), partner<4>(b));
+      if (P > 8) join(partner<8>(a), partner<8>(b));
+      if (gr < g.G && lp % P == 0) sizes[gr] = g.best > 1 && b > kNone ? a + b : a;
     }
   }
-  return sure;
+  wave_sync();
+  float last = INFINITY, next = kNone;
+  bool in = false;
+  for (int gr = mine; gr < g.G; gr += LP) {
+    const float x = sizes[gr];
+    int rank = 0;
+    for (int o = 0; o < g.G; ++o) {
+      const float y = sizes[o];
+      rank += y > x || (y == x && o < gr);
+    }
+    in = rank < g.top_groups;
+    if (in) last = fminf(last, x);
+    else next = fmaxf(next, x);
+    if (whole) break;
+    sp.on[tok][gr] = in;
+  }
+  last = across<LP>(last, [](float p, float q) { return fminf(p, q); });
+  next = across<LP>(next, [](float p, float q) { return fmaxf(p, q); });
+  if (whole) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = in ? key[v] : kNone;
+  } else {
+    wave_sync();
+    int gr = e0 / g.S, r = e0 % g.S;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      key[v] = gr < g.G && sp.on[tok][gr] ? key[v] : kNone;
+      if (++r == g.S) {
+        r = 0;
+        ++gr;
+      }
+    }
+  }
+  return next == kNone || last - next > tol;
 }
 
+// A step's tokens in 64 bits: the chosen ids into sp.pick (bit 30: takes no part).  Rolled loops over the experts, each
+// at its own place in LDS.
 template <typename T, int LP, int V, bool SOFTMAX>
+__device__ __forceinline__ void choose_exactly(const RouteArgs& g, size_t t, bool live, int tok, int lp,
+                                               Space<LP, V>& sp) {
+  constexpr int kAll = LP * V;
+  const T* row = reinterpret_cast<const T*>(g.logits) + t * g.E;
+  double* key = sp.key + tok * kAll;
+  double* sizes = sp.size[tok];
+  auto logit = [&](int e) { return e < g.E && live ? clean(to_f32(row[e])) : kNone; };
+  const bool scores = g.bias || g.G > 1;
+  double m = 0.0, r = 1.0;
+  if (SOFTMAX && scores) {
+    float top = -FLT_MAX;
+#pragma unroll 1
+    for (int e = lp; e < kAll; e += LP) top = fmaxf(top, logit(e));
+    m = across<LP>(top, [](float a, float b) { return fmaxf(a, b); });
+    double z = 0.0;
+#pragma unroll 1
+    for (int e = lp; e < kAll; e += LP) {
+      const float l = logit(e);
+      z += l > kNone ? exp64((double)l - m) : 0.0;
+    }
+    z = across<LP>(z, [](double a, double b) { return a + b; });
+    r = inverse64(fmax(z, 1.0));
+  }
+#pragma unroll 1
+  for (int e = lp; e < kAll; e += LP) {
+    const float l = logit(e);
+    double x = l;
+    if (scores) {
+      const double q = exp64(SOFTMAX ? (double)l - m : -(double)l);
+      x = SOFTMAX ? q * r : inverse64(1.0 + q);
+      if (g.bias && e < g.E) x += (double)g.bias[e];
+    }
+    // (a NaN is not above)
+    key[e] = e >= g.E ? -INFINITY : l > kNone && x > -INFINITY ? fmin(x, 1e300) : kOut;
+  }
+  wave_sync();
+  if (g.G > 1) {
+#pragma unroll 1
+    for (int gr = lp; gr < g.G; gr += LP) {
+      double a = kOut, b = kOut;
+#pragma unroll 1
+      for (int i = 0; i < g.S; ++i) {
+        const double x = key[gr * g.S + i];
+        b = fmax(b, fmin(a, x));
+        a = fmax(a, x);
+      }
+      sizes[gr] = g.best > 1 && b > kOut ? a + b : a;
+    }
+    wave_sync();
+#pragma unroll 1
+    for (int gr = lp; gr < g.G; gr += LP) {
+      const double x = sizes[gr];
+      int rank = 0;
+#pragma unroll 1
+      for (int o = 0; o < g.G; ++o) {
+        const double y = sizes[o];
+        rank += y > x || (y == x && o < gr);
+      }
+      sp.on[tok][gr] = rank < g.top_groups;
+    }
+    wave_sync();
+#pragma unroll 1
+    for (int e = lp; e < g.E; e += LP) {
+      const double x = key[e];
+      key[e] = !sp.on[tok][e / g.S] || x == kOut ? kOut : g.bias ? x : (double)logit(e);
+    }
+    wave_sync();
+  }
+#pragma unroll 1
+  for (int j = 0; j < g.k; ++j) {
+    double best = -INFINITY;
+    int at = kAll;
+#pragma unroll 1
+    for (int e = lp; e < kAll; e += LP) {
+      const double x = key[e];
+      if (x > best) {
+        best = x;
+        at = e;
+      }
+    }
+    const double top = across<LP>(best, [](double a, double b) { return fmax(a, b); });
+    at = across<LP>(best == top ? at : kAll, [](int a, int b) { return min(a, b); });
+    if (lp == 0) {
+      sp.pick[tok][j] = (uint32_t)at | (top > kOut ? 0u : 1u << 30);
+      key[at] = -INFINITY;
+    }
+    wave_sync();
+  }
+}
+
+// NEAR: a bias or groups, for which the scores of all experts are needed.
+template <typename T, int LP, int V, bool SOFTMAX, bool NEAR>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs g) {
-  constexpr int kTokens = kWave / LP;
+  constexpr int kTokens = kWave / LP, kAll = LP * V, L = V < 8 ? V : 8;
+  constexpr int kAgain = 64;   // steps of a wave that wait for their 64-bit turn
+  constexpr int kIdBits = kAll == 16 ? 4 : kAll == 32 ? 5 : kAll == 64 ? 6 : kAll == 128 ? 7 : kAll == 256 ? 8 : 9;
+  static_assert(1 << kIdBits == kAll, "a power of two of places");
+  constexpr float kTop = (float)((1 << (kIdBits < 8 ? 23 : 31 - kIdBits)) - 2);   // the largest key's number, exact as a float
+  constexpr int kSlots = kMaxTopK / LP + 1;   // of k + 1 chosen ones a lane keeps
+  constexpr float kLog2e = 1.44269504088896340736f;
   __shared__ Space<LP, V> space[4];
   __shared__ int s_count[kMaxExpertsWide];
+  __shared__ int s_again[4][kAgain];
   const int w = threadIdx.x / kWave, lane = lane_id();
   const int tok = lane / LP, lp = lane % LP, e0 = lp * V;
   Space<LP, V>& sp = space[w];
+  float* logits = reinterpret_cast<float*>(sp.key) + tok * kAll;   // a token's, by expert
   if (g.counts) {
     for (int e = threadIdx.x; e < g.E; e += 256) s_count[e] = 0;
     __syncthreads();
   }
-  float bias[V];
-  int grp[V];
+  float bias[V], most_bias = 0.0f;   // -infinity for one that is none
+  // The unit of the keys' numbers: of logits, 32 below the largest have numbers of their own; of scores with
+  // a bias, all.
+  float per = (kTop - 2.0f) / 32.0f;
+  if (NEAR && g.bias) {
+    float lo = 0.0f, hi = 0.0f;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const bool in = e0 + v < g.E;
-    bias[v] = in && g.bias ? g.bias[e0 + v] : 0.0f;
-    grp[v] = in ? (e0 + v) / g.S : 0;
-  }
-  unsigned out = 0;   // lanes' places past E
-#pragma unroll
-  for (int v = 0; v < V; ++v) out |= (unsigned)(e0 + v >= g.E) << v;
-
-  const int step = gridDim.x * 4 * kTokens;
-  for (int t0 = (blockIdx.x * 4 + w) * kTokens; t0 < g.N; t0 += step) {
-    const int t = t0 + tok;
-    const bool live = t < g.N;
-    float l[V], s[V];
-    load_logits<T, V>(g, live ? t : 0, e0, live, l);
-#pragma unroll
-    for (int v = 0; v < V; ++v) l[v] = clean(l[v]);
-    scores_of<LP, V, SOFTMAX, float>(l, s);
-
-    // keys of one precision, the groups by them, the choice
-    auto decide = [&](auto zero) {
-      typedef decltype(zero) K;
-      constexpr bool kExact = sizeof(K) == 8;
-      K sk[V], key[V];
-      if constexpr (kExact) {
-        scores_of<LP, V, SOFTMAX, K>(l, sk);
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) sk[v] = s[v];
-      }
-      K big = 0;   // of what the rounding of fp32 keys goes by
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const K x = sk[v] + (K)bias[v];
-        key[v] = l[v] > kNone && x == x ? x : (K)kNone;
-        if (!kExact && key[v] > kNone) big = larger(big, larger(sk[v], (K)fabsf((float)key[v])));
-      }
-      K tol = -1;
-      if constexpr (!kExact) tol = across<LP>(big, [](K a, K b) { return larger(a, b); }) * (K)0x1p-18f;
-      bool sure = true;
-      if (g.G > 1) {
-        sure = choose_groups<LP, V, K>(g, key, e0, tok, lp, 2 * tol, sp);
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (!sp.on[tok][grp[v]]) key[v] = (K)kNone;
-      }
-      if (g.bias) return choose<LP, V, K>(g, key, s, out, e0, tok, lp, kExact ? (K)-1 : tol, sp) && sure;
-      // the order of the logits, which fp32 holds exactly
-      float lk[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) lk[v] = key[v] > (K)kNone ? l[v] : kNone;
-      return choose<LP, V, float>(g, lk, s, out, e0, tok, lp, -1.0f, sp) && sure;
-    };
-    const bool sure = decide(0.0f);
-    if (__ballot(live && !sure)) {
-      wave_sync();
-      decide(0.0);
+    for (int v = 0; v < V; ++v) {
+      bias[v] = g.bias[min(e0 + v, g.E - 1)];   // (past E there is no logit)
+      bias[v] = bias[v] == bias[v] ? bias[v] : kNone;
+      lo = bias[v] > kNone ? fminf(lo, bias[v]) : lo;
+      hi = fmaxf(hi, bias[v]);
     }
-    wave_sync();
-    float D = 0.0f;
-    for (int j = 0; j < g.k; ++j) D += fmaxf(sp.score[tok][j], 0.0f);
+    lo = across<LP>(lo, [](float a, float b) { return fminf(a, b); });
+    hi = across<LP>(hi, [](float a, float b) { return fmaxf(a, b); });
+    per = (kTop - 2.0f) / (1.0f + (hi - lo));
+    most_bias = fmaxf(hi, -lo);
+  }
+  // The outputs of token t0 + tok's chosen ones (entry i LP + lp of the k): id, logit, whether it takes part; m and z the softmax's.
+  auto finish = [&](int t0, const int (&id)[kSlots], const float (&x)[kSlots], const bool (&on)[kSlots], float m, float z)
+      __attribute__((always_inline)) {
+    const int t = t0 + tok;
+    float sc[kSlots], D = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      if constexpr (SOFTMAX) sc[i] = exp_full(x[i] - m) * inverse(z);
+      else sc[i] = inverse(1.0f + exp_full(-x[i]));
+      sc[i] = on[i] ? sc[i] : 0.0f;
+      D += sc[i];
+    }
+    D = across<(LP < 8 ? LP : 8)>(D, [](float a, float b) { return a + b; });   // (lanes 8 .. hold zeros)
     const float r = g.renorm ? g.scale / (D + 1e-20f) : g.scale;
-    for (int j = lp; j < g.k; j += LP) {
-      const float x = sp.score[tok][j];
-      if (live) {
-        g.idx[(size_t)t * g.k + j] = sp.id[tok][j];
-        g.weights[(size_t)t * g.k + j] = x > 0.0f ? x * r : 0.0f;
-        if (g.counts && x >= 0.0f) atomicAdd(&s_count[sp.id[tok][j]], 1);
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      const int j = i * LP + lp;
+      if (j < g.k && t < g.N) {
+        g.idx[(size_t)t * g.k + j] = id[i];
+        g.weights[(size_t)t * g.k + j] = sc[i] * r;
+        if (g.counts && on[i]) atomicAdd(&s_count[id[i]], 1);
       }
     }
     wave_sync();   // before the next token's
+  };
+  auto request = [&](int t0, float (&l)[V]) __attribute__((always_inline)) {
+    const int t = t0 + tok;
+    load_logits<T, V>(g, t < g.N ? t : 0, e0, t < g.N, l);
+  };
+  auto sums = [&](float (&l)[V], float& m, float& z) __attribute__((always_inline)) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) l[v] = clean(l[v]);
+    m = SOFTMAX || NEAR ? largest<LP, V>(l) : 0.0f;
+    z = 0.0f;
+    if constexpr (SOFTMAX) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) z += __builtin_amdgcn_exp2f((l[v] - m) * kLog2e);
+      z = across<LP>(z, [](float a, float b) { return a + b; });
+    }
+  };
+
+  const int step = gridDim.x * 4 * kTokens;
+  int t0 = (blockIdx.x * 4 + w) * kTokens;
+  float ahead[V];   // the next step's logits
+  request(t0, ahead);
+  while (t0 < g.N) {
+    int again = 0;
+    for (; t0 < g.N && again < kAgain; t0 += step) {
+      float l[V], m, z;
+#pragma unroll
+      for (int v = 0; v < V; ++v) l[v] = ahead[v];
+      request(min(t0 + step, g.N), ahead);
+      sums(l, m, z);
+      float key[V], tol = 0.0f;
+      bool sure = true;
+      if constexpr (NEAR) {
+        const float r = SOFTMAX ? (z > 0.0f ? inverse(z) : 0.0f) : 1.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float s = SOFTMAX ? __builtin_amdgcn_exp2f((l[v] - m) * kLog2e) * r
+                                  : inverse(1.0f + __builtin_amdgcn_exp2f(l[v] * -kLog2e));
+          key[v] = l[v] > kNone ? g.bias ? s + bias[v] : s : kNone;
+        }
+        // A key's rounding, of the largest score and bias.  sigmoid: the exponential's argument, 2^-24 |l|, which s (1 - s)
+        // scales, |l| that of the largest score where all are small; 1 + e and the reciprocal 1.5 2^-23; the sum
+        // 2^-24.  softmax: the arguments' 2^-23 |l - m| s, at most 0.4 2^-23 of the largest, the sum and its reciprocal
+        // 2^-22, the rest 2^-23.
+        const float big = (SOFTMAX ? r : inverse(1.0f + __builtin_amdgcn_exp2f(m * -kLog2e))) + most_bias;
+        tol = big * (SOFTMAX ? 3 * 0x1p-22f : (1.5f + 0.25f * fabsf(m)) * 0x1p-22f);
+        if (g.G > 1) sure = choose_groups<LP, V>(g, key, e0, tok, lp, 5 * tol, sp);
+        if (!g.bias) {   // the order of the logits, which are exact
+#pragma unroll
+          for (int v = 0; v < V; ++v) key[v] = key[v] > kNone ? l[v] : kNone;
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = l[v];
+      }
+      float most = key[0];
+#pragma unroll
+      for (int v = 1; v < V; ++v) most = max32(most, key[v]);
+      most = across<LP>(most, [](float a, float b) { return max32(a, b); });
+      most = max32(most, -FLT_MAX);
+      // (-infinity converts to 0, as does what is below the unit's reach)
+      auto number = [&](float k) __attribute__((always_inline)) {
+        return (uint32_t)__builtin_fmaf(k - most, per, kTop);
+      };
+      uint32_t list[V], head[L];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        // (a place past E is none, and behind all experts that are none)
+        list[v] = number(key[v]) << kIdBits | (uint32_t)(kAll - 1 - (e0 + v));
+      }
+      sort_lane<V>(list, head);
+      uint32_t pick[kSlots];
+      int popped = 0;
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) pick[i] = 0;
+#pragma unroll
+      for (int j = 0; j <= kMaxTopK; ++j) {
+        if (j <= g.k) {
+          const uint32_t first = across<LP>(head[0], [](uint32_t a, uint32_t b) { return max(a, b); });
+          const uint32_t mine = head[0] == first ? ~0u : 0u;
+          // (as bits: a choice between neighbours would become a register index)
+#pragma unroll
+          for (int i = 0; i < L; ++i) head[i] = (i + 1 < L ? head[i + 1] & mine : 0) | (head[i] & ~mine);
+          if constexpr (V > L) popped -= (int)mine;
+          pick[j / LP] = lp == j % LP ? first : pick[j / LP];
+        }
+      }
+      // (a list that gave all it had: what follows in the lane is not known)
+      if constexpr (V > L) sure = sure && popped < L;
+#pragma unroll
+      for (int v = 0; v < V; v += 4)
+        *reinterpret_cast<float4*>(logits + e0 + v) = make_float4(l[v], l[v + 1], l[v + 2], l[v + 3]);
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i)
+        if (i * LP + lp <= g.k) sp.pick[tok][i * LP + lp] = pick[i];
+      wave_sync();
+      int id[kSlots];
+      float x[kSlots];
+      bool on[kSlots];
+      const uint32_t near = (uint32_t)fminf(2.0f * tol * per + 4.0f, 0x1p30f);
+      float edge = kNone;   // the last chosen one's logit, where the next has the same number
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        const int j = i * LP + lp;
+        const bool in = j < g.k;
+        const uint32_t p = in ? pick[i] : 0, n = in ? sp.pick[tok][j + 1] : 0;
+        const uint32_t q = p >> kIdBits, qn = n >> kIdBits;
+        id[i] = kAll - 1 - (int)(p & (kAll - 1));
+        on[i] = q > 0;
+        x[i] = in ? logits[id[i]] : kNone;
+        // (out of the unit's reach, or of the groups': in no order)
+        sure = sure && (q > 0 || x[i] == kNone);
+        if (qn > 0) {
+          if (NEAR && g.bias) {
+            sure = sure && q - qn > near;
+          } else if (q == qn) {   // equal logits are in order, others not
+            sure = sure && x[i] == logits[kAll - 1 - (int)(n & (kAll - 1))];
+            if (j + 1 == g.k) edge = x[i];
+          }
+        }
+      }
+      if (__ballot(edge > kNone)) {
+        // are all logits of that number equal?  (those that were not reached may be in any lane)
+        const float ex = across<LP>(edge, [](float a, float b) { return fmaxf(a, b); });
+        const uint32_t eq = number(ex);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (eq > 0 && number(key[v]) == eq && key[v] != ex) sure = false;
+      }
+      if (__ballot(t0 + tok < g.N && !sure)) {
+        s_again[w][again++] = t0;
+        wave_sync();
+      } else {
+        finish(t0, id, x, on, m, z);
+      }
+    }
+#pragma unroll 1
+    for (int i = 0; i < again; ++i) {
+      const int ta = s_again[w][i], t = ta + tok;
+      choose_exactly<T, LP, V, SOFTMAX>(g, t < g.N ? t : 0, t < g.N, tok, lp, sp);
+      float l[V], m, z;
+      request(ta, l);
+      sums(l, m, z);
+#pragma unroll
+      for (int v = 0; v < V; ++v) logits[e0 + v] = l[v];
+      wave_sync();
+      int id[kSlots];
+      float x[kSlots];
+      bool on[kSlots];
+#pragma unroll
+      for (int c = 0; c < kSlots; ++c) {
+        const int j = c * LP + lp;
+        const uint32_t p = j < g.k ? sp.pick[tok][j] : 1u << 30;
+        id[c] = (int)(p & (kAll - 1));
+        on[c] = p >> 30 == 0;
+        x[c] = logits[id[c]];
+      }
+      finish(ta, id, x, on, m, z);
+    }
+    wave_sync();
   }
   if (g.counts) {
     __syncthreads();
@@ -378,7 +688,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs g) {
     load_logits<T, V>(g, live ? t : 0, e0, live, l);
 #pragma unroll
     for (int v = 0; v < V; ++v) l[v] = clean(l[v]);
-    scores_of<LP, V, SOFTMAX, float>(l, s);
+    scores_of<LP, V, SOFTMAX>(l, s);
 #pragma unroll
     for (int v = 0; v < V; ++v) mine[e0 + v] = s[v];
     wave_sync();
@@ -525,13 +835,18 @@ hipError_t for_route(const mgpt_route_config* cfg, Go go) {
   auto with = [&](auto lp, auto v) {
     cfg->score == MGPT_SCORE_SOFTMAX ? go(lp, v, std::true_type{}) : go(lp, v, std::false_type{});
   };
+  auto of = [&](auto lp, auto v) { with(lp, v); };
   const int E = cfg->num_experts;
-  if (E <= 16) with(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-  else if (E <= 32) with(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
-  else if (E <= 64) with(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
-  else if (E <= 128) with(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
-  else if (E <= 256) with(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-  else with(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+  typedef std::integral_constant<int, 4> C4;
+  typedef std::integral_constant<int, 8> C8;
+  typedef std::integral_constant<int, 16> C16;
+  typedef std::integral_constant<int, 32> C32;
+  if (E <= 16) of(C4{}, C4{});
+  else if (E <= 32) of(C4{}, C8{});
+  else if (E <= 64) of(C8{}, C8{});
+  else if (E <= 128) of(C16{}, C8{});
+  else if (E <= 256) of(C16{}, C16{});
+  else of(C32{}, C16{});
   return hipGetLastError();
 }
 
@@ -598,14 +913,17 @@ hipError_t launch_route(const mgpt_route_config* cfg, const RouteArgs& g, bool b
     constexpr int kLP = decltype(lp)::value, kV = decltype(v)::value;
     constexpr bool kSoftmax = decltype(softmax)::value;
     const int per = 4 * (kWave / kLP);
-    const int grid = (int)std::min<long>(((long)g.N + per - 1) / per, (long)compute_units() * 8);
+    const int grid = (int)std::min<long>(((long)g.N + per - 1) / per, (long)compute_units() * (backward ? 8 : 3));
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, g); };
     const bool f32 = cfg->dtype == MGPT_DTYPE_F32;
     if (backward)
       f32 ? launch(route_backward_kernel<float, kLP, kV, kSoftmax>)
           : launch(route_backward_kernel<bf16_t, kLP, kV, kSoftmax>);
+    else if (g.bias || g.G > 1)
+      f32 ? launch(route_kernel<float, kLP, kV, kSoftmax, true>) : launch(route_kernel<bf16_t, kLP, kV, kSoftmax, true>);
     else
-      f32 ? launch(route_kernel<float, kLP, kV, kSoftmax>) : launch(route_kernel<bf16_t, kLP, kV, kSoftmax>);
+      f32 ? launch(route_kernel<float, kLP, kV, kSoftmax, false>)
+          : launch(route_kernel<bf16_t, kLP, kV, kSoftmax, false>);
   });
 }
 
