@@ -608,6 +608,9 @@ typedef struct mgpt_sample_config {
   float min_p;         /* >= 0 */
 } mgpt_sample_config;
 
+/* 0 for rows of up to 8192 (workspace may then be null); 256-byte aligned. */
+int mgpt_sample_workspace_bytes(const mgpt_sample_config* cfg, int num_rows, size_t* bytes);
+
 /* u: [B] fp32, each in [0, 1); temperature, top_p, min_p: [B] fp32 or null; top_k: [B] int32 or null;
  * token: [B] int32; logp: [B] fp32 or null, the logarithm of the token's
  * probability among the kept ones (0 at temperature 0, -infinity for token -1).
@@ -615,7 +618,8 @@ typedef struct mgpt_sample_config {
  * counts as 0 in temperature and u, and as no restriction in top_p. */
 int mgpt_sample(const mgpt_sample_config* cfg, const void* logits, const float* u,
                 const float* temperature, const int32_t* top_k, const float* top_p,
-                const float* min_p, int32_t* token, float* logp, int num_rows, void* stream);
+                const float* min_p, int32_t* token, float* logp, int num_rows, void* workspace,
+                size_t workspace_bytes, void* stream);
 
 /* Description of the last error on this host thread ("" if none). */
 const char* mgpt_moe_last_error(void);

@@ -149,7 +149,8 @@ def lib() -> ctypes.CDLL:
         "mgpt_route_forward": [ctypes.POINTER(RouteConfig)] + [vp] * 5 + [i, vp],
         "mgpt_route_backward": [ctypes.POINTER(RouteConfig)] + [vp] * 6 + [i, vp],
         "mgpt_route_balance": [i, vp, ctypes.c_float, vp, vp],
-        "mgpt_sample": [ctypes.POINTER(SampleConfig)] + [vp] * 8 + [i, vp],
+        "mgpt_sample_workspace_bytes": [ctypes.POINTER(SampleConfig), i, ctypes.POINTER(sz)],
+        "mgpt_sample": [ctypes.POINTER(SampleConfig)] + [vp] * 8 + [i, vp, sz, vp],
         "mgpt_i8_weight_bytes": [ctypes.POINTER(I8Config), ctypes.POINTER(sz)],
         "mgpt_i8_pack_weight": [ctypes.POINTER(I8Config), vp, i, vp, vp, vp],
         "mgpt_i8_pack_quantized": [ctypes.POINTER(I8Config), vp, vp, vp],

@@ -17,7 +17,8 @@ _DT = {"f32": (torch.float32, capi.DTYPE_F32), "bf16": (torch.bfloat16, capi.DTY
 
 
 class Sampler:
-    """Logits are [..., V] in `act`'s type."""
+    """Logits are [..., V] in `act`'s type.  The workspace of a call is allocated
+    with torch for that call (its stream's, or the captured graph's own)."""
 
     def __init__(self, vocab_size: int, act: str = "f32"):
         self.V = vocab_size
@@ -56,6 +57,9 @@ class Sampler:
         with capi.on_device(dev):
             token = torch.empty(shape, dtype=torch.int32, device=dev)
             logp = torch.empty(shape, dtype=torch.float32, device=dev)
+            need = ctypes.c_size_t()
+            capi.check(capi.lib().mgpt_sample_workspace_bytes(ctypes.byref(cfg), token.numel(), ctypes.byref(need)))
+            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
             capi.check(capi.lib().mgpt_sample(ctypes.byref(cfg), ptr, up, *ptrs, token.data_ptr(), logp.data_ptr(),
-                                              token.numel(), capi.stream(dev)))
+                                              token.numel(), ws.data_ptr(), need.value, capi.stream(dev)))
         return token, logp

@@ -228,3 +228,95 @@ def test_rows_at_any_element_streams_graphs():
             torch.cuda.synchronize()
             got = op.forward(l, u, top_k=30, top_p=0.9)
             assert torch.equal(got[0], token) and torch.equal(got[1], logp)
+
+
+@pytest.mark.parametrize("V", [8193, 20011])
+def test_masks_and_far_logits_in_long_rows(V):
+    l, u = inputs(20, V, "f32", seed=V)
+    l[0] = -INF
+    l[1, 1:] = -INF
+    l[2, :-1] = -INF
+    l[3] = float("nan")
+    l[4, ::2] = float("nan")
+    l[5, 7] = INF
+    l[6, 5::900] = INF
+    l[7] = INF
+    l[8] = -BIG
+    l[9, V - 3] = BIG
+    l[10] *= 1e30
+    l[11] *= 1e-30
+    l[12, ::3] = -INF
+    l[13] = -INF
+    l[13, 9] = -BIG
+    l[14] += 1e6
+    l[15, ::2] = 0.0
+    l[15, 1::2] = -0.0
+    for f in FILTERS:
+        check(l, u, **f)
+    for T in (1e-30, 1e-42, 1e30, INF):
+        check(l[11:13].contiguous(), u[:2].contiguous(), T=T, k=11)
+        check(l[15:].contiguous(), u[15:].contiguous(), T=T, p=0.7)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_long_rows_with_their_own_parameters(act):
+    """More rows than a launch takes; lists of few and of many, none, and rows that settle at once, side by side."""
+    B, V = 2077, 9001
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda: torch.rand(B, generator=gen, device="cuda")  # noqa: E731
+    l, u = inputs(B, V, act)
+    T = r() * 2
+    T[::9] = 0
+    k = torch.randint(-1, 1500, (B,), generator=gen, device="cuda", dtype=torch.int32)
+    k[::5] = 0
+    k[1::5] %= 60
+    p, m = r() * 1.2, r() * 0.1
+    m[::3] = 0
+    check(l, u, T, k, p, m)
+    check(l, u, 0.8, 0, p, m)
+
+
+def test_the_list_takes_no_more():
+    """Rows whose bin holds 4096 logits, one fewer and one more, and top_k at the list's own ends."""
+    V = 30000
+    l, u = inputs(8, V, "f32", std=0.5)
+    l.clamp_(max=3.0)
+    for row, n in enumerate((4095, 4096, 4097, 255, 256, 257, 1024, 12000)):
+        l[row, 100:100 + n] = 5.0
+    for k in (1, 2, 255, 256, 257, 1023, 1024, 1025, 4096, 4097, V - 1, V, V + 5):
+        check(l, u, k=k)
+        check(l, u, k=k, p=0.5, m=0.01)
+    check(l, u, p=0.4)
+    check(l, u, p=0.9, T=0.5)
+
+
+def test_long_rows_streams_graphs():
+    from mgpt_amd.sampling import Sampler
+    V = 20001
+    op = Sampler(V, act="bf16")
+    l, u = inputs(9, V, "bf16")
+    kinds = (dict(), dict(top_k=30, top_p=0.9), dict(top_p=0.9), dict(top_k=3000))
+    op.forward(l, u)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [op.forward(l, u, **f) for f in kinds]
+    for seed in (5, 6, 7):
+        nl, nu = inputs(9, V, "bf16", seed)
+        l.copy_(nl), u.copy_(nu)
+        graph.replay()
+        torch.cuda.synchronize()
+        for f, (token, logp) in zip(kinds, out):
+            got = op.forward(l, u, **f)
+            assert torch.equal(got[0], token) and torch.equal(got[1], logp)
+    # two streams at once, a workspace each
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    want = [op.forward(l, u, **f) for f in kinds]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append([op.forward(l, u, **f) for f in kinds])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) for g in got for a, b in zip(g, want))
