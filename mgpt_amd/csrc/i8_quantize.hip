@@ -1,11 +1,10 @@
 // i8_quantize.hip -- rows in 8-bit integers with a scale each: s = max|x| / 127, q = rint(x
 // 127 / max|x|), in the layout of i8.hpp.
 //
-// A block takes a row block; lane l of a wave has 16 neighbouring columns of row l % 32, which are an
-// operand tile's 16 bytes of that lane, so that rows are read as 64-byte pieces and tiles
-// written as whole kilobytes.  One pass finds the maxima, a second one, from
-// registers where the row block fits them, rounds.  x 127 / max|x| is formed in 64 bits: fp32 would put
-// every hundred-thousandth value on the wrong side of a border between two integers, and values on a border
+// A block takes 8 rows of a row block, a wave of it 128 columns of them at a time: 16 neighbouring ones a lane, so
+// that rows are read, and the tiles' parts written, as whole lines.  One pass finds the maxima, a second one, from
+// registers up to 8192 columns, rounds.  x 127 / max|x| is formed in 64 bits, whose rate is that of 32 here: fp32 would
+// put every hundred-thousandth value on the wrong side of a border between two integers, and values on a border
 // (bf16 has many: max|x| / 2 is 63.5) have to be seen there.  A row that holds an infinity or a NaN has
 // the scale NaN, and so have its outputs.
 #include <algorithm>
@@ -15,6 +14,8 @@
 
 namespace mgpt {
 namespace {
+
+constexpr int kPart = 8;   // rows of a block
 
 // 16 values of a row as they are in memory.
 template <QuantizeSource SRC>
@@ -50,33 +51,70 @@ __device__ __forceinline__ Raw<SRC> load_raw(const QuantizeArgs& g, size_t row, 
   return r;
 }
 
+// 2^(e - 141)
+__device__ __forceinline__ float unit_of(int e) { return __uint_as_float((uint32_t)max(e - 14, 1) << 23); }
+
+// The values, kRowsF32 or kRowsBf16.
 template <QuantizeSource SRC>
 __device__ __forceinline__ void values(const QuantizeArgs& g, const Raw<SRC>& r, int c, float rs, float (&x)[16]) {
   const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
-  if constexpr (SRC == kRowsF32) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(w[i]);
-  } else if constexpr (SRC == kRowsBf16) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
-  } else {
-    // (e 255: not finite)
-    const float unit = r.e == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)max(r.e - 14, 1) << 23);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = (float)(int16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFF) * unit;
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (SRC == kRowsF32) x[i] = __uint_as_float(w[i]);
+    else x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
   }
-  if constexpr (SRC != kRowsHidden)
-    if (g.gamma) {
+  if (g.gamma) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = c + i < g.K ? (x[i] * rs) * g.gamma[c + i] : 0.0f;
+    for (int i = 0; i < 16; ++i) x[i] = c + i < g.K ? (x[i] * rs) * g.gamma[c + i] : 0.0f;
+  }
+}
+
+// The largest magnitude's bits as fp32 (infinity's or more: not finite).
+template <QuantizeSource SRC>
+__device__ __forceinline__ uint32_t largest(const QuantizeArgs& g, const Raw<SRC>& r, int c, float rs) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+  uint32_t top = 0;
+  if constexpr (SRC == kRowsHidden) {   // two at a time; within 32767
+    i16x2 most = {0, 0}, least = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const i16x2 v = __builtin_bit_cast(i16x2, w[i]);
+      most = __builtin_elementwise_max(most, v);
+      least = __builtin_elementwise_min(least, v);
     }
+    const int m = max(max((int)most[0], (int)most[1]), -min((int)least[0], (int)least[1]));
+    return r.e == 255 ? 0x7FC00000u : __float_as_uint((float)m * unit_of(r.e));
+  } else if (SRC == kRowsBf16 && !g.gamma) {
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+    return (uint32_t)max(most[0], most[1]) << 16;
+  } else {
+    float x[16];
+    values<SRC>(g, r, c, rs, x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    return top;
+  }
+}
+
+// Four values' integers, as bytes.  x f plus 1.5 2^12 in one rounding, to the nearest 2^-40: a quotient of two floats that
+// is not between two integers is 2^-34 away from there (254 x - (2n + 1) max is a whole number of their units), f's
+// own error 2^-46.  Then to the nearest integer, ties to even (1.5 2^12 is even); its low byte lies in bits 8 to
+// 15 of the upper word.
+__device__ __forceinline__ uint32_t round4(double a, double b, double c, double d, double f) {
+  auto hi = [&](double x) { return (uint32_t)__double2hiint(__builtin_rint(__builtin_fma(x, f, 0x1.8p12))); };
+  const uint32_t ab = __builtin_amdgcn_perm(hi(b), hi(a), 0x00000501), cd = __builtin_amdgcn_perm(hi(d), hi(c), 0x00000501);
+  return __builtin_amdgcn_perm(cd, ab, 0x05040100);
 }
 
 template <QuantizeSource SRC, bool VEC, int NW>
 __global__ __launch_bounds__(NW * kWave) void i8_quantize_kernel(QuantizeArgs g) {
-  constexpr int kHold = 4;   // tiles of a wave that stay in registers
-  __shared__ uint32_t s_top[NW][kI8Rows];
-  const int block = blockIdx.x;
+  constexpr int kHold = 4;   // slabs of a wave that stay in registers
+  __shared__ uint32_t s_top[NW][kPart];
+  const int block = (int)blockIdx.x / (kI8Rows / kPart), part = (int)blockIdx.x % (kI8Rows / kPart);
   int row0, rows;
   if (g.counts) {
     TileInfo t;
@@ -87,7 +125,8 @@ __global__ __launch_bounds__(NW * kWave) void i8_quantize_kernel(QuantizeArgs g)
     row0 = block * kI8Rows;
     rows = g.N - row0;
   }
-  const int w = threadIdx.x / kWave, lane = lane_id(), r = lane & 31, half = lane >> 5;
+  if (g.counts && part * kPart >= rows) return;   // (rows whose products nothing keeps)
+  const int w = threadIdx.x / kWave, lane = lane_id(), chunk = lane / kPart, r = part * kPart + lane % kPart;
   const bool live = r < rows;
   size_t row = 0;
   float rs = 1.0f;
@@ -96,61 +135,53 @@ __global__ __launch_bounds__(NW * kWave) void i8_quantize_kernel(QuantizeArgs g)
     if (g.perm) row = g.perm[row] / g.k;
     if (g.gamma) rs = g.rstd[row];
   }
-  const int tiles = (g.K + kI8Slab - 1) / kI8Slab * (kI8Slab / 32);
-  // neighbouring tiles to a wave, so that it has whole lines of the rows
-  const int per = (tiles + NW - 1) / NW, t0 = w * per, t1 = min(tiles, t0 + per);
+  const int slabs = (g.K + kI8Slab - 1) / kI8Slab;
   Raw<SRC> held[kHold];
   uint32_t top = 0;
-  auto look = [&](const Raw<SRC>& raw, int c) {
-    float x[16];
-    values<SRC>(g, raw, c, rs, x);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  };
-  auto column = [&](int t) { return t * 32 + half * 16; };
+  auto look = [&](const Raw<SRC>& raw, int c) { top = max(top, largest<SRC>(g, raw, c, rs)); };
+  auto column = [&](int t) { return t * kI8Slab + chunk * 16; };
+  auto load = [&](int t) { return load_raw<SRC, VEC>(g, row, column(t), live && column(t) < g.K); };
 #pragma unroll
   for (int u = 0; u < kHold; ++u)
-    if (t0 + u < t1) held[u] = load_raw<SRC, VEC>(g, row, column(t0 + u), live && column(t0 + u) < g.K);
+    if (w + u * NW < slabs) held[u] = load(w + u * NW);
 #pragma unroll
   for (int u = 0; u < kHold; ++u)
-    if (t0 + u < t1) look(held[u], column(t0 + u));
-  for (int t = t0 + kHold; t < t1; ++t) look(load_raw<SRC, VEC>(g, row, column(t), live && column(t) < g.K), column(t));
-  {
-    const auto o = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-    top = max(o[0], o[1]);
-  }
-  if (half == 0) s_top[w][r] = top;
+    if (w + u * NW < slabs) look(held[u], column(w + u * NW));
+  for (int t = w + kHold * NW; t < slabs; t += NW) look(load(t), column(t));
+#pragma unroll
+  for (int d = kPart; d < kWave; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d, kWave));
+  if (chunk == 0) s_top[w][lane] = top;
   __syncthreads();
   top = 0;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) top = max(top, s_top[i][r]);
+  for (int i = 0; i < NW; ++i) top = max(top, s_top[i][lane % kPart]);
   const bool finite = top < 0x7F800000u;
   const float most = __uint_as_float(top);
-  if (w == 0 && half == 0 && live)
+  if (w == 0 && chunk == 0 && live)
     g.scale[(size_t)block * kI8Rows + r] = finite ? most / 127.0f : __uint_as_float(0x7FC00000u);
   const double f = finite && top ? 127.0 / (double)most : 0.0;
-  char* out = g.q + (size_t)block * i8_row_block_bytes(g.K) + lane * 16;
+  // (column c: tile c / 32 of the row block, its half c / 16)
+  char* out = g.q + (size_t)block * i8_row_block_bytes(g.K) + (chunk / 2) * 1024 + (chunk % 2 * kI8Rows + r) * 16;
   auto put = [&](const Raw<SRC>& raw, int t) {
-    float x[16];
-    values<SRC>(g, raw, column(t), rs, x);
     uint32_t q[4];
+    if constexpr (SRC == kRowsHidden) {
+      const uint32_t* v = reinterpret_cast<const uint32_t*>(raw.w);
+      const double fu = f * (double)unit_of(raw.e == 255 ? 0 : raw.e);
+      auto x = [&](int i) { return (double)(i & 1 ? (int)v[i / 2] >> 16 : (int)(int16_t)v[i / 2]); };
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      // To the nearest 2^-40 first: a quotient of two floats that is not between two integers is 2^-34
-      // away from there (254 x - (2n + 1) max is a whole number of their units), the product's rounding 2^-45.
-      // Then to the nearest integer, ties to even, in the low bits.
-      double d = (double)(finite ? x[i] : 0.0f) * f;
-      d = (d + 0x1.8p12) - 0x1.8p12;
-      d += 0x1.8p52;
-      const uint32_t b = (uint32_t)__double2loint(d) & 0xFF;
-      q[i / 4] = i % 4 ? q[i / 4] | b << (8 * (i % 4)) : b;
+      for (int i = 0; i < 4; ++i) q[i] = round4(x(4 * i), x(4 * i + 1), x(4 * i + 2), x(4 * i + 3), fu);
+    } else {
+      float x[16];
+      values<SRC>(g, raw, column(t), rs, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = round4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], f);
     }
-    *reinterpret_cast<uint4*>(out + (size_t)t * 1024) = make_uint4(q[0], q[1], q[2], q[3]);
+    *reinterpret_cast<uint4*>(out + (size_t)t * (kI8Slab * kI8Rows)) = make_uint4(q[0], q[1], q[2], q[3]);
   };
 #pragma unroll
   for (int u = 0; u < kHold; ++u)
-    if (t0 + u < t1) put(held[u], t0 + u);
-  for (int t = t0 + kHold; t < t1; ++t) put(load_raw<SRC, VEC>(g, row, column(t), live && column(t) < g.K), t);
+    if (w + u * NW < slabs) put(held[u], w + u * NW);
+  for (int t = w + kHold * NW; t < slabs; t += NW) put(load(t), t);
 }
 
 __global__ __launch_bounds__(256) void i8_tile_kernel(const int8_t* __restrict__ q, int M, int K,
@@ -178,16 +209,17 @@ hipError_t launch_i8_quantize(QuantizeSource src, const QuantizeArgs& g, int max
   if (src == kRowsHidden && (g.h.Hp != g.K || g.K % 32 != 0 || ((uintptr_t)g.h.q & 15) != 0)) return hipErrorInvalidValue;
   const size_t size = src == kRowsF32 ? 4 : 2;
   const bool vec = src == kRowsHidden || (g.K * size % 16 == 0 && g.ld * size % 16 == 0 && ((uintptr_t)g.src & 15) == 0);
-  const int tiles = (g.K + 31) / 32;
+  const int slabs = (g.K + kI8Slab - 1) / kI8Slab;
   auto go = [&](auto s, auto v) {
     auto launch = [&](auto kernel, int nw) {
-      hipLaunchKernelGGL(kernel, dim3(max_blocks), dim3(nw * kWave), 0, st, g);
+      hipLaunchKernelGGL(kernel, dim3(max_blocks * (kI8Rows / kPart)), dim3(nw * kWave), 0, st, g);
     };
     constexpr QuantizeSource kS = decltype(s)::value;
     constexpr bool kV = decltype(v)::value;
-    // a wave's tiles stay in its registers up to 64 of a row block
-    if (tiles <= 16) launch(i8_quantize_kernel<kS, kV, 4>, 4);
-    else if (tiles <= 32) launch(i8_quantize_kernel<kS, kV, 8>, 8);
+    // the fewest waves whose registers hold the rows
+    if (slabs <= 8) launch(i8_quantize_kernel<kS, kV, 2>, 2);
+    else if (slabs <= 16) launch(i8_quantize_kernel<kS, kV, 4>, 4);
+    else if (slabs <= 32) launch(i8_quantize_kernel<kS, kV, 8>, 8);
     else launch(i8_quantize_kernel<kS, kV, 16>, 16);
   };
   auto with = [&](auto s) { vec ? go(s, std::true_type{}) : go(s, std::false_type{}); };
