@@ -23,13 +23,16 @@ __host__ __device__ inline size_t i8_row_block_bytes(int K) {
   return (size_t)((K + kI8Slab - 1) / kI8Slab) * kI8Slab * kI8Rows;
 }
 
-// Rows of hidden units between the two products of an expert: 16 bits each, with a power of two for
-// every 32: q 2^(e - 141), e the exponent byte of the largest magnitude (16 at least, 255:
-// one of them is not finite).  In bf16 one value in eight would end a step off in the integers
-// that follow (its rounding is 0.03 of their steps, rms); here one in a thousand.
+// Rows of hidden units between the two products of an expert: 20 bits each, with a power of two for
+// every 32: v 2^(e - 145), e the exponent byte (20 at least) of their largest magnitude, which is held as it was, so that
+// a row's is known without its values.  In bf16 one value in eight would end a step off in the integers
+// that follow (its rounding is 0.03 of their steps, rms); in 16 bits so one in four hundred, here one in six thousand.
+// q has the upper 16 bits, signed; n the lower 4: column 32 i + 16 b + 8 a + 4 h + c's in byte 16 i + 8 b + 4 h + c,
+// its lower half where a is 0 (a lane's accumulators and the quantiser's lane both have them in two words).
 struct HiddenRows {
   int16_t* q;      // [rows][Hp]
-  uint8_t* e;      // [rows][Hp / 32]
+  uint8_t* n;      // [rows][Hp / 2]
+  uint32_t* top;   // [rows][Hp / 32]: |h|'s bits as fp32, infinity's or more: one of the 32 is not finite
   int Hp;
 };
 

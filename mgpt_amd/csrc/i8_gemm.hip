@@ -149,27 +149,38 @@ __device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][T
         uint32_t top = 0;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const float x = (float)acc[2 * gi][i][v] * (sa[i] * sg[v]) + bg[v];
-          const float u = (float)acc[2 * gi + 1][i][v] * (sa[i] * su[v]) + bu[v];
+          const float x = fmaf((float)acc[2 * gi][i][v], sa[i] * sg[v], bg[v]);
+          const float u = fmaf((float)acc[2 * gi + 1][i][v], sa[i] * su[v], bu[v]);
           h[v] = x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)) * u;
-          top = max(top, __float_as_uint(h[v]) & 0x7FFFFFFFu);
+          top = max(top, __float_as_uint(h[v]) & 0x7FFFFFFFu);   // (a NaN lies above all)
         }
         const auto o = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-        const int e = max((int)(max(o[0], o[1]) >> 23), 16);
-        // to units of 2^(e - 141): a magnitude that rounds to 2^15 of them stays below
-        const float f = e == 255 ? 0.0f : __uint_as_float((uint32_t)(268 - e) << 23);
-        uint2 q[4];
+        top = max(o[0], o[1]);
+        const int e = max((int)(top >> 23), 20);
+        // to units of 2^(e - 145), in the low bits of a sum; a magnitude that would round to 2^19 of them stays below
+        const float f = __uint_as_float((uint32_t)max(272 - e, 1) << 23);
+        const float most = __uint_as_float((uint32_t)(e - 18) << 23) * 524287.0f;
+        uint32_t q[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          q[v] = __float_as_uint(fmaf(__builtin_amdgcn_fmed3f(h[v], -most, most), f, 0x1.8p23f));
+        uint2 hi[4];
+        uint32_t low[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          uint32_t w[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            w[c] = (uint32_t)(int)fminf(fmaxf(rintf(h[4 * k + c] * f), -32767.0f), 32767.0f) & 0xFFFF;
-          q[k] = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+          const uint32_t *w = q + 4 * k;
+          hi[k] = make_uint2(__builtin_amdgcn_perm(w[1] << 12, w[0] << 12, 0x07060302),
+                             __builtin_amdgcn_perm(w[3] << 12, w[2] << 12, 0x07060302));
+          low[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400),
+                                         __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400), 0x05040100) & 0x0F0F0F0Fu;
         }
+        const auto n = __builtin_amdgcn_permlane32_swap(low[0] | low[1] << 4, low[2] | low[3] << 4, false, false);
         const bool live = row < t.row_end;
-        store_group32(reinterpret_cast<bf16_t*>(g.h.q) + (size_t)row * g.h.Hp + hb, q, half, live);
-        if (live && half == 0) g.h.e[(size_t)row * (g.h.Hp / 32) + hb / 32] = (uint8_t)e;
+        store_group32(reinterpret_cast<bf16_t*>(g.h.q) + (size_t)row * g.h.Hp + hb, hi, half, live);
+        if (live) {
+          *reinterpret_cast<uint2*>(g.h.n + (size_t)row * (g.h.Hp / 2) + hb / 2 + 8 * half) = make_uint2(n[0], n[1]);
+          if (half == 0) g.h.top[(size_t)row * (g.h.Hp / 32) + hb / 32] = top;
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -561,7 +572,7 @@ hipError_t launch_i8_gemm(I8Out kind, const I8Args& args, int num_cus, hipStream
   const int E = g.counts ? g.E : 1;
   g.E = E;
   if (E < 1 || E > kMaxExpertsWide || g.KT < 1 || g.b_blocks < 1 || num_cus <= 0) return hipErrorInvalidValue;
-  if (kind == kI8GateUp && (g.Nf % 64 != 0 || g.h.Hp % 32 != 0 || !g.bias0 || !g.bias1 || ((uintptr_t)g.h.q & 15) != 0 ||
+  if (kind == kI8GateUp && (g.Nf % 64 != 0 || g.h.Hp % 32 != 0 || !g.bias0 || !g.bias1 || ((uintptr_t)g.h.q & 15) != 0 || ((uintptr_t)g.h.n & 7) != 0 ||
                             g.h.Hp < g.Nf / 2 || g.h.Hp % 8 != 0))
     return hipErrorInvalidValue;
   const bool odd = kind != kI8GateUp && (g.Nf % 8 != 0 || g.ldo % 8 != 0 || ((uintptr_t)g.out & 15) != 0);

@@ -21,7 +21,8 @@ constexpr int kPart = 8;   // rows of a block
 template <QuantizeSource SRC>
 struct Raw {
   uint4 w[SRC == kRowsF32 ? 4 : 2];
-  int e;   // kRowsHidden: their exponent
+  uint2 n;        // kRowsHidden: their lower bits,
+  uint32_t top;   // and the largest magnitude of their 32
 };
 
 template <QuantizeSource SRC, bool VEC>
@@ -32,7 +33,8 @@ __device__ __forceinline__ Raw<SRC> load_raw(const QuantizeArgs& g, size_t row, 
     const uint4* p = reinterpret_cast<const uint4*>(g.h.q + row * g.h.Hp + c);
     r.w[0] = p[0];
     r.w[1] = p[1];
-    r.e = g.h.e[row * (g.h.Hp / 32) + c / 32];
+    r.n = *reinterpret_cast<const uint2*>(g.h.n + row * (g.h.Hp / 2) + c / 2);
+    r.top = g.h.top[row * (g.h.Hp / 32) + c / 32];
   } else {
     typedef std::conditional_t<SRC == kRowsF32, uint32_t, uint16_t> T;
     const T* p = reinterpret_cast<const T*>(g.src) + row * g.ld + c;
@@ -51,8 +53,12 @@ __device__ __forceinline__ Raw<SRC> load_raw(const QuantizeArgs& g, size_t row, 
   return r;
 }
 
-// 2^(e - 141)
-__device__ __forceinline__ float unit_of(int e) { return __uint_as_float((uint32_t)max(e - 14, 1) << 23); }
+// Hidden unit i of the 16, in 2^(e - 145).
+__device__ __forceinline__ int hidden(const Raw<kRowsHidden>& r, int i) {
+  const uint32_t w = reinterpret_cast<const uint32_t*>(r.w)[i / 2], n = i & 4 ? r.n.y : r.n.x;
+  const int hi = i & 1 ? (int)w >> 16 : (int)(int16_t)w;
+  return hi << 4 | (int)(n >> (8 * (i & 3) + (i & 8 ? 4 : 0)) & 15);
+}
 
 // The values, kRowsF32 or kRowsBf16.
 template <QuantizeSource SRC>
@@ -73,19 +79,10 @@ __device__ __forceinline__ void values(const QuantizeArgs& g, const Raw<SRC>& r,
 template <QuantizeSource SRC>
 __device__ __forceinline__ uint32_t largest(const QuantizeArgs& g, const Raw<SRC>& r, int c, float rs) {
   typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
   const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
   uint32_t top = 0;
-  if constexpr (SRC == kRowsHidden) {   // two at a time; within 32767
-    i16x2 most = {0, 0}, least = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const i16x2 v = __builtin_bit_cast(i16x2, w[i]);
-      most = __builtin_elementwise_max(most, v);
-      least = __builtin_elementwise_min(least, v);
-    }
-    const int m = max(max((int)most[0], (int)most[1]), -min((int)least[0], (int)least[1]));
-    return r.e == 255 ? 0x7FC00000u : __float_as_uint((float)m * unit_of(r.e));
+  if constexpr (SRC == kRowsHidden) {
+    return r.top;
   } else if (SRC == kRowsBf16 && !g.gamma) {
     u16x2 most = {0, 0};
 #pragma unroll
@@ -165,9 +162,8 @@ __global__ __launch_bounds__(NW * kWave) void i8_quantize_kernel(QuantizeArgs g)
   auto put = [&](const Raw<SRC>& raw, int t) {
     uint32_t q[4];
     if constexpr (SRC == kRowsHidden) {
-      const uint32_t* v = reinterpret_cast<const uint32_t*>(raw.w);
-      const double fu = f * (double)unit_of(raw.e == 255 ? 0 : raw.e);
-      auto x = [&](int i) { return (double)(i & 1 ? (int)v[i / 2] >> 16 : (int)(int16_t)v[i / 2]); };
+      const double fu = f * (double)__uint_as_float((uint32_t)(max((int)(raw.top >> 23), 20) - 18) << 23);
+      auto x = [&](int i) { return (double)hidden(raw, i); };
 #pragma unroll
       for (int i = 0; i < 4; ++i) q[i] = round4(x(4 * i), x(4 * i + 1), x(4 * i + 2), x(4 * i + 3), fu);
     } else {
@@ -206,7 +202,7 @@ __global__ __launch_bounds__(256) void i8_tile_kernel(const int8_t* __restrict__
 
 hipError_t launch_i8_quantize(QuantizeSource src, const QuantizeArgs& g, int max_blocks, hipStream_t st) {
   if (max_blocks <= 0) return hipSuccess;
-  if (src == kRowsHidden && (g.h.Hp != g.K || g.K % 32 != 0 || ((uintptr_t)g.h.q & 15) != 0)) return hipErrorInvalidValue;
+  if (src == kRowsHidden && (g.h.Hp != g.K || g.K % 32 != 0 || ((uintptr_t)g.h.q & 15) != 0 || ((uintptr_t)g.h.n & 7) != 0)) return hipErrorInvalidValue;
   const size_t size = src == kRowsF32 ? 4 : 2;
   const bool vec = src == kRowsHidden || (g.K * size % 16 == 0 && g.ld * size % 16 == 0 && ((uintptr_t)g.src & 15) == 0);
   const int slabs = (g.K + kI8Slab - 1) / kI8Slab;

@@ -171,7 +171,7 @@ struct Layout {
   size_t nrm_part;       // fused block backward: ln2 scale-gradient partials
   // 8-bit integer experts: the gathered rows and the hidden units as row blocks with their
   // scales, and the hidden units' exponents
-  size_t xq, xs, hq, hs, hexp;
+  size_t xq, xs, hq, hs, hlow, htop;
   // a routing of the caller's rule: logits [N][E], and the scores' gradients [E]; last, so
   // that the other regions lie where they do without it
   size_t rlogits, dscore;
@@ -394,7 +394,8 @@ struct mgpt_moe {
       L.xs = take(blocks * kI8Rows * 4);
       L.hq = take(blocks * i8_row_block_bytes(Hp));
       L.hs = take(blocks * kI8Rows * 4);
-      L.hexp = take(A * (Hp / 32));
+      L.hlow = take(A * (Hp / 2));
+      L.htop = take(A * (Hp / 32) * 4);
     }
     if (routed) {
       L.rlogits = take((size_t)N * E * 4);
@@ -882,7 +883,7 @@ int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, co
                const int32_t* counts, const int32_t* perm, char* ws, hipStream_t st, Mark mark) {
   const int C = h->C, Hp = h->Hp, Cp = h->Cp, E = h->E;
   const int blocks = (int)h->row_blocks(A);
-  const HiddenRows hidden{(int16_t*)(ws + L.hbuf), (uint8_t*)(ws + L.hexp), Hp};
+  const HiddenRows hidden{(int16_t*)(ws + L.hbuf), (uint8_t*)(ws + L.hlow), (uint32_t*)(ws + L.htop), Hp};
   QuantizeArgs q{};
   q.src = x;
   q.ld = C;
