@@ -124,17 +124,21 @@ __device__ __forceinline__ f32x16 take_outputs(const float* p, int n, int half) 
   return r;
 }
 
-// Accumulators of TN x TM tiles: outputs fw + 32 j, rows row0 + 32 i of the tile t (row blocks
-// blk + i of A).
-template <int KIND, int TN, int TM>
-__device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][TM], const RowTile& t, int row0, int blk,
-                                      int fw, int lrow, int half) {
-  const size_t eb = (size_t)(g.e_base + t.expert);
-  const float* sb = g.sb + eb * g.ldsb;
-  float sa[TM];
+// The scales of a lane's rows row0 + 32 i + lrow of the tile t.
+template <int TM>
+__device__ __forceinline__ void row_scales(const I8Args& g, const RowTile& t, int row0, int blk, int lrow, float (&sa)[TM]) {
 #pragma unroll
   for (int i = 0; i < TM; ++i)
     sa[i] = row0 + 32 * i + lrow < t.row_end ? g.sa[(size_t)(blk + i) * kI8Rows + lrow] : 0.0f;
+}
+
+// Accumulators of TN x TM tiles: outputs fw + 32 j, rows row0 + 32 i of the tile t (row blocks
+// blk + i of A), and the rows' scales.
+template <int KIND, int TN, int TM>
+__device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][TM], const float (&sa)[TM], const RowTile& t,
+                                      int row0, int fw, int lrow, int half) {
+  const size_t eb = (size_t)(g.e_base + t.expert);
+  const float* sb = g.sb + eb * g.ldsb;
   if constexpr (KIND == kI8GateUp) {
 #pragma unroll
     for (int gi = 0; gi < TN / 2; ++gi) {
@@ -365,6 +369,16 @@ __global__ __launch_bounds__(NW * kWave, 2) void i8_ring_kernel(I8Args g, int gr
       ws[j] = *reinterpret_cast<const i32x4*>(w_base + bslot * kSlot + j * kSlabBytes + ks * kTileBytes);
   };
 
+  // A tile's row scales are loaded a tile ahead: a load waits for the ring's loads before it.
+  float sa[TM];
+  auto scales = [&](const I8Tile& c, float (&to)[TM]) __attribute__((always_inline)) {
+    if constexpr (!ODD) row_scales<TM>(g, c.r, c.r.row0 + wm * W::WTM, c.r.blk0 + wm * TM, lane_id() & 31, to);
+  };
+  scales(cur, sa);
+  if constexpr (!ODD)
+#pragma unroll
+    for (int i = 0; i < TM; ++i) asm volatile("" : "+v"(sa[i]));
+
   // units A0 B0 A1
   next_unit(ua, la);
   issue(kDB, kD);
@@ -432,10 +446,21 @@ __global__ __launch_bounds__(NW * kWave, 2) void i8_ring_kernel(I8Args g, int gr
     int lane_now;
     asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane_now));
     const int row0 = cur.r.row0 + wm * W::WTM, blk = cur.r.blk0 + wm * TM, fw = cur.n0 + wn * W::WTN;
-    if constexpr (ODD) emit8_odd<KIND, TN, TM>(g, acc, cur.r, row0, blk, fw, lane_now & 31, lane_now >> 5);
-    else emit8<KIND, TN, TM>(g, acc, cur.r, row0, blk, fw, lane_now & 31, lane_now >> 5);
     t += G;
-    if (!locate8<BM, BN>(sc, nbx, t, &cur)) break;
+    I8Tile next;
+    const bool more = locate8<BM, BN>(sc, nbx, t, &next);
+    float ahead[TM];
+    if (more) scales(next, ahead);
+    if constexpr (ODD) emit8_odd<KIND, TN, TM>(g, acc, cur.r, row0, blk, fw, lane_now & 31, lane_now >> 5);
+    else emit8<KIND, TN, TM>(g, acc, sa, cur.r, row0, fw, lane_now & 31, lane_now >> 5);
+    if (!more) break;
+    cur = next;
+    if constexpr (!ODD)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        sa[i] = ahead[i];
+        asm volatile("" : "+v"(sa[i]));   // (waited for here)
+      }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the repeated loads at the end
 }
@@ -561,7 +586,11 @@ __global__ __launch_bounds__(kStreamWaves * kWave) void i8_stream_kernel(I8Args 
   }
   if (!busy) return;
   if constexpr (ODD) emit8_odd<KIND, FB, MT>(g, acc, t, t.row0, t.blk0, fb * kI8Rows, lane & 31, lane >> 5);
-  else emit8<KIND, FB, MT>(g, acc, t, t.row0, t.blk0, fb * kI8Rows, lane & 31, lane >> 5);
+  else {
+    float sa[MT];
+    row_scales<MT>(g, t, t.row0, t.blk0, lane & 31, sa);
+    emit8<KIND, FB, MT>(g, acc, sa, t, t.row0, fb * kI8Rows, lane & 31, lane >> 5);
+  }
 }
 
 }  // namespace
