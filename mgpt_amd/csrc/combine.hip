@@ -10,6 +10,7 @@
 // k rows in that order with the same two roundings per term (the file is
 // built with -ffp-contract=off), reading 16 bytes per lane per row chunk.
 #include "common.hpp"
+#include "i8.hpp"
 
 namespace mgpt {
 namespace {
@@ -262,6 +263,61 @@ __global__ __launch_bounds__(256) void combine2_kernel(const ActT* __restrict__ 
   }
 }
 
+// The same sums over Rows16: a wave 512 columns of a token, 8 a lane, AT of its rows in flight; in the order of the
+// experts, by fused multiply-adds (these rows have no sum elsewhere to agree with).
+template <typename OutT, int AT>
+__global__ __launch_bounds__(256) void combine16_kernel(Rows16 rows, const int32_t* __restrict__ topk_idx,
+                                                        const float* __restrict__ topk_p,
+                                                        const int32_t* __restrict__ slot_of, int N, int C, int k,
+                                                        const OutT* __restrict__ resid, OutT* __restrict__ y) {
+  __shared__ int s_slot[kWavesPerBlock][kMaxTopK];
+  __shared__ float s_p[kWavesPerBlock][kMaxTopK];
+  const int w = threadIdx.x / kWave, l = lane_id();
+  const int t = blockIdx.x * kWavesPerBlock + w;
+  if (t >= N) return;   // whole wave exits together; no block barrier below
+  const bool mine = l < k;
+  const int e = mine ? topk_idx[(size_t)t * k + l] : 0, slot = mine ? slot_of[(size_t)t * k + l] : 0;
+  const float p = mine ? topk_p[(size_t)t * k + l] : 0.0f;
+  int rank = 0;
+  for (int i = 0; i < k; ++i) {
+    const int ei = __shfl(e, i, kWave);
+    rank += (ei < e) || (ei == e && i < l);
+  }
+  if (mine) {
+    s_slot[w][rank] = slot;
+    s_p[w][rank] = p;
+  }
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  const int c = ((int)blockIdx.y * kWave + l) * 8;
+  if (c < C) {
+    float acc[8] = {};
+    for (int a0 = 0; a0 < k; a0 += AT) {
+      uint4 raw[AT];
+      uint32_t top[AT];
+#pragma unroll
+      for (int a = 0; a < AT; ++a) {
+        const size_t row = s_slot[w][min(a0 + a, k - 1)];
+        raw[a] = *reinterpret_cast<const uint4*>(rows.q + row * rows.ld + c);
+        top[a] = rows.top[row * (rows.ld / 32) + c / 32];
+      }
+#pragma unroll
+      for (int a = 0; a < AT; ++a) {
+        if (a0 + a >= k) break;
+        // 2^(e - 141)
+        float unit = __uint_as_float((uint32_t)(max((int)(top[a] >> 23), 16) - 14) << 23) * s_p[w][a0 + a];
+        if (top[a] >= 0x7F800000u) unit = __uint_as_float(0x7FC00000u);
+        const uint32_t v[4] = {raw[a].x, raw[a].y, raw[a].z, raw[a].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          acc[i] = fmaf((float)(i & 1 ? (int)v[i / 2] >> 16 : (int)(int16_t)v[i / 2]), unit, acc[i]);
+      }
+    }
+    if (resid) add_resid<OutT, 8>(resid + (size_t)t * C + c, acc);
+    OutVec<OutT, 8>::store(y + (size_t)t * C + c, acc);
+  }
+}
+
 template <typename ActT, typename OutT, int TPW, int KT>
 void launch_combine_k(int chunks, hipStream_t stream, const ActT* out_rows,
                       const int32_t* topk_idx, const float* topk_p, const int32_t* slot_of, int N,
@@ -315,6 +371,25 @@ hipError_t launch_combine(const ActT* out_rows, const int32_t* topk_idx, const f
   }
   return hipGetLastError();
 }
+
+template <typename OutT>
+hipError_t launch_combine16(const Rows16& rows, const int32_t* topk_idx, const float* topk_p, const int32_t* slot_of,
+                            int N, int C, int k, const OutT* resid, OutT* y, hipStream_t stream) {
+  if (N == 0) return hipSuccess;
+  if (k < 1 || k > kMaxTopK || C % 32 != 0 || rows.ld % 32 != 0) return hipErrorInvalidValue;
+  const dim3 grid((N + kWavesPerBlock - 1) / kWavesPerBlock, (C + kWave * 8 - 1) / (kWave * 8));
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, rows, topk_idx, topk_p, slot_of, N, C, k, resid, y);
+  };
+  if (k <= 2) go(combine16_kernel<OutT, 2>);
+  else if (k <= 4) go(combine16_kernel<OutT, 4>);
+  else go(combine16_kernel<OutT, 8>);
+  return hipGetLastError();
+}
+template hipError_t launch_combine16<float>(const Rows16&, const int32_t*, const float*, const int32_t*, int, int, int,
+                                            const float*, float*, hipStream_t);
+template hipError_t launch_combine16<bf16_t>(const Rows16&, const int32_t*, const float*, const int32_t*, int, int, int,
+                                             const bf16_t*, bf16_t*, hipStream_t);
 
 template hipError_t launch_combine<float, float>(const float*, const int32_t*, const float*,
                                                  const int32_t*, int, int, int, const float*,

@@ -23,17 +23,23 @@ __host__ __device__ inline size_t i8_row_block_bytes(int K) {
   return (size_t)((K + kI8Slab - 1) / kI8Slab) * kI8Slab * kI8Rows;
 }
 
-// Rows of hidden units between the two products of an expert: 20 bits each, with a power of two for
-// every 32: v 2^(e - 145), e the exponent byte (20 at least) of their largest magnitude, which is held as it was, so that
-// a row's is known without its values.  In bf16 one value in eight would end a step off in the integers
-// that follow (its rounding is 0.03 of their steps, rms); in 16 bits so one in four hundred, here one in six thousand.
-// q has the upper 16 bits, signed; n the lower 4: column 32 i + 16 b + 8 a + 4 h + c's in byte 16 i + 8 b + 4 h + c,
-// its lower half where a is 0 (a lane's accumulators and the quantiser's lane both have them in two words).
+// Rows that one kernel leaves to another, with a power of two for every 32 values: v 2^(e - 141), v of 16 bits and e the
+// exponent byte (16 at least) of the largest magnitude of the 32, which is held as it was.  At bf16's size they are
+// 2^-16 of that magnitude off at most.
+struct Rows16 {
+  int16_t* q;      // [rows][ld]
+  uint32_t* top;   // [rows][ld / 32]: |x|'s bits as fp32, infinity's or more: one of the 32 is not finite
+  int ld;
+};
+
+// Hidden units between the two products of an expert, with 4 more bits: v 2^(e - 145), e 20 at least.  In bf16 one value in
+// eight would end a step off in the integers that follow (its rounding is 0.03 of their steps, rms), in 16 bits one in
+// four hundred, here one in six thousand.  The largest magnitudes give a row's without its values.
+// n: column 32 i + 16 b + 8 a + 4 h + c's bits in byte 16 i + 8 b + 4 h + c, its lower half where a is 0 (a lane's
+// accumulators and the quantiser's lane both have them in two words).
 struct HiddenRows {
-  int16_t* q;      // [rows][Hp]
-  uint8_t* n;      // [rows][Hp / 2]
-  uint32_t* top;   // [rows][Hp / 32]: |h|'s bits as fp32, infinity's or more: one of the 32 is not finite
-  int Hp;
+  Rows16 r;
+  uint8_t* n;      // [rows][ld / 2]
 };
 
 // Rows to quantise.  Dense: rows 0 .. N - 1 of src.  By experts (counts): slot s of a segment is row
@@ -72,11 +78,12 @@ struct I8Args {
   int E, N;                // N: rows in all
   void* out;               // [rows][ldo]
   size_t ldo;
-  HiddenRows h;            // gate/up: instead
+  HiddenRows h;            // kI8GateUp, and without n kI8Rows16: instead
   int rowsfirst;           // set by the launcher: a lane has an output column
   int e_base;
 };
-enum I8Out { kI8F32, kI8Bf16, kI8GateUp };
+enum I8Out { kI8F32, kI8Bf16, kI8GateUp, kI8Rows16, kI8GateUpF32 };
+// kI8GateUp, kI8GateUpF32, kI8Rows16: Nf is a multiple of 64.
 hipError_t launch_i8_gemm(I8Out kind, const I8Args& g, int num_cus, hipStream_t st);
 
 }  // namespace mgpt

@@ -132,6 +132,45 @@ __device__ __forceinline__ void row_scales(const I8Args& g, const RowTile& t, in
     sa[i] = row0 + 32 * i + lrow < t.row_end ? g.sa[(size_t)(blk + i) * kI8Rows + lrow] : 0.0f;
 }
 
+// Columns col .. col + 31 of a row of Rows16, or of HiddenRows: a lane of each half has 16 values, as an accumulator does,
+// and their largest magnitude's bits.
+template <bool HIDDEN>
+__device__ __forceinline__ void put_group(const HiddenRows& to, const float (&x)[16], uint32_t top, int row, int col,
+                                          int half, bool live) {
+  constexpr int kBits = HIDDEN ? 20 : 16;
+  const auto o = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+  top = max(o[0], o[1]);
+  const int e = max((int)(top >> 23), kBits);
+  // to units of 2^(e - 125 - kBits), in the low bits of a sum; a magnitude that would round to 2^(kBits - 1) of them stays
+  // below
+  const float f = __uint_as_float((uint32_t)max(252 + kBits - e, 1) << 23);
+  const float most = __uint_as_float((uint32_t)(e + 2 - kBits) << 23) * (float)((1 << (kBits - 1)) - 1);
+  uint32_t q[16];
+#pragma unroll
+  for (int v = 0; v < 16; ++v)
+    q[v] = __float_as_uint(fmaf(__builtin_amdgcn_fmed3f(x[v], -most, most), f, 0x1.8p23f));
+  uint2 hi[4];
+  uint32_t low[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t* w = q + 4 * k;
+    if constexpr (HIDDEN) {
+      hi[k] = make_uint2(__builtin_amdgcn_perm(w[1] << 12, w[0] << 12, 0x07060302),
+                         __builtin_amdgcn_perm(w[3] << 12, w[2] << 12, 0x07060302));
+      low[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400),
+                                     __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400), 0x05040100) & 0x0F0F0F0Fu;
+    } else {
+      hi[k] = make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x05040100), __builtin_amdgcn_perm(w[3], w[2], 0x05040100));
+    }
+  }
+  store_group32(reinterpret_cast<bf16_t*>(to.r.q) + (size_t)row * to.r.ld + col, hi, half, live);
+  if constexpr (HIDDEN) {
+    const auto n = __builtin_amdgcn_permlane32_swap(low[0] | low[1] << 4, low[2] | low[3] << 4, false, false);
+    if (live) *reinterpret_cast<uint2*>(to.n + (size_t)row * (to.r.ld / 2) + col / 2 + 8 * half) = make_uint2(n[0], n[1]);
+  }
+  if (live && half == 0) to.r.top[(size_t)row * (to.r.ld / 32) + col / 32] = top;
+}
+
 // Accumulators of TN x TM tiles: outputs fw + 32 j, rows row0 + 32 i of the tile t (row blocks
 // blk + i of A), and the rows' scales.
 template <int KIND, int TN, int TM>
@@ -139,7 +178,7 @@ __device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][T
                                       int row0, int fw, int lrow, int half) {
   const size_t eb = (size_t)(g.e_base + t.expert);
   const float* sb = g.sb + eb * g.ldsb;
-  if constexpr (KIND == kI8GateUp) {
+  if constexpr (KIND == kI8GateUp || KIND == kI8GateUpF32) {
 #pragma unroll
     for (int gi = 0; gi < TN / 2; ++gi) {
       const int f0 = fw + 64 * gi, hb = f0 / 2;
@@ -153,37 +192,25 @@ __device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][T
         uint32_t top = 0;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const float x = fmaf((float)acc[2 * gi][i][v], sa[i] * sg[v], bg[v]);
-          const float u = fmaf((float)acc[2 * gi + 1][i][v], sa[i] * su[v], bu[v]);
-          h[v] = x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)) * u;
+          const float ag = (float)acc[2 * gi][i][v], au = (float)acc[2 * gi + 1][i][v];
+          if constexpr (KIND == kI8GateUpF32) {
+            // each operation's own rounding: the integers of h are those of the formula in fp32
+            const float x = ag * sa[i] * sg[v] + bg[v], u = au * sa[i] * su[v] + bu[v];
+            h[v] = x / (1.0f + expf(-x)) * u;
+          } else {   // (some 2^-22 off, a quarter of what 20 bits are)
+            const float x = fmaf(ag, sa[i] * sg[v], bg[v]), u = fmaf(au, sa[i] * su[v], bu[v]);
+            h[v] = x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)) * u;
+          }
           top = max(top, __float_as_uint(h[v]) & 0x7FFFFFFFu);   // (a NaN lies above all)
         }
-        const auto o = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-        top = max(o[0], o[1]);
-        const int e = max((int)(top >> 23), 20);
-        // to units of 2^(e - 145), in the low bits of a sum; a magnitude that would round to 2^19 of them stays below
-        const float f = __uint_as_float((uint32_t)max(272 - e, 1) << 23);
-        const float most = __uint_as_float((uint32_t)(e - 18) << 23) * 524287.0f;
-        uint32_t q[16];
+        if constexpr (KIND == kI8GateUpF32) {
+          if (row < t.row_end)
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-          q[v] = __float_as_uint(fmaf(__builtin_amdgcn_fmed3f(h[v], -most, most), f, 0x1.8p23f));
-        uint2 hi[4];
-        uint32_t low[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t *w = q + 4 * k;
-          hi[k] = make_uint2(__builtin_amdgcn_perm(w[1] << 12, w[0] << 12, 0x07060302),
-                             __builtin_amdgcn_perm(w[3] << 12, w[2] << 12, 0x07060302));
-          low[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400),
-                                         __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400), 0x05040100) & 0x0F0F0F0Fu;
-        }
-        const auto n = __builtin_amdgcn_permlane32_swap(low[0] | low[1] << 4, low[2] | low[3] << 4, false, false);
-        const bool live = row < t.row_end;
-        store_group32(reinterpret_cast<bf16_t*>(g.h.q) + (size_t)row * g.h.Hp + hb, hi, half, live);
-        if (live) {
-          *reinterpret_cast<uint2*>(g.h.n + (size_t)row * (g.h.Hp / 2) + hb / 2 + 8 * half) = make_uint2(n[0], n[1]);
-          if (half == 0) g.h.top[(size_t)row * (g.h.Hp / 32) + hb / 32] = top;
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + (size_t)row * g.ldo + hb + 8 * k + 4 * half) =
+                  make_float4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+        } else {
+          put_group<true>(g.h, h, top, row, hb, half, row < t.row_end);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -202,7 +229,12 @@ __device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][T
 #pragma unroll
         for (int v = 0; v < 16; ++v) y[v] = (float)acc[j][i][v] * (sa[i] * s[v]) + b[v];
         const bool live = row < t.row_end;
-        if constexpr (KIND == kI8Bf16) {
+        if constexpr (KIND == kI8Rows16) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) top = max(top, __float_as_uint(y[v]) & 0x7FFFFFFFu);
+          put_group<false>(g.h, y, top, row, f0, half, live);
+        } else if constexpr (KIND == kI8Bf16) {
           bf16_t* o = reinterpret_cast<bf16_t*>(g.out) + (size_t)row * g.ldo + f0;
           uint2 q[4];
 #pragma unroll
@@ -601,10 +633,16 @@ hipError_t launch_i8_gemm(I8Out kind, const I8Args& args, int num_cus, hipStream
   const int E = g.counts ? g.E : 1;
   g.E = E;
   if (E < 1 || E > kMaxExpertsWide || g.KT < 1 || g.b_blocks < 1 || num_cus <= 0) return hipErrorInvalidValue;
-  if (kind == kI8GateUp && (g.Nf % 64 != 0 || g.h.Hp % 32 != 0 || !g.bias0 || !g.bias1 || ((uintptr_t)g.h.q & 15) != 0 || ((uintptr_t)g.h.n & 7) != 0 ||
-                            g.h.Hp < g.Nf / 2 || g.h.Hp % 8 != 0))
+  const bool gate_up = kind == kI8GateUp || kind == kI8GateUpF32;
+  if ((kind == kI8GateUp || kind == kI8Rows16) &&
+      (g.h.r.ld % 32 != 0 || g.h.r.ld < (gate_up ? g.Nf / 2 : g.Nf) || ((uintptr_t)g.h.r.q & 15) != 0 ||
+       ((uintptr_t)g.h.n & 7) != 0 || (gate_up && !g.h.n)))
     return hipErrorInvalidValue;
-  const bool odd = kind != kI8GateUp && (g.Nf % 8 != 0 || g.ldo % 8 != 0 || ((uintptr_t)g.out & 15) != 0);
+  if (kind == kI8GateUpF32 && (g.ldo % 4 != 0 || (long)g.ldo < g.Nf / 2 || ((uintptr_t)g.out & 15) != 0))
+    return hipErrorInvalidValue;
+  if ((gate_up || kind == kI8Rows16) && g.Nf % 64 != 0) return hipErrorInvalidValue;
+  if (gate_up && (!g.bias0 || !g.bias1)) return hipErrorInvalidValue;
+  const bool odd = (kind == kI8F32 || kind == kI8Bf16) && (g.Nf % 8 != 0 || g.ldo % 8 != 0 || ((uintptr_t)g.out & 15) != 0);
   auto with = [&](auto k, auto o) {
     constexpr int kK = decltype(k)::value;
     constexpr bool kO = decltype(o)::value;
@@ -639,6 +677,8 @@ hipError_t launch_i8_gemm(I8Out kind, const I8Args& args, int num_cus, hipStream
     else ring(IntC<256>{}, IntC<256>{}, IntC<8>{});
   };
   if (kind == kI8GateUp) with(IntC<kI8GateUp>{}, std::false_type{});
+  else if (kind == kI8GateUpF32) with(IntC<kI8GateUpF32>{}, std::false_type{});
+  else if (kind == kI8Rows16) with(IntC<kI8Rows16>{}, std::false_type{});
   else if (kind == kI8F32) odd ? with(IntC<kI8F32>{}, std::true_type{}) : with(IntC<kI8F32>{}, std::false_type{});
   else odd ? with(IntC<kI8Bf16>{}, std::true_type{}) : with(IntC<kI8Bf16>{}, std::false_type{});
   return hipGetLastError();

@@ -54,6 +54,9 @@ hipError_t launch_permute(const InT*, const int32_t*, const int32_t*, int32_t*, 
 template <typename ActT, typename OutT>
 hipError_t launch_combine(const ActT*, const int32_t*, const float*, const int32_t*, int, int, int,
                           const OutT*, OutT*, hipStream_t);
+template <typename OutT>
+hipError_t launch_combine16(const Rows16&, const int32_t*, const float*, const int32_t*, int, int, int, const OutT*, OutT*,
+                            hipStream_t);
 template <typename T>
 hipError_t launch_copy_cols(const T*, int, T*, int, int, int, int, hipStream_t);
 hipError_t launch_add_jobs(const float*, const AddJobs&, size_t, hipStream_t);
@@ -171,7 +174,7 @@ struct Layout {
   size_t nrm_part;       // fused block backward: ln2 scale-gradient partials
   // 8-bit integer experts: the gathered rows and the hidden units as row blocks with their
   // scales, and the hidden units' exponents
-  size_t xq, xs, hq, hs, hlow, htop;
+  size_t xq, xs, hq, hs, hlow, htop, otop;
   // a routing of the caller's rule: logits [N][E], and the scores' gradients [E]; last, so
   // that the other regions lie where they do without it
   size_t rlogits, dscore;
@@ -335,6 +338,8 @@ struct mgpt_moe {
     return wdt == MGPT_DTYPE_FP8_E4M3 || wdt == MGPT_DTYPE_I8 ? 1 : (wdt == MGPT_DTYPE_BF16 ? 2 : 4);
   }
   bool i8() const { return wdt == MGPT_DTYPE_I8; }
+  // of a hidden unit or expert output (experts in 8 bits with an fp32 caller keep them in fp32)
+  size_t row_bytes() const { return i8() && io == MGPT_DTYPE_F32 ? 4 : act_bytes(); }
   // row blocks that A rows of E experts make up at most
   size_t row_blocks(size_t A) const { return A / kI8Rows + std::min((size_t)E, A); }
   // bytes of an expert's gate/up and down operands in 8-bit integers
@@ -364,8 +369,8 @@ struct mgpt_moe {
     // forward always routes through the logits)
     L.logits = take(E > 16 ? (size_t)(wide() ? N : std::min(N, 4095)) * E * 4 : 0);
     L.xg = take(i8() ? 0 : (A + kRowPad) * C * act_bytes());
-    L.hbuf = take((A + kRowPad) * Hp * act_bytes());
-    L.obuf = take((A + kRowPad) * C * act_bytes());
+    L.hbuf = take((A + kRowPad) * Hp * row_bytes());
+    L.obuf = take((A + kRowPad) * C * row_bytes());
     // fp32 partial tiles of the large-M GEMMs' split last round (one per CU)
     L.partials = take(uses_gemm_dma(N) ? (size_t)num_cus * kGemmPartialBytes : 0);
     L.rstd = take((size_t)N * 4);
@@ -394,8 +399,10 @@ struct mgpt_moe {
       L.xs = take(blocks * kI8Rows * 4);
       L.hq = take(blocks * i8_row_block_bytes(Hp));
       L.hs = take(blocks * kI8Rows * 4);
-      L.hlow = take(A * (Hp / 2));
-      L.htop = take(A * (Hp / 32) * 4);
+      const size_t packed = row_bytes() == 2 ? A : 0;
+      L.hlow = take(packed * (Hp / 2));
+      L.htop = take(packed * (Hp / 32) * 4);
+      L.otop = take(packed * (C / 32) * 4);
     }
     if (routed) {
       L.rlogits = take((size_t)N * E * 4);
@@ -880,10 +887,10 @@ struct BlockArgs {
 // gate/up with SwiGLU, the hidden units quantised in turn, down.
 template <typename IoT, typename Mark>
 int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, const float* gamma, size_t A,
-               const int32_t* counts, const int32_t* perm, char* ws, hipStream_t st, Mark mark) {
+               const int32_t* counts, const int32_t* perm, const Rows16& out, char* ws, hipStream_t st, Mark mark) {
   const int C = h->C, Hp = h->Hp, Cp = h->Cp, E = h->E;
   const int blocks = (int)h->row_blocks(A);
-  const HiddenRows hidden{(int16_t*)(ws + L.hbuf), (uint8_t*)(ws + L.hlow), (uint32_t*)(ws + L.htop), Hp};
+  const HiddenRows hidden{{(int16_t*)(ws + L.hbuf), (uint32_t*)(ws + L.htop), Hp}, (uint8_t*)(ws + L.hlow)};
   QuantizeArgs q{};
   q.src = x;
   q.ld = C;
@@ -914,17 +921,22 @@ int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, co
   g.E = E;
   g.N = (int)A;
   g.h = hidden;
-  HIP_TRY(launch_i8_gemm(kI8GateUp, g, h->num_cus, st));
+  g.out = ws + L.hbuf;
+  g.ldo = Hp;
+  constexpr bool kF32 = sizeof(IoT) == 4;
+  HIP_TRY(launch_i8_gemm(kF32 ? kI8GateUpF32 : kI8GateUp, g, h->num_cus, st));
   HIP_TRY(mark(3));
   QuantizeArgs qh{};
   qh.h = hidden;
+  qh.src = ws + L.hbuf;
+  qh.ld = Hp;
   qh.K = Hp;
   qh.counts = counts;
   qh.E = E;
   qh.k = h->k;
   qh.q = ws + L.hq;
   qh.scale = (float*)(ws + L.hs);
-  HIP_TRY(launch_i8_quantize(kRowsHidden, qh, blocks, st));
+  HIP_TRY(launch_i8_quantize(kF32 ? kRowsF32 : kRowsHidden, qh, blocks, st));
   g.A = ws + L.hq;
   g.sa = (const float*)(ws + L.hs);
   g.B = (const char*)h->wd;
@@ -937,9 +949,10 @@ int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, co
   g.bias0 = h->bd;
   g.bias1 = nullptr;
   g.bias_ld = Cp;
+  g.h = {out, nullptr};
   g.out = ws + L.obuf;
   g.ldo = C;
-  HIP_TRY(launch_i8_gemm(kI8Bf16, g, h->num_cus, st));
+  HIP_TRY(launch_i8_gemm(kF32 ? kI8F32 : kI8Rows16, g, h->num_cus, st));
   return MGPT_OK;
 }
 
@@ -1030,8 +1043,9 @@ int forward_impl(mgpt_moe* h, const IoT* x, IoT* y, int N, char* ws, bool train,
     HIP_TRY((launch_permute<IoT, ActT>(xi, idx, block_hist, base, N, C, E, k, counts, perm, slot_of,
                                        h->i8() ? nullptr : xg, rstd, gamma, st)));
   HIP_TRY(mark(2));
+  const Rows16 rows16{(int16_t*)ob, (uint32_t*)(ws + L.otop), C};   // the outputs of experts in 8 bits
   if (h->i8()) {
-    if (int rc = i8_experts<IoT>(h, L, xi, rstd, gamma, A, counts, perm, ws, st, mark)) return rc;
+    if (int rc = i8_experts<IoT>(h, L, xi, rstd, gamma, A, counts, perm, rows16, ws, st, mark)) return rc;
   } else if constexpr (sizeof(ActT) == 4) {
     HIP_TRY(launch_gemm_f32<kEpiGateUp>(xg, (const float*)h->wgu, h->bg, h->bu, counts, E, C, 2 * Hp,
                                         2 * Hp, Hp, hb, Hp, A, gu, 2 * Hp, h->num_cus, st));
@@ -1113,8 +1127,14 @@ int forward_impl(mgpt_moe* h, const IoT* x, IoT* y, int N, char* ws, bool train,
     }
   }
   HIP_TRY(mark(4));
-  HIP_TRY((launch_combine<ActT, IoT>(ob, idx, topp, slot_of, N, C, k, gamma ? xi : nullptr, yi,
-                                     st)));
+  if (h->i8() && sizeof(IoT) == 4)
+    HIP_TRY((launch_combine<float, float>((const float*)ob, idx, topp, slot_of, N, C, k,
+                                          gamma ? (const float*)xi : nullptr, (float*)yi, st)));
+  else if (h->i8())
+    HIP_TRY(launch_combine16<IoT>(rows16, idx, topp, slot_of, N, C, k, gamma ? xi : nullptr, yi, st));
+  else
+    HIP_TRY((launch_combine<ActT, IoT>(ob, idx, topp, slot_of, N, C, k, gamma ? xi : nullptr, yi,
+                                       st)));
   if (h->padded()) HIP_TRY(launch_copy_cols<IoT>(yi, C, y, Cx, N, Cx, Cx, st));
   HIP_TRY(mark(5));
   if (prof) ++h->prof_count;

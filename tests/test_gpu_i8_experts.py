@@ -1,8 +1,8 @@
 """MoELayer(weights="i8") against its formula in 64 bits: rows quantised as gathered, gate and
 up, h = silu(g) u, h quantised in turn, down, weighted.
 
-What the device's h differs from the exact one by (2^-16 of a group's largest for the 16 bits
-it is held in, and some 2^-20 of g and u) moves it across a border between two integers with that probability, in integer
+What the device's h differs from the exact one by (for bf16 the 20 bits it is held in, at most 2^-16 of a group's
+largest; some 2^-20 of g and u) moves it across a border between two integers with that probability, in integer
 steps up to 2 127 2^-16 + 127 2^-18 < 0.005.  An output's error is a sum over k of such steps, each of at most b = 127 sh sd and with a
 variance of at most 0.005 (sh qd_k sd)^2, v in sum: by Bernstein's inequality it passes t = c b + sqrt((c b)^2 + 6 c v) with
 a probability of 2 exp(-3 c); c = 20 / 3 makes that 4e-9 of an output.  Beside t the tolerance has 2^-7 of the summed
@@ -27,7 +27,7 @@ def gpu():
 
 def quantised(a):
     top = a.double().abs().amax(-1, keepdim=True)
-    q = torch.where(top > 0, torch.round(a.double() * 127 / top), torch.zeros(()).double().to(a.device))
+    q = torch.where(top > 0, torch.round(a.double() * (127 / top)), torch.zeros(()).double().to(a.device))
     return q, (top / 127).squeeze(-1)
 
 

@@ -2,8 +2,7 @@
 
 Tolerance, u = 2^-24: the sum as a float, the token's scale, its product with the output's,
 the product and the bias each round once: 6 u of the terms' magnitudes, and half a step of the
-output's type, 2^-8 of the value in bf16.  The integers are the same on both sides: 127 x is exact in 64 bits, and so is
-its quotient where it lies between two integers.
+output's type, 2^-8 of the value in bf16.  The integers are the same on both sides: x times 127 (1 / max|x|), in 64 bits.
 """
 import pytest
 
@@ -25,7 +24,7 @@ def gpu():
 
 def quantised(x):
     top = x.double().abs().amax(1, keepdim=True)
-    q = torch.where(top > 0, torch.round(x.double() * 127 / top), torch.zeros(()).double().to(x.device))
+    q = torch.where(top > 0, torch.round(x.double() * (127 / top)), torch.zeros(()).double().to(x.device))
     return q, (top / 127).squeeze(1)
 
 
