@@ -608,21 +608,31 @@ __global__ __launch_bounds__(kStreamWaves * kWave) void i8_stream_kernel(I8Args 
 #pragma unroll
           for (int v = 0; v < 16; ++v) atomicAdd(mine + ((j * MT + i) * 16 + v) * kWave, acc[j][i][v]);
     __syncthreads();
-    if (s > 0) return;
-#pragma unroll
-    for (int j = 0; j < FB; ++j)
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) acc[j][i][v] = mine[((j * MT + i) * 16 + v) * kWave];
   }
   if (!busy) return;
-  if constexpr (ODD) emit8_odd<KIND, FB, MT>(g, acc, t, t.row0, t.blk0, fb * kI8Rows, lane & 31, lane >> 5);
-  else {
-    float sa[MT];
-    row_scales<MT>(g, t, t.row0, t.blk0, lane & 31, sa);
-    emit8<KIND, FB, MT>(g, acc, sa, t, t.row0, fb * kI8Rows, lane & 31, lane >> 5);
-  }
+  // Outputs JF row blocks at a time (gate and up together).  The waves that share them take them in turn.
+  constexpr int JF = KIND == kI8GateUp || KIND == kI8GateUpF32 ? 2 : 1;
+  static_assert(FB % JF == 0, "gate and up are neighbours");
+#pragma unroll
+  for (int j = 0; j < FB; j += JF)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if (KS > 1 && (j / JF * MT + i) % KS != s) continue;
+      i32x16 part[JF][1];
+#pragma unroll
+      for (int q = 0; q < JF; ++q)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          part[q][0][v] = KS > 1 ? s_acc[(((f * FB + j + q) * MT + i) * 16 + v) * kWave + lane] : acc[j + q][i][v];
+      const int row0 = t.row0 + 32 * i, blk = t.blk0 + i, fw = (fb + j) * kI8Rows, lrow = lane & 31, half = lane >> 5;
+      if constexpr (ODD) {
+        emit8_odd<KIND, JF, 1>(g, part, t, row0, blk, fw, lrow, half);
+      } else {
+        float sa[1];
+        row_scales<1>(g, t, row0, blk, lrow, sa);
+        emit8<KIND, JF, 1>(g, part, sa, t, row0, fw, lrow, half);
+      }
+    }
 }
 
 }  // namespace
@@ -671,8 +681,13 @@ hipError_t launch_i8_gemm(I8Out kind, const I8Args& args, int num_cus, hipStream
       hipLaunchKernelGGL((i8_ring_kernel<kK, kO, BM, BN, NW>), dim3(grid, groups), dim3(NW * kWave), 0, st, g,
                          (E + groups - 1) / groups);
     };
-    if ((long)g.N <= 32L * E) stream(IntC<1>{});
-    else if ((long)g.N <= 64L * E) stream(IntC<2>{});
+    // The stream kernel for few rows a segment, or little work in all, `units` waves' of it: up to two a CU it takes 15 us
+    // where the ring of 128 x 128 tiles has 18 (1024 x 2048 x 1024), from four on 25 against 19 (2048 rows).  A wave takes 64
+    // rows where 32 would make many units (16384 outputs of 64 rows: 14.6 us against 15.5; 4096: 12.5 against 11.3), unless
+    // they are short (512 columns, 1024 x 1024: 9.8 us against 11.4).
+    const long units = (g.counts ? (long)g.N / 32 + std::min(E, g.N) : ((long)g.N + 31) / 32) * ((g.Nf + 63) / 64);
+    if ((long)g.N <= 32L * E || units <= num_cus || (units <= 2L * num_cus && g.KT < 16)) stream(IntC<1>{});
+    else if ((long)g.N <= 64L * E || units <= 2L * num_cus) stream(IntC<2>{});
     else if (((long)g.N / 256 + E) * ((g.Nf + 255) / 256) < num_cus) ring(IntC<128>{}, IntC<128>{}, IntC<4>{});
     else ring(IntC<256>{}, IntC<256>{}, IntC<8>{});
   };
