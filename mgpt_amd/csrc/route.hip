@@ -23,9 +23,11 @@
 //
 // Keys with a bias, and sizes of groups, are those of 64 bits, and logits may have the same number without being equal:
 // where what is compared is not further apart than its rounding, the wave does its tokens again in 64 bits (one in
-// thousands), in rolled loops through LDS: code that a wave comes to once, by itself, costs its fetches.  At 32768 x 256
-// (8 groups, a bias), us: 64 bits throughout 52, a wave to a token that searches for each maximum 57, again in
-// 64 bits by unrolled code 64, so 43 (17 of them the waves' mean).
+// thousands), by code that is short, since a wave that comes to it alone waits for every fetch of it, and whose
+// invariants are formed there (ahead of the loop they took a hundred registers).  At 32768 x 256 (8 groups, a bias), us:
+// 64 bits throughout 52, a wave to a token that searches for each maximum 57, again in 64 bits by unrolled code 64, by
+// loops that load the logits one by one 43, so 30, 8 of them for those tokens.  1100 vector instructions a step of four tokens
+// bound it, 15 us; 40001 x 160 bf16 (8 groups of 20, softmax) takes 36 forward, 17 backward; 16384 x 16 3.6 and 3.3.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -115,6 +117,17 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// The number, of which the compiler knows nothing here: what follows from it is not computed ahead of a loop, where it
+// would take registers for code that hardly ever runs.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+__device__ __forceinline__ int here_lane(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // A lane's V logits of a token, e0 .. e0 + V - 1; experts past E have -infinity.
 template <typename T, int V>
 __device__ __forceinline__ void load_logits(const RouteArgs& g, size_t t, int e0, bool live, float (&l)[V]) {
@@ -137,9 +150,10 @@ __device__ __forceinline__ void load_logits(const RouteArgs& g, size_t t, int e0
       }
     }
   } else {
+    const int n = here(g.E) - e0;
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (e0 + v < g.E) l[v] = to_f32(p[e0 + v]);
+      if (v < n) l[v] = to_f32(p[e0 + v]);
   }
 }
 
@@ -291,6 +305,8 @@ __device__ __forceinline__ bool choose_groups(const RouteArgs& g, float (&key)[V
     mine = lp / lanes;
     if (lp % lanes == 0 && mine < g.G) sizes[mine] = g.best > 1 && b > kNone ? a + b : a;
   } else {
+    const int G = here(g.G), S = here(g.S);
+    lp = here_lane(lp);
     float* keys = reinterpret_cast<float*>(sp.key) + tok * LP * V;
 #pragma unroll
     for (int v = 0; v < V; v += 4)
@@ -298,17 +314,17 @@ __device__ __forceinline__ bool choose_groups(const RouteArgs& g, float (&key)[V
     wave_sync();
     // P lanes to a group, a power of two (at most 16)
     int P = 1;
-    while (2 * P * g.G <= LP && P < 16) P *= 2;
-    for (int gr0 = 0; gr0 < g.G; gr0 += LP / P) {
+    while (2 * P * G <= LP && P < 16) P *= 2;
+    for (int gr0 = 0; gr0 < G; gr0 += LP / P) {
       const int gr = gr0 + lp / P;
       a = b = kNone;
-      if (gr < g.G)
-        for (int i = lp % P; i < g.S; i += P) take(keys[gr * g.S + i]);
+      if (gr < G)
+        for (int i = lp % P; i < S; i += P) take(keys[gr * S + i]);
       if (P > 1) join(partner<1>(a), partner<1>(b));
       if (P > 2) join(partner<2>(a), partner<2>(b));
       if (P > 4) join(partner<4>(a), partner<4>(b));
       if (P > 8) join(partner<8>(a), partner<8>(b));
-      if (gr < g.G && lp % P == 0) sizes[gr] = g.best > 1 && b > kNone ? a + b : a;
+      if (gr < G && lp % P == 0) sizes[gr] = g.best > 1 && b > kNone ? a + b : a;
     }
   }
   wave_sync();
@@ -334,11 +350,12 @@ __device__ __forceinline__ bool choose_groups(const RouteArgs& g, float (&key)[V
     for (int v = 0; v < V; ++v) key[v] = in ? key[v] : kNone;
   } else {
     wave_sync();
-    int gr = e0 / g.S, r = e0 % g.S;
+    const int G = here(g.G), S = here(g.S);
+    int gr = here_lane(e0) / S, r = e0 - gr * S;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      key[v] = gr < g.G && sp.on[tok][gr] ? key[v] : kNone;
-      if (++r == g.S) {
+      key[v] = gr < G && sp.on[tok][gr] ? key[v] : kNone;
+      if (++r == S) {
         r = 0;
         ++gr;
       }
@@ -347,50 +364,55 @@ __device__ __forceinline__ bool choose_groups(const RouteArgs& g, float (&key)[V
   return next == kNone || last - next > tol;
 }
 
-// A step's tokens in 64 bits: the chosen ids into sp.pick (bit 30: takes no part).  Rolled loops over the experts, each
-// at its own place in LDS.
-template <typename T, int LP, int V, bool SOFTMAX>
-__device__ __forceinline__ void choose_exactly(const RouteArgs& g, size_t t, bool live, int tok, int lp,
+// A step's tokens in 64 bits, from their (clean) logits: the chosen ids into sp.pick (bit 30: takes no part).  Scores and
+// sizes in rolled loops over LDS, the k rounds from registers.  bias: in LDS.
+template <int LP, int V, bool SOFTMAX>
+__device__ __forceinline__ void choose_exactly(RouteArgs g, const float (&l)[V], const float* bias, int tok, int lp,
                                                Space<LP, V>& sp) {
   constexpr int kAll = LP * V;
-  const T* row = reinterpret_cast<const T*>(g.logits) + t * g.E;
+  g.E = here(g.E);
+  g.G = here(g.G);
+  g.S = here(g.S);
+  g.k = here(g.k);
+  g.top_groups = here(g.top_groups);
+  lp = here_lane(lp);
+  tok = here_lane(tok);
+  const int e0 = lp * V;
   double* key = sp.key + tok * kAll;
   double* sizes = sp.size[tok];
-  auto logit = [&](int e) { return e < g.E && live ? clean(to_f32(row[e])) : kNone; };
   const bool scores = g.bias || g.G > 1;
+#pragma unroll
+  for (int v = 0; v < V; ++v) key[e0 + v] = e0 + v < g.E ? (double)l[v] : -INFINITY;
   double m = 0.0, r = 1.0;
-  if (SOFTMAX && scores) {
-    float top = -FLT_MAX;
-#pragma unroll 1
-    for (int e = lp; e < kAll; e += LP) top = fmaxf(top, logit(e));
-    m = across<LP>(top, [](float a, float b) { return fmaxf(a, b); });
-    double z = 0.0;
-#pragma unroll 1
-    for (int e = lp; e < kAll; e += LP) {
-      const float l = logit(e);
-      z += l > kNone ? exp64((double)l - m) : 0.0;
-    }
-    z = across<LP>(z, [](double a, double b) { return a + b; });
-    r = inverse64(fmax(z, 1.0));
-  }
-#pragma unroll 1
-  for (int e = lp; e < kAll; e += LP) {
-    const float l = logit(e);
-    double x = l;
-    if (scores) {
-      const double q = exp64(SOFTMAX ? (double)l - m : -(double)l);
-      x = SOFTMAX ? q * r : inverse64(1.0 + q);
-      if (g.bias && e < g.E) x += (double)g.bias[e];
-    }
-    // (a NaN is not above)
-    key[e] = e >= g.E ? -INFINITY : l > kNone && x > -INFINITY ? fmin(x, 1e300) : kOut;
-  }
+  if (SOFTMAX && scores) m = largest<LP, V>(l);
   wave_sync();
+  if (scores) {
+    if constexpr (SOFTMAX) {
+      double z = 0.0;
+#pragma unroll 2
+      for (int e = lp; e < kAll; e += LP) {
+        const double x = key[e];
+        z += x > -INFINITY ? exp64(x - m) : 0.0;
+      }
+      z = across<LP>(z, [](double a, double b) { return a + b; });
+      r = inverse64(fmax(z, 1.0));
+    }
+#pragma unroll 2
+    for (int e = lp; e < kAll; e += LP) {
+      const double x = key[e];
+      const double q = exp64(SOFTMAX ? x - m : -x);
+      double s = SOFTMAX ? q * r : inverse64(1.0 + q);
+      if (g.bias) s += (double)bias[e];
+      // (a NaN is not above)
+      key[e] = e >= g.E ? -INFINITY : x > -INFINITY && s > -INFINITY ? fmin(s, 1e300) : kOut;
+    }
+    wave_sync();
+  }
   if (g.G > 1) {
 #pragma unroll 1
     for (int gr = lp; gr < g.G; gr += LP) {
       double a = kOut, b = kOut;
-#pragma unroll 1
+#pragma unroll 4
       for (int i = 0; i < g.S; ++i) {
         const double x = key[gr * g.S + i];
         b = fmax(b, fmin(a, x));
@@ -403,7 +425,7 @@ __device__ __forceinline__ void choose_exactly(const RouteArgs& g, size_t t, boo
     for (int gr = lp; gr < g.G; gr += LP) {
       const double x = sizes[gr];
       int rank = 0;
-#pragma unroll 1
+#pragma unroll 4
       for (int o = 0; o < g.G; ++o) {
         const double y = sizes[o];
         rank += y > x || (y == x && o < gr);
@@ -411,38 +433,47 @@ __device__ __forceinline__ void choose_exactly(const RouteArgs& g, size_t t, boo
       sp.on[tok][gr] = rank < g.top_groups;
     }
     wave_sync();
-#pragma unroll 1
-    for (int e = lp; e < g.E; e += LP) {
-      const double x = key[e];
-      key[e] = !sp.on[tok][e / g.S] || x == kOut ? kOut : g.bias ? x : (double)logit(e);
+  }
+  double kd[V];
+  {
+    int gr = g.G > 1 ? e0 / g.S : 0, i = g.G > 1 ? e0 % g.S : 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const bool in = e0 + v < g.E;
+      double x = key[e0 + v];
+      if (!(x > -INFINITY)) x = kOut;
+      if (g.G > 1) {
+        if (in && !sp.on[tok][gr]) x = kOut;
+        if (++i == g.S) {
+          i = 0;
+          ++gr;
+        }
+      }
+      if (!g.bias && x > kOut) x = (double)l[v];   // the order of the logits
+      kd[v] = in ? x : -INFINITY;
     }
-    wave_sync();
   }
 #pragma unroll 1
   for (int j = 0; j < g.k; ++j) {
-    double best = -INFINITY;
-    int at = kAll;
-#pragma unroll 1
-    for (int e = lp; e < kAll; e += LP) {
-      const double x = key[e];
-      if (x > best) {
-        best = x;
-        at = e;
-      }
-    }
+    double best = kd[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) best = fmax(best, kd[v]);
     const double top = across<LP>(best, [](double a, double b) { return fmax(a, b); });
-    at = across<LP>(best == top ? at : kAll, [](int a, int b) { return min(a, b); });
-    if (lp == 0) {
-      sp.pick[tok][j] = (uint32_t)at | (top > kOut ? 0u : 1u << 30);
-      key[at] = -INFINITY;
-    }
-    wave_sync();
+    int at = kAll;
+#pragma unroll
+    for (int v = V - 1; v >= 0; --v) at = kd[v] == top ? e0 + v : at;
+    at = across<LP>(at, [](int a, int b) { return min(a, b); });
+#pragma unroll
+    for (int v = 0; v < V; ++v) kd[v] = at == e0 + v ? -INFINITY : kd[v];
+    if (lp == 0) sp.pick[tok][j] = (uint32_t)at | (top > kOut ? 0u : 1u << 30);
   }
+  wave_sync();
 }
 
+// (Three blocks a CU: with two or four 33 and 34 us at 32768 x 256.)
 // NEAR: a bias or groups, for which the scores of all experts are needed.
 template <typename T, int LP, int V, bool SOFTMAX, bool NEAR>
-__global__ __launch_bounds__(256) void route_kernel(RouteArgs g) {
+__global__ __launch_bounds__(256, 3) void route_kernel(RouteArgs g) {
   constexpr int kTokens = kWave / LP, kAll = LP * V, L = V < 8 ? V : 8;
   constexpr int kAgain = 64;   // steps of a wave that wait for their 64-bit turn
   constexpr int kIdBits = kAll == 16 ? 4 : kAll == 32 ? 5 : kAll == 64 ? 6 : kAll == 128 ? 7 : kAll == 256 ? 8 : 9;
@@ -453,14 +484,20 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs g) {
   __shared__ Space<LP, V> space[4];
   __shared__ int s_count[kMaxExpertsWide];
   __shared__ int s_again[4][kAgain];
+  __shared__ float s_bias[NEAR ? kAll : 1];
   const int w = threadIdx.x / kWave, lane = lane_id();
   const int tok = lane / LP, lp = lane % LP, e0 = lp * V;
   Space<LP, V>& sp = space[w];
   float* logits = reinterpret_cast<float*>(sp.key) + tok * kAll;   // a token's, by expert
   if (g.counts) {
     for (int e = threadIdx.x; e < g.E; e += 256) s_count[e] = 0;
-    __syncthreads();
   }
+  if (NEAR && g.bias)
+    for (int e = threadIdx.x; e < kAll; e += 256) {
+      const float b = e < g.E ? g.bias[e] : 0.0f;   // (past E there is no logit)
+      s_bias[e] = b == b ? b : kNone;
+    }
+  __syncthreads();
   float bias[V], most_bias = 0.0f;   // -infinity for one that is none
   // The unit of the keys' numbers: of logits, 32 below the largest have numbers of their own; of scores with
   // a bias, all.
@@ -469,8 +506,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs g) {
     float lo = 0.0f, hi = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      bias[v] = g.bias[min(e0 + v, g.E - 1)];   // (past E there is no logit)
-      bias[v] = bias[v] == bias[v] ? bias[v] : kNone;
+      bias[v] = s_bias[e0 + v];
       lo = bias[v] > kNone ? fminf(lo, bias[v]) : lo;
       hi = fmaxf(hi, bias[v]);
     }
@@ -506,7 +542,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs g) {
   };
   auto request = [&](int t0, float (&l)[V]) __attribute__((always_inline)) {
     const int t = t0 + tok;
-    load_logits<T, V>(g, t < g.N ? t : 0, e0, t < g.N, l);
+    load_logits<T, V>(g, t < g.N ? t : 0, here_lane(e0), t < g.N, l);
   };
   auto sums = [&](float (&l)[V], float& m, float& z) __attribute__((always_inline)) {
 #pragma unroll
@@ -573,6 +609,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs g) {
         list[v] = number(key[v]) << kIdBits | (uint32_t)(kAll - 1 - (e0 + v));
       }
       sort_lane<V>(list, head);
+      const int lq = here_lane(lp);
       uint32_t pick[kSlots];
       int popped = 0;
 #pragma unroll
@@ -586,7 +623,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs g) {
 #pragma unroll
           for (int i = 0; i < L; ++i) head[i] = (i + 1 < L ? head[i + 1] & mine : 0) | (head[i] & ~mine);
           if constexpr (V > L) popped -= (int)mine;
-          pick[j / LP] = lp == j % LP ? first : pick[j / LP];
+          pick[j / LP] = lq == j % LP ? first : pick[j / LP];
         }
       }
       // (a list that gave all it had: what follows in the lane is not known)
@@ -640,11 +677,11 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs g) {
     }
 #pragma unroll 1
     for (int i = 0; i < again; ++i) {
-      const int ta = s_again[w][i], t = ta + tok;
-      choose_exactly<T, LP, V, SOFTMAX>(g, t < g.N ? t : 0, t < g.N, tok, lp, sp);
+      const int ta = here(__builtin_amdgcn_readfirstlane(s_again[w][i]));
       float l[V], m, z;
       request(ta, l);
       sums(l, m, z);
+      choose_exactly<LP, V, SOFTMAX>(g, l, s_bias, tok, lp, sp);
 #pragma unroll
       for (int v = 0; v < V; ++v) logits[e0 + v] = l[v];
       wave_sync();
