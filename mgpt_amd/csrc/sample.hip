@@ -237,8 +237,18 @@ struct End {
   int n;
 };
 
+// LDS of finish_few.
+template <int WAVES>
+struct FewShared {
+  u64 key[kFewer], weight[kFewer];
+  u64 red[WAVES];
+};
+
 struct Shared {
-  u64 bins[kBins];
+  union {
+    u64 bins[kBins];
+    FewShared<kWaves> few;
+  };
   int sizes[kBins];
   u64 digit[256];
   int digit_n[256];
@@ -565,6 +575,74 @@ __device__ __forceinline__ int under(u64 before, u64 w, int n, double bound) {
   return lo;
 }
 
+// Sums of v over the threads before this one, and of all, in the order of the threads.
+template <int WAVES>
+__device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64* all) {
+  const u64 incl = wave_scan(v);
+  __syncthreads();
+  if (lane_id() == kWave - 1) red[threadIdx.x / kWave] = incl;
+  __syncthreads();
+  u64 before = incl - v;
+  *all = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    if (i < (int)threadIdx.x / kWave) before += red[i];
+    *all += red[i];
+  }
+  return before;
+}
+
+// The token of a row from the running sums of its kept weights: this logit's, `before` it, of `all`.
+__device__ __forceinline__ void draw_one(const SampleArgs& g, int b, const Params& p, const Scale& s, u64 x, u64 w,
+                                         u64 before, u64 all) {
+  const double target = (double)(p.u > 0.0f ? p.u : 0.0f) * (double)all;
+  auto past = [&](u64 r) { return (double)r > target || r >= all; };
+  if (!w || (before > 0 && past(before)) || !past(before + w)) return;
+  g.token[b] = (int)~(uint32_t)x;
+  if (g.logp) {
+    const double z = ((double)logit_of((uint32_t)(x >> 32)) - (double)s.top) / (double)p.temp;
+    g.logp[b] = (float)(z - log((double)all / kUnits));
+  }
+}
+
+// The rest of a top_k row from a short list, x a thread's logit of it: places and sums of a logit by comparison with all others.
+template <int THREADS>
+__device__ __forceinline__ void finish_few(const SampleArgs& g, int b, const Params& p, const Scale& s, int n, u64 x,
+                                           FewShared<THREADS / kWave>& sh) {
+  static_assert(kFewer <= THREADS, "a logit a thread");
+  const int t = threadIdx.x;
+  u64 w = t < n ? weight_of(logit_of((uint32_t)(x >> 32)), s) : 0;
+  if (t < kFewer) {
+    sh.key[t] = x;
+    sh.weight[t] = w;
+  }
+  __syncthreads();
+  int place = 0;
+  u64 before = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const bool above = sh.key[j] > x;
+    place += above;
+    before += above ? sh.weight[j] : 0;
+  }
+  u64 all;
+  block_scan<THREADS / kWave>(place < p.k ? w : 0, sh.red, &all);   // (its syncs end the reads above)
+  const bool keep = place < p.k && (place == 0 || (((double)before < (double)p.top_p * (double)all || !(p.top_p < 1.0f)) &&
+                                                   (double)w >= (double)p.min_p * kUnits));
+  if (!keep) w = 0;
+  if (t < kFewer) sh.weight[t] = w;
+  __syncthreads();
+  before = 0;
+  all = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const u64 o = sh.weight[j];
+    all += o;
+    before += (uint32_t)sh.key[j] > (uint32_t)x ? o : 0;   // (the ids' complements)
+  }
+  draw_one(g, b, p, s, x, w, before, all);
+}
+
 // The end of top_p among n <= kList logits of a bin (sh.list) and the `ties` that are its smallest, `before` lying
 // before them; weights' sum of the bin.
 template <int THREADS, typename T, typename S, typename In>
@@ -584,8 +662,8 @@ __device__ __forceinline__ End end_of_mass(const Row<T, THREADS>& row, S& sh, in
   return cut;
 }
 
-// A row by one block.
-template <typename T, int THREADS>
+// A row by one block.  FEW: a short list may do for a top_k.
+template <typename T, int THREADS, bool FEW>
 __device__ void whole_row(const SampleArgs& g, int b, Shared& sh, u64* sums, int* piece_ties) {
   const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
   const Row<T, THREADS> row{reinterpret_cast<const T*>(g.logits) + (size_t)b * g.V, g.V};
@@ -624,6 +702,18 @@ __device__ void whole_row(const SampleArgs& g, int b, Shared& sh, u64* sums, int
     const int bin = (int)sh.found[0];
     const u64 before = sh.found[1];
     const int n = sh.sizes[bin];
+    if (const int last = min(bin, kBins - 2), few = (int)before + (bin == last ? n : 0); FEW && before + n <= kFewer) {
+      __syncthreads();   // (bins is free, sizes has been read)
+      u64* keys = sh.bins;
+      row.each([&](float l, int i) {
+        if (i < V && bin_of(l, s) <= last) keys[atomicAdd(&sh.count, 1)] = (u64)order_of(l) << 32 | (uint32_t)~(uint32_t)i;
+      });
+      __syncthreads();
+      const u64 x = tid < few ? keys[tid] : 0;
+      __syncthreads();
+      finish_few<THREADS>(g, b, p, s, few, x, sh.few);
+      return;
+    }
     // (the last bin's weights are 0: whether they are kept makes no difference)
     if (bin < kBins - 1) {
       auto in = [&](float l) { return bin_of(l, s) == bin; };
@@ -700,7 +790,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs g) {
   __shared__ Shared sh;
   extern __shared__ u64 sums[];   // the pieces', then their ties
-  whole_row<T, kThreads>(g, blockIdx.x, sh, sums, reinterpret_cast<int*>(sums + (g.V + kWave * Piece<T>::N - 1) / (kWave * Piece<T>::N)));
+  whole_row<T, kThreads, true>(g, blockIdx.x, sh, sums, reinterpret_cast<int*>(sums + (g.V + kWave * Piece<T>::N - 1) / (kWave * Piece<T>::N)));
 }
 
 // ------------------------------------------------------------------ in chunks
@@ -814,22 +904,6 @@ __global__ __launch_bounds__(kChunkThreads) void sample_scan_kernel(SampleArgs g
   }
 }
 
-// Sums of v over the threads before this one, and of all, in the order of the threads.
-__device__ __forceinline__ u64 block_scan(u64 v, u64* red, u64* all) {
-  const u64 incl = wave_scan(v);
-  __syncthreads();
-  if (lane_id() == kWave - 1) red[threadIdx.x / kWave] = incl;
-  __syncthreads();
-  u64 before = incl - v;
-  *all = 0;
-#pragma unroll
-  for (int i = 0; i < kChunkWaves; ++i) {
-    if (i < (int)threadIdx.x / kWave) before += red[i];
-    *all += red[i];
-  }
-  return before;
-}
-
 // Where the end lies: the last bin with items before which less than `bound` lies.
 struct Place {
   int bin;
@@ -850,7 +924,7 @@ __device__ __forceinline__ Place place_of(const SampleArgs& g, int b, const Para
     w[q] = bins[q];
     sum += w[q];
   }
-  u64 run = block_scan(sum, sh.red, &all);
+  u64 run = block_scan<kChunkWaves>(sum, sh.red, &all);
   Place at{-1, 0, 0, mode == kTopP ? fmax((double)p.top_p * (double)all, 0.0) : (double)p.k};
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -964,10 +1038,8 @@ __device__ __forceinline__ void sort_down(u64* x, int n) {
 // LDS of the cut: a row's list (top_k), or what refine needs (top_p).
 struct CutShared {
   union {
-    struct {
-      u64 key[kList];
-      u64 weight[kFewer];
-    };
+    u64 key[kList];
+    FewShared<kChunkWaves> few;
     struct {
       uint32_t list[kList];
       u64 digit[256];
@@ -978,55 +1050,6 @@ struct CutShared {
   u64 red[kChunkWaves];
   PlaceShared place;
 };
-
-// The token of a row from the running sums of its kept weights: this logit's, `before` it, of `all`.
-__device__ __forceinline__ void draw_one(const SampleArgs& g, int b, const Params& p, const Scale& s, u64 x, u64 w,
-                                         u64 before, u64 all) {
-  const double target = (double)(p.u > 0.0f ? p.u : 0.0f) * (double)all;
-  auto past = [&](u64 r) { return (double)r > target || r >= all; };
-  if (!w || (before > 0 && past(before)) || !past(before + w)) return;
-  g.token[b] = (int)~(uint32_t)x;
-  if (g.logp) {
-    const double z = ((double)logit_of((uint32_t)(x >> 32)) - (double)s.top) / (double)p.temp;
-    g.logp[b] = (float)(z - log((double)all / kUnits));
-  }
-}
-
-// The rest of a top_k row from a short list: places and sums of a logit by comparison with all others.
-__device__ __forceinline__ void finish_few(const SampleArgs& g, int b, const Params& p, const Scale& s, int n,
-                                           CutShared& sh) {
-  static_assert(kFewer == kChunkThreads, "a logit a thread");
-  const int t = threadIdx.x;
-  const u64 x = t < n ? g.list[(size_t)b * kList + t] : 0;
-  u64 w = t < n ? weight_of(logit_of((uint32_t)(x >> 32)), s) : 0;
-  sh.key[t] = x;
-  sh.weight[t] = w;
-  __syncthreads();
-  int place = 0;
-  u64 before = 0;
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) {
-    const bool above = sh.key[j] > x;
-    place += above;
-    before += above ? sh.weight[j] : 0;
-  }
-  u64 all;
-  block_scan(place < p.k ? w : 0, sh.red, &all);   // (its syncs end the reads above)
-  const bool keep = place < p.k && (place == 0 || (((double)before < (double)p.top_p * (double)all || !(p.top_p < 1.0f)) &&
-                                                   (double)w >= (double)p.min_p * kUnits));
-  if (!keep) w = 0;
-  sh.weight[t] = w;
-  __syncthreads();
-  before = 0;
-  all = 0;
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) {
-    const u64 o = sh.weight[j];
-    all += o;
-    before += (uint32_t)sh.key[j] > (uint32_t)x ? o : 0;   // (the ids' complements)
-  }
-  draw_one(g, b, p, s, x, w, before, all);
-}
 
 // The rest of a top_k row, from the list of its logits: by a block.
 __device__ __forceinline__ void finish_top_k(const SampleArgs& g, int b, const Params& p, const Scale& s, int n,
@@ -1047,7 +1070,7 @@ __device__ __forceinline__ void finish_top_k(const SampleArgs& g, int b, const P
     w[q] = i < n ? weight_of(logit_of((uint32_t)(x[q] >> 32)), s) : 0;
     sum += w[q];
   }
-  u64 run = block_scan(sum, sh.red, &all);
+  u64 run = block_scan<kChunkWaves>(sum, sh.red, &all);
   const double bound = (double)p.top_p * (double)all, least = (double)p.min_p * kUnits;
   // the kept ones, by id: their order's complement is the number's lower half
 #pragma unroll
@@ -1073,7 +1096,7 @@ __device__ __forceinline__ void finish_top_k(const SampleArgs& g, int b, const P
     w[q] = x[q] ? weight_of(logit_of((uint32_t)x[q]), s) : 0;
     sum += w[q];
   }
-  run = block_scan(sum, sh.red, &all);
+  run = block_scan<kChunkWaves>(sum, sh.red, &all);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     draw_one(g, b, p, s, x[q] << 32 | x[q] >> 32, w[q], run, all);
@@ -1098,8 +1121,10 @@ __global__ __launch_bounds__(kChunkThreads) void sample_cut_kernel(SampleArgs g)
   if (mode == kOpen || mode == kWhole) return;
   if (n > kList) return;
   if (mode == kTopK) {
-    if (chunk == 0 && n <= kFewer) finish_few(g, b, p, s, n, sh);
-    else if (chunk == 0) finish_top_k(g, b, p, s, n, sh);
+    if (chunk == 0 && n <= kFewer)
+      finish_few<kChunkThreads>(g, b, p, s, n, (int)threadIdx.x < n ? g.list[(size_t)b * kList + threadIdx.x] : 0, sh.few);
+    else if (chunk == 0)
+      finish_top_k(g, b, p, s, n, sh);
     return;
   }
   // (every block of the row finds the end for itself)
@@ -1124,7 +1149,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs g) {
   u64* sums = g.sums + (size_t)b * g.pieces;
   int* ties = g.ties + (size_t)b * g.pieces;
   if (mode == kWhole || (mode != kOpen && g.list_n[b] > kList)) {
-    whole_row<T, kThreads>(g, b, sh, sums, ties);
+    whole_row<T, kThreads, false>(g, b, sh, sums, ties);
   } else if (mode == kTopP && threadIdx.x < kWave) {
     lay_out_pow(sh.pow);   // (written and read by this wave alone, in order)
     __builtin_amdgcn_wave_barrier();
