@@ -563,7 +563,7 @@ int mgpt_route_balance(int num_experts, const int32_t* counts, float rate, float
                        void* stream);
 
 /* A linear layer in 8-bit integers with a scale for each token and each output:
- *   sx[n] = max|x[n]| / 127,  q = rint(x 127 / max|x[n]|),
+ *   sx[n] = max|x[n]| / 127,  q = rint(x r), r = 127 (1 / max|x[n]|), both products in 64 bits,
  *   y[n][m] = (sum over k of q[n][k] w[m][k]) sx[n] scales[m] + bias[m]
  * x [N,K], y [N,M] in dtype; the weight is kept as the kernels read it, packed once
  * from int8 [M,K] with scales of the caller's or from float rows by the same rule.

@@ -180,6 +180,8 @@ __global__ __launch_bounds__(NW * kWave) void i8_quantize_kernel(QuantizeArgs g)
   for (int t = w + kHold * NW; t < slabs; t += NW) put(load(t), t);
 }
 
+// VEC: a lane's 16 columns are a vector or past K.
+template <bool VEC>
 __global__ __launch_bounds__(256) void i8_tile_kernel(const int8_t* __restrict__ q, int M, int K,
                                                       char* __restrict__ out) {
   const size_t block = blockIdx.x;
@@ -188,13 +190,19 @@ __global__ __launch_bounds__(256) void i8_tile_kernel(const int8_t* __restrict__
   const int tiles = (K + kI8Slab - 1) / kI8Slab * (kI8Slab / 32);
   for (int t = blockIdx.y * 4 + threadIdx.x / kWave; t < tiles; t += gridDim.y * 4) {
     const int c = t * 32 + (lane >> 5) * 16;
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (row < (size_t)M)
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (row < (size_t)M) {
+      if constexpr (VEC) {
+        if (c < K) w = *reinterpret_cast<const uint4*>(q + row * K + c);
+      } else {
+        uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (c + i < K) w[i / 4] |= (uint32_t)(uint8_t)q[row * K + c + i] << (8 * (i % 4));
-    *reinterpret_cast<uint4*>(out + block * i8_row_block_bytes(K) + (size_t)t * 1024 + lane * 16) =
-        make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < 16; ++i)
+          if (c + i < K) u[i / 4] |= (uint32_t)(uint8_t)q[row * K + c + i] << (8 * (i % 4));
+        w = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+    }
+    *reinterpret_cast<uint4*>(out + block * i8_row_block_bytes(K) + (size_t)t * 1024 + lane * 16) = w;
   }
 }
 
@@ -227,8 +235,11 @@ hipError_t launch_i8_quantize(QuantizeSource src, const QuantizeArgs& g, int max
 
 hipError_t launch_i8_tile(const int8_t* q, int M, int K, char* out, hipStream_t st) {
   if (M <= 0) return hipSuccess;
-  hipLaunchKernelGGL(i8_tile_kernel, dim3((M + kI8Rows - 1) / kI8Rows, std::min(8, (K + 127) / 128)), dim3(256), 0, st,
-                     q, M, K, out);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((M + kI8Rows - 1) / kI8Rows, std::min(8, (K + 127) / 128)), dim3(256), 0, st, q, M,
+                       K, out);
+  };
+  K % 16 == 0 && ((uintptr_t)q & 15) == 0 ? go(i8_tile_kernel<true>) : go(i8_tile_kernel<false>);
   return hipGetLastError();
 }
 
