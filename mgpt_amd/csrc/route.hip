@@ -27,7 +27,8 @@
 // invariants are formed there (ahead of the loop they took a hundred registers).  At 32768 x 256 (8 groups, a bias), us:
 // 64 bits throughout 52, a wave to a token that searches for each maximum 57, again in 64 bits by unrolled code 64, by
 // loops that load the logits one by one 43, so 30, 8 of them for those tokens.  1100 vector instructions a step of four tokens
-// bound it, 15 us; 40001 x 160 bf16 (8 groups of 20, softmax) takes 36 forward, 17 backward; 16384 x 16 3.6 and 3.3.
+// bound it, 15 us.  The backward, whose next step's loads are on their way, takes 22 (67 MB, 13 at a copy's rate);
+// 40001 x 160 bf16 (8 groups of 20, softmax) 36 and 13.5, 16384 x 16 3.6 and 2.9.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -180,25 +181,20 @@ __device__ __forceinline__ float largest(const float (&l)[V]) {
   return max32(across<LP>(m, [](float a, float b) { return max32(a, b); }), -FLT_MAX);   // (a row without experts)
 }
 
-// Scores to some 2^-22.
-template <int LP, int V, bool SOFTMAX>
-__device__ __forceinline__ void scores_of(const float (&l)[V], float (&s)[V]) {
-  if constexpr (SOFTMAX) {
-    const float m = largest<LP, V>(l);
-    float z = 0.0f;
+// Softmax to some 2^-22.
+template <int LP, int V>
+__device__ __forceinline__ void softmax_of(const float (&l)[V], float (&s)[V]) {
+  const float m = largest<LP, V>(l);
+  float z = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      s[v] = exp_full(l[v] - m);
-      z += s[v];
-    }
-    z = across<LP>(z, [](float a, float b) { return a + b; });
-    const float r = z > 0.0f ? inverse(z) : 0.0f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v] *= r;
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = inverse(1.0f + exp_full(-l[v]));
+  for (int v = 0; v < V; ++v) {
+    s[v] = exp_full(l[v] - m);
+    z += s[v];
   }
+  z = across<LP>(z, [](float a, float b) { return a + b; });
+  const float r = z > 0.0f ? inverse(z) : 0.0f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) s[v] *= r;
 }
 
 // exp(x) in 64 bits to 2^-51, x up to 700 in magnitude (beyond: as there): 2^t by its whole part and a polynomial of degree 10 on
@@ -709,7 +705,7 @@ __global__ __launch_bounds__(256, 3) void route_kernel(RouteArgs g) {
 
 template <typename T, int LP, int V, bool SOFTMAX>
 __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs g) {
-  constexpr int kTokens = kWave / LP;
+  constexpr int kTokens = kWave / LP, kSlots = (kMaxTopK + LP - 1) / LP;
   __shared__ float s_all[4][kWave * V];
   const int w = threadIdx.x / kWave, lane = lane_id();
   const int tok = lane / LP, lp = lane % LP, e0 = lp * V;
@@ -718,41 +714,69 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs g) {
 #pragma unroll
   for (int v = 0; v < V; ++v) up[v] = g.dscore && e0 + v < g.E ? g.dscore[e0 + v] : 0.0f;
   const int step = gridDim.x * 4 * kTokens;
-  for (int t0 = (blockIdx.x * 4 + w) * kTokens; t0 < g.N; t0 += step) {
+  // A step's logits, and the lane's chosen ones (entry i LP + lp of the k), a step ahead.
+  struct Step {
+    float l[V], w[kSlots], dw[kSlots];
+    int e[kSlots];
+  };
+  auto request = [&](int t0, Step& x) __attribute__((always_inline)) {
     const int t = t0 + tok;
     const bool live = t < g.N;
-    float l[V], s[V];
-    load_logits<T, V>(g, live ? t : 0, e0, live, l);
+    load_logits<T, V>(g, live ? t : 0, here_lane(e0), live, x.l);
 #pragma unroll
-    for (int v = 0; v < V; ++v) l[v] = clean(l[v]);
-    scores_of<LP, V, SOFTMAX>(l, s);
-#pragma unroll
-    for (int v = 0; v < V; ++v) mine[e0 + v] = s[v];
-    wave_sync();
-    // the chosen experts, the same in all of the token's lanes
-    int id[kMaxTopK];
-    float sc[kMaxTopK], dw[kMaxTopK];
-    float D = 0.0f, dot = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kMaxTopK; ++j) {
-      id[j] = -1;
-      sc[j] = dw[j] = 0.0f;
+    for (int i = 0; i < kSlots; ++i) {
+      const int j = i * LP + lp;
+      x.e[i] = 0;
+      x.w[i] = x.dw[i] = 0.0f;
       if (j < g.k && live) {
-        const int e = g.bidx[(size_t)t * g.k + j];
-        const float wj = g.bw[(size_t)t * g.k + j];
-        if (wj != 0.0f && (unsigned)e < (unsigned)g.E) {
-          id[j] = e;
-          sc[j] = mine[e];
-          dw[j] = g.dw[(size_t)t * g.k + j];
-          D += sc[j];
-        }
+        const size_t f = (size_t)t * g.k + j;
+        x.e[i] = g.bidx[f];
+        x.w[i] = g.bw[f];
+        x.dw[i] = g.dw[f];
       }
+    }
+  };
+  auto plus = [](float a, float b) { return a + b; };
+  int t0 = (blockIdx.x * 4 + w) * kTokens;
+  Step ahead;
+  request(t0, ahead);
+  for (; t0 < g.N; t0 += step) {
+    const int t = t0 + tok;
+    const bool live = t < g.N;
+    const Step now = ahead;
+    request(min(t0 + step, g.N), ahead);
+    float l[V], s[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) l[v] = clean(now.l[v]);
+    if constexpr (SOFTMAX) {
+      softmax_of<LP, V>(l, s);
+#pragma unroll
+      for (int v = 0; v < V; ++v) mine[e0 + v] = s[v];
+    } else {
+      // e = exp(-|l|), r = 1 / (1 + e): s = r or e r, and s (1 - s) = e r^2, without a difference
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float e = exp_full(-fabsf(l[v])), r = inverse(1.0f + e), er = e * r;
+        mine[e0 + v] = l[v] >= 0.0f ? r : er;
+        s[v] = er * r;
+      }
+    }
+    wave_sync();
+    bool on[kSlots];
+    float sc[kSlots], D = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      on[i] = now.w[i] != 0.0f && (unsigned)now.e[i] < (unsigned)g.E;
+      sc[i] = on[i] ? mine[now.e[i]] : 0.0f;
+      D += sc[i];
     }
     float inv = 1.0f;
     if (g.renorm) {
+      D = across<LP>(D, plus);
       inv = 1.0f / (D + 1e-20f);
 #pragma unroll
-      for (int j = 0; j < kMaxTopK; ++j) dot += dw[j] * (sc[j] * inv);
+      for (int i = 0; i < kSlots; ++i) dot += on[i] ? now.dw[i] * (sc[i] * inv) : 0.0f;
+      dot = across<LP>(dot, plus);
     }
     wave_sync();
 #pragma unroll
@@ -761,13 +785,16 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs g) {
     const float c = g.scale * inv;
     float sum = 0.0f;   // of ds_e s_e
 #pragma unroll
-    for (int j = 0; j < kMaxTopK; ++j) {
-      const float d = c * (dw[j] - dot);
-      if (id[j] >= 0 && lp == j % LP) mine[id[j]] = d;
-      // (renormalised, the chosen ones' terms cancel but for 1e-20 of c dot)
-      if (!g.renorm && id[j] >= 0) sum += d * sc[j];
+    for (int i = 0; i < kSlots; ++i) {
+      const float d = c * (now.dw[i] - dot);
+      if (on[i]) {
+        mine[now.e[i]] = d;
+        sum += d * sc[i];
+      }
     }
+    // (renormalised, the chosen ones' terms cancel but for 1e-20 of c dot)
     if (g.renorm) sum = c * dot * 1e-20f;
+    else sum = across<LP>(sum, plus);
     wave_sync();
     float ds[V];
 #pragma unroll
@@ -783,9 +810,8 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs g) {
     float o[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      // (1 - s from the other side: s may be near 1)
       if constexpr (SOFTMAX) o[v] = s[v] * (ds[v] - sum);
-      else o[v] = ds[v] * (s[v] * inverse(1.0f + exp_full(l[v])));
+      else o[v] = ds[v] * s[v];   // (s (1 - s) there)
       if (!(l[v] > kNone)) o[v] = 0.0f;
     }
     if (live) {
