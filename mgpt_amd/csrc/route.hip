@@ -22,8 +22,8 @@
 // lanes' first ones, by moves within rows of 16 lanes, and pop it.
 //
 // Keys with a bias, and sizes of groups, are those of 64 bits, and logits may have the same number without being equal:
-// where what is compared is not further apart than its rounding, the wave does its tokens again in 64 bits (one in
-// thousands), by code that is short, since a wave that comes to it alone waits for every fetch of it, and whose
+// where what is compared is not further apart than its rounding, the wave does its tokens again in 64 bits (few steps),
+// by code that is short, since a wave that comes to it alone waits for every fetch of it, and whose
 // invariants are formed there (ahead of the loop they took a hundred registers).  At 32768 x 256 (8 groups, a bias), us:
 // 64 bits throughout 52, a wave to a token that searches for each maximum 57, again in 64 bits by unrolled code 64, by
 // loops that load the logits one by one 43, so 30, 8 of them for those tokens.  1100 vector instructions a step of four tokens
