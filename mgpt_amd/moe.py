@@ -122,6 +122,8 @@ class MoELayer:
         self._workspace(max_tokens, dev, train)
 
     def _workspace(self, n: int, device, train: bool = False) -> torch.Tensor:
+        if self._route_bias is not None and self._route_bias.device != device:
+            raise ValueError("the routing's bias is on another device")
         need = self.train_workspace_bytes(n) if train else self.workspace_bytes(n)
         if self._ws is None or self._ws.numel() < need or self._ws.device != device:
             self._ws = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
