@@ -176,10 +176,11 @@ _HERE = contextlib.nullcontext()
 
 
 def on_device(device):
-    """A context in which `device` (a torch.device with an index) is the current
-    one; nothing to enter where it is already."""
+    """A context in which `device` (that of a tensor on the GPU) is the current
+    one; nothing to enter where it is already.  (The call that
+    torch.cuda.current_device ends in.)"""
     import torch
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def stream(device):

@@ -13,6 +13,7 @@
 //    registers that the matrix instruction takes, a slab ahead, the rows' from the caches. Waves split a
 //    long contraction and add their integers up in LDS.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/mgpt_moe.h"
@@ -733,11 +734,14 @@ I8Layout i8_layout(const mgpt_i8_config* cfg, int N) {
   return l;
 }
 
+// (the device's number is a part of each call's 3 us: asked for once)
 int compute_units() {
+  static std::atomic<int> known[64];
   int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-    return 256;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 256;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

@@ -31,6 +31,7 @@ class ExpertRouting:
         self.config = capi.RouteConfig(num_experts, top_k, _SCORE[score], groups,
                                        groups if top_groups is None else top_groups, group_best, int(renormalise),
                                        scale, dt)
+        self._cfg = ctypes.byref(self.config)
 
     @staticmethod
     def _check(t, dtype, shape, device, what):
@@ -38,43 +39,44 @@ class ExpertRouting:
             raise ValueError(f"{what} must be a CUDA tensor on the device of logits")
         if t.dtype != dtype:
             raise TypeError(f"{what} must be {dtype}")
-        if tuple(t.shape) != shape or not t.is_contiguous():
+        if t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous with shape {list(shape)}")
         return t.data_ptr()
 
     def _logits(self, logits):
-        if logits.dim() < 1 or logits.shape[-1] != self.E:
+        """(address, device, the shape before the experts)"""
+        shape, dev = logits.shape, logits.device
+        if not shape or shape[-1] != self.E:
             raise ValueError(f"logits must have {self.E} columns")
-        return self._check(logits, self.dtype, tuple(logits.shape), logits.device, "logits")
+        return self._check(logits, self.dtype, shape, dev, "logits"), dev, shape[:-1]
 
     def forward(self, logits, bias=None, counts=None):
         """(idx, weights): int32 and float32 [..., k].  bias: float32 [E], for
         the choice alone.  counts: int32 [E], to which the tokens of each
         expert are added."""
-        ptr, dev = self._logits(logits), logits.device
+        ptr, dev, rows = self._logits(logits)
         b = None if bias is None else self._check(bias, torch.float32, (self.E,), dev, "bias")
         c = None if counts is None else self._check(counts, torch.int32, (self.E,), dev, "counts")
         with capi.on_device(dev):
-            idx = torch.empty((*logits.shape[:-1], self.k), dtype=torch.int32, device=dev)
-            weights = torch.empty(idx.shape, dtype=torch.float32, device=dev)
-            capi.check(capi.lib().mgpt_route_forward(ctypes.byref(self.config), ptr, b, idx.data_ptr(),
-                                                     weights.data_ptr(), c, logits.numel() // self.E,
-                                                     capi.stream(dev)))
+            idx = torch.empty((*rows, self.k), dtype=torch.int32, device=dev)
+            weights = torch.empty_like(idx, dtype=torch.float32)
+            capi.check(capi.lib().mgpt_route_forward(self._cfg, ptr, b, idx.data_ptr(), weights.data_ptr(), c,
+                                                     logits.numel() // self.E, capi.stream(dev)))
         return idx, weights
 
     def backward(self, logits, idx, weights, dweights, dscores=None):
         """The gradient of logits, in their type, for dweights (float32 [..., k])
         and dscores (float32 [E]: of every token's score of each expert), from
         forward's input and outputs; the choice is taken as given."""
-        ptr, dev = self._logits(logits), logits.device
-        shape = (*logits.shape[:-1], self.k)
+        ptr, dev, rows = self._logits(logits)
+        shape = (*rows, self.k)
         ptrs = [self._check(idx, torch.int32, shape, dev, "idx"),
                 self._check(weights, torch.float32, shape, dev, "weights"),
                 self._check(dweights, torch.float32, shape, dev, "dweights"),
                 None if dscores is None else self._check(dscores, torch.float32, (self.E,), dev, "dscores")]
         with capi.on_device(dev):
             dlogits = torch.empty_like(logits)
-            capi.check(capi.lib().mgpt_route_backward(ctypes.byref(self.config), ptr, *ptrs, dlogits.data_ptr(),
+            capi.check(capi.lib().mgpt_route_backward(self._cfg, ptr, *ptrs, dlogits.data_ptr(),
                                                       logits.numel() // self.E, capi.stream(dev)))
         return dlogits
 

@@ -30,7 +30,7 @@ class Sampler:
             raise ValueError(f"{what} must be a CUDA tensor on the device of logits")
         if t.dtype != dtype:
             raise TypeError(f"{what} must be {dtype}")
-        if tuple(t.shape) != shape or not t.is_contiguous():
+        if t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous with shape {list(shape)}")
         return t.data_ptr()
 
@@ -42,8 +42,8 @@ class Sampler:
         nothing but -inf has token -1."""
         if logits.dim() < 1 or logits.shape[-1] != self.V:
             raise ValueError(f"logits must have {self.V} columns")
-        dev, shape = logits.device, tuple(logits.shape[:-1])
-        ptr = self._check(logits, self.dtype, tuple(logits.shape), dev, "logits")
+        dev, shape = logits.device, logits.shape[:-1]
+        ptr = self._check(logits, self.dtype, logits.shape, dev, "logits")
         up = self._check(u, torch.float32, shape, dev, "u")
         cfg = capi.SampleConfig(self.V, self._dt, 1.0, 0, 1.0, 0.0)
         ptrs = []
@@ -56,7 +56,7 @@ class Sampler:
                 ptrs.append(None)
         with capi.on_device(dev):
             token = torch.empty(shape, dtype=torch.int32, device=dev)
-            logp = torch.empty(shape, dtype=torch.float32, device=dev)
+            logp = torch.empty_like(token, dtype=torch.float32)
             need = ctypes.c_size_t()
             capi.check(capi.lib().mgpt_sample_workspace_bytes(ctypes.byref(cfg), token.numel(), ctypes.byref(need)))
             ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
