@@ -122,12 +122,14 @@ class MoELayer:
         self._workspace(max_tokens, dev, train)
 
     def _workspace(self, n: int, device, train: bool = False) -> torch.Tensor:
-        if self._route_bias is not None and self._route_bias.device != device:
-            raise ValueError("the routing's bias is on another device")
         need = self.train_workspace_bytes(n) if train else self.workspace_bytes(n)
         if self._ws is None or self._ws.numel() < need or self._ws.device != device:
             self._ws = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
         return self._ws
+
+    def _check_routing(self, x: torch.Tensor) -> None:
+        if self._route_bias is not None and self._route_bias.device != x.device:
+            raise ValueError("the routing's bias is on another device than x")
 
     def forward_into(self, x: torch.Tensor, out: torch.Tensor, train: bool = False) -> None:
         """out = MoE(x).  train=True also keeps what backward() needs (the
@@ -141,6 +143,7 @@ class MoELayer:
         if not x.is_contiguous() or not out.is_contiguous():
             raise ValueError("x and out must be contiguous")
         n = x.numel() // self.C
+        self._check_routing(x)
         ws = self._workspace(n, x.device, train)
         stream = torch.cuda.current_stream(x.device).cuda_stream
         fn = capi.lib().mgpt_moe_forward_train if train else capi.lib().mgpt_moe_forward
@@ -182,6 +185,7 @@ class MoELayer:
                 raise ValueError(f"{what} must be a contiguous {dt} tensor of shape {list(shape)} on the device of x")
         out = torch.empty_like(x)
         n = x.numel() // self.C
+        self._check_routing(x)
         ws = self._workspace(n, x.device)
         capi.check(capi.lib().mgpt_moe_forward_routed(self._h, x.data_ptr(), idx.data_ptr(), weights.data_ptr(),
                                                       out.data_ptr(), n, ws.data_ptr(), ws.numel(),
@@ -212,6 +216,7 @@ class MoELayer:
         if g.numel() != self.C:
             raise ValueError("gamma must have C elements")
         n = x.numel() // self.C
+        self._check_routing(x)
         ws = self._workspace(n, x.device, train)
         stream = torch.cuda.current_stream(x.device).cuda_stream
         fn = (capi.lib().mgpt_moe_forward_block_train if train
