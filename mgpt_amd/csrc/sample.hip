@@ -23,10 +23,10 @@
 //          of equal logits)
 // Short rows are done whole, by a block each, in one launch.
 //
-// Measured: 256 rows of 131072 bf16 with top_p and min_p 113 us, of it max 14 (4.7 TB/s), scan 37 (bound by the 26
-// vector instructions of a weight), list 25, cut 35, draw 8; 64 rows of 100003 fp32, all open, 32 us; one row of
-// 50257 with top_k 24 us, of it five launches' latency.  A block for each row and all steps took 191, 71 and
-// 61 us.
+// Measured: 256 rows of 131072 bf16 with top_p and min_p 101 us, of it max 14 (4.7 TB/s), scan 26 (38 with the 26 vector
+// instructions of a weight for every logit), list 24, cut 35, draw 8; 64 rows of 100003 fp32, all open, 32 us; one
+// row of 50257 with top_k 25 us, of it five launches' latency; one of 8192 16 us.  A block for each row and all
+// steps took 191, 71 and 61 us for the first three.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -49,6 +49,8 @@ constexpr double kUnits = 0x1p40;
 
 constexpr int kFew = 1024;           // top_k up to which the list serves
 constexpr int kFewer = 256;          // logits of a list that need no sorting
+constexpr uint32_t kValues = 4096;   // of bf16, counted by themselves: 16 powers of two of either sign
+constexpr uint32_t kLeastValue = (127 - 8) << 7;   // 2^-8
 constexpr int kCopies = 4;           // of a block's histogram, so that a wave's lanes meet less
 constexpr int kChunkThreads = 256, kChunkWaves = kChunkThreads / kWave;
 constexpr int kMaxChunks = 64;
@@ -178,6 +180,10 @@ struct Piece {
   __device__ __forceinline__ float raw(int q) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[q]);
     else return __uint_as_float(q & 1 ? w[q / 2] & 0xFFFF0000u : w[q / 2] << 16);
+  }
+  __device__ __forceinline__ uint32_t bits(int q) const {   // T's own
+    if constexpr (sizeof(T) == 4) return w[q];
+    else return q & 1 ? w[q / 2] >> 16 : w[q / 2] & 0xFFFF;
   }
   __device__ __forceinline__ float operator[](int q) const { return clean_logit(raw(q)); }
 };
@@ -865,7 +871,10 @@ __global__ __launch_bounds__(kChunkThreads) void sample_max_kernel(SampleArgs g)
 
 template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void sample_scan_kernel(SampleArgs g) {
-  __shared__ u64 s_bins[kBins * kCopies];
+  constexpr bool kByValue = sizeof(T) == 2;
+  constexpr int kBinCopies = kByValue ? 1 : kCopies;
+  __shared__ u64 s_bins[kBins * kBinCopies];
+  __shared__ uint32_t s_value[kByValue ? kValues : 1];
   __shared__ double s_pow[16];
   const int b = blockIdx.y, chunk = blockIdx.x;
   Pieces<T> part = pieces_of<T>(g, b, chunk);
@@ -882,25 +891,52 @@ __global__ __launch_bounds__(kChunkThreads) void sample_scan_kernel(SampleArgs g
     piece_sums(part, kept, g.sums + (size_t)b * g.pieces, g.ties + (size_t)b * g.pieces);
     return;
   }
-  for (int i = threadIdx.x; i < kCopies * kBins; i += kChunkThreads) s_bins[i] = 0;
+  for (int i = threadIdx.x; i < kBinCopies * kBins; i += kChunkThreads) s_bins[i] = 0;
+  if constexpr (kByValue)
+    for (int i = threadIdx.x; i < kValues; i += kChunkThreads) s_value[i] = 0;
   __syncthreads();
-  u64* mine = s_bins + threadIdx.x % kCopies;
-  if (mode == kTopK) {
-    part.each([&](float l, int i) {
-      if (i < g.V) atomicAdd(reinterpret_cast<uint32_t*>(mine + bin_of(l, s) * kCopies), 1u);
-    });
-  } else {
-    part.each([&](float l, int) {
+  u64* mine = s_bins + threadIdx.x % kBinCopies;
+  // `n` logits l
+  auto add = [&](float l, uint32_t n) {
+    if (mode == kTopK) {
+      atomicAdd(reinterpret_cast<uint32_t*>(mine + bin_of(l, s) * kBinCopies), n);
+    } else {
       int bin;
       const u64 w = weight_of(l, s, &bin);
-      if (w) atomicAdd(mine + bin * kCopies, w);
+      if (w) atomicAdd(mine + bin * kBinCopies, w * n);
+    }
+  };
+  if constexpr (kByValue) {
+    // bf16 has few values: those of 2^-8 to 2^8 in magnitude are counted, and weighed once each
+    part.run([&](const Piece<T>& x, int) {
+#pragma unroll
+      for (int q = 0; q < Piece<T>::N; ++q) {
+        const uint32_t bits = x.bits(q), i = (bits & 0x7FFF) - kLeastValue;
+        if (i < kValues / 2) {
+          atomicAdd(s_value + (i | (bits >> 15) * (kValues / 2)), 1u);
+        } else {
+          const float l = x[q];
+          if (l > -INFINITY) add(l, 1);
+        }
+      }
     });
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kValues; i += kChunkThreads) {
+      const uint32_t bits = (i % (kValues / 2) + kLeastValue) | (i / (kValues / 2)) << 15;
+      if (const uint32_t n = s_value[i]) add(__uint_as_float(bits << 16), n);
+    }
+  } else if (mode == kTopK) {
+    part.each([&](float l, int i) {
+      if (i < g.V) add(l, 1);
+    });
+  } else {
+    part.each([&](float l, int) { add(l, 1); });
   }
   __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += kChunkThreads) {
     u64 w = 0;
 #pragma unroll
-    for (int c = 0; c < kCopies; ++c) w += s_bins[i * kCopies + c];
+    for (int c = 0; c < kBinCopies; ++c) w += s_bins[i * kBinCopies + c];
     if (w) atomicAdd(g.bins + (size_t)b * kBins + i, w);
   }
 }

@@ -320,3 +320,34 @@ def test_long_rows_streams_graphs():
                 got.append([op.forward(l, u, **f) for f in kinds])
     torch.cuda.synchronize()
     assert all(torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) for g in got for a, b in zip(g, want))
+
+
+def test_bf16_values_of_any_size_in_long_rows():
+    """Values inside and outside 2^-8 to 2^8, which are counted apart, in one row and alone; few values, many times."""
+    V = 20011
+    l, u = inputs(16, V, "bf16", seed=8)
+    f = l.float()
+    f[0] *= 2.0 ** -12
+    f[1] *= 2.0 ** 12
+    f[2, ::2] *= 2.0 ** -10
+    f[3, ::2] *= 2.0 ** 7
+    f[4] = f[4].abs() + 250
+    f[5] = 256 - f[5].abs() * 2
+    f[6] = 2.0 ** -8
+    f[7] = -2.0 ** -8
+    f[7, ::3] = 2.0 ** -9
+    f[8] = -3e38
+    f[8, 5::1000] = -2.9e38
+    f[9] = f[9].round()
+    f[10, ::2] = -INF
+    f[11, 1::2] = float("nan")
+    f[12, 77] = INF
+    f[13] = 0.0
+    f[13, ::2] = -0.0
+    f[14] = (f[14] * 4).round() / 4 + 255
+    l = f.bfloat16()
+    for kw in FILTERS:
+        check(l, u, **kw)
+    for T in (100.0, 1e-3):
+        check(l, u, T=T, p=0.9)
+        check(l, u, T=T, k=300, p=0.9)
