@@ -507,7 +507,7 @@ int mgpt_lm_loss_backward(const mgpt_lm_loss_config* cfg, const void* x, const v
  * idx [N,k]: the k largest keys, descending, the lower id first where equal;
  * where fewer take part the lowest other ids follow, with weight 0.  weights [N,k] fp32:
  * scale s_j / (sum of the k's s + 1e-20) if renormalise is not 0, else scale
- * s_j.  Keys with a bias and the groups' sizes are compared as 64 bits hold
+ * s_j; an s below 2^-126 may count as 0.  Keys with a bias and the groups' sizes are compared as 64 bits hold
  * them.  The layer's own router (mgpt_moe_forward) is the engine's; see
  * mgpt_moe_set_routing. */
 typedef enum mgpt_score {

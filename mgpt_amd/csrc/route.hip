@@ -8,7 +8,7 @@
 //   top_groups largest groups take part, and of their experts the k largest keys, in
 //   descending order, the lower id first where equal; where fewer are left, the lowest of the other ids
 //   follow, with weight 0:
-//   w_j = c s_j / D,  D = sum_j s_j + 1e-20 (renormalised) or 1
+//   w_j = c s_j / D,  D = sum_j s_j + 1e-20 (renormalised) or 1;  a score below 2^-126 may count as 0 here
 // Backward, for the upstream gradients dw of the weights and g_e of expert e's score in every token:
 //   d_j = (c dw_j - sum_i dw_i w_i) / D (or c dw_j),  ds = g + d scattered to the chosen ones
 //   sigmoid: dl = ds s (1 - s),   softmax: dl = s (ds - sum_e ds_e s_e)
@@ -637,6 +637,7 @@ __global__ __launch_bounds__(256, 3) void route_kernel(RouteArgs g) {
       bool on[kSlots];
       const uint32_t near = (uint32_t)fminf(2.0f * tol * per + 4.0f, 0x1p30f);
       float edge = kNone;   // the last chosen one's logit, where the next has the same number
+      bool out = false;     // one is chosen that takes no part
 #pragma unroll
       for (int i = 0; i < kSlots; ++i) {
         const int j = i * LP + lp;
@@ -648,6 +649,7 @@ __global__ __launch_bounds__(256, 3) void route_kernel(RouteArgs g) {
         x[i] = in ? logits[id[i]] : kNone;
         // (out of the unit's reach, or of the groups': in no order)
         sure = sure && (q > 0 || x[i] == kNone);
+        out = out || (in && q == 0);
         if (qn > 0) {
           if (NEAR && g.bias) {
             sure = sure && q - qn > near;
@@ -656,6 +658,12 @@ __global__ __launch_bounds__(256, 3) void route_kernel(RouteArgs g) {
             if (j + 1 == g.k) edge = x[i];
           }
         }
+      }
+      if (__ballot(out)) {
+        // does one take part that is out of the unit's reach?
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (key[v] > kNone && number(key[v]) == 0) sure = false;
       }
       if (__ballot(edge > kNone)) {
         // are all logits of that number equal?  (those that were not reached may be in any lane)

@@ -310,3 +310,23 @@ def test_balance_evens_the_load():
     last = load()
     assert int(first.sum()) == int(last.sum()) == 4096 * 4
     assert int(last.max()) - int(last.min()) < (int(first.max()) - int(first.min())) // 4
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("E,groups", [(3, 1), (16, 4), (60, 1), (160, 8), (256, 8), (512, 1)])
+def test_far_logits_beside_masked_ones(E, groups, act):
+    """Experts that are out come behind all that are not, however far those lie below the largest."""
+    N = 200
+    gen = torch.Generator(device="cuda").manual_seed(E)
+    for gap in (20.0, 31.0, 34.0, 60.0, 300.0, 1e5):
+        l = logits_of(N, E, act, seed=E)
+        l[:, ::2] = -INF
+        l[:, 1::4] -= gap
+        l[torch.arange(N, device="cuda"), torch.randint(0, E, (N,), generator=gen, device="cuda")] = 3.0
+        l[5] = -INF
+        l[5, E - 1] = -gap
+        for k in (1, min(4, E), min(8, E)):
+            for score in ("softmax", "sigmoid"):
+                check(l, k, score, renormalise=False)
+                if groups > 1:
+                    check(l, k, score, groups=groups, top_groups=max(1, groups // 2), renormalise=False)
