@@ -198,10 +198,10 @@ __device__ __forceinline__ void softmax_of(const float (&l)[V], float (&s)[V]) {
   for (int v = 0; v < V; ++v) s[v] *= r;
 }
 
-// exp(x) in 64 bits to 2^-51, x up to 700 in magnitude (beyond: as there): 2^t by its whole part and a polynomial of degree 10 on
-// [-1/2, 1/2] (least maximum relative error, 2^-52).
+// exp(x) in 64 bits to 2^-51, x <= 0 (down to 0 itself): 2^t by its whole part and a polynomial of degree 10 on [-1/2, 1/2]
+// (least maximum relative error, 2^-52).
 __device__ __forceinline__ double exp64(double x) {
-  const double t = fmin(fmax(x * 1.4426950408889634, -1000.0), 1000.0);
+  const double t = fmax(x * 1.4426950408889634, -1100.0);
   const double n = (t + 0x1.8p52) - 0x1.8p52, f = t - n;
   double q = 0x1.e3992178bd0ddp-28;
   q = __builtin_fma(q, f, 0x1.b6740fb0785eap-24);
@@ -397,8 +397,8 @@ __device__ __forceinline__ void choose_exactly(RouteArgs g, const float (&l)[V],
 #pragma unroll 2
     for (int e = lp; e < kAll; e += LP) {
       const double x = key[e];
-      const double q = exp64(SOFTMAX ? x - m : -x);
-      double s = SOFTMAX ? q * r : inverse64(1.0 + q);
+      const double q = exp64(SOFTMAX ? x - m : -fabs(x)), i = SOFTMAX ? r : inverse64(1.0 + q);
+      double s = SOFTMAX || x < 0.0 ? q * i : i;
       if (g.bias) s += (double)bias[e];
       // (a NaN is not above)
       key[e] = e >= g.E ? -INFINITY : x > -INFINITY && s > -INFINITY ? fmin(s, 1e300) : kOut;

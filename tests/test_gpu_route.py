@@ -330,3 +330,14 @@ def test_far_logits_beside_masked_ones(E, groups, act):
                 check(l, k, score, renormalise=False)
                 if groups > 1:
                     check(l, k, score, groups=groups, top_groups=max(1, groups // 2), renormalise=False)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_groups_of_the_smallest_scores(score):
+    """Sizes of groups down to 64 bits' smallest normal number are in order."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    l = -694 - 13 * torch.rand(300, 16, generator=gen, device="cuda")
+    if score == "softmax":
+        l[:, 0] = 0.0
+    for groups, top in ((16, 5), (8, 3), (4, 2)):
+        check(l, 2, score, groups=groups, top_groups=top, renormalise=False)
