@@ -134,3 +134,56 @@ def test_training_steps_even_the_load():
         spread = (counts.max() - counts.min()).item()
         first = spread if first is None else first
     assert int(counts.sum()) == N * k and spread < first
+
+
+def test_a_row_without_a_batch_and_no_rows():
+    """Tensors of one dimension, and none: the values of a batch of one, and empty outputs."""
+    from mgpt_amd.linear8 import I8Linear
+    from mgpt_amd.routing import ExpertRouting
+    from mgpt_amd.sampling import Sampler
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+    route = ExpertRouting(24, 3, score="sigmoid")
+    l = r(24)
+    one, many = route.forward(l), route.forward(l[None])
+    assert one[0].shape == (3,) and torch.equal(one[0], many[0][0]) and torch.equal(one[1], many[1][0])
+    assert torch.equal(route.backward(l, *one, one[1]), route.backward(l[None], *many, many[1])[0])
+    assert route.forward(l.new_empty(0, 24))[0].shape == (0, 3)
+    assert route.backward(l.new_empty(0, 24), *route.forward(l.new_empty(0, 24)), l.new_empty(0, 3)).shape == (0, 24)
+    head = I8Linear(40, 70, act="f32")
+    head.load(r(70, 40))
+    x = r(40)
+    assert head.forward(x).shape == (70,) and torch.equal(head.forward(x), head.forward(x[None])[0])
+    assert head.forward(x.new_empty(0, 40)).shape == (0, 70)
+    for V in (300, 9000):
+        sampler = Sampler(V)
+        l, u = r(V), torch.rand((), generator=gen, device="cuda")
+        one, many = sampler.forward(l, u, top_p=0.9), sampler.forward(l[None], u[None], top_p=0.9)
+        assert one[0].shape == () and torch.equal(one[0], many[0][0]) and torch.equal(one[1], many[1][0])
+        assert sampler.forward(l.new_empty(0, V), u.new_empty(0))[0].shape == (0,)
+
+
+@pytest.mark.parametrize("E,k", [(80, 4), (200, 8)])
+def test_training_by_a_rule_with_many_experts(E, k):
+    """Forward, backward and the loads of a layer of more than 64 experts, against the layer in 64 bits."""
+    from test_gpu_layer_routing import of
+    c = Case(128, 64, E, k, "f32", "f32")
+    r = rule(E, k, score="sigmoid", groups=8, top_groups=4)
+    c.op.set_routing(r, balance=0.1)
+    N = 300
+    x = c.x(N)
+    y = c.op.forward(x, train=True)
+    idx, w, on = of(r, c.logits(x), None)
+    dout = torch.randn(N, 128, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda")
+    c.op.zero_grad()
+    dx = c.op.backward(dout)
+    xd, wr = x.double().requires_grad_(), c.wr.double().requires_grad_()
+    s = torch.sigmoid(xd @ wr + c.br.double())
+    chosen = s.gather(1, idx.cuda())
+    want = c.experts(xd, idx.cuda(), chosen / (chosen.sum(1, keepdim=True) + 1e-20))
+    counts = torch.bincount(idx.reshape(-1), minlength=E).double().cuda()
+    loss = (want * dout.double()).sum() + (0.1 * E * counts / N / N * s).sum()
+    loss.backward()
+    assert rel(y, want.detach()) < 1e-5
+    assert rel(dx, xd.grad) < 1e-5
+    assert rel(c.op.get_gradients()[0], wr.grad) < 1e-5
