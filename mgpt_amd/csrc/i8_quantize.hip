@@ -8,7 +8,7 @@
 // row often has, is on the border of 63 and 64; r's rounding decides, in a program of 64-bit operations as here.)  A
 // row that holds an infinity or a NaN has the scale NaN, and so have its outputs.
 //
-// Measured: 16384 x 2048 bf16 28 us (3.6 TB/s), one row 4 us; hidden units 32768 x 2816 70 us (4.6 TB/s).  Blocks of
+// Measured: 16384 x 2048 bf16 25 us (4.0 TB/s), one row 4 us; hidden units 32768 x 2816 70 us (4.6 TB/s).  Blocks of
 // whole row blocks, 64 bytes of a row at a time, took 44 and 8 us, and 110 for hidden units of 16 bits.
 #include <algorithm>
 #include <type_traits>
@@ -107,9 +107,9 @@ __device__ __forceinline__ uint32_t round4(double a, double b, double c, double 
   return __builtin_amdgcn_perm(cd, ab, 0x05040100);
 }
 
-template <QuantizeSource SRC, bool VEC, int NW>
+// HOLD: slabs of a wave that stay in registers
+template <QuantizeSource SRC, bool VEC, int NW, int HOLD>
 __global__ __launch_bounds__(NW * kWave) void i8_quantize_kernel(QuantizeArgs g) {
-  constexpr int kHold = 4;   // slabs of a wave that stay in registers
   __shared__ uint32_t s_top[NW][kPart];
   const int block = (int)blockIdx.x / (kI8Rows / kPart), part = (int)blockIdx.x % (kI8Rows / kPart);
   int row0, rows;
@@ -133,18 +133,18 @@ __global__ __launch_bounds__(NW * kWave) void i8_quantize_kernel(QuantizeArgs g)
     if (g.gamma) rs = g.rstd[row];
   }
   const int slabs = (g.K + kI8Slab - 1) / kI8Slab;
-  Raw<SRC> held[kHold];
+  Raw<SRC> held[HOLD];
   uint32_t top = 0;
   auto look = [&](const Raw<SRC>& raw, int c) { top = max(top, largest<SRC>(g, raw, c, rs)); };
   auto column = [&](int t) { return t * kI8Slab + chunk * 16; };
   auto load = [&](int t) { return load_raw<SRC, VEC>(g, row, column(t), live && column(t) < g.K); };
 #pragma unroll
-  for (int u = 0; u < kHold; ++u)
+  for (int u = 0; u < HOLD; ++u)
     if (w + u * NW < slabs) held[u] = load(w + u * NW);
 #pragma unroll
-  for (int u = 0; u < kHold; ++u)
+  for (int u = 0; u < HOLD; ++u)
     if (w + u * NW < slabs) look(held[u], column(w + u * NW));
-  for (int t = w + kHold * NW; t < slabs; t += NW) look(load(t), column(t));
+  for (int t = w + HOLD * NW; t < slabs; t += NW) look(load(t), column(t));
 #pragma unroll
   for (int d = kPart; d < kWave; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d, kWave));
   if (chunk == 0) s_top[w][lane] = top;
@@ -175,9 +175,9 @@ __global__ __launch_bounds__(NW * kWave) void i8_quantize_kernel(QuantizeArgs g)
     *reinterpret_cast<uint4*>(out + (size_t)t * (kI8Slab * kI8Rows)) = make_uint4(q[0], q[1], q[2], q[3]);
   };
 #pragma unroll
-  for (int u = 0; u < kHold; ++u)
+  for (int u = 0; u < HOLD; ++u)
     if (w + u * NW < slabs) put(held[u], w + u * NW);
-  for (int t = w + kHold * NW; t < slabs; t += NW) put(load(t), t);
+  for (int t = w + HOLD * NW; t < slabs; t += NW) put(load(t), t);
 }
 
 // VEC: a lane's 16 columns are a vector or past K.
@@ -220,11 +220,13 @@ hipError_t launch_i8_quantize(QuantizeSource src, const QuantizeArgs& g, int max
     };
     constexpr QuantizeSource kS = decltype(s)::value;
     constexpr bool kV = decltype(v)::value;
-    // the fewest waves whose registers hold the rows
-    if (slabs <= 8) launch(i8_quantize_kernel<kS, kV, 2>, 2);
-    else if (slabs <= 16) launch(i8_quantize_kernel<kS, kV, 4>, 4);
-    else if (slabs <= 32) launch(i8_quantize_kernel<kS, kV, 8>, 8);
-    else launch(i8_quantize_kernel<kS, kV, 16>, 16);
+    // Waves whose registers hold the rows: two slabs each, of long rows four (at 16 slabs 4 and 2 a wave take 28 and 25 us
+    // for 16384 rows, at 22 of hidden units 72 and, on 16 waves, 84).
+    if (slabs <= 4) launch(i8_quantize_kernel<kS, kV, 2, 2>, 2);
+    else if (slabs <= 8) launch(i8_quantize_kernel<kS, kV, 4, 2>, 4);
+    else if (slabs <= 16) launch(i8_quantize_kernel<kS, kV, 8, 2>, 8);
+    else if (slabs <= 32) launch(i8_quantize_kernel<kS, kV, 8, 4>, 8);
+    else launch(i8_quantize_kernel<kS, kV, 16, 4>, 16);
   };
   auto with = [&](auto s) { vec ? go(s, std::true_type{}) : go(s, std::false_type{}); };
   if (src == kRowsF32) with(std::integral_constant<QuantizeSource, kRowsF32>{});
