@@ -65,9 +65,11 @@ typedef struct mgpt_moe_config {
                         and BF16 / FP8 weights the caller's tensors stay fp32:
                         routing on the fp32 rows, expert products in bf16,
                         fp32 outputs (inference only).  I8 (inference only):
-                        the experts' rows and hidden units are quantised with a
-                        scale each (as mgpt_i8_linear_forward's) and both
-                        products run in integers */
+                        the experts' rows, hidden units and weights are
+                        quantised as mgpt_i8_linear_forward's rows, but for
+                        the scale, max|x| (1 / 127) in fp32, and both products
+                        run in integers.  Hidden units h = g / (1 + exp(-g)) u:
+                        for act F32 in fp32, each operation rounded by itself */
 } mgpt_moe_config;
 
 typedef struct mgpt_moe mgpt_moe;   /* opaque handle; owns packed weights */

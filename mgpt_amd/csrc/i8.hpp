@@ -52,6 +52,7 @@ struct QuantizeArgs {
   const int32_t *counts, *perm;
   int E, k;
   const float *rstd, *gamma;
+  int by_product;          // scales are max|x| (1 / 127), both factors of 32 bits, instead of the quotient
   char* q;                 // row blocks
   float* scale;            // [row blocks][32]
 };

@@ -201,7 +201,8 @@ __device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][T
         for (int v = 0; v < 16; ++v) {
           const float ag = (float)acc[2 * gi][i][v], au = (float)acc[2 * gi + 1][i][v];
           if constexpr (KIND == kI8GateUpF32) {
-            // each operation's own rounding: the integers of h are those of the formula in fp32
+            // each operation's own rounding: the integers of h are those of the formula in 32 bits, scales included
+            // (QuantizeArgs::by_product)
             const float x = ag * sa[i] * sg[v] + bg[v], u = au * sa[i] * su[v] + bu[v];
             h[v] = x / (1.0f + expf(-x)) * u;
           } else {   // (some 2^-22 off, a quarter of what 20 bits are)

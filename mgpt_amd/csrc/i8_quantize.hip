@@ -155,7 +155,8 @@ __global__ __launch_bounds__(NW * kWave) void i8_quantize_kernel(QuantizeArgs g)
   const bool finite = top < 0x7F800000u;
   const float most = __uint_as_float(top);
   if (w == 0 && chunk == 0 && live)
-    g.scale[(size_t)block * kI8Rows + r] = finite ? most / 127.0f : __uint_as_float(0x7FC00000u);
+    g.scale[(size_t)block * kI8Rows + r] =
+        !finite ? __uint_as_float(0x7FC00000u) : g.by_product ? most * (1.0f / 127.0f) : most / 127.0f;
   const double f = finite && top ? 127.0 * (1.0 / (double)most) : 0.0;
   // (column c: tile c / 32 of the row block, its half c / 16)
   char* out = g.q + (size_t)block * i8_row_block_bytes(g.K) + (chunk / 2) * 1024 + (chunk % 2 * kI8Rows + r) * 16;

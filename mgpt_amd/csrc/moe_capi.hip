@@ -763,6 +763,7 @@ int mgpt_moe_load_parameters(mgpt_moe* h, const float* const* params, int num_pa
       a.ld = K;
       a.N = rows;
       a.K = K;
+      a.by_product = 1;
       a.q = q;
       a.scale = scale;
       return launch_i8_quantize(kRowsF32, a, rows / kI8Rows, st);
@@ -884,7 +885,10 @@ struct BlockArgs {
 };
 
 // The experts in 8-bit integers: rows of x (normalised, with gamma) quantised as they are gathered,
-// gate/up with SwiGLU, the hidden units quantised in turn, down.
+// gate/up with SwiGLU, the hidden units quantised in turn, down.  Hidden units decide integers, so an fp32 caller's have
+// the bits of a torch program's: each operation rounded by itself, and scales by the product with 1 / 127 that torch
+// makes of a division by a number on the GPU (by the quotient one scale in twenty differed in its last bit, and of the
+// hidden units that they scale one in ten million came out an integer further: outputs 1e-5 to 3e-5 apart in norm).
 template <typename IoT, typename Mark>
 int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, const float* gamma, size_t A,
                const int32_t* counts, const int32_t* perm, const Rows16& out, char* ws, hipStream_t st, Mark mark) {
@@ -901,6 +905,7 @@ int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, co
   q.k = h->k;
   q.rstd = rstd;
   q.gamma = gamma;
+  q.by_product = 1;
   q.q = ws + L.xq;
   q.scale = (float*)(ws + L.xs);
   HIP_TRY(launch_i8_quantize(sizeof(IoT) == 4 ? kRowsF32 : kRowsBf16, q, blocks, st));
@@ -934,6 +939,7 @@ int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, co
   qh.counts = counts;
   qh.E = E;
   qh.k = h->k;
+  qh.by_product = 1;
   qh.q = ws + L.hq;
   qh.scale = (float*)(ws + L.hs);
   HIP_TRY(launch_i8_quantize(kF32 ? kRowsF32 : kRowsHidden, qh, blocks, st));
