@@ -263,13 +263,13 @@ __global__ __launch_bounds__(256) void combine2_kernel(const ActT* __restrict__ 
   }
 }
 
-// The same sums over Rows16: a wave 512 columns of a token, 8 a lane, AT of its rows in flight; in the order of the
-// experts, by fused multiply-adds (these rows have no sum elsewhere to agree with).  16384 x 1024, k 2: 20 us, 5.0 TB/s.
-template <typename OutT, int AT>
-__global__ __launch_bounds__(256) void combine16_kernel(Rows16 rows, const int32_t* __restrict__ topk_idx,
+// The same sums over Rows24: a wave 512 columns of a token, 8 a lane, AT of its rows in flight; in the order of the
+// experts, by fused multiply-adds (these rows have no sum elsewhere to agree with).
+template <int AT>
+__global__ __launch_bounds__(256) void combine24_kernel(Rows24 rows, const int32_t* __restrict__ topk_idx,
                                                         const float* __restrict__ topk_p,
                                                         const int32_t* __restrict__ slot_of, int N, int C, int k,
-                                                        const OutT* __restrict__ resid, OutT* __restrict__ y) {
+                                                        const bf16_t* __restrict__ resid, bf16_t* __restrict__ y) {
   __shared__ int s_slot[kWavesPerBlock][kMaxTopK];
   __shared__ float s_p[kWavesPerBlock][kMaxTopK];
   const int w = threadIdx.x / kWave, l = lane_id();
@@ -294,27 +294,28 @@ __global__ __launch_bounds__(256) void combine16_kernel(Rows16 rows, const int32
     float acc[8] = {};
     for (int a0 = 0; a0 < k; a0 += AT) {
       uint4 raw[AT];
-      uint32_t top[AT];
+      uint2 low[AT];
 #pragma unroll
       for (int a = 0; a < AT; ++a) {
         const size_t row = s_slot[w][min(a0 + a, k - 1)];
-        raw[a] = *reinterpret_cast<const uint4*>(rows.q + row * rows.ld + c);
-        top[a] = rows.top[row * (rows.ld / 32) + c / 32];
+        raw[a] = *reinterpret_cast<const uint4*>(rows.hi + row * rows.ld + c);
+        low[a] = *reinterpret_cast<const uint2*>(rows.low + row * rows.ld + c);
       }
 #pragma unroll
       for (int a = 0; a < AT; ++a) {
         if (a0 + a >= k) break;
-        // 2^(e - 141)
-        float unit = __uint_as_float((uint32_t)(max((int)(top[a] >> 23), 16) - 14) << 23) * s_p[w][a0 + a];
-        if (top[a] >= 0x7F800000u) unit = __uint_as_float(0x7FC00000u);
+        const float p = s_p[w][a0 + a];
         const uint32_t v[4] = {raw[a].x, raw[a].y, raw[a].z, raw[a].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          acc[i] = fmaf((float)(i & 1 ? (int)v[i / 2] >> 16 : (int)(int16_t)v[i / 2]), unit, acc[i]);
+        for (int i = 0; i < 8; ++i) {   // bytes: zero, the lower one, the two upper ones
+          const uint32_t bits = __builtin_amdgcn_perm(v[i / 2], i < 4 ? low[a].x : low[a].y,
+                                                      (i & 1 ? 0x0706000cu : 0x0504000cu) | (uint32_t)(i % 4) << 8);
+          acc[i] = fmaf(__uint_as_float(bits), p, acc[i]);
+        }
       }
     }
-    if (resid) add_resid<OutT, 8>(resid + (size_t)t * C + c, acc);
-    OutVec<OutT, 8>::store(y + (size_t)t * C + c, acc);
+    if (resid) add_resid<bf16_t, 8>(resid + (size_t)t * C + c, acc);
+    OutVec<bf16_t, 8>::store(y + (size_t)t * C + c, acc);
   }
 }
 
@@ -372,24 +373,19 @@ hipError_t launch_combine(const ActT* out_rows, const int32_t* topk_idx, const f
   return hipGetLastError();
 }
 
-template <typename OutT>
-hipError_t launch_combine16(const Rows16& rows, const int32_t* topk_idx, const float* topk_p, const int32_t* slot_of,
-                            int N, int C, int k, const OutT* resid, OutT* y, hipStream_t stream) {
+hipError_t launch_combine24(const Rows24& rows, const int32_t* topk_idx, const float* topk_p, const int32_t* slot_of,
+                            int N, int C, int k, const bf16_t* resid, bf16_t* y, hipStream_t stream) {
   if (N == 0) return hipSuccess;
   if (k < 1 || k > kMaxTopK || C % 32 != 0 || rows.ld % 32 != 0) return hipErrorInvalidValue;
   const dim3 grid((N + kWavesPerBlock - 1) / kWavesPerBlock, (C + kWave * 8 - 1) / (kWave * 8));
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, rows, topk_idx, topk_p, slot_of, N, C, k, resid, y);
   };
-  if (k <= 2) go(combine16_kernel<OutT, 2>);
-  else if (k <= 4) go(combine16_kernel<OutT, 4>);
-  else go(combine16_kernel<OutT, 8>);
+  if (k <= 2) go(combine24_kernel<2>);
+  else if (k <= 4) go(combine24_kernel<4>);
+  else go(combine24_kernel<8>);
   return hipGetLastError();
 }
-template hipError_t launch_combine16<float>(const Rows16&, const int32_t*, const float*, const int32_t*, int, int, int,
-                                            const float*, float*, hipStream_t);
-template hipError_t launch_combine16<bf16_t>(const Rows16&, const int32_t*, const float*, const int32_t*, int, int, int,
-                                             const bf16_t*, bf16_t*, hipStream_t);
 
 template hipError_t launch_combine<float, float>(const float*, const int32_t*, const float*,
                                                  const int32_t*, int, int, int, const float*,

@@ -23,23 +23,27 @@ __host__ __device__ inline size_t i8_row_block_bytes(int K) {
   return (size_t)((K + kI8Slab - 1) / kI8Slab) * kI8Slab * kI8Rows;
 }
 
-// Rows that one kernel leaves to another, with a power of two for every 32 values: v 2^(e - 141), v of 16 bits and e the
-// exponent byte (16 at least) of the largest magnitude of the 32, which is held as it was.  At bf16's size they are
-// 2^-16 of that magnitude off at most.
-struct Rows16 {
-  int16_t* q;      // [rows][ld]
-  uint32_t* top;   // [rows][ld / 32]: |x|'s bits as fp32, infinity's or more: one of the 32 is not finite
-  int ld;
-};
-
-// Hidden units between the two products of an expert, with 4 more bits: v 2^(e - 145), e 20 at least.  In bf16 one value in
+// Hidden units of a bf16 caller between the two products of an expert: 20 bits each, with a power of two for every 32:
+// v 2^(e - 145), e the exponent byte (20 at least) of the largest magnitude of the 32, which is held as it was.  They are
+// rounded to a step of max|h| / 127 of the whole row next, of which these bits are 2^-12 at most; in bf16 one value in
 // eight would end a step off in the integers that follow (its rounding is 0.03 of their steps, rms), in 16 bits one in
 // four hundred, here one in six thousand.  The largest magnitudes give a row's without its values.
-// n: column 32 i + 16 b + 8 a + 4 h + c's bits in byte 16 i + 8 b + 4 h + c, its lower half where a is 0 (a lane's
-// accumulators and the quantiser's lane both have them in two words).
 struct HiddenRows {
-  Rows16 r;
-  uint8_t* n;      // [rows][ld / 2]
+  int16_t* q;      // [rows][ld]: v's upper 16 bits
+  uint32_t* top;   // [rows][ld / 32]: |x|'s bits as fp32, infinity's or more: one of the 32 is not finite
+  int ld;
+  // [rows][ld / 2]: column 32 i + 16 b + 8 a + 4 h + c's lower bits in byte 16 i + 8 b + 4 h + c, its lower half where
+  // a is 0 (a lane's accumulators and the quantiser's lane both have them in two words)
+  uint8_t* n;
+};
+
+// Expert outputs of a bf16 caller between the down product and the combine: the upper 24 bits of the fp32 number, so
+// that each is off by 2^-16 of itself at most, whatever its neighbours (outputs that share an exponent lose their bits
+// beside a channel that is hundreds of times as large, as models have them), against the 2^-8 that y is rounded to.
+struct Rows24 {
+  uint16_t* hi;    // [rows][ld]
+  uint8_t* low;    // [rows][ld]
+  int ld;
 };
 
 // Rows to quantise.  Dense: rows 0 .. N - 1 of src.  By experts (counts): slot s of a segment is row
@@ -79,12 +83,13 @@ struct I8Args {
   int E, N;                // N: rows in all
   void* out;               // [rows][ldo]
   size_t ldo;
-  HiddenRows h;            // kI8GateUp, and without n kI8Rows16: instead
+  HiddenRows h;            // kI8GateUp: instead
+  Rows24 o;                // kI8Rows24: instead
   int rowsfirst;           // set by the launcher: a lane has an output column
   int e_base;
 };
-enum I8Out { kI8F32, kI8Bf16, kI8GateUp, kI8Rows16, kI8GateUpF32 };
-// kI8GateUp, kI8GateUpF32, kI8Rows16: Nf is a multiple of 64.
+enum I8Out { kI8F32, kI8Bf16, kI8GateUp, kI8Rows24, kI8GateUpF32 };
+// kI8GateUp, kI8GateUpF32, kI8Rows24: Nf is a multiple of 64.
 hipError_t launch_i8_gemm(I8Out kind, const I8Args& g, int num_cus, hipStream_t st);
 
 }  // namespace mgpt

@@ -139,12 +139,11 @@ __device__ __forceinline__ void row_scales(const I8Args& g, const RowTile& t, in
     sa[i] = row0 + 32 * i + lrow < t.row_end ? g.sa[(size_t)(blk + i) * kI8Rows + lrow] : 0.0f;
 }
 
-// Columns col .. col + 31 of a row of Rows16, or of HiddenRows: a lane of each half has 16 values, as an accumulator does,
-// and their largest magnitude's bits.
-template <bool HIDDEN>
-__device__ __forceinline__ void put_group(const HiddenRows& to, const float (&x)[16], uint32_t top, int row, int col,
-                                          int half, bool live) {
-  constexpr int kBits = HIDDEN ? 20 : 16;
+// Columns col .. col + 31 of a row of HiddenRows: a lane of each half has 16 values, as an accumulator does, and their
+// largest magnitude's bits.
+__device__ __forceinline__ void put_hidden(const HiddenRows& to, const float (&x)[16], uint32_t top, int row, int col,
+                                           int half, bool live) {
+  constexpr int kBits = 20;
   const auto o = __builtin_amdgcn_permlane32_swap(top, top, false, false);
   top = max(o[0], o[1]);
   const int e = max((int)(top >> 23), kBits);
@@ -161,21 +160,33 @@ __device__ __forceinline__ void put_group(const HiddenRows& to, const float (&x)
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const uint32_t* w = q + 4 * k;
-    if constexpr (HIDDEN) {
-      hi[k] = make_uint2(__builtin_amdgcn_perm(w[1] << 12, w[0] << 12, 0x07060302),
-                         __builtin_amdgcn_perm(w[3] << 12, w[2] << 12, 0x07060302));
-      low[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400),
-                                     __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400), 0x05040100) & 0x0F0F0F0Fu;
-    } else {
-      hi[k] = make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x05040100), __builtin_amdgcn_perm(w[3], w[2], 0x05040100));
-    }
+    hi[k] = make_uint2(__builtin_amdgcn_perm(w[1] << 12, w[0] << 12, 0x07060302),
+                       __builtin_amdgcn_perm(w[3] << 12, w[2] << 12, 0x07060302));
+    low[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400),
+                                   __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400), 0x05040100) & 0x0F0F0F0Fu;
   }
-  store_group32(reinterpret_cast<bf16_t*>(to.r.q) + (size_t)row * to.r.ld + col, hi, half, live);
-  if constexpr (HIDDEN) {
-    const auto n = __builtin_amdgcn_permlane32_swap(low[0] | low[1] << 4, low[2] | low[3] << 4, false, false);
-    if (live) *reinterpret_cast<uint2*>(to.n + (size_t)row * (to.r.ld / 2) + col / 2 + 8 * half) = make_uint2(n[0], n[1]);
+  store_group32(reinterpret_cast<bf16_t*>(to.q) + (size_t)row * to.ld + col, hi, half, live);
+  const auto n = __builtin_amdgcn_permlane32_swap(low[0] | low[1] << 4, low[2] | low[3] << 4, false, false);
+  if (live) *reinterpret_cast<uint2*>(to.n + (size_t)row * (to.ld / 2) + col / 2 + 8 * half) = make_uint2(n[0], n[1]);
+  if (live && half == 0) to.top[(size_t)row * (to.ld / 32) + col / 32] = top;
+}
+
+// The same of Rows24.
+__device__ __forceinline__ void put24(const Rows24& to, const float (&x)[16], int row, int col, int half, bool live) {
+  uint2 hi[4];
+  uint32_t low[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[q] = __float_as_uint(x[4 * k + q]) + (x[4 * k + q] == x[4 * k + q] ? 0x80u : 0u);   // (a NaN stays one)
+    hi[k] = make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x07060302), __builtin_amdgcn_perm(w[3], w[2], 0x07060302));
+    low[k] = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0501) | __builtin_amdgcn_perm(w[3], w[2], 0x05010c0c);
   }
-  if (live && half == 0) to.r.top[(size_t)row * (to.r.ld / 32) + col / 32] = top;
+  store_group32(to.hi + (size_t)row * to.ld + col, hi, half, live);
+  const auto a = __builtin_amdgcn_permlane32_swap(low[0], low[2], false, false);   // columns 16 half .. + 3, + 4 .. 7
+  const auto b = __builtin_amdgcn_permlane32_swap(low[1], low[3], false, false);
+  if (live) *reinterpret_cast<uint4*>(to.low + (size_t)row * to.ld + col + 16 * half) = make_uint4(a[0], a[1], b[0], b[1]);
 }
 
 // Accumulators of TN x TM tiles: outputs fw + 32 j, rows row0 + 32 i of the tile t (row blocks
@@ -218,7 +229,7 @@ __device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][T
               *reinterpret_cast<float4*>(reinterpret_cast<float*>(g.out) + (size_t)row * g.ldo + hb + 8 * k + 4 * half) =
                   make_float4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
         } else {
-          put_group<true>(g.h, h, top, row, hb, half, row < t.row_end);
+          put_hidden(g.h, h, top, row, hb, half, row < t.row_end);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -237,11 +248,8 @@ __device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][T
 #pragma unroll
         for (int v = 0; v < 16; ++v) y[v] = (float)acc[j][i][v] * (sa[i] * s[v]) + b[v];
         const bool live = row < t.row_end;
-        if constexpr (KIND == kI8Rows16) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int v = 0; v < 16; ++v) top = max(top, __float_as_uint(y[v]) & 0x7FFFFFFFu);
-          put_group<false>(g.h, y, top, row, f0, half, live);
+        if constexpr (KIND == kI8Rows24) {
+          put24(g.o, y, row, f0, half, live);
         } else if constexpr (KIND == kI8Bf16) {
           bf16_t* o = reinterpret_cast<bf16_t*>(g.out) + (size_t)row * g.ldo + f0;
           uint2 q[4];
@@ -652,13 +660,14 @@ hipError_t launch_i8_gemm(I8Out kind, const I8Args& args, int num_cus, hipStream
   g.E = E;
   if (E < 1 || E > kMaxExpertsWide || g.KT < 1 || g.b_blocks < 1 || num_cus <= 0) return hipErrorInvalidValue;
   const bool gate_up = kind == kI8GateUp || kind == kI8GateUpF32;
-  if ((kind == kI8GateUp || kind == kI8Rows16) &&
-      (g.h.r.ld % 32 != 0 || g.h.r.ld < (gate_up ? g.Nf / 2 : g.Nf) || ((uintptr_t)g.h.r.q & 15) != 0 ||
-       ((uintptr_t)g.h.n & 7) != 0 || (gate_up && !g.h.n)))
+  if (kind == kI8GateUp && (g.h.ld % 32 != 0 || g.h.ld < g.Nf / 2 || ((uintptr_t)g.h.q & 15) != 0 ||
+                            ((uintptr_t)g.h.n & 7) != 0 || !g.h.n))
+    return hipErrorInvalidValue;
+  if (kind == kI8Rows24 && (g.o.ld % 32 != 0 || g.o.ld < g.Nf || (((uintptr_t)g.o.hi | (uintptr_t)g.o.low) & 15) != 0))
     return hipErrorInvalidValue;
   if (kind == kI8GateUpF32 && (g.ldo % 4 != 0 || (long)g.ldo < g.Nf / 2 || ((uintptr_t)g.out & 15) != 0))
     return hipErrorInvalidValue;
-  if ((gate_up || kind == kI8Rows16) && g.Nf % 64 != 0) return hipErrorInvalidValue;
+  if ((gate_up || kind == kI8Rows24) && g.Nf % 64 != 0) return hipErrorInvalidValue;
   if (gate_up && (!g.bias0 || !g.bias1)) return hipErrorInvalidValue;
   const bool odd = (kind == kI8F32 || kind == kI8Bf16) && (g.Nf % 8 != 0 || g.ldo % 8 != 0 || ((uintptr_t)g.out & 15) != 0);
   auto with = [&](auto k, auto o) {
@@ -701,7 +710,7 @@ hipError_t launch_i8_gemm(I8Out kind, const I8Args& args, int num_cus, hipStream
   };
   if (kind == kI8GateUp) with(IntC<kI8GateUp>{}, std::false_type{});
   else if (kind == kI8GateUpF32) with(IntC<kI8GateUpF32>{}, std::false_type{});
-  else if (kind == kI8Rows16) with(IntC<kI8Rows16>{}, std::false_type{});
+  else if (kind == kI8Rows24) with(IntC<kI8Rows24>{}, std::false_type{});
   else if (kind == kI8F32) odd ? with(IntC<kI8F32>{}, std::true_type{}) : with(IntC<kI8F32>{}, std::false_type{});
   else odd ? with(IntC<kI8Bf16>{}, std::true_type{}) : with(IntC<kI8Bf16>{}, std::false_type{});
   return hipGetLastError();

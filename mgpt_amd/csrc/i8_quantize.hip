@@ -33,11 +33,11 @@ __device__ __forceinline__ Raw<SRC> load_raw(const QuantizeArgs& g, size_t row, 
   Raw<SRC> r{};
   if (!live) return r;
   if constexpr (SRC == kRowsHidden) {
-    const uint4* p = reinterpret_cast<const uint4*>(g.h.r.q + row * g.h.r.ld + c);
+    const uint4* p = reinterpret_cast<const uint4*>(g.h.q + row * g.h.ld + c);
     r.w[0] = p[0];
     r.w[1] = p[1];
-    r.n = *reinterpret_cast<const uint2*>(g.h.n + row * (g.h.r.ld / 2) + c / 2);
-    r.top = g.h.r.top[row * (g.h.r.ld / 32) + c / 32];
+    r.n = *reinterpret_cast<const uint2*>(g.h.n + row * (g.h.ld / 2) + c / 2);
+    r.top = g.h.top[row * (g.h.ld / 32) + c / 32];
   } else {
     typedef std::conditional_t<SRC == kRowsF32, uint32_t, uint16_t> T;
     const T* p = reinterpret_cast<const T*>(g.src) + row * g.ld + c;
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(256) void i8_tile_kernel(const int8_t* __restrict__
 
 hipError_t launch_i8_quantize(QuantizeSource src, const QuantizeArgs& g, int max_blocks, hipStream_t st) {
   if (max_blocks <= 0) return hipSuccess;
-  if (src == kRowsHidden && (g.h.r.ld != g.K || g.K % 32 != 0 || ((uintptr_t)g.h.r.q & 15) != 0 || ((uintptr_t)g.h.n & 7) != 0)) return hipErrorInvalidValue;
+  if (src == kRowsHidden && (g.h.ld != g.K || g.K % 32 != 0 || ((uintptr_t)g.h.q & 15) != 0 || ((uintptr_t)g.h.n & 7) != 0)) return hipErrorInvalidValue;
   const size_t size = src == kRowsF32 ? 4 : 2;
   const bool vec = src == kRowsHidden || (g.K * size % 16 == 0 && g.ld * size % 16 == 0 && ((uintptr_t)g.src & 15) == 0);
   const int slabs = (g.K + kI8Slab - 1) / kI8Slab;

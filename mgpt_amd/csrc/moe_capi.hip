@@ -54,9 +54,8 @@ hipError_t launch_permute(const InT*, const int32_t*, const int32_t*, int32_t*, 
 template <typename ActT, typename OutT>
 hipError_t launch_combine(const ActT*, const int32_t*, const float*, const int32_t*, int, int, int,
                           const OutT*, OutT*, hipStream_t);
-template <typename OutT>
-hipError_t launch_combine16(const Rows16&, const int32_t*, const float*, const int32_t*, int, int, int, const OutT*, OutT*,
-                            hipStream_t);
+hipError_t launch_combine24(const Rows24&, const int32_t*, const float*, const int32_t*, int, int, int, const bf16_t*,
+                            bf16_t*, hipStream_t);
 template <typename T>
 hipError_t launch_copy_cols(const T*, int, T*, int, int, int, int, hipStream_t);
 hipError_t launch_add_jobs(const float*, const AddJobs&, size_t, hipStream_t);
@@ -173,8 +172,8 @@ struct Layout {
   size_t dypad, dxpad;   // padded width: dy and dx at width C
   size_t nrm_part;       // fused block backward: ln2 scale-gradient partials
   // 8-bit integer experts: the gathered rows and the hidden units as row blocks with their
-  // scales, and the hidden units' exponents
-  size_t xq, xs, hq, hs, hlow, htop, otop;
+  // scales, and of a bf16 caller the hidden units' and the outputs' further bits
+  size_t xq, xs, hq, hs, hlow, htop, olow;
   // a routing of the caller's rule: logits [N][E], and the scores' gradients [E]; last, so
   // that the other regions lie where they do without it
   size_t rlogits, dscore;
@@ -402,7 +401,7 @@ struct mgpt_moe {
       const size_t packed = row_bytes() == 2 ? A : 0;
       L.hlow = take(packed * (Hp / 2));
       L.htop = take(packed * (Hp / 32) * 4);
-      L.otop = take(packed * (C / 32) * 4);
+      L.olow = take(packed * C);
     }
     if (routed) {
       L.rlogits = take((size_t)N * E * 4);
@@ -891,10 +890,10 @@ struct BlockArgs {
 // hidden units that they scale one in ten million came out an integer further: outputs 1e-5 to 3e-5 apart in norm).
 template <typename IoT, typename Mark>
 int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, const float* gamma, size_t A,
-               const int32_t* counts, const int32_t* perm, const Rows16& out, char* ws, hipStream_t st, Mark mark) {
+               const int32_t* counts, const int32_t* perm, const Rows24& out, char* ws, hipStream_t st, Mark mark) {
   const int C = h->C, Hp = h->Hp, Cp = h->Cp, E = h->E;
   const int blocks = (int)h->row_blocks(A);
-  const HiddenRows hidden{{(int16_t*)(ws + L.hbuf), (uint32_t*)(ws + L.htop), Hp}, (uint8_t*)(ws + L.hlow)};
+  const HiddenRows hidden{(int16_t*)(ws + L.hbuf), (uint32_t*)(ws + L.htop), Hp, (uint8_t*)(ws + L.hlow)};
   QuantizeArgs q{};
   q.src = x;
   q.ld = C;
@@ -955,10 +954,10 @@ int i8_experts(mgpt_moe* h, const Layout& L, const IoT* x, const float* rstd, co
   g.bias0 = h->bd;
   g.bias1 = nullptr;
   g.bias_ld = Cp;
-  g.h = {out, nullptr};
+  g.o = out;
   g.out = ws + L.obuf;
   g.ldo = C;
-  HIP_TRY(launch_i8_gemm(kF32 ? kI8F32 : kI8Rows16, g, h->num_cus, st));
+  HIP_TRY(launch_i8_gemm(kF32 ? kI8F32 : kI8Rows24, g, h->num_cus, st));
   return MGPT_OK;
 }
 
@@ -1049,9 +1048,9 @@ int forward_impl(mgpt_moe* h, const IoT* x, IoT* y, int N, char* ws, bool train,
     HIP_TRY((launch_permute<IoT, ActT>(xi, idx, block_hist, base, N, C, E, k, counts, perm, slot_of,
                                        h->i8() ? nullptr : xg, rstd, gamma, st)));
   HIP_TRY(mark(2));
-  const Rows16 rows16{(int16_t*)ob, (uint32_t*)(ws + L.otop), C};   // the outputs of experts in 8 bits
+  const Rows24 rows24{(uint16_t*)ob, (uint8_t*)(ws + L.olow), C};   // outputs of experts in 8 bits, of a bf16 caller
   if (h->i8()) {
-    if (int rc = i8_experts<IoT>(h, L, xi, rstd, gamma, A, counts, perm, rows16, ws, st, mark)) return rc;
+    if (int rc = i8_experts<IoT>(h, L, xi, rstd, gamma, A, counts, perm, rows24, ws, st, mark)) return rc;
   } else if constexpr (sizeof(ActT) == 4) {
     HIP_TRY(launch_gemm_f32<kEpiGateUp>(xg, (const float*)h->wgu, h->bg, h->bu, counts, E, C, 2 * Hp,
                                         2 * Hp, Hp, hb, Hp, A, gu, 2 * Hp, h->num_cus, st));
@@ -1133,12 +1132,18 @@ int forward_impl(mgpt_moe* h, const IoT* x, IoT* y, int N, char* ws, bool train,
     }
   }
   HIP_TRY(mark(4));
-  if (h->i8() && sizeof(IoT) == 4)
-    HIP_TRY((launch_combine<float, float>((const float*)ob, idx, topp, slot_of, N, C, k,
-                                          gamma ? (const float*)xi : nullptr, (float*)yi, st)));
-  else if (h->i8())
-    HIP_TRY(launch_combine16<IoT>(rows16, idx, topp, slot_of, N, C, k, gamma ? xi : nullptr, yi, st));
-  else
+  bool combined = false;
+  if constexpr (sizeof(ActT) == 2) {
+    if (h->i8()) {
+      const IoT* resid = gamma ? xi : nullptr;
+      if constexpr (sizeof(IoT) == 4)
+        HIP_TRY((launch_combine<float, float>((const float*)ob, idx, topp, slot_of, N, C, k, resid, yi, st)));
+      else
+        HIP_TRY(launch_combine24(rows24, idx, topp, slot_of, N, C, k, resid, yi, st));
+      combined = true;
+    }
+  }
+  if (!combined)
     HIP_TRY((launch_combine<ActT, IoT>(ob, idx, topp, slot_of, N, C, k, gamma ? xi : nullptr, yi,
                                        st)));
   if (h->padded()) HIP_TRY(launch_copy_cols<IoT>(yi, C, y, Cx, N, Cx, Cx, st));

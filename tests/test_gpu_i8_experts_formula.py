@@ -5,6 +5,9 @@ bits, as a torch program has them on the GPU: their integers are that program's,
 output, the sum as a float, its two products, the bias, the weight and the sums over the token's experts round once each,
 6 + k steps of 2^-24 of the terms' magnitudes.  A unit on the other side of a border would be a step, max|h| / 127 times a
 weight, thousands of times as much.
+
+bf16 callers: outputs of an expert keep 2^-16 of themselves, whatever the other channels' sizes; y is rounded to bf16 (2^-8).
+What hidden units of 20 bits do to a channel is a sum of integer steps, which the channel's own weights scale.
 """
 import pytest
 
@@ -74,3 +77,43 @@ def test_integers_of_fp32_callers(N, C, H, E, k):
         bad = ((y.double() - want).abs() > (6 + k) * U * mag).any(1)
         assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].flatten().tolist())
         assert ((y.double() - want).norm() / want.norm()).item() < 2e-6
+
+
+def big_channels(L, at, factor):
+    """The same layer, the output channels `at` factor times as large."""
+    params = [L.wr, L.br]
+    L.W["d"][:, :, at] *= factor
+    L.b["d"][:, at] *= factor
+    for e in range(L.E):
+        for n in "gud":
+            params += [L.W[n][e], L.b[n][e]]
+    L.op.load_parameters(params)
+
+
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+@pytest.mark.parametrize("N", [40, 600])
+@pytest.mark.parametrize("factor", [1.0, 256.0, 4096.0, 32768.0])
+def test_channels_of_other_sizes(factor, N, act):
+    L = Layer(256, 384, 4, 2, act)
+    big_channels(L, slice(5, None, 32), factor)
+    x, idx, w = L.inputs(N)
+    y = L.op.forward_routed(x, idx, w)
+    want = L.check(y, x, idx, w)     # each output, by its own terms
+    # each channel: y's rounding, 2^-8 of each, and the integer steps: with a probability of 1 / 6000 (2^-22 for fp32)
+    # for each of 384 units of 2 experts, a step is 1 / (sqrt(384) 20) of an output and of 40 rows 8 have one: 0.0012; twice that
+    off = (y.double() - want).norm(dim=0) / want.norm(dim=0)
+    assert off.max().item() < (2.0 ** -8 + 0.0024 if act == "bf16" else 0.0006), off.max().item()
+
+
+@pytest.mark.parametrize("act", ["bf16", "f32"])
+def test_an_infinite_channel_leaves_the_others(act):
+    L = Layer(128, 256, 4, 2, act)
+    x, idx, w = L.inputs(50)
+    clean = L.op.forward_routed(x, idx, w)
+    L.b["d"][:, 37] = float("inf")
+    L.b["d"][:, 70] = float("nan")
+    big_channels(L, slice(0, 0), 1.0)
+    y = L.op.forward_routed(x, idx, w)
+    keep = [c for c in range(128) if c not in (37, 70)]
+    assert torch.equal(y[:, keep], clean[:, keep])
+    assert (y[:, 37] == float("inf")).all() and y[:, 70].isnan().all()
