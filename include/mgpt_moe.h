@@ -161,6 +161,9 @@ int mgpt_moe_get_rstd(const mgpt_moe* h, int num_tokens, void* workspace, float*
  *   softmax probabilities, not renormalised), counts [E] int32,
  *   perm [N*k] int32 (slot -> flat assignment id t*k+j, expert-major,
  *   ascending flat id within an expert), slot_of [N*k] int32 (its inverse).
+ * A place that no expert takes (mgpt_moe_forward_routed)
+ * has topk_idx -1, topk_p 0 and slot_of -1, is not in counts, and leaves a -1
+ * at perm's end.
  * Replaces the reference's cached_top_indices, cached_top_probs,
  * cached_expert_counts and cached_sorted_token_ids (layers/MoELayer.h:18-28),
  * which it stores as float; these are int32. */
@@ -554,8 +557,8 @@ int mgpt_route_backward(const mgpt_route_config* cfg, const void* logits, const 
 int mgpt_moe_set_routing(mgpt_moe* h, const mgpt_route_config* cfg, const float* bias, float balance);
 
 /* mgpt_moe_forward with a routing that is given: idx, weights [N,k] device memory, y[t] = the sum of
- * weights[t][j] expert(idx[t][j])(x[t]).  An idx outside 0 .. E - 1 counts as expert 0 with weight 0; the
- * same expert may come twice.  Inference only. */
+ * weights[t][j] expert(idx[t][j])(x[t]).  An idx outside 0 .. E - 1 and a weight of 0 count for nothing, whatever
+ * x[t] holds, and no expert runs for them; the same expert may come twice.  Inference only. */
 int mgpt_moe_forward_routed(mgpt_moe* h, const void* x, const int32_t* idx, const float* weights,
                             void* y, int num_tokens, void* workspace, size_t workspace_bytes,
                             void* stream);

@@ -9,6 +9,9 @@
 // one wave per token sorts its k choices by expert id and accumulates the
 // k rows in that order with the same two roundings per term (the file is
 // built with -ffp-contract=off), reading 16 bytes per lane per row chunk.
+// A choice of slot -1 (an id that the permute skipped) adds nothing, as the
+// reference's scatter, which walks slots, does not meet it; its row is read at
+// slot 0, and left.
 #include "common.hpp"
 #include "i8.hpp"
 
@@ -142,7 +145,9 @@ __global__ __launch_bounds__(256) void combine_kernel(const ActT* __restrict__ o
       for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
         for (int i = 0; i < VN; ++i) acc[u][ch][i] = 0.0f;
-    auto add_row = [&](int u, const uint4 (&raw)[CH], float p) __attribute__((always_inline)) {
+    auto add_row = [&](int u, int a, const uint4 (&raw)[CH]) __attribute__((always_inline)) {
+      const float p = s_p[w][u][a];
+      if (s_slot[w][u][a] < 0) return;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch) {
         float v[VN];
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const ActT* __restrict__ o
       }
     };
     auto load_row = [&](int u, int a, uint4 (&raw)[CH]) __attribute__((always_inline)) {
-      const ActT* src = out_rows + (size_t)s_slot[w][u][a] * C;
+      const ActT* src = out_rows + (size_t)max(s_slot[w][u][a], 0) * C;
 #pragma unroll
       for (int ch = 0; ch < CH; ++ch) {
         const int c = c0 + (ch * kWave + l) * VN;
@@ -171,13 +176,13 @@ __global__ __launch_bounds__(256) void combine_kernel(const ActT* __restrict__ o
       for (int u = 0; u < TPW; ++u)
         if (u < nt)
 #pragma unroll
-          for (int a = 0; a < KT; ++a) add_row(u, raw[u][a], s_p[w][u][a]);
+          for (int a = 0; a < KT; ++a) add_row(u, a, raw[u][a]);
     } else {
       for (int u = 0; u < nt; ++u)
         for (int a = 0; a < k; ++a) {
           uint4 raw[CH];
           load_row(u, a, raw);
-          add_row(u, raw, s_p[w][u][a]);
+          add_row(u, a, raw);
         }
     }
 #pragma unroll
@@ -233,7 +238,7 @@ __global__ __launch_bounds__(256) void combine2_kernel(const ActT* __restrict__ 
     for (int u = 0; u < TPW; ++u)
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        const ActT* src = out_rows + (size_t)sl[u][a] * C;
+        const ActT* src = out_rows + (size_t)max(sl[u][a], 0) * C;
 #pragma unroll
         for (int ch = 0; ch < CH; ++ch) {
           const int c = c0 + (ch * kWave + l) * VN;
@@ -250,6 +255,7 @@ __global__ __launch_bounds__(256) void combine2_kernel(const ActT* __restrict__ 
         for (int i = 0; i < VN; ++i) acc[i] = 0.0f;
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
+          if (sl[u][a] < 0) continue;
           Vec16<ActT>::unpack(raw[u][a][ch], v);
 #pragma unroll
           for (int i = 0; i < VN; ++i) acc[i] = acc[i] + v[i] * pr[u][a];
@@ -297,13 +303,14 @@ __global__ __launch_bounds__(256) void combine24_kernel(Rows24 rows, const int32
       uint2 low[AT];
 #pragma unroll
       for (int a = 0; a < AT; ++a) {
-        const size_t row = s_slot[w][min(a0 + a, k - 1)];
+        const size_t row = max(s_slot[w][min(a0 + a, k - 1)], 0);
         raw[a] = *reinterpret_cast<const uint4*>(rows.hi + row * rows.ld + c);
         low[a] = *reinterpret_cast<const uint2*>(rows.low + row * rows.ld + c);
       }
 #pragma unroll
       for (int a = 0; a < AT; ++a) {
         if (a0 + a >= k) break;
+        if (s_slot[w][a0 + a] < 0) continue;
         const float p = s_p[w][a0 + a];
         const uint32_t v[4] = {raw[a].x, raw[a].y, raw[a].z, raw[a].w};
 #pragma unroll

@@ -266,6 +266,10 @@ __global__ __launch_bounds__(256) void permute_kernel(
       }
       carry += __shfl(incl, kWave - 1, kWave);
     }
+    // (ids were skipped: the slots at the end have none)
+    if (writer && carry < N * k)
+      for (int f = tid; f < nflat; f += kWave)
+        if ((int)flat0 + f >= carry) perm[flat0 + f] = -1;
   }
   __syncthreads();
   if (tid < kWave) {
@@ -279,9 +283,12 @@ __global__ __launch_bounds__(256) void permute_kernel(
       const int f = f0 + l;
       int e = ids[u];
       // Ids outside [0, E) are skipped, as the reference's histogram and
-      // gather skip them (utils/Tensor.cpp:1348, :1368).
+      // gather skip them (utils/Tensor.cpp:1348, :1368), and have slot -1.
       const bool valid = e >= 0 && e < E;
-      if (!valid) e = 0;
+      if (!valid) {
+        e = 0;
+        if (writer && f < nflat) slot_of[flat0 + f] = -1;
+      }
       unsigned long long match = __ballot(valid);
 #pragma unroll
       for (int bit = 0; bit < 9; ++bit) {

@@ -147,7 +147,7 @@ struct DScan {
 // block of the gathering gate/up kernel instead of a separate permute
 // launch: per-expert counts, expert-major slots in
 // flat order within each expert (the permute's assignment, dispatch.hip),
-// and the slot -> token map s_tok.  Ids outside [0, E) get no slot, as in
+// and the slot -> token map s_tok.  Ids outside [0, E) get slot -1, as in
 // the permute.  With publish set the block also writes counts, perm and
 // slot_of for the down GEMM, the combine and the caller.  All threads call
 // it; wave 0 does the work.
@@ -177,9 +177,12 @@ __device__ __forceinline__ void decode_rank(const int32_t* __restrict__ topk_idx
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int cnt = l < E ? s_cnt[l] : 0;
-    s_base[l] = wave_incl_scan(cnt) - cnt;
+    const int incl = wave_incl_scan(cnt);
+    s_base[l] = incl - cnt;
     s_run[l] = 0;
     if (publish && l < E) counts[l] = cnt;
+    if (publish)   // (ids were skipped: the slots at the end have none)
+      for (int f = __shfl(incl, kWave - 1, kWave) + l; f < nflat; f += kWave) perm[f] = -1;
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const unsigned long long lt = (l == 0) ? 0ull : (~0ull >> (kWave - l));
@@ -190,7 +193,10 @@ __device__ __forceinline__ void decode_rank(const int32_t* __restrict__ topk_idx
       const int f = f0 + l;
       int e = ids[u];
       const bool valid = e >= 0 && e < E;
-      if (!valid) e = 0;
+      if (!valid) {
+        e = 0;
+        if (publish && f < nflat) slot_of[f] = -1;
+      }
       unsigned long long match = __ballot(valid);
 #pragma unroll
       for (int bit = 0; bit < 6; ++bit) {

@@ -873,14 +873,15 @@ __global__ __launch_bounds__(256) void route_take_kernel(const int32_t* from, co
     int e;
     if (from) {
       e = from[f0 + f];
-      const bool in = (unsigned)e < (unsigned)E;
-      w[f0 + f] = in ? from_w[f0 + f] : 0.0f;
-      e = in ? e : 0;
+      const float p = from_w[f0 + f];
+      const bool in = (unsigned)e < (unsigned)E && p != 0.0f;
+      w[f0 + f] = in ? p : 0.0f;
+      e = in ? e : -1;
       idx[f0 + f] = e;
     } else {
       e = idx[f0 + f];
     }
-    if (hist) atomicAdd(&s_hist[e], 1);
+    if (hist && e >= 0) atomicAdd(&s_hist[e], 1);
   }
   if (!hist) return;
   __syncthreads();

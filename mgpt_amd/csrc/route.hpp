@@ -24,8 +24,8 @@ struct RouteArgs {
 int check_route(const mgpt_route_config* cfg, int N);   // a status
 RouteArgs route_args(const mgpt_route_config* cfg, const void* logits, const void* dlogits, int N);
 hipError_t launch_route(const mgpt_route_config* cfg, const RouteArgs& g, bool backward, hipStream_t st);
-// A routing for the layer: ids outside 0 .. E - 1 become expert 0 with weight 0 (from -> idx, w; null:
-// idx as it is), and hist[e][block of 64 tokens], where not null, as the permute reads it.
+// A routing for the layer: ids outside 0 .. E - 1 and those of weight 0 become -1 with weight 0 (from -> idx, w; null:
+// idx as it is), and hist[e][block of 64 tokens], where not null, as the permute reads it, without the ids -1.
 hipError_t launch_route_take(const int32_t* from, const float* from_w, int N, int E, int k, int32_t* idx, float* w,
                              int32_t* hist, hipStream_t st);
 // dscore[e] = alpha E counts[e] / N^2: the balance loss' gradient for every token's score.

@@ -176,7 +176,7 @@ class MoELayer:
     def forward_routed(self, x: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
         """The layer with a routing that is given: the sum over j of weights[..., j]
         (float32) times expert idx[..., j] (int32) of x; an idx outside 0 .. E - 1
-        counts for nothing.  Inference only."""
+        and a weight of 0 count for nothing.  Inference only."""
         if not x.is_cuda or x.dtype != self.dtype or x.shape[-1] != self.C or not x.is_contiguous():
             raise ValueError("x must be a contiguous device tensor [..., C] of the layer's dtype")
         shape = (*x.shape[:-1], self.k)
@@ -321,7 +321,8 @@ class MoELayer:
     def routing(self) -> dict:
         """Device views (torch tensors) of the last forward's routing:
         topk_idx [N,k] int32, topk_p [N,k] f32, counts [E], perm [N*k],
-        slot_of [N*k]."""
+        slot_of [N*k].  A place that no expert takes (an id out of range or a
+        weight of 0 in forward_routed) has id -1, weight 0, slot -1 and is in no count."""
         if self._last_n is None:
             raise RuntimeError("no forward has been run")
         n = self._last_n
