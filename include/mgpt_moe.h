@@ -161,7 +161,7 @@ int mgpt_moe_get_rstd(const mgpt_moe* h, int num_tokens, void* workspace, float*
  *   softmax probabilities, not renormalised), counts [E] int32,
  *   perm [N*k] int32 (slot -> flat assignment id t*k+j, expert-major,
  *   ascending flat id within an expert), slot_of [N*k] int32 (its inverse).
- * A place that no expert takes (mgpt_moe_forward_routed)
+ * A place that no expert takes (mgpt_moe_set_routing, mgpt_moe_forward_routed)
  * has topk_idx -1, topk_p 0 and slot_of -1, is not in counts, and leaves a -1
  * at perm's end.
  * Replaces the reference's cached_top_indices, cached_top_probs,
@@ -552,7 +552,8 @@ int mgpt_route_backward(const mgpt_route_config* cfg, const void* logits, const 
  * (cfg->dtype: F32; num_experts and top_k the layer's).  bias: device [E] fp32 or null, read by
  * every forward from then on (it may be updated in place; the caller keeps it alive).  balance >= 0: the factor of
  * the load-balance loss whose gradient the backward adds to every token's
- * scores, balance E (counts[e] / N) / N (the engine's router: 0.01).  Workspaces grow with it: query them
+ * scores, balance E (counts[e] / N) / N (the engine's router: 0.01).  Where fewer than k experts take part, the
+ * other places are none's: not in y, nor in counts.  Workspaces grow with it: query them
  * again.  A backward needs a training forward under the same setting. */
 int mgpt_moe_set_routing(mgpt_moe* h, const mgpt_route_config* cfg, const float* bias, float balance);
 

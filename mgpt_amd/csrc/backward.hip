@@ -67,6 +67,7 @@ __global__ __launch_bounds__(256) void scatter_bwd_kernel(
   if (slot >= A) return;
   const int lane = lane_id();
   const int flat = perm[slot];
+  if (flat < 0) return;   // (of ids that were skipped)
   const int t = flat / k;
   const float p = topk_p[flat];
   const uint4* d4 = reinterpret_cast<const uint4*>(dy + (size_t)t * C);
@@ -233,6 +234,7 @@ __global__ __launch_bounds__(64) void token_dx_kernel(const ActT* __restrict__ d
 #pragma unroll
     for (int q = 0; q < 8; ++q) gs[q] = 0.0f;
     for (int j = 0; j < k; ++j) {
+      if (s_slot[r][j] < 0) continue;   // (an id that was skipped)
       const ActT* src = dxe + (size_t)s_slot[r][j] * C + c0;
 #pragma unroll
       for (int h = 0; h < 8 / V::N; ++h) {

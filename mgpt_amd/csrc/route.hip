@@ -530,7 +530,7 @@ __global__ __launch_bounds__(256, 3) void route_kernel(RouteArgs g) {
     for (int i = 0; i < kSlots; ++i) {
       const int j = i * LP + lp;
       if (j < g.k && t < g.N) {
-        g.idx[(size_t)t * g.k + j] = id[i];
+        g.idx[(size_t)t * g.k + j] = g.drop && !on[i] ? -1 : id[i];
         g.weights[(size_t)t * g.k + j] = sc[i] * r;
         if (g.counts && on[i]) atomicAdd(&s_count[id[i]], 1);
       }

@@ -19,6 +19,7 @@ struct RouteArgs {
   int N, E, k, G, S, top_groups, best;   // S = E / G
   float scale;
   int renorm, vec;
+  int drop;              // what takes no part has the id -1, instead of the lowest ids left
 };
 
 int check_route(const mgpt_route_config* cfg, int N);   // a status

@@ -322,7 +322,8 @@ class MoELayer:
         """Device views (torch tensors) of the last forward's routing:
         topk_idx [N,k] int32, topk_p [N,k] f32, counts [E], perm [N*k],
         slot_of [N*k].  A place that no expert takes (an id out of range or a
-        weight of 0 in forward_routed) has id -1, weight 0, slot -1 and is in no count."""
+        weight of 0 in forward_routed, a rule that fewer than k experts pass)
+        has id -1, weight 0, slot -1 and is in no count."""
         if self._last_n is None:
             raise RuntimeError("no forward has been run")
         n = self._last_n
