@@ -312,8 +312,9 @@ __device__ __forceinline__ Kept kept_of(const Scale& s, End end, float min_p) {
   k.end = end;
   const double least = (double)(min_p > 0.0f ? min_p : 0.0f) * kUnits;   // (at most kUnits: more has been settled)
   k.least = (u64)ceil(least);
-  // (wider than the logarithm's error; the difference's rounding to 32 bits passes no logit)
-  const double span = least >= 1.0 ? 40.01 - (double)log2f((float)least) : 42.0;
+  // (a weight is the nearest whole number, so it has `least` units from half a unit below on; wider by more than the
+  // logarithm's error; the difference's rounding to 32 bits passes no logit)
+  const double span = k.least > 0 ? 40.01 - (double)log2f((float)((double)k.least - 0.5)) : 42.0;
   k.from = fmaxf((float)((double)s.top - span / s.c), -FLT_MAX);
   k.at = __builtin_nanf("");
   k.tie = 0;
