@@ -621,7 +621,7 @@ int mgpt_sample_workspace_bytes(const mgpt_sample_config* cfg, int num_rows, siz
  * token: [B] int32; logp: [B] fp32 or null, the logarithm of the token's
  * probability among the kept ones (0 at temperature 0, -infinity for token -1).
  * All device memory.  The arrays' values are not checked: what is not a number
- * counts as 0 in temperature and u, and as no restriction in top_p. */
+ * counts as 0 in temperature and u, and as no restriction in top_p and min_p. */
 int mgpt_sample(const mgpt_sample_config* cfg, const void* logits, const float* u,
                 const float* temperature, const int32_t* top_k, const float* top_p,
                 const float* min_p, int32_t* token, float* logp, int num_rows, void* workspace,

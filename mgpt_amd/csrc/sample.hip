@@ -271,7 +271,8 @@ struct Params {
   int k;
 };
 __device__ __forceinline__ Params params_of(const SampleArgs& g, int b) {
-  return {g.T ? g.T[b] : g.T0, g.p ? g.p[b] : g.p0, g.m ? g.m[b] : g.m0, g.u[b], g.k ? g.k[b] : g.k0};
+  const float m = g.m ? g.m[b] : g.m0;
+  return {g.T ? g.T[b] : g.T0, g.p ? g.p[b] : g.p0, m > 0.0f ? m : 0.0f, g.u[b], g.k ? g.k[b] : g.k0};
 }
 __device__ __forceinline__ Scale scale_of(float top, float temp, const double* pow) {
   Scale s;
@@ -310,7 +311,7 @@ __device__ __forceinline__ Kept kept_of(const Scale& s, End end, float min_p) {
   Kept k;
   k.s = s;
   k.end = end;
-  const double least = (double)(min_p > 0.0f ? min_p : 0.0f) * kUnits;   // (at most kUnits: more has been settled)
+  const double least = (double)min_p * kUnits;   // (at most kUnits: more has been settled)
   k.least = (u64)ceil(least);
   // (a weight is the nearest whole number, so it has `least` units from half a unit below on; wider by more than the
   // logarithm's error; the difference's rounding to 32 bits passes no logit)

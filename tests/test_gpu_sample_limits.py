@@ -1,10 +1,13 @@
-"""Sampler: min_p down to the units of the weights.  The reference and its tolerances are test_gpu_sample.py's."""
+"""Sampler: min_p down to the units of the weights, parameters that are no numbers.  The reference
+and its tolerances are test_gpu_sample.py's."""
+import math
+
 import pytest
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from test_gpu_sample import check  # noqa: E402
+from test_gpu_sample import check, inputs  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -35,3 +38,37 @@ def test_min_p_of_a_few_units(V, units):
             check(l, u, m=m, **kw)
     token, kept = check(l, u, m=units * 2.0 ** -40)
     assert (token != V // 3).any()
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [500, 8000, 9001, 30000])
+def test_parameters_that_are_no_numbers(V, act):
+    """NaN in a device array: temperature and u as 0, top_p and min_p as no restriction."""
+    from mgpt_amd.sampling import Sampler
+    B = 12
+    l, u = inputs(B, V, act, seed=V)
+    op = Sampler(V, act=act)
+    full = lambda v: torch.full((B,), v, device="cuda")  # noqa: E731
+    for k in (0, 5, 60, 900, V // 2):
+        want = op.forward(l, u, temperature=0.8, top_k=k, top_p=0.9)
+        got = op.forward(l, u, temperature=full(0.8), top_k=k, top_p=full(0.9), min_p=full(math.nan))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
+        want = op.forward(l, u, temperature=0.8, top_k=k, min_p=0.01)
+        got = op.forward(l, u, temperature=0.8, top_k=k, top_p=full(math.nan), min_p=full(0.01))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
+        want = op.forward(l, u, temperature=0.0, top_k=k)
+        got = op.forward(l, u, temperature=full(math.nan), top_k=k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
+        want = op.forward(l, full(0.0), top_k=k)
+        got = op.forward(l, full(math.nan), top_k=k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
+
+
+def test_negative_min_p_restricts_nothing():
+    from mgpt_amd.sampling import Sampler
+    for V in (500, 20000):
+        l, u = inputs(8, V, "f32")
+        for k in (0, 60):
+            want = Sampler(V).forward(l, u, top_k=k)
+            got = Sampler(V).forward(l, u, top_k=k, min_p=torch.full((8,), -1.0, device="cuda"))
+            assert torch.equal(got[0], want[0])
