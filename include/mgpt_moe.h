@@ -618,7 +618,7 @@ typedef struct mgpt_sample_config {
 int mgpt_sample_workspace_bytes(const mgpt_sample_config* cfg, int num_rows, size_t* bytes);
 
 /* u: [B] fp32, each in [0, 1); temperature, top_p, min_p: [B] fp32 or null; top_k: [B] int32 or null;
- * token: [B] int32; logp: [B] fp32 or null, the logarithm of the token's
+ * num_rows up to 2^24; token: [B] int32; logp: [B] fp32 or null, the logarithm of the token's
  * probability among the kept ones (0 at temperature 0, -infinity for token -1).
  * All device memory.  The arrays' values are not checked: what is not a number
  * counts as 0 in temperature and u, and as no restriction in top_p and min_p. */

@@ -1206,6 +1206,7 @@ using namespace mgpt;
 namespace {
 
 constexpr int kSlice = 1024;   // rows of a launch in chunks (44 KB of workspace each)
+constexpr int kWholeSlice = 1 << 20;   // rows of a launch by whole blocks (a launch takes fewer than 2^32 threads)
 
 // Rows of up to 8192 are whole blocks' work in one launch.
 bool in_chunks(const mgpt_sample_config* cfg) { return cfg->vocab_size > 8192; }
@@ -1264,23 +1265,20 @@ int check_sample(const mgpt_sample_config* cfg, int num_rows) {
 
 template <typename T>
 hipError_t launch_sample(SampleArgs g, const SampleLayout& l, int num_rows, char* ws, bool cut, hipStream_t st) {
-  if (l.rows == 0) {
-    const int piece = kWave * Piece<T>::N;
-    const size_t lds = (size_t)((g.V + piece - 1) / piece) * 12;
-    hipLaunchKernelGGL(sample_kernel<T>, dim3(num_rows), dim3(kThreads), lds, st, g);
-    return hipGetLastError();
+  if (l.rows > 0) {
+    g.chunks = l.chunks;
+    g.pieces = l.pieces;
+    g.best = (u64*)(ws + l.best);
+    g.bins = (u64*)(ws + l.bins);
+    g.list = (u64*)(ws + l.list);
+    g.sums = (u64*)(ws + l.sums);
+    g.ties = (int*)(ws + l.ties);
+    g.list_n = (int*)(ws + l.list_n);
+    g.cut = (End*)(ws + l.cut);
   }
-  g.chunks = l.chunks;
-  g.pieces = l.pieces;
-  g.best = (u64*)(ws + l.best);
-  g.bins = (u64*)(ws + l.bins);
-  g.list = (u64*)(ws + l.list);
-  g.sums = (u64*)(ws + l.sums);
-  g.ties = (int*)(ws + l.ties);
-  g.list_n = (int*)(ws + l.list_n);
-  g.cut = (End*)(ws + l.cut);
-  for (int r = 0; r < num_rows; r += l.rows) {
-    const int n = std::min(l.rows, num_rows - r);
+  const int slice = l.rows > 0 ? l.rows : kWholeSlice;
+  for (int r = 0; r < num_rows; r += slice) {
+    const int n = std::min(slice, num_rows - r);
     SampleArgs a = g;
     a.logits = (const T*)g.logits + (size_t)r * g.V;
     a.u += r;
@@ -1290,6 +1288,12 @@ hipError_t launch_sample(SampleArgs g, const SampleLayout& l, int num_rows, char
     if (a.k) a.k += r;
     a.token += r;
     if (a.logp) a.logp += r;
+    if (l.rows == 0) {
+      const int piece = kWave * Piece<T>::N;
+      const size_t lds = (size_t)((g.V + piece - 1) / piece) * 12;
+      hipLaunchKernelGGL(sample_kernel<T>, dim3(n), dim3(kThreads), lds, st, a);
+      continue;
+    }
     const dim3 grid(l.chunks, n), block(kChunkThreads);
     hipLaunchKernelGGL(sample_max_kernel<T>, grid, block, 0, st, a);
     hipLaunchKernelGGL(sample_scan_kernel<T>, grid, block, 0, st, a);

@@ -1,5 +1,5 @@
-"""Sampler: min_p down to the units of the weights, parameters that are no numbers.  The reference
-and its tolerances are test_gpu_sample.py's."""
+"""Sampler: min_p down to the units of the weights, parameters that are no numbers, very many rows.
+The reference and its tolerances are test_gpu_sample.py's."""
 import math
 
 import pytest
@@ -72,3 +72,11 @@ def test_negative_min_p_restricts_nothing():
             want = Sampler(V).forward(l, u, top_k=k)
             got = Sampler(V).forward(l, u, top_k=k, min_p=torch.full((8,), -1.0, device="cuda"))
             assert torch.equal(got[0], want[0])
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^22 blocks of 1024 threads are more than a grid holds."""
+    B = (1 << 22) + 1000
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    l = torch.randn(B, 3, generator=gen, device="cuda").bfloat16()
+    check(l, torch.rand(B, generator=gen, device="cuda"), T=torch.rand(B, generator=gen, device="cuda"), k=2, p=0.9)
