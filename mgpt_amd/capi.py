@@ -183,6 +183,13 @@ def on_device(device):
     return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
+def rows(n: int) -> int:
+    """A number of rows as the C ABI takes it, which ctypes would cut to 32 bits."""
+    if n > 0x7FFFFFFF:
+        raise ValueError(f"{n} rows are more than 2^31 - 1")
+    return n
+
+
 def stream(device):
     """The current stream of `device`, as the C ABI takes it.  (The call that
     torch.cuda.current_stream ends in: 0.1 us, where making its Stream object

@@ -78,7 +78,7 @@ class I8Linear:
             raise TypeError(f"x must be {self.dtype}")
         if x.dim() < 1 or x.shape[-1] != self.K or not x.is_contiguous():
             raise ValueError(f"x must be contiguous with {self.K} columns")
-        n = x.numel() // self.K
+        n = capi.rows(x.numel() // self.K)
         with capi.on_device(dev):
             y = torch.empty((*x.shape[:-1], self.M), dtype=self.dtype, device=dev)
             need = ctypes.c_size_t()

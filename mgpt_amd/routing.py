@@ -55,13 +55,14 @@ class ExpertRouting:
         the choice alone.  counts: int32 [E], to which the tokens of each
         expert are added."""
         ptr, dev, rows = self._logits(logits)
+        n = capi.rows(rows.numel())
         b = None if bias is None else self._check(bias, torch.float32, (self.E,), dev, "bias")
         c = None if counts is None else self._check(counts, torch.int32, (self.E,), dev, "counts")
         with capi.on_device(dev):
             idx = torch.empty((*rows, self.k), dtype=torch.int32, device=dev)
             weights = torch.empty_like(idx, dtype=torch.float32)
-            capi.check(capi.lib().mgpt_route_forward(self._cfg, ptr, b, idx.data_ptr(), weights.data_ptr(), c,
-                                                     logits.numel() // self.E, capi.stream(dev)))
+            capi.check(capi.lib().mgpt_route_forward(self._cfg, ptr, b, idx.data_ptr(), weights.data_ptr(), c, n,
+                                                     capi.stream(dev)))
         return idx, weights
 
     def backward(self, logits, idx, weights, dweights, dscores=None):
@@ -69,6 +70,7 @@ class ExpertRouting:
         and dscores (float32 [E]: of every token's score of each expert), from
         forward's input and outputs; the choice is taken as given."""
         ptr, dev, rows = self._logits(logits)
+        n = capi.rows(rows.numel())
         shape = (*rows, self.k)
         ptrs = [self._check(idx, torch.int32, shape, dev, "idx"),
                 self._check(weights, torch.float32, shape, dev, "weights"),
@@ -76,8 +78,8 @@ class ExpertRouting:
                 None if dscores is None else self._check(dscores, torch.float32, (self.E,), dev, "dscores")]
         with capi.on_device(dev):
             dlogits = torch.empty_like(logits)
-            capi.check(capi.lib().mgpt_route_backward(self._cfg, ptr, *ptrs, dlogits.data_ptr(),
-                                                      logits.numel() // self.E, capi.stream(dev)))
+            capi.check(capi.lib().mgpt_route_backward(self._cfg, ptr, *ptrs, dlogits.data_ptr(), n,
+                                                      capi.stream(dev)))
         return dlogits
 
     def balance(self, bias, counts, rate: float) -> None:

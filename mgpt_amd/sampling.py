@@ -43,6 +43,7 @@ class Sampler:
         if logits.dim() < 1 or logits.shape[-1] != self.V:
             raise ValueError(f"logits must have {self.V} columns")
         dev, shape = logits.device, logits.shape[:-1]
+        n = capi.rows(shape.numel())
         ptr = self._check(logits, self.dtype, logits.shape, dev, "logits")
         up = self._check(u, torch.float32, shape, dev, "u")
         cfg = capi.SampleConfig(self.V, self._dt, 1.0, 0, 1.0, 0.0)
@@ -52,14 +53,15 @@ class Sampler:
             if isinstance(v, torch.Tensor):
                 ptrs.append(self._check(v, dt, shape, dev, name))
             else:
-                setattr(cfg, name, v)
+                # (32 bits: a top_k past the vocabulary is all of it, as one below 1)
+                setattr(cfg, name, max(0, min(v, self.V)) if name == "top_k" else v)
                 ptrs.append(None)
         with capi.on_device(dev):
             token = torch.empty(shape, dtype=torch.int32, device=dev)
             logp = torch.empty_like(token, dtype=torch.float32)
             need = ctypes.c_size_t()
-            capi.check(capi.lib().mgpt_sample_workspace_bytes(ctypes.byref(cfg), token.numel(), ctypes.byref(need)))
+            capi.check(capi.lib().mgpt_sample_workspace_bytes(ctypes.byref(cfg), n, ctypes.byref(need)))
             ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
             capi.check(capi.lib().mgpt_sample(ctypes.byref(cfg), ptr, up, *ptrs, token.data_ptr(), logp.data_ptr(),
-                                              token.numel(), ws.data_ptr(), need.value, capi.stream(dev)))
+                                              n, ws.data_ptr(), need.value, capi.stream(dev)))
         return token, logp

@@ -75,7 +75,7 @@ def test_negative_min_p_restricts_nothing():
 
 
 def test_more_rows_than_a_launch_takes():
-    """2^22 blocks of 1024 threads are more than a grid holds."""
+    """2^22 blocks of 1024 threads are more than a grid holds: it ran those past them alone."""
     B = (1 << 22) + 1000
     gen = torch.Generator(device="cuda").manual_seed(1)
     l = torch.randn(B, 3, generator=gen, device="cuda").bfloat16()
