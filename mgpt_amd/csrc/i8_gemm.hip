@@ -189,6 +189,9 @@ __device__ __forceinline__ void put24(const Rows24& to, const float (&x)[16], in
   if (live) *reinterpret_cast<uint4*>(to.low + (size_t)row * to.ld + col + 16 * half) = make_uint4(a[0], a[1], b[0], b[1]);
 }
 
+// The outputs' scales come first: those of rows reach from the smallest to the largest numbers, and a product of the two
+// scales alone would leave them (0 times infinity for a sum of 0, bits lost below 2^-126).
+//
 // Accumulators of TN x TM tiles: outputs fw + 32 j, rows row0 + 32 i of the tile t (row blocks
 // blk + i of A), and the rows' scales.
 template <int KIND, int TN, int TM>
@@ -217,7 +220,7 @@ __device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][T
             const float x = ag * sa[i] * sg[v] + bg[v], u = au * sa[i] * su[v] + bu[v];
             h[v] = x / (1.0f + expf(-x)) * u;
           } else {   // (some 2^-22 off, a quarter of what 20 bits are)
-            const float x = fmaf(ag, sa[i] * sg[v], bg[v]), u = fmaf(au, sa[i] * su[v], bu[v]);
+            const float x = fmaf(ag * sg[v], sa[i], bg[v]), u = fmaf(au * su[v], sa[i], bu[v]);
             h[v] = x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)) * u;
           }
           top = max(top, __float_as_uint(h[v]) & 0x7FFFFFFFu);   // (a NaN lies above all)
@@ -246,7 +249,7 @@ __device__ __forceinline__ void emit8(const I8Args& g, const i32x16 (&acc)[TN][T
         const int row = row0 + 32 * i + lrow;
         float y[16];
 #pragma unroll
-        for (int v = 0; v < 16; ++v) y[v] = (float)acc[j][i][v] * (sa[i] * s[v]) + b[v];
+        for (int v = 0; v < 16; ++v) y[v] = (float)acc[j][i][v] * s[v] * sa[i] + b[v];
         const bool live = row < t.row_end;
         if constexpr (KIND == kI8Rows24) {
           put24(g.o, y, row, f0, half, live);
@@ -296,7 +299,7 @@ __device__ __forceinline__ void emit8_odd(const I8Args& g, const i32x16 (&acc)[T
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         const int row = row0 + 32 * i + 8 * (v / 4) + 4 * half + v % 4;
-        const float y = (float)acc[j][i][v] * (sa[v] * s) + b;
+        const float y = (float)acc[j][i][v] * s * sa[v] + b;
         if (in && row < t.row_end) {
           if constexpr (KIND == kI8Bf16) store_act(reinterpret_cast<bf16_t*>(g.out) + (size_t)row * g.ldo + f, y);
           else reinterpret_cast<float*>(g.out)[(size_t)row * g.ldo + f] = y;
