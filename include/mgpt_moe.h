@@ -110,7 +110,8 @@ int mgpt_moe_workspace_bytes(const mgpt_moe* h, int num_tokens, size_t* bytes);
 /* y[N,C] = MoE(x[N,C]) on `stream`, no host synchronisation.  x and y are
  * act_dtype, row-major, device memory; y must not alias x.  The workspace
  * (>= mgpt_moe_workspace_bytes) holds the routing of this call until the
- * next call that uses it.  num_tokens = 0 is a no-op.  Replaces
+ * next call that uses it.  num_tokens = 0 is a no-op; 2^26 or more (in
+ * training, times top_k) are refused.  Replaces
  * MoELayer::forward_into (layers/MoELayer.cpp:28-128) on the device.
  * No allocation, copy, memset or host synchronisation happens inside, so
  * the call may be captured into a HIP graph (stream capture) and replayed,

@@ -215,6 +215,8 @@ hipError_t launch_i8_quantize(QuantizeSource src, const QuantizeArgs& g, int max
   const size_t size = src == kRowsF32 ? 4 : 2;
   const bool vec = src == kRowsHidden || (g.K * size % 16 == 0 && g.ld * size % 16 == 0 && ((uintptr_t)g.src & 15) == 0);
   const int slabs = (g.K + kI8Slab - 1) / kI8Slab;
+  if ((long)max_blocks * (kI8Rows / kPart) * (slabs <= 4 ? 2 : slabs <= 8 ? 4 : slabs <= 32 ? 8 : 16) * kWave >= 1L << 32)
+    return hipErrorInvalidConfiguration;   // (more threads than a grid holds)
   auto go = [&](auto s, auto v) {
     auto launch = [&](auto kernel, int nw) {
       hipLaunchKernelGGL(kernel, dim3(max_blocks * (kI8Rows / kPart)), dim3(nw * kWave), 0, st, g);

@@ -1380,6 +1380,9 @@ int check_forward_args(const mgpt_moe* h, const void* x, const void* y, int num_
   if (!h->loaded) return fail(MGPT_ERR_NOT_READY, "parameters not loaded");
   if (num_tokens < 0) return fail(MGPT_ERR_INVALID_ARGUMENT, "negative num_tokens");
   if (num_tokens == 0) return MGPT_OK;
+  // a wave for each token in the combine, and for each slot in the backward, and a grid holds fewer than 2^32 threads
+  if ((train ? (long)num_tokens * h->k : (long)num_tokens) >= 1L << 26)
+    return fail(MGPT_ERR_UNSUPPORTED, "num_tokens %d%s >= 2^26", num_tokens, train ? " * top_k" : "");
   if (!x || !y || !workspace) return fail(MGPT_ERR_INVALID_ARGUMENT, "null x, y or workspace");
   if (((uintptr_t)x | (uintptr_t)y) % 16 != 0)
     return fail(MGPT_ERR_INVALID_ARGUMENT, "x and y must be 16-byte aligned");

@@ -54,3 +54,21 @@ def test_top_k_of_any_size():
         for k in (0, -1, V, V + 1, 2 ** 31, 2 ** 32 + 3, -(2 ** 32) + 3, 2 ** 70):
             got = op.forward(l, u, top_k=k)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
+
+
+def test_more_tokens_than_a_grid_holds():
+    import ctypes
+    from mgpt_amd import capi
+    from mgpt_amd.moe import MoELayer
+    for weights, k in (("bf16", 2), ("i8", 4)):
+        L = MoELayer(64, 64, 4, k, act="bf16", weights=weights)
+        r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+        L.load_parameters([r(64, 4), r(4)] + 4 * [r(64, 64), r(64), r(64, 64), r(64), r(64, 64), r(64)])
+        x, y, ws = (ctypes.c_void_p(a << 20) for a in (1, 1 << 30, 1 << 31))     # never read: refused before
+        lib = capi.lib()
+        for n, status in ((1 << 26, capi.MGPT_ERR_UNSUPPORTED), ((1 << 26) - 1, capi.MGPT_ERR_WORKSPACE_TOO_SMALL)):
+            assert lib.mgpt_moe_forward(L._h, x, y, n, ws, 0, None) == status
+            assert lib.mgpt_moe_forward_routed(L._h, x, x, x, y, n, ws, 0, None) == status
+    L = MoELayer(64, 64, 4, 2, act="bf16")
+    L.load_parameters([r(64, 4), r(4)] + 4 * [r(64, 64), r(64), r(64, 64), r(64), r(64, 64), r(64)])
+    assert lib.mgpt_moe_forward_train(L._h, x, y, 1 << 25, ws, 0, None) == capi.MGPT_ERR_UNSUPPORTED
