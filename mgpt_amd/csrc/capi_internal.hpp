@@ -7,6 +7,9 @@ namespace mgpt {
 // thread and returns `code`.
 int fail(int code, const char* fmt, ...);
 
+// CUs of the current device (moe_capi.hip), 256 where they cannot be asked for.
+int compute_units();
+
 }  // namespace mgpt
 
 // Returns MGPT_ERR_HIP, with the call that failed as the description, from a

@@ -19,7 +19,6 @@
 // 2048 x 50257 21 us (4.9 TB/s), 512 rows of 64 experts, 2048 x 2816 80 (4.6), 1408 x 2048 35 (5.2); 999 x 500 x 1003 8
 // (ring of 128 x 128 tiles: 15).
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "../../include/mgpt_moe.h"
@@ -751,17 +750,6 @@ I8Layout i8_layout(const mgpt_i8_config* cfg, int N) {
   l.scale = row_blocks(N) * i8_row_block_bytes(cfg->in_features);   // (a multiple of 4 KB)
   l.total = l.scale + (row_blocks(N) * kI8Rows * 4 + 255) / 256 * 256;
   return l;
-}
-
-// (the device's number is a part of each call's 3 us: asked for once)
-int compute_units() {
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 256;
-  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
-  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
-  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
-  return n;
 }
 
 QuantizeArgs dense_rows(const void* x, int N, int K, char* q, float* scale) {

@@ -1082,14 +1082,6 @@ __global__ __launch_bounds__(1024) void colsum_kernel(const float* __restrict__ 
   }
 }
 
-int compute_units() {
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-    return 256;
-  return n;
-}
-
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 int div_up(int a, int b) { return (a + b - 1) / b; }
 

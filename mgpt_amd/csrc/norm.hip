@@ -603,14 +603,6 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(
   else group_sums[(size_t)g * C + c] = u;
 }
 
-int compute_units() {
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-    return 256;
-  return n;
-}
-
 // Waves and vectors of a row.  Forward: 1024 columns a wave, whose gains then serve more
 // of a row (16384 x 1024: 22.4 us, with 512 24.5; 32768 x 2048: 95 / 110).  Backward: 512,
 // for twice the waves on a CU (norm_backward_kernel, us with 1024 / 512: 16384 x 1024 53 /

@@ -30,7 +30,6 @@
 // bound it, 15 us.  The backward, whose next step's loads are on their way, takes 22 (67 MB, 13 at a copy's rate);
 // 40001 x 160 bf16 (8 groups of 20, softmax) 36 and 13.5, 16384 x 16 3.6 and 2.9.
 #include <algorithm>
-#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -892,17 +891,6 @@ __global__ __launch_bounds__(512) void route_dscore_kernel(const int32_t* __rest
                                                            float alpha, float* __restrict__ dscore) {
   const int e = threadIdx.x;
   if (e < E) dscore[e] = (alpha * (float)E * ((float)counts[e] / (float)N)) / (float)N;
-}
-
-// (the device's number is a part of each call's 3 us: asked for once)
-int compute_units() {
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 256;
-  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
-  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
-  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
-  return n;
 }
 
 // Calls go(lanes per token, experts per lane, softmax) for the config.

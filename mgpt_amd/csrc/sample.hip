@@ -28,7 +28,6 @@
 // row of 50257 with top_k 25 us, of it five launches' latency; one of 8192 16 us.  A block for each row and all
 // steps took 191, 71 and 61 us for the first three.
 #include <algorithm>
-#include <atomic>
 #include <cfloat>
 #include <cmath>
 
@@ -1239,17 +1238,6 @@ SampleLayout sample_layout(const mgpt_sample_config* cfg, int num_rows, int cus)
   l.cut = take(R * sizeof(End));
   l.total = off;
   return l;
-}
-
-// (the device's number is a part of each call's 3 us: asked for once)
-int compute_units() {
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 256;
-  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
-  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
-  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
-  return n;
 }
 
 int check_sample(const mgpt_sample_config* cfg, int num_rows) {
