@@ -1040,7 +1040,7 @@ int forward_impl(mgpt_moe* h, const IoT* x, IoT* y, int N, char* ws, bool train,
     ra.bias = h->route_bias;
     ra.idx = idx;
     ra.weights = topp;
-    ra.drop = 1;
+    ra.how |= kRouteDrop;
     HIP_TRY(launch_route(&h->route, ra, false, st));
     if (block_hist) HIP_TRY(launch_route_take(nullptr, nullptr, N, E, k, idx, topp, block_hist, st));
     if (train) h->route_trained = h->route_set;

@@ -524,12 +524,12 @@ __global__ __launch_bounds__(256, 3) void route_kernel(RouteArgs g) {
       D += sc[i];
     }
     D = across<(LP < 8 ? LP : 8)>(D, [](float a, float b) { return a + b; });   // (lanes 8 .. hold zeros)
-    const float r = g.renorm ? g.scale / (D + 1e-20f) : g.scale;
+    const float r = g.how & kRouteRenorm ? g.scale / (D + 1e-20f) : g.scale;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
       const int j = i * LP + lp;
       if (j < g.k && t < g.N) {
-        g.idx[(size_t)t * g.k + j] = g.drop && !on[i] ? -1 : id[i];
+        g.idx[(size_t)t * g.k + j] = id[i] | (on[i] ? 0 : g.how >> 31);
         g.weights[(size_t)t * g.k + j] = sc[i] * r;
         if (g.counts && on[i]) atomicAdd(&s_count[id[i]], 1);
       }
@@ -779,7 +779,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs g) {
       D += sc[i];
     }
     float inv = 1.0f;
-    if (g.renorm) {
+    if (g.how & kRouteRenorm) {
       D = across<LP>(D, plus);
       inv = 1.0f / (D + 1e-20f);
 #pragma unroll
@@ -801,7 +801,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(RouteArgs g) {
       }
     }
     // (renormalised, the chosen ones' terms cancel but for 1e-20 of c dot)
-    if (g.renorm) sum = c * dot * 1e-20f;
+    if (g.how & kRouteRenorm) sum = c * dot * 1e-20f;
     else sum = across<LP>(sum, plus);
     wave_sync();
     float ds[V];
@@ -951,7 +951,7 @@ RouteArgs route_args(const mgpt_route_config* cfg, const void* logits, const voi
   g.top_groups = cfg->top_groups;
   g.best = cfg->group_best;
   g.scale = cfg->scale;
-  g.renorm = cfg->renormalise;
+  g.how = cfg->renormalise ? kRouteRenorm : 0;
   const uintptr_t row = cfg->dtype == MGPT_DTYPE_F32 ? 16 : 8;
   g.vec = g.E % 4 == 0 && (((uintptr_t)logits | (uintptr_t)dlogits) & (row - 1)) == 0;
   return g;

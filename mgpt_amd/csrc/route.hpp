@@ -6,6 +6,9 @@
 
 namespace mgpt {
 
+constexpr int kRouteRenorm = 1;
+constexpr int kRouteDrop = (int)0x80000000;   // what takes no part has the id -1, instead of the lowest ids left
+
 struct RouteArgs {
   const void* logits;    // [N][E]
   const float* bias;     // [E] or null
@@ -18,8 +21,8 @@ struct RouteArgs {
   void* dlogits;
   int N, E, k, G, S, top_groups, best;   // S = E / G
   float scale;
-  int renorm, vec;
-  int drop;              // what takes no part has the id -1, instead of the lowest ids left
+  int vec;
+  int how;               // one register: kRouteRenorm, kRouteDrop
 };
 
 int check_route(const mgpt_route_config* cfg, int N);   // a status
