@@ -270,7 +270,8 @@ __global__ __launch_bounds__(256) void combine2_kernel(const ActT* __restrict__ 
 }
 
 // The same sums over Rows24: a wave 512 columns of a token, 8 a lane, AT of its rows in flight; in the order of the
-// experts, by fused multiply-adds (these rows have no sum elsewhere to agree with).
+// experts, by fused multiply-adds (these rows have no sum elsewhere to agree with).  16384 x 1024, k 2: 23 us (134 MB, of
+// which the last-level cache holds a part; 2 bytes a value and an exponent for 32 took 20).
 template <int AT>
 __global__ __launch_bounds__(256) void combine24_kernel(Rows24 rows, const int32_t* __restrict__ topk_idx,
                                                         const float* __restrict__ topk_p,

@@ -15,7 +15,8 @@
 //
 // Measured: ring, 16384 x 2048 x 8192 250 us (2200 TOP/s; a library's int8 product of 8192^3 2090); gate/up of 32768 rows x
 // 1024 x 5632 in 16 segments 263 us (1440), of it some 70 the epilogue, which a block that fills the CU has nothing to
-// hide behind (row scales loaded in it, behind the ring's loads, cost 25 more); down, x 2816 x 1024, 123.  Stream, 1 x
+// hide behind (row scales loaded in it, behind the ring's loads, cost 25 more); down, x 2816 x 1024, 127; the two of an fp32
+// caller 302 (a full exponential and a division for each unit, 32 bytes of a row a store) and 140.  Stream, 1 x
 // 2048 x 50257 21 us (4.9 TB/s), 512 rows of 64 experts, 2048 x 2816 80 (4.6), 1408 x 2048 35 (5.2); 999 x 500 x 1003 8
 // (ring of 128 x 128 tiles: 15).
 #include <algorithm>

@@ -1204,7 +1204,9 @@ using namespace mgpt;
 
 namespace {
 
-constexpr int kSlice = 1024;   // rows of a launch in chunks (44 KB of workspace each)
+// Rows of a launch in chunks.  Of workspace each has 40 KB (bins and list), 8 bytes a chunk and 12 bytes for every 256 (fp32)
+// or 512 (bf16) logits: up to 89 KB, at 2^20 fp32 logits, and 89 MB for all of them.
+constexpr int kSlice = 1024;
 constexpr int kWholeSlice = 1 << 20;   // rows of a launch by whole blocks (a launch takes fewer than 2^32 threads)
 
 // Rows of up to 8192 are whole blocks' work in one launch.
