@@ -134,6 +134,29 @@ def test_training_with_fewer_than_k(act, N, masked):
             assert rel(gW, leaves[2 + i].grad) < BAR[act] and rel(gb, leaves[5 + i].grad) < BAR[act]
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("N", [1, 70, 1200])
+def test_training_of_no_expert_at_all(act, N):
+    """Every expert masked: y, dx and all gradients are 0, by the layer alone and in the block (y = x, dx = dy)."""
+    E, k, C = 8, 2, 64
+    c = Case(C, 96, E, k, act, act)
+    c.op.set_routing(rule(E, k, score="sigmoid"), bias=torch.full((E,), -INF, device="cuda"), balance=0.5)
+    x, gamma = c.x(N), torch.ones(C, device="cuda")
+    dy = torch.randn(N, C, device="cuda").to(x.dtype)
+    c.op.reserve(N, train=True)
+    c.op._ws.fill_(255)
+    c.op.zero_grad()
+    y = c.op.forward(x, train=True)
+    dx = c.op.backward(dy)
+    assert (y == 0).all() and (dx == 0).all() and (c.op.routing()["counts"] == 0).all()
+    assert all((g == 0).all() for g in c.op.get_gradients())
+    out = torch.empty_like(x)
+    c.op.forward_block_into(x, gamma, 1e-5, out, train=True)
+    dx, dgamma = c.op.backward_block(dy)
+    assert torch.equal(out, x) and torch.equal(dx, dy) and (dgamma == 0).all()
+    assert all((g == 0).all() for g in c.op.get_gradients())
+
+
 def test_replayed_graph():
     c = Case(64, 96, 8, 2, "bf16", "i8")
     for N in (30, 500):
